@@ -50,6 +50,7 @@ extern "C" {
 
 #define MOE_DTYPE_F32   0
 #define MOE_DTYPE_BF16  1
+#define MOE_DTYPE_FP8   2      /* e4m3fn: the caches of the attention entry points */
 
 #define MOE_ROUTE_SOFTMAX 0   /* select on logits; weights = softmax over all experts      */
 #define MOE_ROUTE_SIGMOID 1   /* scores = sigmoid(logit); select on scores + bias          */
@@ -59,6 +60,8 @@ extern "C" {
 
 #define MOE_MAX_EXPERTS 1024
 #define MOE_MAX_TOPK    32
+#define MOE_MAX_REQUESTS 4096   /* requests of one step of the paged cache */
+#define MOE_MAX_PAGE    1024    /* tokens of a cache page (a power of two) */
 
 /*
  * Library version and the gfx target it was built for.  The version changes whenever a caller built against an
@@ -378,6 +381,79 @@ int moe_layer_fp8_static(void *stream, const void *x_bf16, int T, int H,
 size_t moe_router_logits_workspace_bytes(int T, int H, int E);
 int moe_router_logits(void *stream, const void *x_bf16, int T, int H, const void *router_w_bf16, int E,
                       void *logits_bf16, void *workspace, size_t workspace_bytes);
+
+/*
+ * ---- a serving step around the layer: paged cache, attention, answers -------------------------------------------------
+ * No counterparts among the reference's MoE ops.  What a decoder step with drafted tokens does beside the experts: the
+ * cache's bookkeeping, norms and rotation of queries and keys into the cache, attention over it, and what the logits say
+ * about given tokens.  Lengths, tables and slots stay on the device; nothing is read back by the host.
+ *
+ *   cache      K and V: [n_blocks, page_size, Hkv, D] each, bf16 or e4m3fn, the last three dimensions contiguous, blocks
+ *              *_block_stride elements apart (both may lie in one allocation).  page_size: a power of two.
+ *   slot       block * page_size + place in the page, int64; -1: none.
+ *   tokens     of all requests one after another: request b holds rows [cu_tokens[b], cu_tokens[b + 1]), cu_tokens [B + 1].
+ *   tree       parents [T] int32: of a drafted token, the place of its parent among its own request's (before its own), -1 for
+ *              one that follows the cached text directly.  masks [T] int64: bit i = sees its request's token i.
+ */
+
+/*
+ * What one step needs, from lengths: request b holds lens[b] cached tokens and brings counts[b] new ones (0: idle).
+ * New pages come from the top of the stack free_blocks[0 .. n_free), request by request, and are appended to
+ * block_tables [B, table_width] (rows table_stride apart); n_free_out is what is left of the stack (not the same address as
+ * n_free).  A request is refused - kv_lens 0, its rows' positions and slots -1, masks 0, its table untouched - when its tokens do not
+ * fit its table row or the batch's T rows, when a tree has more than 64 tokens, or when the pages needed by it and the requests before it are more than
+ * there are; the others are granted.  Outputs: cu_tokens [B + 1]; positions [T] int32 (a tree's token: cached
+ * length + depth); slots [T]; masks [T] with parents (without: causal order, masks not written); kv_lens [B] = lens +
+ * counts.  Rows of no request get -1 / -1 / 0.  B <= MOE_MAX_REQUESTS.
+ */
+int moe_cache_plan(void *stream, int32_t *block_tables, int64_t table_stride, int B, int table_width, const int32_t *lens,
+                   const int32_t *counts, const int32_t *free_blocks, int n_free_max, const int32_t *n_free, int page_size,
+                   const int32_t *parents, int T, int32_t *cu_tokens, int32_t *positions, int64_t *slots, int64_t *masks,
+                   int32_t *kv_lens, int32_t *n_free_out);
+
+/*
+ * qkv [T, (Hq + 2 Hkv) D] bf16 (rows row_stride apart): query, key and value heads of a token.  Queries and keys are normalised
+ * per head, y = x rsqrt(mean(x^2) + eps) weight (a NULL weight: not normalised; weights [D] of weight_dtype), then their
+ * first R elements rotated by the angles of the token's position, cos_sin [P, R] fp32 = R/2 cosines, then R/2 sines; pairs
+ * (i, i + R/2), or (2i, 2i + 1) with interleaved.  fp32 throughout, one rounding at the end.
+ * q_out [T, Hq, D] bf16; k_out [T, Hkv, D] bf16 or NULL.  With caches (both or none): keys and values go to slots[t],
+ * in e4m3 after a division by k_scale[head] / v_scale[head] (fp32, NULL: 1).  A position outside [0, P): the q and k rows are zero and nothing is
+ * stored; a slot outside the cache: nothing is stored.  D a multiple of 8 and at most 256, R of 16.
+ */
+int moe_qk_norm_rope(void *stream, const void *qkv_bf16, int64_t row_stride, int T, int Hq, int Hkv, int D,
+                     const int32_t *positions, const float *cos_sin, int P, int R, int interleaved, const void *q_weight,
+                     const void *k_weight, int weight_dtype, float eps, void *q_out_bf16, void *k_out_bf16, void *k_cache,
+                     void *v_cache, int cache_dtype, int n_blocks, int64_t k_block_stride, int64_t v_block_stride, int page_size,
+                     const int64_t *slots, const float *k_scale, const float *v_scale);
+
+/*
+ * Attention of the new tokens over the cache, which holds their own keys and values too (moe_qk_norm_rope has stored
+ * them).  Of request b's kv_lens[b] keys the last n = cu_tokens[b + 1] - cu_tokens[b] are the new tokens'; every new token sees all
+ * before them, and of the new ones those of its mask (masks NULL: itself and the ones before it).
+ * q [T, Hq, D] bf16 (rows q_stride apart), query head h on cache head h / (Hq / Hkv); scores scale * q.k (times k_scale
+ * of the head), out [T, Hq, D] bf16 (times v_scale), lse [T, Hq] fp32 or NULL = log of the sum of exponentials.
+ * A row that sees no key, of a refused request (kv_lens < n) or of no request: out 0, lse -inf.
+ * D 64 or 128; masks cover requests of at most 64 new tokens, without masks there is no limit.
+ * workspace: moe_tree_attention_workspace_bytes(...) bytes, 256-byte aligned.
+ */
+size_t moe_tree_attention_workspace_bytes(int T, int Hq, int Hkv, int D, int B);
+int moe_tree_attention(void *stream, const void *q_bf16, int64_t q_stride, int T, int Hq, int Hkv, int D, const void *k_cache,
+                       const void *v_cache, int cache_dtype, int n_blocks, int64_t k_block_stride, int64_t v_block_stride,
+                       int page_size, const int32_t *block_tables, int64_t table_stride, int table_width, const int32_t *kv_lens,
+                       const int32_t *cu_tokens, int B, const int64_t *masks, float scale, const float *k_scale,
+                       const float *v_scale, void *out_bf16, float *lse, void *workspace, size_t workspace_bytes);
+
+/*
+ * logits [T, V] fp32 or bf16 (rows row_stride apart) divided by temperature: logprobs [T] of tokens [T] int64, entropy [T]
+ * in nats, and with k > 0 the k most likely tokens, top_ids [T, k] int32 and top_logprobs [T, k], equal logits by the lower index.  All
+ * results fp32.  A logit of -inf is a token that cannot come; a row of nothing else: logprobs -inf, entropy 0.  A token
+ * outside [0, V): -inf.  A row with a NaN or +inf: NaN (NaN logits are no alternatives: id -1 where others run out).
+ * workspace: moe_token_logprobs_workspace_bytes(...) bytes, 256-byte aligned.  k <= MOE_MAX_TOPK.
+ */
+size_t moe_token_logprobs_workspace_bytes(int T, int V, int k, int logits_dtype);
+int moe_token_logprobs(void *stream, const void *logits, int logits_dtype, int64_t row_stride, int T, int V, const int64_t *tokens,
+                       int k, float temperature, float *logprobs, float *entropy, float *top_logprobs, int32_t *top_ids,
+                       void *workspace, size_t workspace_bytes);
 
 #ifdef __cplusplus
 }

@@ -16,10 +16,10 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmoe_hip.so")
 PROBE_LIB = os.path.join(HERE, "libmoe_bench_probe.so")
 SOURCES = ["route.hip", "permute.hip", "quant_reduce.hip", "gemm_fp8.hip", "dense_small.hip", "decode_prep.hip", "router_front.hip",
-           "capi.hip"]
+           "cache_plan.hip", "qk_norm_rope.hip", "tree_attention.hip", "token_logprobs.hip", "capi.hip"]
 PROBE_SOURCES = ["probe.hip"]
 SHIM_LIB = os.path.join(HERE, "libmy_ops_torch.so")
-SHIM_SOURCE = "my_ops.cpp"
+SHIM_SOURCES = ["my_ops.cpp", "serving_ops.cpp"]
 # packed fp32 VALU ops are switched off for every kernel in this library
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-Wno-inline-asm",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
@@ -33,14 +33,14 @@ def hipcc():
 
 
 def build_shim(verbose=True):
-    """csrc/my_ops.cpp -> libmy_ops_torch.so: TORCH_LIBRARY(my_ops, ...) on top of libmoe_hip.so, plain host C++."""
+    """csrc/my_ops.cpp, csrc/serving_ops.cpp -> libmy_ops_torch.so: TORCH_LIBRARY(my_ops, ...) on top of libmoe_hip.so, plain host C++."""
     import torch
     tdir = os.path.dirname(os.path.abspath(torch.__file__))
     cxx = os.environ.get("CXX", "g++")
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wno-unknown-pragmas", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-I" + os.path.join(tdir, "include"), "-I" + os.path.join(tdir, "include", "torch", "csrc", "api", "include"),
-           "-I/opt/rocm/include", os.path.join(CSRC, SHIM_SOURCE), "-o", SHIM_LIB,
+           "-I/opt/rocm/include", *(os.path.join(CSRC, s) for s in SHIM_SOURCES), "-o", SHIM_LIB,
            "-L" + os.path.join(tdir, "lib"), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-lamdhip64", "-L" + HERE, "-lmoe_hip",
            "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
