@@ -6,16 +6,21 @@
 // One pass over the keys with the running maximum and sum of the softmax, both fp32, as is the output until its one
 // rounding.  A token that sees nothing gives 0 and -inf.
 #include <math.h>
+#include <type_traits>
 #include "moe_common.h"
 #include "moe_layout.h"
 #include "../../include/moe_hip.h"
 
 namespace moe {
 
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+
 struct AttnArgs {
   const uint16_t *q;
   int64_t q_stride;
-  int T, Hq, Hkv, D, B, n_blocks, page_log2, table_width;
+  int T, Hq, Hkv, G, B, n_blocks, page_log2, table_width;
   const uint8_t *k_cache, *v_cache;
   int64_t k_block_bytes, v_block_bytes, table_stride;
   const int32_t *tables, *kv_lens, *cu;
@@ -24,104 +29,656 @@ struct AttnArgs {
   const float *k_scale, *v_scale;
   uint16_t *out;
   float *lse;
+  int min_units, groups;               // least units of a workgroup; workgroups of the main launch
+  float *part_o, *part_ml;             // [2 groups][rows][D]; [2 groups][rows][2]
+  int32_t *records;                    // [groups][8]: of the tile that begins in a stretch and goes on: last stretch, request, head, tile, part
 };
 
-// the request whose tokens hold row t: the last one with cu[b] <= t
-__device__ __forceinline__ int attn_request(const int32_t *cu, int B, int t) {
-  int lo = 0, hi = B - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (cu[mid] <= t) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
+// ---- who does what ----------------------------------------------------------------------------------------------------
+// The work is a line of units: for each request, each cache head, each tile of ROWS of its rows (a row: a token and a query
+// head of the cache head's group), each UNIT keys that the tile sees.  Every workgroup takes an equal stretch of the line,
+// which may begin and end inside a tile and hold several, so that ragged lengths cost nothing.  A tile that lies in one stretch
+// is finished there; of the others each stretch leaves (max, sum, weighted values), which the second launch joins in
+// order.  The line's length is on the device, so every workgroup adds it up.
+struct AttnRequest {
+  int t0, n, kv, prefix;
+};
+__device__ __forceinline__ AttnRequest attn_request(const AttnArgs &a, int b) {
+  const int t0 = min(max(a.cu[b], 0), a.T), t1 = min(max(a.cu[b + 1], t0), a.T);
+  const int kv = (int)min((int64_t)a.kv_lens[b], (int64_t)a.table_width << a.page_log2);
+  return {t0, t1 - t0, kv, kv - (t1 - t0)};
+}
+// rows of tile m see keys below this
+template <int ROWS>
+__device__ __forceinline__ int attn_tile_end(const AttnArgs &a, const AttnRequest &r, int m) {
+  if (a.masks || r.n == 1) return r.kv;
+  return r.prefix + min(r.n, (min((m + 1) * ROWS, r.n * a.G) - 1) / a.G + 1);
+}
+template <int ROWS, int UNIT>
+__device__ __forceinline__ int64_t attn_head_units(const AttnArgs &a, const AttnRequest &r) {
+  if (r.n <= 0 || r.prefix < 0) return 0;
+  const int tiles = (r.n * a.G + ROWS - 1) / ROWS;
+  if (a.masks || r.n == 1) return (int64_t)tiles * ((r.kv + UNIT - 1) / UNIT);
+  int64_t sum = 0;
+  for (int m = 0; m < tiles; m++) sum += (attn_tile_end<ROWS>(a, r, m) + UNIT - 1) / UNIT;
+  return sum;
 }
 
-// A workgroup for each token and query head; groups of LPK lanes take keys in turn, 8 elements a lane.
-template <int LPK, bool FP8>
-__global__ __launch_bounds__(256) void tree_attention_simple_kernel(const AttnArgs a) {
-  constexpr int G = 256 / LPK;
-  __shared__ float sh_m[G], sh_l[G], sh_o[G][LPK * 8 + 1];
-  const int t = blockIdx.x / a.Hq, h = blockIdx.x % a.Hq, kh = h / (a.Hq / a.Hkv);
-  const int grp = threadIdx.x / LPK, L = threadIdx.x % LPK, e = 8 * L;
-  const bool live = e < a.D;
-  const int b = attn_request(a.cu, a.B, t);
-  const int t0 = a.cu[b], n = min(a.cu[b + 1], a.T) - t0, j = t - t0;
-  const int kv = min(a.kv_lens[b], a.table_width << a.page_log2), prefix = kv - n;
-  const bool here = j >= 0 && j < n && prefix >= 0;
-  const uint64_t mask = a.masks ? (uint64_t)a.masks[t] : 0;
-  const float sc = a.scale * (a.k_scale ? a.k_scale[kh] : 1.f) * 1.4426950408889634f;
-  float q[8], o[8], m = -INFINITY, l = 0.f;
-  const v4i raw = live ? *(const v4i *)(a.q + (size_t)t * a.q_stride + (size_t)h * a.D + e) : (v4i){0, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    q[i] = bf16_to_f32((uint16_t)((uint32_t)raw[i / 2] >> (16 * (i & 1))));
-    o[i] = 0.f;
-  }
-  const auto load8 = [&](const uint8_t *at, float *v) {
-    if (FP8) {
-      const v2i r = *(const v2i *)at;
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(r[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(r[i], true);
-        v[4 * i] = lo[0], v[4 * i + 1] = lo[1], v[4 * i + 2] = hi[0], v[4 * i + 3] = hi[1];
-      }
-    } else {
-      const v4i r = *(const v4i *)at;
-#pragma unroll
-      for (int i = 0; i < 8; i++) v[i] = bf16_to_f32((uint16_t)((uint32_t)r[i / 2] >> (16 * (i & 1))));
-    }
-  };
-  if (here)
-    for (int key = grp; key < kv; key += G) {
-      const int i = key - prefix;
-      if (i >= 0 && !(a.masks ? i < 64 && (mask >> i & 1) : i <= j)) continue;
-      const int block = min(max(a.tables[(size_t)b * a.table_stride + (key >> a.page_log2)], 0), a.n_blocks - 1);
-      const int64_t within = (((int64_t)(key & ((1 << a.page_log2) - 1)) * a.Hkv + kh) * a.D + e) * (FP8 ? 1 : 2);
-      float k[8], v[8], s = 0.f;
-      if (live) {
-        load8(a.k_cache + block * a.k_block_bytes + within, k);
-        load8(a.v_cache + block * a.v_block_bytes + within, v);
-#pragma unroll
-        for (int x = 0; x < 8; x++) s = fmaf(q[x], k[x], s);
-      }
-#pragma unroll
-      for (int d = 1; d < LPK; d <<= 1) s += __shfl_xor(s, d, 64);
-      s *= sc;
-      const float m2 = fmaxf(m, s), base = m2 == -INFINITY ? 0.f : m2;
-      const float f = exp2f(m - base), p = exp2f(s - base);
-      m = m2;
-      l = l * f + p;
-      if (live)
-#pragma unroll
-        for (int x = 0; x < 8; x++) o[x] = o[x] * f + p * v[x];
-    }
-  if (L == 0) sh_m[grp] = m, sh_l[grp] = l;
-#pragma unroll
-  for (int x = 0; x < 8; x++) sh_o[grp][e + x] = o[x];
-  __syncthreads();
-  float top = -INFINITY;
-  for (int i = 0; i < G; i++) top = fmaxf(top, sh_m[i]);
-  const float base = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
-  for (int i = 0; i < G; i++) sum += sh_l[i] * exp2f(sh_m[i] - base);
-  const float vs = a.v_scale ? a.v_scale[kh] : 1.f;
-  for (int d = threadIdx.x; d < a.D; d += 256) {
-    float r = 0.f;
-    for (int i = 0; i < G; i++) {
-      const float f = exp2f(sh_m[i] - base);
-      if (f != 0.f) r += sh_o[i][d] * f;
-    }
-    a.out[((size_t)t * a.Hq + h) * a.D + d] = f32_to_bf16(top == -INFINITY && sum == 0.f ? 0.f : r / sum * vs);
-  }
-  if (a.lse && threadIdx.x == 0) a.lse[(size_t)t * a.Hq + h] = (top == -INFINITY && sum == 0.f) ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
+struct AttnLine {
+  int64_t waves[4];
+  int64_t before;
+  int b;
+};
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)v) | (int64_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32;
 }
+
+// The line's length; sh.b and sh.before: the request that holds place which(total) of it, and the units before that.
+template <int ROWS, int UNIT, typename Which>
+__device__ __forceinline__ int64_t attn_line(const AttnArgs &a, AttnLine &sh, Which which) {
+  const int tid = threadIdx.x, lane = tid & 63, per = (a.B + 255) / 256, b0 = tid * per;
+  int64_t mine = 0;
+  for (int b = b0; b < min(b0 + per, a.B); b++) mine += attn_head_units<ROWS, UNIT>(a, attn_request(a, b)) * a.Hkv;
+  int64_t upto = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t o = __shfl_up(upto, d, 64);
+    if (lane >= d) upto += o;
+  }
+  if (lane == 63) sh.waves[tid >> 6] = upto;
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if (i < (tid >> 6)) upto += sh.waves[i];
+    total += sh.waves[i];
+  }
+  const int64_t place = which(total);
+  int64_t before = upto - mine;
+  if (place >= before && place < upto) {
+    int b = b0;
+    for (;; b++) {
+      const int64_t units = attn_head_units<ROWS, UNIT>(a, attn_request(a, b)) * a.Hkv;
+      if (place < before + units) break;
+      before += units;
+    }
+    sh.b = b;
+    sh.before = before;
+  }
+  __syncthreads();
+  return uniform(total);
+}
+__device__ __forceinline__ int64_t attn_stretch(const AttnArgs &a, int64_t total) {
+  const int64_t even = (total + a.groups - 1) / a.groups;
+  return even > a.min_units ? even : a.min_units;
+}
+
+// ---- softmax and products of 32 keys ----------------------------------------------------------------------------------
+// Scores are formed transposed, S^T = K Q^T, so that a lane holds for ONE query (lane % 16) the keys 4 g + i, g = lane / 16, of two
+// tiles of 16.  Those eight are at once the lane's operand of O^T = V^T P^T, if the reduction runs over the keys in that
+// order: no probability changes its lane.  V^T comes from row-major values in LDS by the transposing read.
+// p = 2^(s c - m): m follows the maximum only when that has grown by more than 8, so p stays below 2^8 and the output is
+// seldom rescaled.  p is rounded to bf16 for the product (what the matrix cores take; an error of 2^-9 of each term, as the
+// output's own rounding); its sum is taken before that, in fp32.
+__device__ __forceinline__ float over_groups(float v, bool sum) {
+  v2u r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = sum ? __uint_as_float(r[0]) + __uint_as_float(r[1]) : fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return sum ? __uint_as_float(r[0]) + __uint_as_float(r[1]) : fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+template <int NQ, int DT>
+struct AttnState {
+  v4f o[DT][NQ];
+  float m[NQ], off[NQ], l[NQ];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int qc = 0; qc < NQ; qc++) {
+      m[qc] = -INFINITY;
+      off[qc] = l[qc] = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < DT; dt++) o[dt][qc] = (v4f){0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  // s -> probabilities, as the second product's operand
+  __device__ __forceinline__ void softmax(const v4f (&s)[2][NQ], float c, v8bf (&p)[NQ]) {
+    float top[NQ];
+    bool grown = false;
+#pragma unroll
+    for (int qc = 0; qc < NQ; qc++) {
+      float t = fmaxf(fmaxf(s[0][qc][0], s[0][qc][1]), s[0][qc][2]);
+      t = fmaxf(fmaxf(t, s[0][qc][3]), s[1][qc][0]);
+      t = fmaxf(fmaxf(t, s[1][qc][1]), s[1][qc][2]);
+      top[qc] = fmaxf(t, s[1][qc][3]) * c;
+      grown |= top[qc] > m[qc] + 8.f;
+    }
+    if (__any(grown)) {
+#pragma unroll
+      for (int qc = 0; qc < NQ; qc++) {
+        const float t = over_groups(top[qc], false), now = t > m[qc] + 8.f ? t : m[qc];
+        const float f = now == m[qc] ? 1.f : __builtin_amdgcn_exp2f(m[qc] - now);
+        m[qc] = now;
+        off[qc] = now == -INFINITY ? 0.f : now;
+        l[qc] *= f;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) o[dt][qc] *= f;
+      }
+    }
+#pragma unroll
+    for (int qc = 0; qc < NQ; qc++) {
+      float e[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) e[i] = __builtin_amdgcn_exp2f(fmaf(s[i / 4][qc][i % 4], c, -off[qc]));
+      l[qc] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+      const v4i w = {(int)pack2_bf16(e[0], e[1]), (int)pack2_bf16(e[2], e[3]), (int)pack2_bf16(e[4], e[5]), (int)pack2_bf16(e[6], e[7])};
+      p[qc] = __builtin_bit_cast(v8bf, w);
+    }
+  }
+  // o += V^T p; `at`: this lane's address in the first 16 rows of the values
+  template <int LD>
+  __device__ __forceinline__ void add_values(const uint8_t *at, const v8bf (&p)[NQ]) {
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) {
+      typedef __attribute__((address_space(3))) v4s lds_v4s;
+      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(at + 32 * dt));
+      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(at + 16 * LD + 32 * dt));
+      const v8bf v = __builtin_bit_cast(v8bf, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+      for (int qc = 0; qc < NQ; qc++) o[dt][qc] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[qc], o[dt][qc], 0, 0, 0);
+    }
+  }
+};
+
+// what a lane's queries see of the new tokens
+template <int NQ>
+struct AttnSight {
+  uint64_t mask[NQ];
+  int last[NQ];                        // without masks: the last key seen
+  __device__ __forceinline__ bool sees(const AttnArgs &a, const AttnRequest &r, int qc, int key) const {
+    const int i = key - r.prefix;
+    return a.masks ? i < 0 || (key < r.kv && i < 64 && (mask[qc] >> (i & 63) & 1)) : key <= last[qc];
+  }
+};
+
+// Hides what a lane's queries do not see; the scores left are scaled already.
+template <int NQ>
+__device__ __forceinline__ void attn_hide(const AttnArgs &a, const AttnRequest &r, const AttnSight<NQ> &sight, int first_key, float c,
+                                          v4f (&s)[2][NQ]) {
+  const int g4 = 4 * ((threadIdx.x & 63) >> 4);
+#pragma unroll
+  for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+    for (int qc = 0; qc < NQ; qc++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) s[kt][qc][i] = sight.sees(a, r, qc, first_key + 16 * kt + g4 + i) ? s[kt][qc][i] * c : -INFINITY;
+}
+
+// 16 bytes of the cache -> operands of 8 bf16: themselves, or two of e4m3 codes
+__device__ __forceinline__ v8bf attn_widen(const v4i raw, int half) {
+  const uint32_t w0 = (uint32_t)raw[2 * half], w1 = (uint32_t)raw[2 * half + 1];
+  const v4i w = {__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, 1.0f, false)),
+                 __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, 1.0f, true)),
+                 __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, 1.0f, false)),
+                 __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, 1.0f, true))};
+  return __builtin_bit_cast(v8bf, w);
+}
+// two bf16 in a word: which are NaN or infinite -> 0xffff in their place
+__device__ __forceinline__ uint32_t no_numbers(uint32_t w) {
+  return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+}
+
+__device__ __forceinline__ int attn_block(const AttnArgs &a, const int32_t *table, int key) {
+  return min(max(table[key >> a.page_log2], 0), a.n_blocks - 1);
+}
+// where a head's key or value of a block lies
+template <int BYTES>
+__device__ __forceinline__ const uint8_t *attn_row(const AttnArgs &a, const uint8_t *cache, int64_t block_bytes, int block, int kh, int key) {
+  return cache + block * block_bytes + (uint32_t)(((key & ((1 << a.page_log2) - 1)) * a.Hkv + kh) * BYTES);
+}
+
+// A value that is NaN or infinite would, times a probability of 0, reach rows that do not see its key.  Where new tokens are among
+// the keys such values are staged as 0, and this adds them to the rows that do see them.
+template <int NQ, int DT, bool FP8>
+__device__ __forceinline__ void attn_add_no_numbers(const AttnArgs &a, const AttnRequest &r, const AttnSight<NQ> &sight, const int32_t *table,
+                                                 int kh, int first_key, int keys, AttnState<NQ, DT> &st) {
+  const int g4 = 4 * ((threadIdx.x & 63) >> 4);
+  for (int key = first_key; key < min(first_key + keys, r.kv); key++) {
+    const uint8_t *row = attn_row<DT * (FP8 ? 16 : 32)>(a, a.v_cache, a.v_block_bytes, attn_block(a, table, key), kh, key);
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int d = 16 * dt + g4 + i;
+        const float v = FP8 ? __builtin_amdgcn_cvt_f32_fp8((uint32_t)row[d], 0) : bf16_to_f32(((const uint16_t *)row)[d]);
+        if (__builtin_isfinite(v)) continue;
+#pragma unroll
+        for (int qc = 0; qc < NQ; qc++)
+          if (sight.sees(a, r, qc, key)) st.o[dt][qc][i] += v;
+      }
+  }
+}
+
+// a lane's queries as the scores' second operand: element j of step s is d = 32 s + 8 g + j, or with e4m3 keys, of which a lane reads
+// 16 at a time, d = 64 (s / 2) + 16 g + 8 (s % 2) + j
+template <int NQ, int D, bool FP8>
+__device__ __forceinline__ void attn_queries(const AttnArgs &a, const AttnRequest &r, int kh, int first_row, v8bf (&q)[NQ][D / 32],
+                                             AttnSight<NQ> &sight) {
+  const int lane = threadIdx.x & 63, g = lane >> 4;
+#pragma unroll
+  for (int qc = 0; qc < NQ; qc++) {
+    const int row = min(first_row + 16 * qc + (lane & 15), r.n * a.G - 1), j = row / a.G, h = kh * a.G + row - j * a.G;
+    const uint16_t *src = a.q + (size_t)(r.t0 + j) * a.q_stride + (size_t)h * D;
+#pragma unroll
+    for (int s = 0; s < D / 32; s++) q[qc][s] = *(const v8bf *)(src + (FP8 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g));
+    sight.mask[qc] = a.masks ? (uint64_t)a.masks[r.t0 + j] : 0;
+    sight.last[qc] = r.prefix + j;
+  }
+}
+
+// Four neighbouring outputs of a row: finished, or as a stretch's part of it.
+template <int ROWS, int D>
+__device__ __forceinline__ void attn_store(const AttnArgs &a, const AttnRequest &r, int kh, int m_tile, int row_in_tile, int d, bool whole,
+                                           int64_t part, const v4f o, float m, float l) {
+  const int row = m_tile * ROWS + row_in_tile;
+  if (row >= r.n * a.G) return;
+  if (!whole) {
+    *(v4f *)(a.part_o + ((size_t)part * ROWS + row_in_tile) * D + d) = o;
+    if (d == 0) {
+      a.part_ml[((size_t)part * ROWS + row_in_tile) * 2] = m;
+      a.part_ml[((size_t)part * ROWS + row_in_tile) * 2 + 1] = l;
+    }
+    return;
+  }
+  const int j = row / a.G, h = kh * a.G + row - j * a.G;
+  const size_t at = (size_t)(r.t0 + j) * a.Hq + h;
+  const bool none = m == -INFINITY && l == 0.f;
+  const float f = none ? 0.f : (a.v_scale ? a.v_scale[kh] : 1.f) / l;
+  *(v2i *)(a.out + at * D + d) = (v2i){(int)pack2_bf16(o[0] * f, o[1] * f), (int)pack2_bf16(o[2] * f, o[3] * f)};
+  if (a.lse && d == 0) a.lse[at] = none ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+}
+
+// A workgroup's way along its stretch: calls segment(request, head, tile, units c0 .. c1 of the tile's u, part) for each piece.
+template <int ROWS, int UNIT, typename Segment>
+__device__ __forceinline__ void attn_walk(const AttnArgs &a, AttnLine &line, Segment segment) {
+  int64_t start = 0, per = 1;
+  const int64_t total = attn_line<ROWS, UNIT>(a, line, [&](int64_t t) {
+    per = attn_stretch(a, t);
+    start = (int64_t)blockIdx.x * per;
+    return start;
+  });
+  per = uniform(per);
+  start = uniform(start);
+  int64_t at = start, end = start + per < total ? start + per : total;
+  if (threadIdx.x == 0) a.records[8 * blockIdx.x] = -1;
+  if (at >= end) return;
+  int b = __builtin_amdgcn_readfirstlane(line.b);
+  int64_t before = uniform(line.before);
+  while (at < end) {
+    const AttnRequest r = attn_request(a, b);
+    const int64_t head = attn_head_units<ROWS, UNIT>(a, r);
+    if (at >= before + head * a.Hkv) {
+      before += head * a.Hkv;
+      b++;
+      continue;
+    }
+    const int kh = (int)((at - before) / head);
+    const int64_t in_head = at - before - kh * head;
+    int m = 0, u = (r.kv + UNIT - 1) / UNIT;
+    int64_t first = 0;
+    if (a.masks || r.n == 1) {
+      m = (int)(in_head / u);
+      first = (int64_t)m * u;
+    } else {
+      for (;; m++) {
+        u = (attn_tile_end<ROWS>(a, r, m) + UNIT - 1) / UNIT;
+        if (in_head < first + u) break;
+        first += u;
+      }
+    }
+    const int c0 = (int)(in_head - first), c1 = (int)(u < c0 + (end - at) ? u : c0 + (end - at));
+    if (threadIdx.x == 0 && c0 == 0 && c1 < u) {
+      int32_t *rec = a.records + 8 * blockIdx.x;
+      rec[0] = (int32_t)((at + u - 1) / per), rec[1] = b, rec[2] = kh, rec[3] = m, rec[4] = at > start;
+    }
+    segment(r, b, kh, m, c0, c1, c0 == 0 && c1 == u, 2 * (int64_t)blockIdx.x + (at - c0 > start ? 1 : 0));
+    at += c1 - c0;
+  }
+}
+
+// ---- few rows: the four wavefronts take the keys in turn --------------------------------------------------------------
+// Up to 64 rows to a cached key the cache's bytes bound it.  A wavefront takes 32 keys of a unit of 128 by itself: keys go
+// from memory straight into operand registers, values through LDS that no other wavefront touches, so nothing waits at a
+// barrier, and the next keys and values are asked for before the present ones are worked on.  The wavefronts' results meet in
+// LDS at the end of a tile.
+template <int D, bool FP8, int NQ>
+__global__ __launch_bounds__(256, 2) void attn_keys_kernel(const AttnArgs a) {
+  constexpr int ROWS = 16 * NQ, UNIT = 128, DT = D / 16, LD = 2 * D + 32, P = FP8 ? D / 64 : D / 32;   // P: 16-byte pieces of a lane's key
+  constexpr int kValues = 4 * 32 * LD, kMerge = 4 * DT * NQ * 64 * 16;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kValues > kMerge ? kValues : kMerge];
+  __shared__ float sh_m[4][ROWS], sh_l[4][ROWS];
+  __shared__ AttnLine line;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c16 = lane & 15;
+  uint8_t *values = lds + w * 32 * LD;
+  const uint8_t *read_at = values + (4 * g + c16 / 4) * LD + 8 * (c16 % 4);
+  attn_walk<ROWS, UNIT>(a, line, [&](const AttnRequest r, int b, int kh, int m_tile, int c0, int c1, bool whole, int64_t part) {
+    const int32_t *table = a.tables + (size_t)b * a.table_stride;
+    const float scale = a.scale * (a.k_scale ? a.k_scale[kh] : 1.f) * 1.4426950408889634f;
+    v8bf q[NQ][D / 32];
+    AttnSight<NQ> sight;
+    attn_queries<NQ, D, FP8>(a, r, kh, m_tile * ROWS, q, sight);
+    const int clear = a.masks ? r.prefix : r.prefix + m_tile * ROWS / a.G + 1;      // keys below it are seen by every row
+    AttnState<NQ, DT> st;
+    st.clear();
+    // The block of a key is read two units ahead of the key, so that no load waits for another one.
+    v4i kr[2][P], vr[2][P];
+    int block[2];
+    const auto key_of = [&](int unit, int kt) { return min(unit * UNIT + 32 * w + 16 * kt + c16, r.kv - 1); };
+    const auto blocks = [&](int unit) {
+#pragma unroll
+      for (int kt = 0; kt < 2; kt++) block[kt] = attn_block(a, table, key_of(unit, kt));
+    };
+    const auto load = [&](const uint8_t *cache, int64_t block_bytes, int unit, v4i (&to)[2][P]) {
+#pragma unroll
+      for (int kt = 0; kt < 2; kt++) {
+        const uint8_t *row = attn_row<FP8 ? D : 2 * D>(a, cache, block_bytes, block[kt], kh, key_of(unit, kt)) + 16 * g;
+#pragma unroll
+        for (int p = 0; p < P; p++) to[kt][p] = *(const v4i *)(row + 64 * p);
+      }
+    };
+    blocks(c0);
+    load(a.k_cache, a.k_block_bytes, c0, kr);
+    load(a.v_cache, a.v_block_bytes, c0, vr);
+    blocks(min(c0 + 1, c1 - 1));
+    for (int c = c0; c < c1; c++) {
+      const int key0 = c * UNIT + 32 * w;
+      v4f s[2][NQ];
+#pragma unroll
+      for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+        for (int qc = 0; qc < NQ; qc++) {
+          s[kt][qc] = (v4f){0.f, 0.f, 0.f, 0.f};
+        }
+#pragma unroll
+      for (int x = 0; x < D / 32; x++)
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++) {
+          const v8bf k = FP8 ? attn_widen(kr[kt][x / 2], x % 2) : __builtin_bit_cast(v8bf, kr[kt][FP8 ? 0 : x]);
+#pragma unroll
+          for (int qc = 0; qc < NQ; qc++) s[kt][qc] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[qc][x], s[kt][qc], 0, 0, 0);
+        }
+      load(a.k_cache, a.k_block_bytes, min(c + 1, c1 - 1), kr);
+      const bool edge = key0 + 32 > clear;
+      // values into LDS, rows of bf16
+      uint32_t odd = 0;
+#pragma unroll
+      for (int kt = 0; kt < 2; kt++) {
+        uint8_t *row = values + (16 * kt + c16) * LD + (FP8 ? 32 : 16) * g;
+        const bool there = key0 + 16 * kt + c16 < r.kv;
+#pragma unroll
+        for (int x = 0; x < D / 32; x++) {
+          v4i v = FP8 ? __builtin_bit_cast(v4i, attn_widen(vr[kt][x / 2], x % 2)) : vr[kt][FP8 ? 0 : x];
+          if (edge) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const uint32_t bad = no_numbers((uint32_t)v[i]);
+              odd |= there ? bad : 0;
+              v[i] = there ? v[i] & (int)~bad : 0;
+            }
+          }
+          *(v4i *)(row + (FP8 ? 128 * (x / 2) + 16 * (x % 2) : 64 * x)) = v;
+        }
+      }
+      load(a.v_cache, a.v_block_bytes, min(c + 1, c1 - 1), vr);
+      blocks(min(c + 2, c1 - 1));
+      float scl = scale;
+      if (edge) {
+        attn_hide<NQ>(a, r, sight, key0, scale, s);
+        scl = 1.f;
+      }
+      v8bf p[NQ];
+      st.softmax(s, scl, p);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      st.template add_values<LD>(read_at, p);
+      if (edge && __any(odd != 0)) attn_add_no_numbers<NQ, DT, FP8>(a, r, sight, table, kh, key0, 32, st);
+      __builtin_amdgcn_wave_barrier();
+    }
+    // the wavefronts' results, each scaled to the common maximum, a quarter of the columns to each wavefront
+    __syncthreads();
+#pragma unroll
+    for (int qc = 0; qc < NQ; qc++) {
+      const float l = over_groups(st.l[qc], true);
+      if (g == 0) {
+        sh_m[w][16 * qc + c16] = st.m[qc];
+        sh_l[w][16 * qc + c16] = l;
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; dt++) *(v4f *)(lds + (((size_t)w * DT + dt) * NQ + qc) * 1024 + lane * 16) = st.o[dt][qc];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int qc = 0; qc < NQ; qc++) {
+      const int row = 16 * qc + c16;
+      float m = sh_m[0][row], l = 0.f, f[4];
+#pragma unroll
+      for (int i = 1; i < 4; i++) m = fmaxf(m, sh_m[i][row]);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        f[i] = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(sh_m[i][row] - m);
+        l += sh_l[i][row] * f[i];
+      }
+#pragma unroll
+      for (int x = 0; x < DT / 4; x++) {
+        const int dt = w * (DT / 4) + x;
+        v4f o = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4; i++) o += *(const v4f *)(lds + (((size_t)i * DT + dt) * NQ + qc) * 1024 + lane * 16) * f[i];
+        attn_store<ROWS, D>(a, r, kh, m_tile, row, 16 * dt + 4 * g, whole, part, o, m, l);
+      }
+    }
+    __syncthreads();
+  });
+}
+
+// ---- many rows: the four wavefronts take the rows, and share the keys ----------------------------------------------------
+// From about 100 rows to a cached key on the products bound it.  A workgroup stages 64 keys and values at a time in LDS, two
+// stages of them, and every wavefront takes its rows past all of them: one barrier a stage, the next stage's bytes in
+// registers meanwhile.
+template <int D, bool FP8, int NQ>
+__global__ __launch_bounds__(256, 2) void attn_rows_kernel(const AttnArgs a) {
+  constexpr int ROWS = 64 * NQ, UNIT = 64, DT = D / 16, LK = 2 * D + 16, LV = 2 * D + 32, STAGE = UNIT * (LK + LV);
+  constexpr int BYTES = FP8 ? D : 2 * D, PER_ROW = BYTES / 16, RPI = 256 / PER_ROW, NU = UNIT / RPI;   // 16-byte pieces of a row; rows at a time
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
+  __shared__ AttnLine line;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c16 = lane & 15;
+  attn_walk<ROWS, UNIT>(a, line, [&](const AttnRequest r, int b, int kh, int m_tile, int c0, int c1, bool whole, int64_t part) {
+    const int32_t *table = a.tables + (size_t)b * a.table_stride;
+    const float scale = a.scale * (a.k_scale ? a.k_scale[kh] : 1.f) * 1.4426950408889634f;
+    v8bf q[NQ][D / 32];
+    AttnSight<NQ> sight;
+    attn_queries<NQ, D, false>(a, r, kh, m_tile * ROWS + 16 * NQ * w, q, sight);
+    const int clear = a.masks ? r.prefix : r.prefix + m_tile * ROWS / a.G + 1;
+    const bool idle = m_tile * ROWS + 16 * NQ * w >= r.n * a.G;                     // a wavefront without rows only helps with the bytes
+    AttnState<NQ, DT> st;
+    st.clear();
+    v4i kr[NU], vr[NU];
+    int block[NU], key[NU];                            // two units ahead, as above
+    const auto blocks = [&](int unit) {
+#pragma unroll
+      for (int u = 0; u < NU; u++) {
+        key[u] = min(unit * UNIT + u * RPI + tid / PER_ROW, r.kv - 1);
+        block[u] = attn_block(a, table, key[u]);
+      }
+    };
+    const auto load = [&]() {
+#pragma unroll
+      for (int u = 0; u < NU; u++) {
+        kr[u] = *(const v4i *)(attn_row<BYTES>(a, a.k_cache, a.k_block_bytes, block[u], kh, key[u]) + 16 * (tid % PER_ROW));
+        vr[u] = *(const v4i *)(attn_row<BYTES>(a, a.v_cache, a.v_block_bytes, block[u], kh, key[u]) + 16 * (tid % PER_ROW));
+      }
+    };
+    // the registers' bytes into a stage; -> whether a value of an edge unit is no number
+    const auto put = [&](int unit) -> uint32_t {
+      uint8_t *stage = lds + (unit & 1) * STAGE;
+      const bool edge = (unit + 1) * UNIT > clear;
+      uint32_t odd = 0;
+#pragma unroll
+      for (int u = 0; u < NU; u++) {
+        const int row = u * RPI + tid / PER_ROW;
+        const bool there = unit * UNIT + row < r.kv;
+#pragma unroll
+        for (int h = 0; h < (FP8 ? 2 : 1); h++) {
+          const v4i k = FP8 ? __builtin_bit_cast(v4i, attn_widen(kr[u], h)) : kr[u];
+          v4i v = FP8 ? __builtin_bit_cast(v4i, attn_widen(vr[u], h)) : vr[u];
+          if (edge) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const uint32_t bad = no_numbers((uint32_t)v[i]);
+              odd |= there ? bad : 0;
+              v[i] = there ? v[i] & (int)~bad : 0;
+            }
+          }
+          const int col = (FP8 ? 32 : 16) * (tid % PER_ROW) + 16 * h;
+          *(v4i *)(stage + row * LK + col) = k;
+          *(v4i *)(stage + UNIT * LK + row * LV + col) = v;
+        }
+      }
+      return odd;
+    };
+    blocks(c0);
+    load();
+    blocks(min(c0 + 1, c1 - 1));
+    uint32_t odd = put(c0);
+    bool any_odd = __syncthreads_or(odd != 0);
+    for (int c = c0; c < c1; c++) {
+      load();
+      blocks(min(c + 2, c1 - 1));
+      const uint8_t *stage = lds + (c & 1) * STAGE;
+      const bool edge = (c + 1) * UNIT > clear;
+      if (!idle) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          v4f s[2][NQ];
+#pragma unroll
+          for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+            for (int qc = 0; qc < NQ; qc++) s[kt][qc] = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int x = 0; x < D / 32; x++)
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++) {
+              const v8bf k = *(const v8bf *)(stage + (32 * h + 16 * kt + c16) * LK + 64 * x + 16 * g);
+#pragma unroll
+              for (int qc = 0; qc < NQ; qc++) s[kt][qc] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[qc][x], s[kt][qc], 0, 0, 0);
+            }
+          float scl = scale;
+          if (edge) {
+            attn_hide<NQ>(a, r, sight, c * UNIT + 32 * h, scale, s);
+            scl = 1.f;
+          }
+          v8bf p[NQ];
+          st.softmax(s, scl, p);
+          st.template add_values<LV>(stage + UNIT * LK + (32 * h + 4 * g + c16 / 4) * LV + 8 * (c16 % 4), p);
+        }
+        if (edge && any_odd) attn_add_no_numbers<NQ, DT, FP8>(a, r, sight, table, kh, c * UNIT, UNIT, st);
+      }
+      if (c + 1 < c1) odd = put(c + 1);
+      any_odd = __syncthreads_or(odd != 0);
+    }
+#pragma unroll
+    for (int qc = 0; qc < NQ; qc++) {
+      const float l = over_groups(st.l[qc], true);
+#pragma unroll
+      for (int dt = 0; dt < DT; dt++)
+        attn_store<ROWS, D>(a, r, kh, m_tile, 16 * NQ * w + 16 * qc + c16, 16 * dt + 4 * g, whole, part, st.o[dt][qc], st.m[qc], l);
+    }
+  });
+}
+
+// ---- joining ------------------------------------------------------------------------------------------------------------
+// Row blocks of the tile that began in stretch blockIdx.x and went on in later ones: the parts in the stretches' order.  A row is taken by
+// SPLIT groups of D / 4 lanes, each a share of the parts, which meet in LDS.  Rows of no request and of refused ones become 0.
+template <int ROWS, int D, int SPLIT>
+__global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
+  constexpr int lanes = D / 4, per_block = 256 / (lanes * SPLIT);
+  __shared__ v4f sh_o[256];
+  __shared__ float sh_m[256 / lanes], sh_l[256 / lanes];
+  const int tid = threadIdx.x, group = tid / lanes, d = 4 * (tid % lanes), split = group % SPLIT;
+  if (blockIdx.y == 0) {
+    const auto nothing = [&](int t) {
+      for (int i = tid; i < a.Hq * lanes; i += 256) *(v2i *)(a.out + ((size_t)t * a.Hq * lanes + i) * 4) = (v2i){0, 0};
+      if (a.lse)
+        for (int i = tid; i < a.Hq; i += 256) a.lse[(size_t)t * a.Hq + i] = -INFINITY;
+    };
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+      const AttnRequest r = attn_request(a, b);
+      if (r.prefix < 0)
+        for (int j = 0; j < r.n; j++) nothing(r.t0 + j);
+    }
+    for (int t = min(max(a.cu[a.B], 0), a.T) + (int)blockIdx.x; t < a.T; t += gridDim.x) nothing(t);
+  }
+  const int *rec = a.records + 8 * blockIdx.x;
+  const int w1 = rec[0], b = rec[1], kh = rec[2], m_tile = rec[3], side = rec[4], w0 = blockIdx.x;
+  if (w1 <= w0) return;
+  const AttnRequest r = attn_request(a, b);
+  const int in_tile = blockIdx.y * per_block + group / SPLIT, row = m_tile * ROWS + in_tile;
+  if (m_tile * ROWS + (int)blockIdx.y * per_block >= r.n * a.G) return;
+  const auto part = [&](int w) { return (size_t)(2 * w + (w == w0 ? side : 0)) * ROWS + in_tile; };
+  float m = -INFINITY, l = 0.f;
+  v4f o = (v4f){0.f, 0.f, 0.f, 0.f};
+  if (row < r.n * a.G) {
+#pragma unroll 8
+    for (int w = w0 + split; w <= w1; w += SPLIT) {
+      const size_t at = part(w);
+      const float pm = a.part_ml[at * 2], pl = a.part_ml[at * 2 + 1], top = fmaxf(m, pm);
+      const v4f po = *(const v4f *)(a.part_o + at * D + d);
+      const float fo = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top), fp = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(pm - top);
+      m = top;
+      l = l * fo + pl * fp;
+      o = o * fo + po * fp;
+    }
+  }
+  if (SPLIT > 1) {
+    sh_o[tid] = o;
+    if (d == 0) sh_m[group] = m, sh_l[group] = l;
+    __syncthreads();
+    if (split) return;
+    m = sh_m[group];
+#pragma unroll
+    for (int i = 1; i < SPLIT; i++) m = fmaxf(m, sh_m[group + i]);
+    l = 0.f;
+    o = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < SPLIT; i++) {
+      const float f = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(sh_m[group + i] - m);
+      l += sh_l[group + i] * f;
+      o += sh_o[tid + i * lanes] * f;
+    }
+  }
+  attn_store<ROWS, D>(a, r, kh, m_tile, in_tile, d, true, 0, o, m, l);
+}
+
+// ---- which kernel -------------------------------------------------------------------------------------------------------
+// By the rows to a cached key that a request has on average.
+struct AttnPlan {
+  int rows, keys;                      // rows of a tile; whether the wavefronts split the keys
+};
+static AttnPlan attn_plan(int T, int Hq, int Hkv, int B) {
+  const int64_t rows = B > 0 ? ((int64_t)T * (Hq / Hkv) + B - 1) / B : 1;
+  if (rows <= 16) return {16, 1};
+  if (rows <= 32) return {32, 1};
+  if (rows <= 64) return {64, 0};
+  return {128, 0};
+}
+constexpr int kAttnGroups = 512;
 
 }  // namespace moe
 
 extern "C" size_t moe_tree_attention_workspace_bytes(int T, int Hq, int Hkv, int D, int B) {
+  using namespace moe;
   if (T < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || D < 1 || B < 0) return 0;
-  return 256;
+  const size_t rows = attn_plan(T, Hq, Hkv, B).rows, parts = 2 * kAttnGroups;
+  return align_up(parts * rows * D * 4, 256) + align_up(parts * rows * 8, 256) + kAttnGroups * 32;
 }
 
 extern "C" int moe_tree_attention(void *stream, const void *q_bf16, int64_t q_stride, int T, int Hq, int Hkv, int D,
@@ -147,14 +704,39 @@ extern "C" int moe_tree_attention(void *stream, const void *q_bf16, int64_t q_st
   if ((uintptr_t)workspace % 256) return MOE_E_ALIGN;
   if (workspace_bytes < moe_tree_attention_workspace_bytes(T, Hq, Hkv, D, B)) return MOE_E_WORKSPACE;
   const int fp8 = cache_dtype == MOE_DTYPE_FP8, wide = fp8 ? 1 : 2;
-  AttnArgs a{(const uint16_t *)q_bf16, q_stride, T, Hq, Hkv, D, B, n_blocks, __builtin_ctz(page_size), n_blocks ? table_width : 0,
+  const AttnPlan plan = attn_plan(T, Hq, Hkv, B);
+  const size_t parts = 2 * kAttnGroups;
+  AttnArgs a{(const uint16_t *)q_bf16, q_stride, T, Hq, Hkv, Hq / Hkv, B, n_blocks, __builtin_ctz(page_size), n_blocks ? table_width : 0,
              (const uint8_t *)k_cache, (const uint8_t *)v_cache, k_block_stride * wide, v_block_stride * wide, table_stride, block_tables,
-             kv_lens, cu_tokens, masks, scale, k_scale, v_scale, (uint16_t *)out_bf16, lse};
+             kv_lens, cu_tokens, masks, scale, k_scale, v_scale, (uint16_t *)out_bf16, lse, 2, kAttnGroups, (float *)workspace,
+             (float *)((uint8_t *)workspace + align_up(parts * plan.rows * D * 4, 256)),
+             (int32_t *)((uint8_t *)workspace + align_up(parts * plan.rows * D * 4, 256) + align_up(parts * plan.rows * 8, 256))};
   hipStream_t st = (hipStream_t)stream;
-  const unsigned grid = (unsigned)((int64_t)T * Hq);
-  if (D == 64 && fp8) tree_attention_simple_kernel<8, true><<<grid, 256, 0, st>>>(a);
-  else if (D == 64) tree_attention_simple_kernel<8, false><<<grid, 256, 0, st>>>(a);
-  else if (fp8) tree_attention_simple_kernel<16, true><<<grid, 256, 0, st>>>(a);
-  else tree_attention_simple_kernel<16, false><<<grid, 256, 0, st>>>(a);
+  using std::integral_constant;
+  const auto run = [&](auto dim, auto narrow) {
+    constexpr int Dc = decltype(dim)::value;
+    constexpr bool F = decltype(narrow)::value;
+    const auto join = [&](auto rows, auto split) {
+      constexpr int R = decltype(rows)::value, S = decltype(split)::value;
+      attn_join_kernel<R, Dc, S><<<dim3(a.groups, R * Dc * S / 1024), 256, 0, st>>>(a);
+    };
+    if (plan.rows == 16) {
+      attn_keys_kernel<Dc, F, 1><<<a.groups, 256, 0, st>>>(a);
+      join(integral_constant<int, 16>(), integral_constant<int, 8>());
+    } else if (plan.rows == 32) {
+      attn_keys_kernel<Dc, F, 2><<<a.groups, 256, 0, st>>>(a);
+      join(integral_constant<int, 32>(), integral_constant<int, 4>());
+    } else if (plan.rows == 64) {
+      attn_rows_kernel<Dc, F, 1><<<a.groups, 256, 0, st>>>(a);
+      join(integral_constant<int, 64>(), integral_constant<int, 2>());
+    } else {
+      attn_rows_kernel<Dc, F, 2><<<a.groups, 256, 0, st>>>(a);
+      join(integral_constant<int, 128>(), integral_constant<int, 1>());
+    }
+  };
+  if (D == 64 && fp8) run(integral_constant<int, 64>(), integral_constant<bool, true>());
+  else if (D == 64) run(integral_constant<int, 64>(), integral_constant<bool, false>());
+  else if (fp8) run(integral_constant<int, 128>(), integral_constant<bool, true>());
+  else run(integral_constant<int, 128>(), integral_constant<bool, false>());
   return (int)hipGetLastError();
 }
