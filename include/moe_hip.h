@@ -433,10 +433,11 @@ int moe_qk_norm_rope(void *stream, const void *qkv_bf16, int64_t row_stride, int
  * q [T, Hq, D] bf16 (rows q_stride apart), query head h on cache head h / (Hq / Hkv); scores scale * q.k (times k_scale
  * of the head), out [T, Hq, D] bf16 (times v_scale), lse [T, Hq] fp32 or NULL = log of the sum of exponentials.
  * A row that sees no key, of a refused request (kv_lens < n) or of no request: out 0, lse -inf.
- * D 64 or 128; masks cover requests of at most 64 new tokens, without masks there is no limit.
+ * D 64 or 128; masks cover requests of at most 64 new tokens, without masks there is no limit.  Scales are positive.
+ * (T Hq / (16 Hkv) + B) Hkv table_width page_size / 64 below 2^31.
  * workspace: moe_tree_attention_workspace_bytes(...) bytes, 256-byte aligned.
  */
-size_t moe_tree_attention_workspace_bytes(int T, int Hq, int Hkv, int D, int B);
+size_t moe_tree_attention_workspace_bytes(int T, int Hq, int Hkv, int D, int B, int cache_dtype);
 int moe_tree_attention(void *stream, const void *q_bf16, int64_t q_stride, int T, int Hq, int Hkv, int D, const void *k_cache,
                        const void *v_cache, int cache_dtype, int n_blocks, int64_t k_block_stride, int64_t v_block_stride,
                        int page_size, const int32_t *block_tables, int64_t table_stride, int table_width, const int32_t *kv_lens,

@@ -63,7 +63,7 @@ def test_qk_norm_rope_refusals(pkg):
 def test_tree_attention_refusals(pkg):
     names = ["q", "qs", "T", "Hq", "Hkv", "D", "kc", "vc", "ct", "blocks", "ks", "vs", "page", "bt", "bts", "W", "lens", "cu", "B", "masks", "scale",
              "kscale", "vscale", "out", "lse", "ws", "wsb"]
-    ws = lib().moe_tree_attention_workspace_bytes(4, 8, 2, 128, 3)
+    ws = lib().moe_tree_attention_workspace_bytes(4, 8, 2, 128, 3, 1)
     assert ws > 0 and ws % 256 == 0
     good = dict(q=fake, qs=1024, T=4, Hq=8, Hkv=2, D=128, kc=fake, vc=fake, ct=1, blocks=5, ks=16 * 256, vs=16 * 256, page=16, bt=fake, bts=4, W=4,
                 lens=fake, cu=fake, B=3, masks=None, scale=0.1, kscale=None, vscale=None, out=fake, lse=None, ws=fake, wsb=ws)
@@ -81,7 +81,8 @@ def test_tree_attention_refusals(pkg):
     for name in ("q", "kc", "vc", "bt", "lens", "cu", "out", "ws"):
         assert call(**{name: None}) == E_NULL, name
     assert call(T=0, q=None, out=None) == 0
-    assert lib().moe_tree_attention_workspace_bytes(4, 8, 3, 128, 3) == 0
+    assert lib().moe_tree_attention_workspace_bytes(4, 8, 3, 128, 3, 1) == 0
+    assert lib().moe_tree_attention_workspace_bytes(4, 8, 2, 128, 3, 0) == 0
 
 
 def test_token_logprobs_refusals(pkg):

@@ -186,7 +186,7 @@ std::tuple<Tensor, OptTensor> tree_attention(const Tensor &q, const Tensor &k_ca
   OptTensor lse;
   if (return_lse) lse = at::empty({T, Hq}, q.options().dtype(at::kFloat));
   const int t = fits_int(T, "tokens"), h = fits_int(Hq, "heads"), b = fits_int(B, "requests");
-  const size_t need = moe_tree_attention_workspace_bytes(t, h, c.heads, c.dim, b);
+  const size_t need = moe_tree_attention_workspace_bytes(t, h, c.heads, c.dim, b, c.dtype);
   const Tensor ws = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
   check_rc(moe_tree_attention(current_stream(q), q.data_ptr(), T > 1 ? q.stride(0) : Hq * D, t, h, c.heads, c.dim, k_cache.data_ptr(),
                               v_cache.data_ptr(), c.dtype, c.n_blocks, c.k_stride, c.v_stride, c.page, block_tables.data_ptr<int32_t>(),

@@ -22,16 +22,19 @@ struct AttnArgs {
   int64_t q_stride;
   int T, Hq, Hkv, G, B, n_blocks, page_log2, table_width;
   const uint8_t *k_cache, *v_cache;
-  int64_t k_block_bytes, v_block_bytes, table_stride;
+  uint32_t k_block_bytes, v_block_bytes;
+  int64_t table_stride;
   const int32_t *tables, *kv_lens, *cu;
   const int64_t *masks;
   float scale;
   const float *k_scale, *v_scale;
   uint16_t *out;
   float *lse;
-  int min_units, groups;               // least units of a workgroup; workgroups of the main launch
+  int groups;                          // workgroups of the main launch
+  float cut;                           // see attn_walk
   float *part_o, *part_ml;             // [2 groups][rows][D]; [2 groups][rows][2]
-  int32_t *records;                    // [groups][8]: of the tile that begins in a stretch and goes on: last stretch, request, head, tile, part
+  int32_t *records;                    // [groups][8]: of the tile that begins in a stretch and goes on: last stretch, the
+                                       // request's first row and rows, head, tile, part
 };
 
 // ---- who does what ----------------------------------------------------------------------------------------------------
@@ -39,7 +42,7 @@ struct AttnArgs {
 // head of the cache head's group), each UNIT keys that the tile sees.  Every workgroup takes an equal stretch of the line,
 // which may begin and end inside a tile and hold several, so that ragged lengths cost nothing.  A tile that lies in one stretch
 // is finished there; of the others each stretch leaves (max, sum, weighted values), which the second launch joins in
-// order.  The line's length is on the device, so every workgroup adds it up.
+// order.
 struct AttnRequest {
   int t0, n, kv, prefix;
 };
@@ -55,70 +58,108 @@ __device__ __forceinline__ int attn_tile_end(const AttnArgs &a, const AttnReques
   return r.prefix + min(r.n, (min((m + 1) * ROWS, r.n * a.G) - 1) / a.G + 1);
 }
 template <int ROWS, int UNIT>
-__device__ __forceinline__ int64_t attn_head_units(const AttnArgs &a, const AttnRequest &r) {
+__device__ __forceinline__ int attn_head_units(const AttnArgs &a, const AttnRequest &r) {
   if (r.n <= 0 || r.prefix < 0) return 0;
   const int tiles = (r.n * a.G + ROWS - 1) / ROWS;
-  if (a.masks || r.n == 1) return (int64_t)tiles * ((r.kv + UNIT - 1) / UNIT);
-  int64_t sum = 0;
+  if (a.masks || r.n == 1) return tiles * ((r.kv + UNIT - 1) / UNIT);
+  int sum = 0;
   for (int m = 0; m < tiles; m++) sum += (attn_tile_end<ROWS>(a, r, m) + UNIT - 1) / UNIT;
   return sum;
 }
 
-struct AttnLine {
-  int64_t waves[4];
-  int64_t before;
-  int b;
-};
-__device__ __forceinline__ int64_t uniform(int64_t v) {
-  return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)v) | (int64_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32;
-}
-
-// The line's length; sh.b and sh.before: the request that holds place which(total) of it, and the units before that.
-template <int ROWS, int UNIT, typename Which>
-__device__ __forceinline__ int64_t attn_line(const AttnArgs &a, AttnLine &sh, Which which) {
-  const int tid = threadIdx.x, lane = tid & 63, per = (a.B + 255) / 256, b0 = tid * per;
-  int64_t mine = 0;
-  for (int b = b0; b < min(b0 + per, a.B); b++) mine += attn_head_units<ROWS, UNIT>(a, attn_request(a, b)) * a.Hkv;
-  int64_t upto = mine;
+// A workgroup's way along its stretch: calls segment(request, head, tile, units c0 .. c1 of the tile's u, part) for each piece.
+// Every wavefront adds the line up for itself, 64 requests at a time, and finds its first request among them: one trip to
+// memory and no barrier stand in front of the work.  (The host has seen to it that the line's length fits an int.)
+template <int ROWS, int UNIT, typename Segment>
+__device__ __forceinline__ void attn_walk(const AttnArgs &a, Segment segment) {
+  const int lane = threadIdx.x & 63;
+  AttnRequest mine{0, 0, 0, -1};
+  int units = 0, total = 0, longest = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    if (b0 + lane < a.B) mine = attn_request(a, b0 + lane);
+    else mine.n = 0;
+    units = attn_head_units<ROWS, UNIT>(a, mine) * a.Hkv;
+    total += units;
+    if (units > 0) longest = max(longest, (mine.kv + UNIT - 1) / UNIT);
+  }
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const int64_t o = __shfl_up(upto, d, 64);
-    if (lane >= d) upto += o;
+    total += __shfl_xor(total, d, 64);
+    longest = max(longest, __shfl_xor(longest, d, 64));
   }
-  if (lane == 63) sh.waves[tid >> 6] = upto;
-  __syncthreads();
-  int64_t total = 0;
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    if (i < (tid >> 6)) upto += sh.waves[i];
-    total += sh.waves[i];
-  }
-  const int64_t place = which(total);
-  int64_t before = upto - mine;
-  if (place >= before && place < upto) {
-    int b = b0;
-    for (;; b++) {
-      const int64_t units = attn_head_units<ROWS, UNIT>(a, attn_request(a, b)) * a.Hkv;
-      if (place < before + units) break;
-      before += units;
+  total = __builtin_amdgcn_readfirstlane(total);
+  longest = __builtin_amdgcn_readfirstlane(longest);
+  // An equal share for every workgroup, but of one long tile no more than pays: n units cut into stretches of x take x steps of a unit, then
+  // a join of n / x parts, least at x = sqrt(n cut), cut the time of a part over that of a unit.  (One token over 32767 keys: 28, 23.5 and
+  // 26 us with stretches of 2, 4 and 8 units; over 1000 keys 14.8 and 17.8 us with 2 and 4.)
+  const int even = (total + a.groups - 1) / a.groups, least = __builtin_amdgcn_readfirstlane((int)ceilf(sqrtf((float)longest * a.cut)));
+  const int per = max(max(even, least), 1);
+  // Neighbouring stretches, whose tiles have keys in common, on one XCD and so behind one L2: workgroups go to the eight XCDs in turn.
+  const int eighth = ((total + per - 1) / per + 7) / 8, wg = blockIdx.x, place = wg < 8 * eighth ? wg % 8 * eighth + wg / 8 : wg;
+  const int start = (int)min((int64_t)place * per, (int64_t)total), end = min(start + per, total);
+  if (threadIdx.x == 0) a.records[8 * place] = -1;
+  if (start >= end) return;
+  int b = 0, before = 0;
+  AttnRequest r{};
+  for (int b0 = 0;; b0 += 64) {                        // (ends: start < total)
+    if (a.B > 64) {
+      if (b0 + lane < a.B) mine = attn_request(a, b0 + lane);
+      else mine.n = 0;
+      units = attn_head_units<ROWS, UNIT>(a, mine) * a.Hkv;
     }
-    sh.b = b;
-    sh.before = before;
+    int upto = units;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(upto, d, 64);
+      if (lane >= d) upto += o;
+    }
+    const uint64_t past = __ballot(start < before + upto);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      b = b0 + l;
+      before += __builtin_amdgcn_readlane(upto - units, l);
+      r = {__builtin_amdgcn_readlane(mine.t0, l), __builtin_amdgcn_readlane(mine.n, l), __builtin_amdgcn_readlane(mine.kv, l),
+           __builtin_amdgcn_readlane(mine.prefix, l)};
+      break;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
   }
-  __syncthreads();
-  return uniform(total);
-}
-__device__ __forceinline__ int64_t attn_stretch(const AttnArgs &a, int64_t total) {
-  const int64_t even = (total + a.groups - 1) / a.groups;
-  return even > a.min_units ? even : a.min_units;
+  for (int at = start;;) {
+    const int head = attn_head_units<ROWS, UNIT>(a, r);
+    if (at >= before + head * a.Hkv) {
+      before += head * a.Hkv;
+      r = attn_request(a, ++b);
+      continue;
+    }
+    const int kh = (at - before) / head, in_head = at - before - kh * head;
+    int m = 0, u = (r.kv + UNIT - 1) / UNIT, first = 0;
+    if (a.masks || r.n == 1) {
+      m = in_head / u;
+      first = m * u;
+    } else {
+      for (;; m++) {
+        u = (attn_tile_end<ROWS>(a, r, m) + UNIT - 1) / UNIT;
+        if (in_head < first + u) break;
+        first += u;
+      }
+    }
+    const int c0 = in_head - first, c1 = min(u, c0 + (end - at));
+    if (threadIdx.x == 0 && c0 == 0 && c1 < u) {
+      int32_t *rec = a.records + 8 * place;
+      rec[0] = (at + u - 1) / per, rec[1] = r.t0, rec[2] = r.n, rec[3] = kh, rec[4] = m, rec[5] = at > start;
+    }
+    segment(r, b, kh, m, c0, c1, c0 == 0 && c1 == u, 2 * place + (at - c0 > start ? 1 : 0));
+    at += c1 - c0;
+    if (at >= end) break;
+  }
 }
 
 // ---- softmax and products of 32 keys ----------------------------------------------------------------------------------
 // Scores are formed transposed, S^T = K Q^T, so that a lane holds for ONE query (lane % 16) the keys 4 g + i, g = lane / 16, of two
 // tiles of 16.  Those eight are at once the lane's operand of O^T = V^T P^T, if the reduction runs over the keys in that
 // order: no probability changes its lane.  V^T comes from row-major values in LDS by the transposing read.
-// p = 2^(s c - m): m follows the maximum only when that has grown by more than 8, so p stays below 2^8 and the output is
-// seldom rescaled.  p is rounded to bf16 for the product (what the matrix cores take; an error of 2^-9 of each term, as the
+// p = 2^(s c - m): m is the maximum of a tile's first keys and follows it later only where sums exceed 2^60: in between p, the
+// sums and the output merely have another exponent, nothing is lost, and no maximum is formed nor anything rescaled.  p is rounded to bf16 for the product (what the matrix cores take; an error of 2^-9 of each term, as the
 // output's own rounding); its sum is taken before that, in fp32.
 __device__ __forceinline__ float over_groups(float v, bool sum) {
   v2u r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -130,83 +171,142 @@ __device__ __forceinline__ float over_groups(float v, bool sum) {
 template <int NQ, int DT>
 struct AttnState {
   v4f o[DT][NQ];
-  float m[NQ], off[NQ], l[NQ];
+  float m[NQ], l[NQ];
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int qc = 0; qc < NQ; qc++) {
       m[qc] = -INFINITY;
-      off[qc] = l[qc] = 0.f;
+      l[qc] = 0.f;
 #pragma unroll
       for (int dt = 0; dt < DT; dt++) o[dt][qc] = (v4f){0.f, 0.f, 0.f, 0.f};
     }
   }
-  // s -> probabilities, as the second product's operand
-  __device__ __forceinline__ void softmax(const v4f (&s)[2][NQ], float c, v8bf (&p)[NQ]) {
+  // lets m follow the largest of KT tiles' scores
+  template <int KT>
+  __device__ __forceinline__ void raise(const v4f (&s)[KT][NQ], float c) {
     float top[NQ];
     bool grown = false;
 #pragma unroll
     for (int qc = 0; qc < NQ; qc++) {
-      float t = fmaxf(fmaxf(s[0][qc][0], s[0][qc][1]), s[0][qc][2]);
-      t = fmaxf(fmaxf(t, s[0][qc][3]), s[1][qc][0]);
-      t = fmaxf(fmaxf(t, s[1][qc][1]), s[1][qc][2]);
-      top[qc] = fmaxf(t, s[1][qc][3]) * c;
+      float t = s[0][qc][0];
+#pragma unroll
+      for (int x = 1; x + 1 < 4 * KT; x += 2) t = fmaxf(fmaxf(t, s[x / 4][qc][x % 4]), s[(x + 1) / 4][qc][(x + 1) % 4]);
+      top[qc] = fmaxf(t, s[KT - 1][qc][3]) * c;
       grown |= top[qc] > m[qc] + 8.f;
     }
-    if (__any(grown)) {
+    if (__builtin_expect(__any(grown), 0)) {
 #pragma unroll
       for (int qc = 0; qc < NQ; qc++) {
         const float t = over_groups(top[qc], false), now = t > m[qc] + 8.f ? t : m[qc];
         const float f = now == m[qc] ? 1.f : __builtin_amdgcn_exp2f(m[qc] - now);
         m[qc] = now;
-        off[qc] = now == -INFINITY ? 0.f : now;
         l[qc] *= f;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) o[dt][qc] *= f;
       }
     }
+  }
+  // KT tiles' scores -> probabilities, as the second product's operands.  sure: m follows the maximum first (a tile's first
+  // keys, and keys that some rows do not see); else m is left alone unless the sums show that it is far too low.
+  template <int KT>
+  __device__ __forceinline__ void softmax(const v4f (&s)[KT][NQ], float c, bool sure, v8bf (&p)[KT / 2][NQ]) {
+    float sum[NQ];
+    for (bool rise = sure;;) {
+      if (__builtin_expect(rise, 0)) raise<KT>(s, c);
+      weigh<KT>(s, c, p, sum);
+      bool far = false;
+#pragma unroll
+      for (int qc = 0; qc < NQ; qc++) far |= sum[qc] > 0x1p60f;
+      if (__builtin_expect(rise || !__any(far), 1)) break;
+      rise = true;
+    }
+#pragma unroll
+    for (int qc = 0; qc < NQ; qc++) l[qc] += sum[qc];
+  }
+  template <int KT>
+  __device__ __forceinline__ void weigh(const v4f (&s)[KT][NQ], float c, v8bf (&p)[KT / 2][NQ], float (&sum)[NQ]) const {
 #pragma unroll
     for (int qc = 0; qc < NQ; qc++) {
-      float e[8];
+      sum[qc] = 0.f;
+      const float off = m[qc] == -INFINITY ? 0.f : m[qc];
 #pragma unroll
-      for (int i = 0; i < 8; i++) e[i] = __builtin_amdgcn_exp2f(fmaf(s[i / 4][qc][i % 4], c, -off[qc]));
-      l[qc] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-      const v4i w = {(int)pack2_bf16(e[0], e[1]), (int)pack2_bf16(e[2], e[3]), (int)pack2_bf16(e[4], e[5]), (int)pack2_bf16(e[6], e[7])};
-      p[qc] = __builtin_bit_cast(v8bf, w);
-    }
-  }
-  // o += V^T p; `at`: this lane's address in the first 16 rows of the values
-  template <int LD>
-  __device__ __forceinline__ void add_values(const uint8_t *at, const v8bf (&p)[NQ]) {
+      for (int h = 0; h < KT / 2; h++) {
+        float e[8];
 #pragma unroll
-    for (int dt = 0; dt < DT; dt++) {
-      typedef __attribute__((address_space(3))) v4s lds_v4s;
-      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(at + 32 * dt));
-      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(at + 16 * LD + 32 * dt));
-      const v8bf v = __builtin_bit_cast(v8bf, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-      for (int qc = 0; qc < NQ; qc++) o[dt][qc] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[qc], o[dt][qc], 0, 0, 0);
+        for (int i = 0; i < 8; i++) e[i] = __builtin_amdgcn_exp2f(fmaf(s[2 * h + i / 4][qc][i % 4], c, -off));
+        sum[qc] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+        const v4i w = {(int)pack2_bf16(e[0], e[1]), (int)pack2_bf16(e[2], e[3]), (int)pack2_bf16(e[4], e[5]), (int)pack2_bf16(e[6], e[7])};
+        p[h][qc] = __builtin_bit_cast(v8bf, w);
+      }
     }
   }
 };
+
+// The products' operands come from LDS some hundred cycles after they are asked for, a group of matrix instructions takes 32 to 64: operands
+// are asked for AHEAD groups before their use, and the order written here is kept (left to itself the compiler asks
+// and waits in turn; 64 keys of 32 rows then took 2.3 us, half of it such waits).
+__device__ __forceinline__ void in_this_order() { __builtin_amdgcn_sched_barrier(0); }
+__device__ __forceinline__ void made_here(v4f &x) { asm volatile("" : "+v"(x)); }      // (products are moved freely otherwise)
+
+// 16 columns of the values of 32 keys as the product's first operand; `at`: this lane's address in the first 16 rows
+template <int LD>
+__device__ __forceinline__ v8bf attn_values(const uint8_t *at, int dt) {
+  typedef __attribute__((address_space(3))) v4s lds_v4s;
+  const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(at + 32 * dt));
+  const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(at + 16 * LD + 32 * dt));
+  return __builtin_bit_cast(v8bf, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+// o += V^T p over H times 32 keys; v: the first AHEAD operands, asked for already
+template <int AHEAD, int H, int LD, int NQ, int DT>
+__device__ __forceinline__ void attn_add_values(AttnState<NQ, DT> &st, const uint8_t *at, const v8bf (&p)[H][NQ], v8bf (&v)[H * DT]) {
+#pragma unroll
+  for (int i = 0; i < H * DT; i++) {
+    if (i + AHEAD < H * DT) v[i + AHEAD] = attn_values<LD>(at + 32 * ((i + AHEAD) / DT) * LD, (i + AHEAD) % DT);
+    in_this_order();
+#pragma unroll
+    for (int qc = 0; qc < NQ; qc++) {
+      st.o[i % DT][qc] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[i], p[i / DT][qc], st.o[i % DT][qc], 0, 0, 0);
+      made_here(st.o[i % DT][qc]);
+    }
+    in_this_order();
+  }
+}
+// scores of KT tiles of 16 keys, rows LK apart in LDS from `at` (this lane's row of the first tile and its 16 bytes) on
+template <int AHEAD, int KT, int LK, int NQ, int X>
+__device__ __forceinline__ void attn_scores(const uint8_t *at, const v8bf (&q)[NQ][X], v4f (&s)[KT][NQ]) {
+  v8bf k[KT * X];
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++) k[i] = *(const v8bf *)(at + (i / X) * 16 * LK + 64 * (i % X));
+#pragma unroll
+  for (int i = 0; i < KT * X; i++) {
+    if (i + AHEAD < KT * X) k[i + AHEAD] = *(const v8bf *)(at + ((i + AHEAD) / X) * 16 * LK + 64 * ((i + AHEAD) % X));
+    in_this_order();
+#pragma unroll
+    for (int qc = 0; qc < NQ; qc++) {
+      s[i / X][qc] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[i], q[qc][i % X], i % X ? s[i / X][qc] : (v4f){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+      made_here(s[i / X][qc]);
+    }
+    in_this_order();
+  }
+}
 
 // what a lane's queries see of the new tokens
 template <int NQ>
 struct AttnSight {
-  uint64_t mask[NQ];
-  int last[NQ];                        // without masks: the last key seen
+  uint64_t mask[NQ];                   // without masks: the last key seen
   __device__ __forceinline__ bool sees(const AttnArgs &a, const AttnRequest &r, int qc, int key) const {
     const int i = key - r.prefix;
-    return a.masks ? i < 0 || (key < r.kv && i < 64 && (mask[qc] >> (i & 63) & 1)) : key <= last[qc];
+    return a.masks ? i < 0 || (key < r.kv && i < 64 && (mask[qc] >> (i & 63) & 1)) : key <= (int)mask[qc];
   }
 };
 
 // Hides what a lane's queries do not see; the scores left are scaled already.
-template <int NQ>
+template <int NQ, int KT>
 __device__ __forceinline__ void attn_hide(const AttnArgs &a, const AttnRequest &r, const AttnSight<NQ> &sight, int first_key, float c,
-                                          v4f (&s)[2][NQ]) {
+                                          v4f (&s)[KT][NQ]) {
   const int g4 = 4 * ((threadIdx.x & 63) >> 4);
 #pragma unroll
-  for (int kt = 0; kt < 2; kt++)
+  for (int kt = 0; kt < KT; kt++)
 #pragma unroll
     for (int qc = 0; qc < NQ; qc++)
 #pragma unroll
@@ -230,10 +330,11 @@ __device__ __forceinline__ uint32_t no_numbers(uint32_t w) {
 __device__ __forceinline__ int attn_block(const AttnArgs &a, const int32_t *table, int key) {
   return min(max(table[key >> a.page_log2], 0), a.n_blocks - 1);
 }
-// where a head's key or value of a block lies
+// where a head's key or value of a block lies (one 32 x 32 -> 64 bit multiplication and one of 24 bits)
 template <int BYTES>
-__device__ __forceinline__ const uint8_t *attn_row(const AttnArgs &a, const uint8_t *cache, int64_t block_bytes, int block, int kh, int key) {
-  return cache + block * block_bytes + (uint32_t)(((key & ((1 << a.page_log2) - 1)) * a.Hkv + kh) * BYTES);
+__device__ __forceinline__ const uint8_t *attn_row(const AttnArgs &a, const uint8_t *cache, uint32_t block_bytes, int block, int kh, int key) {
+  return cache + (uint64_t)(uint32_t)block * block_bytes +
+         (__umul24((uint32_t)key & ((1u << a.page_log2) - 1), (uint32_t)a.Hkv * BYTES) + (uint32_t)kh * BYTES);
 }
 
 // A value that is NaN or infinite would, times a probability of 0, reach rows that do not see its key.  Where new tokens are among
@@ -242,18 +343,21 @@ template <int NQ, int DT, bool FP8>
 __device__ __forceinline__ void attn_add_no_numbers(const AttnArgs &a, const AttnRequest &r, const AttnSight<NQ> &sight, const int32_t *table,
                                                  int kh, int first_key, int keys, AttnState<NQ, DT> &st) {
   const int g4 = 4 * ((threadIdx.x & 63) >> 4);
+#pragma unroll 1
   for (int key = first_key; key < min(first_key + keys, r.kv); key++) {
     const uint8_t *row = attn_row<DT * (FP8 ? 16 : 32)>(a, a.v_cache, a.v_block_bytes, attn_block(a, table, key), kh, key);
+    bool sees[NQ];
+#pragma unroll
+    for (int qc = 0; qc < NQ; qc++) sees[qc] = sight.sees(a, r, qc, key);
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const int d = 16 * dt + g4 + i;
-        const float v = FP8 ? __builtin_amdgcn_cvt_f32_fp8((uint32_t)row[d], 0) : bf16_to_f32(((const uint16_t *)row)[d]);
-        if (__builtin_isfinite(v)) continue;
+        float v = FP8 ? __builtin_amdgcn_cvt_f32_fp8((uint32_t)row[d], 0) : bf16_to_f32(((const uint16_t *)row)[d]);
+        v = __builtin_isfinite(v) ? 0.f : v;
 #pragma unroll
-        for (int qc = 0; qc < NQ; qc++)
-          if (sight.sees(a, r, qc, key)) st.o[dt][qc][i] += v;
+        for (int qc = 0; qc < NQ; qc++) st.o[dt][qc][i] += sees[qc] ? v : 0.f;
       }
   }
 }
@@ -270,15 +374,14 @@ __device__ __forceinline__ void attn_queries(const AttnArgs &a, const AttnReques
     const uint16_t *src = a.q + (size_t)(r.t0 + j) * a.q_stride + (size_t)h * D;
 #pragma unroll
     for (int s = 0; s < D / 32; s++) q[qc][s] = *(const v8bf *)(src + (FP8 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g));
-    sight.mask[qc] = a.masks ? (uint64_t)a.masks[r.t0 + j] : 0;
-    sight.last[qc] = r.prefix + j;
+    sight.mask[qc] = a.masks ? (uint64_t)a.masks[r.t0 + j] : (uint64_t)(r.prefix + j);
   }
 }
 
 // Four neighbouring outputs of a row: finished, or as a stretch's part of it.
 template <int ROWS, int D>
 __device__ __forceinline__ void attn_store(const AttnArgs &a, const AttnRequest &r, int kh, int m_tile, int row_in_tile, int d, bool whole,
-                                           int64_t part, const v4f o, float m, float l) {
+                                           int part, const v4f o, float m, float l) {
   const int row = m_tile * ROWS + row_in_tile;
   if (row >= r.n * a.G) return;
   if (!whole) {
@@ -297,54 +400,6 @@ __device__ __forceinline__ void attn_store(const AttnArgs &a, const AttnRequest 
   if (a.lse && d == 0) a.lse[at] = none ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
-// A workgroup's way along its stretch: calls segment(request, head, tile, units c0 .. c1 of the tile's u, part) for each piece.
-template <int ROWS, int UNIT, typename Segment>
-__device__ __forceinline__ void attn_walk(const AttnArgs &a, AttnLine &line, Segment segment) {
-  int64_t start = 0, per = 1;
-  const int64_t total = attn_line<ROWS, UNIT>(a, line, [&](int64_t t) {
-    per = attn_stretch(a, t);
-    start = (int64_t)blockIdx.x * per;
-    return start;
-  });
-  per = uniform(per);
-  start = uniform(start);
-  int64_t at = start, end = start + per < total ? start + per : total;
-  if (threadIdx.x == 0) a.records[8 * blockIdx.x] = -1;
-  if (at >= end) return;
-  int b = __builtin_amdgcn_readfirstlane(line.b);
-  int64_t before = uniform(line.before);
-  while (at < end) {
-    const AttnRequest r = attn_request(a, b);
-    const int64_t head = attn_head_units<ROWS, UNIT>(a, r);
-    if (at >= before + head * a.Hkv) {
-      before += head * a.Hkv;
-      b++;
-      continue;
-    }
-    const int kh = (int)((at - before) / head);
-    const int64_t in_head = at - before - kh * head;
-    int m = 0, u = (r.kv + UNIT - 1) / UNIT;
-    int64_t first = 0;
-    if (a.masks || r.n == 1) {
-      m = (int)(in_head / u);
-      first = (int64_t)m * u;
-    } else {
-      for (;; m++) {
-        u = (attn_tile_end<ROWS>(a, r, m) + UNIT - 1) / UNIT;
-        if (in_head < first + u) break;
-        first += u;
-      }
-    }
-    const int c0 = (int)(in_head - first), c1 = (int)(u < c0 + (end - at) ? u : c0 + (end - at));
-    if (threadIdx.x == 0 && c0 == 0 && c1 < u) {
-      int32_t *rec = a.records + 8 * blockIdx.x;
-      rec[0] = (int32_t)((at + u - 1) / per), rec[1] = b, rec[2] = kh, rec[3] = m, rec[4] = at > start;
-    }
-    segment(r, b, kh, m, c0, c1, c0 == 0 && c1 == u, 2 * (int64_t)blockIdx.x + (at - c0 > start ? 1 : 0));
-    at += c1 - c0;
-  }
-}
-
 // ---- few rows: the four wavefronts take the keys in turn --------------------------------------------------------------
 // Up to 64 rows to a cached key the cache's bytes bound it.  A wavefront takes 32 keys of a unit of 128 by itself: keys go
 // from memory straight into operand registers, values through LDS that no other wavefront touches, so nothing waits at a
@@ -356,11 +411,10 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(const AttnArgs a) {
   constexpr int kValues = 4 * 32 * LD, kMerge = 4 * DT * NQ * 64 * 16;
   __shared__ __attribute__((aligned(16))) uint8_t lds[kValues > kMerge ? kValues : kMerge];
   __shared__ float sh_m[4][ROWS], sh_l[4][ROWS];
-  __shared__ AttnLine line;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c16 = lane & 15;
   uint8_t *values = lds + w * 32 * LD;
   const uint8_t *read_at = values + (4 * g + c16 / 4) * LD + 8 * (c16 % 4);
-  attn_walk<ROWS, UNIT>(a, line, [&](const AttnRequest r, int b, int kh, int m_tile, int c0, int c1, bool whole, int64_t part) {
+  attn_walk<ROWS, UNIT>(a, [&](const AttnRequest r, int b, int kh, int m_tile, int c0, int c1, bool whole, int part) {
     const int32_t *table = a.tables + (size_t)b * a.table_stride;
     const float scale = a.scale * (a.k_scale ? a.k_scale[kh] : 1.f) * 1.4426950408889634f;
     v8bf q[NQ][D / 32];
@@ -377,7 +431,7 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(const AttnArgs a) {
 #pragma unroll
       for (int kt = 0; kt < 2; kt++) block[kt] = attn_block(a, table, key_of(unit, kt));
     };
-    const auto load = [&](const uint8_t *cache, int64_t block_bytes, int unit, v4i (&to)[2][P]) {
+    const auto load = [&](const uint8_t *cache, uint32_t block_bytes, int unit, v4i (&to)[2][P]) {
 #pragma unroll
       for (int kt = 0; kt < 2; kt++) {
         const uint8_t *row = attn_row<FP8 ? D : 2 * D>(a, cache, block_bytes, block[kt], kh, key_of(unit, kt)) + 16 * g;
@@ -431,16 +485,18 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(const AttnArgs a) {
       load(a.v_cache, a.v_block_bytes, min(c + 1, c1 - 1), vr);
       blocks(min(c + 2, c1 - 1));
       float scl = scale;
-      if (edge) {
-        attn_hide<NQ>(a, r, sight, key0, scale, s);
+      if (__builtin_expect(edge, 0)) {
+        attn_hide(a, r, sight, key0, scale, s);
         scl = 1.f;
       }
-      v8bf p[NQ];
-      st.softmax(s, scl, p);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
-      st.template add_values<LD>(read_at, p);
-      if (edge && __any(odd != 0)) attn_add_no_numbers<NQ, DT, FP8>(a, r, sight, table, kh, key0, 32, st);
+      v8bf p[1][NQ], v[DT];
+#pragma unroll
+      for (int i = 0; i < 3; i++) v[i] = attn_values<LD>(read_at, i);
+      st.template softmax<2>(s, scl, edge || c == c0, p);
+      attn_add_values<3, 1, LD>(st, read_at, p, v);
+      if (__builtin_expect(edge && __any(odd != 0), 0)) attn_add_no_numbers<NQ, DT, FP8>(a, r, sight, table, kh, key0, 32, st);
       __builtin_amdgcn_wave_barrier();
     }
     // the wavefronts' results, each scaled to the common maximum, a quarter of the columns to each wavefront
@@ -480,118 +536,260 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(const AttnArgs a) {
   });
 }
 
-// ---- many rows: the four wavefronts take the rows, and share the keys ----------------------------------------------------
-// From about 100 rows to a cached key on the products bound it.  A workgroup stages 64 keys and values at a time in LDS, two
-// stages of them, and every wavefront takes its rows past all of them: one barrier a stage, the next stage's bytes in
-// registers meanwhile.
+// ---- staging in LDS (the two kernels below) ---------------------------------------------------------------------------
+// Rows of a stage are 32 bytes longer than their values: operands are read without bank conflicts then (counted: none).  TPR
+// threads write a row, 16 bytes of it at a time; which row thread group i takes is chosen so that the rows of one write fall into different
+// banks as well: four rows 4 apart, or of bytes widened to 32 apart 0, 1, 8 and 9.
+template <bool FP8, int TPR>
+__device__ __forceinline__ int attn_stage_row(int i) {
+  if (FP8) return TPR == 4 ? (i & ~15) | (i & 1) | (i & 2) << 2 | (i >> 1 & 6) : i;
+  return TPR == 4 ? (i & ~15) | (i & 3) << 2 | (i >> 2 & 3) : (i & ~15) | (i & 1) << 3 | (i >> 1 & 7);
+}
+template <bool FP8, int TPR, int NU>
+__device__ __forceinline__ void attn_put(uint8_t *at, const v4i (&raw)[NU]) {
+#pragma unroll
+  for (int u = 0; u < NU; u++)
+#pragma unroll
+    for (int h = 0; h < (FP8 ? 2 : 1); h++)
+      *(v4i *)(at + (FP8 ? 32 : 16) * TPR * u + 16 * h) = FP8 ? __builtin_bit_cast(v4i, attn_widen(raw[u], h)) : raw[u];
+}
+// The same for values.  edge: the unit holds new tokens' values or ends the request: what is no number becomes 0 and is told, what
+// is beyond the end (there: this row is not) becomes 0.
+template <bool FP8, int TPR, int NU>
+__device__ __forceinline__ void attn_put_values(uint8_t *at, const v4i (&raw)[NU], bool edge, bool there, int *any_odd) {
+#pragma unroll
+  for (int u = 0; u < NU; u++)
+#pragma unroll
+    for (int h = 0; h < (FP8 ? 2 : 1); h++) {
+      v4i v = FP8 ? __builtin_bit_cast(v4i, attn_widen(raw[u], h)) : raw[u];
+      if (__builtin_expect(edge, 0)) {
+        uint32_t odd = 0;
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+          const uint32_t bad = no_numbers((uint32_t)v[x]);
+          odd |= there ? bad : 0;
+          v[x] = there ? v[x] & (int)~bad : 0;
+        }
+        if (odd) *any_odd = 1;
+      }
+      *(v4i *)(at + (FP8 ? 32 : 16) * TPR * u + 16 * h) = v;
+    }
+}
+
+// ---- more rows: the wavefronts take the rows, and share the keys ---------------------------------------------------------
+// Up to about 128 rows to a cached key both the bytes and the products count.  A workgroup stages 64 keys and values at a time in
+// LDS, two stages of them, and every wavefront takes its rows past all of them, one barrier a stage.  The bytes of the stages after
+// that wait in registers, of two stages where there are enough (a stage takes less time than the way to memory).
 template <int D, bool FP8, int NQ>
 __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const AttnArgs a) {
-  constexpr int ROWS = 64 * NQ, UNIT = 64, DT = D / 16, LK = 2 * D + 16, LV = 2 * D + 32, STAGE = UNIT * (LK + LV);
-  constexpr int BYTES = FP8 ? D : 2 * D, PER_ROW = BYTES / 16, RPI = 256 / PER_ROW, NU = UNIT / RPI;   // 16-byte pieces of a row; rows at a time
+  constexpr int ROWS = 64 * NQ, UNIT = 64, DT = D / 16, LD = 2 * D + 32, STAGE = 2 * UNIT * LD;
+  constexpr int BYTES = FP8 ? D : 2 * D, TPR = 4, NU = BYTES / (16 * TPR);           // a row's threads; a thread's 16-byte pieces of its row
+  constexpr int SETS = NQ == 1 ? 2 : 1;
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
-  __shared__ AttnLine line;
+  __shared__ int any_odd;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c16 = lane & 15;
-  attn_walk<ROWS, UNIT>(a, line, [&](const AttnRequest r, int b, int kh, int m_tile, int c0, int c1, bool whole, int64_t part) {
+  attn_walk<ROWS, UNIT>(a, [&](const AttnRequest r, int b, int kh, int m_tile, int c0, int c1, bool whole, int part) {
     const int32_t *table = a.tables + (size_t)b * a.table_stride;
     const float scale = a.scale * (a.k_scale ? a.k_scale[kh] : 1.f) * 1.4426950408889634f;
-    v8bf q[NQ][D / 32];
-    AttnSight<NQ> sight;
-    attn_queries<NQ, D, false>(a, r, kh, m_tile * ROWS + 16 * NQ * w, q, sight);
-    const int clear = a.masks ? r.prefix : r.prefix + m_tile * ROWS / a.G + 1;
-    const bool idle = m_tile * ROWS + 16 * NQ * w >= r.n * a.G;                     // a wavefront without rows only helps with the bytes
-    AttnState<NQ, DT> st;
-    st.clear();
+    const int clear = a.masks ? r.prefix : r.prefix + m_tile * ROWS / a.G + 1;      // keys below it are seen by every row
+    const int last = c1 - 1;
+    const int stage_row = attn_stage_row<FP8, TPR>(tid / TPR), piece = tid % TPR;
+    uint8_t *const stage_at = lds + stage_row * LD + (FP8 ? 32 : 16) * piece;
+    v4i kr[SETS][NU], vr[SETS][NU];
+    int block;                                         // of the unit that is asked for next
+    const auto key_of = [&](int unit) { return min(min(unit, last) * UNIT + stage_row, r.kv - 1); };
+    const auto ask = [&](int unit, v4i (&k)[NU], v4i (&v)[NU]) {
+      const uint8_t *ka = attn_row<BYTES>(a, a.k_cache, a.k_block_bytes, block, kh, key_of(unit)) + 16 * piece;
+      const uint8_t *va = attn_row<BYTES>(a, a.v_cache, a.v_block_bytes, block, kh, key_of(unit)) + 16 * piece;
+#pragma unroll
+      for (int u = 0; u < NU; u++) {
+        k[u] = *(const v4i *)(ka + 16 * TPR * u);
+        v[u] = *(const v4i *)(va + 16 * TPR * u);
+      }
+      block = attn_block(a, table, key_of(unit + 1));
+    };
+    const auto put = [&](int unit, const v4i (&k)[NU], const v4i (&v)[NU]) {
+      attn_put<FP8, TPR, NU>(stage_at + (unit & 1) * STAGE, k);
+      attn_put_values<FP8, TPR, NU>(stage_at + (unit & 1) * STAGE + UNIT * LD, v, (unit + 1) * UNIT > clear,
+                                    unit * UNIT + stage_row < r.kv, &any_odd);
+    };
+    if (tid == 0) any_odd = 0;
+    block = attn_block(a, table, key_of(c0));
+    ask(c0, kr[0], vr[0]);
+    if (SETS == 2) ask(c0 + 1, kr[SETS - 1], vr[SETS - 1]);
+    __syncthreads();
+    put(c0, kr[0], vr[0]);
+    ask(c0 + SETS, kr[0], vr[0]);
+    __syncthreads();
+    // a stage: `work` on it, the next one's bytes from registers to LDS, the one's after those asked for
+    const auto stages = [&](auto work) {
+      const auto step = [&](int c, v4i (&k)[NU], v4i (&v)[NU]) {
+        work(c, lds + (c & 1) * STAGE);
+        put(c + 1, k, v);
+        ask(c + 1 + SETS, k, v);
+        __syncthreads();
+      };
+      if (SETS == 1) {
+        for (int c = c0; c < c1; c++) step(c, kr[0], vr[0]);
+      } else {
+        for (int c = c0; c < c1; c += 2) {
+          step(c, kr[SETS - 1], vr[SETS - 1]);
+          if (c + 1 < c1) step(c + 1, kr[0], vr[0]);
+        }
+      }
+    };
+    if (m_tile * ROWS + 16 * NQ * w < r.n * a.G) {
+      v8bf q[NQ][D / 32];
+      AttnSight<NQ> sight;
+      attn_queries<NQ, D, false>(a, r, kh, m_tile * ROWS + 16 * NQ * w, q, sight);
+      AttnState<NQ, DT> st;
+      st.clear();
+      stages([&](int c, const uint8_t *stage) {
+        const bool edge = (c + 1) * UNIT > clear;
+        v4f s[4][NQ];
+        attn_scores<3, 4, LD>(stage + c16 * LD + 16 * g, q, s);
+        const uint8_t *read_at = stage + UNIT * LD + (4 * g + c16 / 4) * LD + 8 * (c16 % 4);
+        v8bf p[2][NQ], va[2 * DT];
+#pragma unroll
+        for (int i = 0; i < 3; i++) va[i] = attn_values<LD>(read_at, i);
+        float scl = scale;
+        if (__builtin_expect(edge, 0)) {
+          attn_hide(a, r, sight, c * UNIT, scale, s);
+          scl = 1.f;
+        }
+        st.template softmax<4>(s, scl, edge || c == c0, p);
+        attn_add_values<3, 2, LD>(st, read_at, p, va);
+      });
+      if (__builtin_expect(any_odd, 0)) {
+        const int from = max(c0, clear / UNIT) * UNIT;          // the first unit whose values were looked at
+        attn_add_no_numbers<NQ, DT, FP8>(a, r, sight, table, kh, from, c1 * UNIT - from, st);
+      }
+#pragma unroll
+      for (int qc = 0; qc < NQ; qc++) {
+        const float l = over_groups(st.l[qc], true);
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+          attn_store<ROWS, D>(a, r, kh, m_tile, 16 * NQ * w + 16 * qc + c16, 16 * dt + 4 * g, whole, part, st.o[dt][qc], st.m[qc], l);
+      }
+    } else {                                           // a wavefront without rows only helps with the bytes
+      stages([](int, const uint8_t *) {});
+    }
+    __syncthreads();
+  });
+}
+
+// ---- many rows: two groups of wavefronts, one at the products while the other is at the exponentials ---------------------
+// The matrix cores and the vector unit of a SIMD work at the same time only for different wavefronts, and two that share every barrier
+// would always want the same one.  So wavefronts 4 to 7, one on each SIMD beside one of 0 to 3, run the same steps a slot later:
+//   slot      0          1          2                     3
+//   first     scores 0   weigh 0    scores 1, values 0    weigh 1 ...
+//   second    -          scores 0   weigh 0               scores 1, values 0 ...
+// A barrier ends a slot.  While it weighs unit c a wavefront also stages its share of the keys of c + 1 and the values of c, the
+// second group's a unit further on, so that each stage is whole a slot before the first group needs it and is written when the second
+// group has left it (two stages of each).
+template <int D, bool FP8, int NQ>
+__global__ __launch_bounds__(512, 2) void attn_pairs_kernel(const AttnArgs a) {
+  constexpr int ROWS = 128 * NQ, UNIT = 64, DT = D / 16, X = D / 32, LD = 2 * D + 32, HALF = UNIT * LD;
+  constexpr int BYTES = FP8 ? D : 2 * D, TPR = BYTES / 16 < 8 ? BYTES / 16 : 8, NU = BYTES / (16 * TPR);
+  __shared__ __attribute__((aligned(16))) uint8_t lds[4 * HALF];
+  __shared__ int any_odd;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c16 = lane & 15;
+  const int late = __builtin_amdgcn_readfirstlane(w) >> 2;
+  attn_walk<ROWS, UNIT>(a, [&](const AttnRequest r, int b, int kh, int m_tile, int c0, int c1, bool whole, int part) {
+    const int32_t *table = a.tables + (size_t)b * a.table_stride;
+    const float scale = a.scale * (a.k_scale ? a.k_scale[kh] : 1.f) * 1.4426950408889634f;
+    const int clear = a.masks ? r.prefix : r.prefix + m_tile * ROWS / a.G + 1;      // keys below it are seen by every row
+    const int last = c1 - 1;
+    const int i = tid / TPR, piece = tid % TPR, stage_row = attn_stage_row<FP8, TPR>(i);
+    const bool stages = i < UNIT;                      // (narrow rows take fewer threads)
+    uint8_t *const stage_at = lds + stage_row * LD + (FP8 ? 32 : 16) * piece;
     v4i kr[NU], vr[NU];
-    int block[NU], key[NU];                            // two units ahead, as above
-    const auto blocks = [&](int unit) {
+    int block, block_v;                                // of the key, of the value that is asked for next
+    const auto key_of = [&](int unit) { return min(min(unit, last) * UNIT + stage_row, r.kv - 1); };
+    const auto ask = [&](const uint8_t *cache, uint32_t block_bytes, int blk, int unit, v4i (&to)[NU]) {
+      const uint8_t *at = attn_row<BYTES>(a, cache, block_bytes, blk, kh, key_of(unit)) + 16 * piece;
 #pragma unroll
-      for (int u = 0; u < NU; u++) {
-        key[u] = min(unit * UNIT + u * RPI + tid / PER_ROW, r.kv - 1);
-        block[u] = attn_block(a, table, key[u]);
-      }
+      for (int u = 0; u < NU; u++) to[u] = *(const v4i *)(at + 16 * TPR * u);
     };
-    const auto load = [&]() {
-#pragma unroll
-      for (int u = 0; u < NU; u++) {
-        kr[u] = *(const v4i *)(attn_row<BYTES>(a, a.k_cache, a.k_block_bytes, block[u], kh, key[u]) + 16 * (tid % PER_ROW));
-        vr[u] = *(const v4i *)(attn_row<BYTES>(a, a.v_cache, a.v_block_bytes, block[u], kh, key[u]) + 16 * (tid % PER_ROW));
-      }
+    const auto put_keys = [&](int unit) {
+      if (stages) attn_put<FP8, TPR, NU>(stage_at + (unit & 1) * HALF, kr);
     };
-    // the registers' bytes into a stage; -> whether a value of an edge unit is no number
-    const auto put = [&](int unit) -> uint32_t {
-      uint8_t *stage = lds + (unit & 1) * STAGE;
-      const bool edge = (unit + 1) * UNIT > clear;
-      uint32_t odd = 0;
-#pragma unroll
-      for (int u = 0; u < NU; u++) {
-        const int row = u * RPI + tid / PER_ROW;
-        const bool there = unit * UNIT + row < r.kv;
-#pragma unroll
-        for (int h = 0; h < (FP8 ? 2 : 1); h++) {
-          const v4i k = FP8 ? __builtin_bit_cast(v4i, attn_widen(kr[u], h)) : kr[u];
-          v4i v = FP8 ? __builtin_bit_cast(v4i, attn_widen(vr[u], h)) : vr[u];
-          if (edge) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-              const uint32_t bad = no_numbers((uint32_t)v[i]);
-              odd |= there ? bad : 0;
-              v[i] = there ? v[i] & (int)~bad : 0;
-            }
-          }
-          const int col = (FP8 ? 32 : 16) * (tid % PER_ROW) + 16 * h;
-          *(v4i *)(stage + row * LK + col) = k;
-          *(v4i *)(stage + UNIT * LK + row * LV + col) = v;
-        }
-      }
-      return odd;
+    const auto put_values = [&](int unit) {
+      if (stages)
+        attn_put_values<FP8, TPR, NU>(stage_at + (2 + (unit & 1)) * HALF, vr, (unit + 1) * UNIT > clear, unit * UNIT + stage_row < r.kv, &any_odd);
     };
-    blocks(c0);
-    load();
-    blocks(min(c0 + 1, c1 - 1));
-    uint32_t odd = put(c0);
-    bool any_odd = __syncthreads_or(odd != 0);
-    for (int c = c0; c < c1; c++) {
-      load();
-      blocks(min(c + 2, c1 - 1));
-      const uint8_t *stage = lds + (c & 1) * STAGE;
-      const bool edge = (c + 1) * UNIT > clear;
-      if (!idle) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-          v4f s[2][NQ];
-#pragma unroll
-          for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-            for (int qc = 0; qc < NQ; qc++) s[kt][qc] = (v4f){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int x = 0; x < D / 32; x++)
-#pragma unroll
-            for (int kt = 0; kt < 2; kt++) {
-              const v8bf k = *(const v8bf *)(stage + (32 * h + 16 * kt + c16) * LK + 64 * x + 16 * g);
-#pragma unroll
-              for (int qc = 0; qc < NQ; qc++) s[kt][qc] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[qc][x], s[kt][qc], 0, 0, 0);
-            }
-          float scl = scale;
-          if (edge) {
-            attn_hide<NQ>(a, r, sight, c * UNIT + 32 * h, scale, s);
-            scl = 1.f;
-          }
-          v8bf p[NQ];
-          st.softmax(s, scl, p);
-          st.template add_values<LV>(stage + UNIT * LK + (32 * h + 4 * g + c16 / 4) * LV + 8 * (c16 % 4), p);
-        }
-        if (edge && any_odd) attn_add_no_numbers<NQ, DT, FP8>(a, r, sight, table, kh, c * UNIT, UNIT, st);
-      }
-      if (c + 1 < c1) odd = put(c + 1);
-      any_odd = __syncthreads_or(odd != 0);
+    // keys of unit c + 1 and values of c into LDS, the next of both asked for
+    const auto stage = [&](int c) {
+      put_keys(c + 1);
+      put_values(c);
+      ask(a.k_cache, a.k_block_bytes, block, c + 2, kr);
+      ask(a.v_cache, a.v_block_bytes, block_v, c + 1, vr);
+      block_v = block;
+      block = attn_block(a, table, key_of(c + 3));
+    };
+
+    if (tid == 0) any_odd = 0;
+    block = attn_block(a, table, key_of(c0));
+    ask(a.k_cache, a.k_block_bytes, block, c0, kr);
+    ask(a.v_cache, a.v_block_bytes, block, c0, vr);
+    block = block_v = attn_block(a, table, key_of(c0 + 1));
+    put_keys(c0);
+    ask(a.k_cache, a.k_block_bytes, block, c0 + 1, kr);
+    block = attn_block(a, table, key_of(c0 + 2));
+    __syncthreads();
+    if (late) {                                        // slot 0
+      stage(c0);
+      __syncthreads();
     }
+    if (m_tile * ROWS + 16 * NQ * w < r.n * a.G) {
+      v8bf q[NQ][X];
+      AttnSight<NQ> sight;
+      attn_queries<NQ, D, false>(a, r, kh, m_tile * ROWS + 16 * NQ * w, q, sight);
+      AttnState<NQ, DT> st;
+      st.clear();
+      v4f s[4][NQ];
+      attn_scores<4, 4, LD>(lds + (c0 & 1) * HALF + c16 * LD + 16 * g, q, s);
+      __syncthreads();
+      for (int c = c0; c < c1; c++) {
+        stage(c + late);
+        const bool edge = (c + 1) * UNIT > clear;
+        float scl = scale;
+        if (__builtin_expect(edge, 0)) {
+          attn_hide(a, r, sight, c * UNIT, scale, s);
+          scl = 1.f;
+        }
+        v8bf p[2][NQ], v[2 * DT];
+        st.template softmax<4>(s, scl, edge || c == c0, p);
+        __syncthreads();
+        attn_scores<4, 4, LD>(lds + ((c + 1) & 1) * HALF + c16 * LD + 16 * g, q, s);       // (past the last unit: of no use)
+        const uint8_t *at = lds + (2 + (c & 1)) * HALF + (4 * g + c16 / 4) * LD + 8 * (c16 % 4);
 #pragma unroll
-    for (int qc = 0; qc < NQ; qc++) {
-      const float l = over_groups(st.l[qc], true);
+        for (int x = 0; x < 4; x++) v[x] = attn_values<LD>(at, x);
+        attn_add_values<4, 2, LD>(st, at, p, v);
+        __syncthreads();
+      }
+      if (!late) __syncthreads();
+      if (__builtin_expect(any_odd, 0)) {
+        const int from = max(c0, clear / UNIT) * UNIT;          // the first unit whose values were looked at
+        attn_add_no_numbers<NQ, DT, FP8>(a, r, sight, table, kh, from, c1 * UNIT - from, st);
+      }
 #pragma unroll
-      for (int dt = 0; dt < DT; dt++)
-        attn_store<ROWS, D>(a, r, kh, m_tile, 16 * NQ * w + 16 * qc + c16, 16 * dt + 4 * g, whole, part, st.o[dt][qc], st.m[qc], l);
+      for (int qc = 0; qc < NQ; qc++) {
+        const float l = over_groups(st.l[qc], true);
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+          attn_store<ROWS, D>(a, r, kh, m_tile, 16 * NQ * w + 16 * qc + c16, 16 * dt + 4 * g, whole, part, st.o[dt][qc], st.m[qc], l);
+      }
+    } else {                                           // a wavefront without rows only helps with the bytes
+      __syncthreads();
+      for (int c = c0; c < c1; c++) {
+        stage(c + late);
+        __syncthreads();
+        __syncthreads();
+      }
+      if (!late) __syncthreads();
     }
+    __syncthreads();
   });
 }
 
@@ -604,7 +802,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
   __shared__ v4f sh_o[256];
   __shared__ float sh_m[256 / lanes], sh_l[256 / lanes];
   const int tid = threadIdx.x, group = tid / lanes, d = 4 * (tid % lanes), split = group % SPLIT;
-  if (blockIdx.y == 0) {
+  if (blockIdx.y == gridDim.y - 1) {
     const auto nothing = [&](int t) {
       for (int i = tid; i < a.Hq * lanes; i += 256) *(v2i *)(a.out + ((size_t)t * a.Hq * lanes + i) * 4) = (v2i){0, 0};
       if (a.lse)
@@ -616,11 +814,12 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
         for (int j = 0; j < r.n; j++) nothing(r.t0 + j);
     }
     for (int t = min(max(a.cu[a.B], 0), a.T) + (int)blockIdx.x; t < a.T; t += gridDim.x) nothing(t);
+    return;
   }
   const int *rec = a.records + 8 * blockIdx.x;
-  const int w1 = rec[0], b = rec[1], kh = rec[2], m_tile = rec[3], side = rec[4], w0 = blockIdx.x;
+  const int w1 = rec[0], kh = rec[3], m_tile = rec[4], side = rec[5], w0 = blockIdx.x;
+  const AttnRequest r{rec[1], rec[2], 0, 0};
   if (w1 <= w0) return;
-  const AttnRequest r = attn_request(a, b);
   const int in_tile = blockIdx.y * per_block + group / SPLIT, row = m_tile * ROWS + in_tile;
   if (m_tile * ROWS + (int)blockIdx.y * per_block >= r.n * a.G) return;
   const auto part = [&](int w) { return (size_t)(2 * w + (w == w0 ? side : 0)) * ROWS + in_tile; };
@@ -661,24 +860,25 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
 // ---- which kernel -------------------------------------------------------------------------------------------------------
 // By the rows to a cached key that a request has on average.
 struct AttnPlan {
-  int rows, keys;                      // rows of a tile; whether the wavefronts split the keys
+  int rows, groups;                    // rows of a tile; workgroups, a multiple of 8
+  float cut;
 };
-static AttnPlan attn_plan(int T, int Hq, int Hkv, int B) {
+static AttnPlan attn_plan(int T, int Hq, int Hkv, int B, int cache_dtype) {
   const int64_t rows = B > 0 ? ((int64_t)T * (Hq / Hkv) + B - 1) / B : 1;
-  if (rows <= 16) return {16, 1};
-  if (rows <= 32) return {32, 1};
-  if (rows <= 64) return {64, 0};
-  return {128, 0};
+  if (rows <= 16) return {16, cache_dtype == MOE_DTYPE_FP8 ? 512 : 256, 0.0625f};
+  if (rows <= 64) return {64, 512, 0.125f};
+  if (rows <= 128) return {128, 512, 0.125f};
+  return {256, 256, 0.25f};
 }
-constexpr int kAttnGroups = 512;
 
 }  // namespace moe
 
-extern "C" size_t moe_tree_attention_workspace_bytes(int T, int Hq, int Hkv, int D, int B) {
+extern "C" size_t moe_tree_attention_workspace_bytes(int T, int Hq, int Hkv, int D, int B, int cache_dtype) {
   using namespace moe;
-  if (T < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || D < 1 || B < 0) return 0;
-  const size_t rows = attn_plan(T, Hq, Hkv, B).rows, parts = 2 * kAttnGroups;
-  return align_up(parts * rows * D * 4, 256) + align_up(parts * rows * 8, 256) + kAttnGroups * 32;
+  if (T < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || D < 1 || B < 0 || (cache_dtype != MOE_DTYPE_BF16 && cache_dtype != MOE_DTYPE_FP8)) return 0;
+  const AttnPlan plan = attn_plan(T, Hq, Hkv, B, cache_dtype);
+  const size_t rows = plan.rows, parts = 2 * plan.groups;
+  return align_up(parts * rows * D * 4, 256) + align_up(parts * rows * 8, 256) + plan.groups * 32;
 }
 
 extern "C" int moe_tree_attention(void *stream, const void *q_bf16, int64_t q_stride, int T, int Hq, int Hkv, int D,
@@ -695,6 +895,7 @@ extern "C" int moe_tree_attention(void *stream, const void *q_bf16, int64_t q_st
       v_block_stride < page_size * row || table_width < 0 || (B > 1 && table_stride < table_width) || q_stride < (int64_t)Hq * D ||
       (int64_t)table_width * page_size >= (1ll << 31) || (int64_t)T * Hq >= (1ll << 31))
     return MOE_E_SHAPE;
+  if (k_block_stride >= (1ll << 31) || v_block_stride >= (1ll << 31) || row >= (1 << 22)) return MOE_E_SHAPE;
   if (q_stride % 8 || k_block_stride % 16 || v_block_stride % 16) return MOE_E_ALIGN;
   if (T == 0) return MOE_OK;
   if (B == 0 || !q_bf16 || !out_bf16 || !kv_lens || !cu_tokens || !workspace) return MOE_E_NULL;
@@ -702,13 +903,15 @@ extern "C" int moe_tree_attention(void *stream, const void *q_bf16, int64_t q_st
   for (const void *p : {q_bf16, k_cache, v_cache, (const void *)out_bf16})
     if ((uintptr_t)p % 16) return MOE_E_ALIGN;
   if ((uintptr_t)workspace % 256) return MOE_E_ALIGN;
-  if (workspace_bytes < moe_tree_attention_workspace_bytes(T, Hq, Hkv, D, B)) return MOE_E_WORKSPACE;
+  if (workspace_bytes < moe_tree_attention_workspace_bytes(T, Hq, Hkv, D, B, cache_dtype)) return MOE_E_WORKSPACE;
   const int fp8 = cache_dtype == MOE_DTYPE_FP8, wide = fp8 ? 1 : 2;
-  const AttnPlan plan = attn_plan(T, Hq, Hkv, B);
-  const size_t parts = 2 * kAttnGroups;
+  const AttnPlan plan = attn_plan(T, Hq, Hkv, B, cache_dtype);
+  // the line's length at most, in units
+  if (((int64_t)T * (Hq / Hkv) / plan.rows + B) * Hkv * (((int64_t)table_width * page_size + 63) / 64) >= (1ll << 31)) return MOE_E_SHAPE;
+  const size_t parts = 2 * plan.groups;
   AttnArgs a{(const uint16_t *)q_bf16, q_stride, T, Hq, Hkv, Hq / Hkv, B, n_blocks, __builtin_ctz(page_size), n_blocks ? table_width : 0,
-             (const uint8_t *)k_cache, (const uint8_t *)v_cache, k_block_stride * wide, v_block_stride * wide, table_stride, block_tables,
-             kv_lens, cu_tokens, masks, scale, k_scale, v_scale, (uint16_t *)out_bf16, lse, 2, kAttnGroups, (float *)workspace,
+             (const uint8_t *)k_cache, (const uint8_t *)v_cache, (uint32_t)(k_block_stride * wide), (uint32_t)(v_block_stride * wide), table_stride,
+             block_tables, kv_lens, cu_tokens, masks, scale, k_scale, v_scale, (uint16_t *)out_bf16, lse, plan.groups, plan.cut, (float *)workspace,
              (float *)((uint8_t *)workspace + align_up(parts * plan.rows * D * 4, 256)),
              (int32_t *)((uint8_t *)workspace + align_up(parts * plan.rows * D * 4, 256) + align_up(parts * plan.rows * 8, 256))};
   hipStream_t st = (hipStream_t)stream;
@@ -718,20 +921,20 @@ extern "C" int moe_tree_attention(void *stream, const void *q_bf16, int64_t q_st
     constexpr bool F = decltype(narrow)::value;
     const auto join = [&](auto rows, auto split) {
       constexpr int R = decltype(rows)::value, S = decltype(split)::value;
-      attn_join_kernel<R, Dc, S><<<dim3(a.groups, R * Dc * S / 1024), 256, 0, st>>>(a);
+      attn_join_kernel<R, Dc, S><<<dim3(a.groups, R * Dc * S / 1024 + 1), 256, 0, st>>>(a);
     };
     if (plan.rows == 16) {
       attn_keys_kernel<Dc, F, 1><<<a.groups, 256, 0, st>>>(a);
       join(integral_constant<int, 16>(), integral_constant<int, 8>());
-    } else if (plan.rows == 32) {
-      attn_keys_kernel<Dc, F, 2><<<a.groups, 256, 0, st>>>(a);
-      join(integral_constant<int, 32>(), integral_constant<int, 4>());
     } else if (plan.rows == 64) {
       attn_rows_kernel<Dc, F, 1><<<a.groups, 256, 0, st>>>(a);
       join(integral_constant<int, 64>(), integral_constant<int, 2>());
-    } else {
+    } else if (plan.rows == 128) {
       attn_rows_kernel<Dc, F, 2><<<a.groups, 256, 0, st>>>(a);
       join(integral_constant<int, 128>(), integral_constant<int, 1>());
+    } else {
+      attn_pairs_kernel<Dc, F, 2><<<a.groups, 512, 0, st>>>(a);
+      join(integral_constant<int, 256>(), integral_constant<int, 1>());
     }
   };
   if (D == 64 && fp8) run(integral_constant<int, 64>(), integral_constant<bool, true>());
