@@ -8,9 +8,10 @@
 // three rescaled when m grows; then entropy = ln 2 (log2 s - w / s).  Few rows are cut into segments, whose results a second
 // launch joins.
 // For the alternatives a value and its index become one whole number, (value's bits in order, ~index), so that no two are
-// equal.  The k-th best of the threads' best keys is a bound that at least k keys reach and that only k threads' keys can
-// pass; what passes it is collected in LDS, later chunks add what beats the bound, and the rank of a key at the end is the
-// count of larger ones.
+// equal.  The first chunk gives a bound: the k-th best of 64 groups' best keys, which at least k keys reach.  What reaches it there
+// and later - some k keys a chunk where values come in no order - is collected in LDS and sorted by wavefronts, 64 keys at a time.
+// Where values come in rising order more is collected than there is room for: the row is then looked over again, the
+// bound raised with every chunk.
 #include <math.h>
 #include "moe_common.h"
 #include "moe_layout.h"
@@ -19,7 +20,8 @@
 namespace moe {
 
 constexpr int kLpThreads = 256, kLpVectors = 4;        // vectors of 16 bytes that a thread holds of a chunk
-constexpr int kLpRoom = 2048;                          // keys collected at a time
+// keys collected at a time: what k groups of four threads hold of a chunk at the most, beside the k kept from before
+constexpr int kLpRoom = MOE_MAX_TOPK * 4 * 8 * kLpVectors + 2 * MOE_MAX_TOPK;
 constexpr int kLpSegments = 64;
 
 struct LpArgs {
@@ -63,13 +65,85 @@ struct LpShared {
   int count;
 };
 
+// the value of lane ^ D, without a trip through LDS
+template <int D>
+__device__ __forceinline__ uint32_t lp_across(uint32_t v) {
+  typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+  if (D == 1) return __builtin_amdgcn_update_dpp(v, v, 0xb1, 0xf, 0xf, false);         // quad_perm 1 0 3 2
+  if (D == 2) return __builtin_amdgcn_update_dpp(v, v, 0x4e, 0xf, 0xf, false);         // quad_perm 2 3 0 1
+  if (D == 4) {                                                                        // from 4 lanes up and down in a row
+    const uint32_t up = __builtin_amdgcn_update_dpp(v, v, 0x104, 0xf, 0x5, false);
+    return __builtin_amdgcn_update_dpp(up, v, 0x114, 0xf, 0xa, false);
+  }
+  if (D == 8) return __builtin_amdgcn_update_dpp(v, v, 0x128, 0xf, 0xf, false);        // row rotated by 8
+  const v2u r = D == 16 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return (threadIdx.x & D) ? r[0] : r[1];
+}
+template <int D>
+__device__ __forceinline__ uint64_t lp_across(uint64_t v) {
+  return (uint64_t)lp_across<D>((uint32_t)(v >> 32)) << 32 | lp_across<D>((uint32_t)v);
+}
+template <int D>
+__device__ __forceinline__ float lp_across(float v) { return __uint_as_float(lp_across<D>(__float_as_uint(v))); }
+
+// a step of a sorting network: lanes D apart, the larger value to the lower lane where `down`
+template <int D>
+__device__ __forceinline__ uint64_t lp_step(uint64_t v, bool down) {
+  const uint64_t o = lp_across<D>(v);
+  return (((threadIdx.x & D) == 0) == down) == (v > o) ? v : o;
+}
+template <int D>
+__device__ __forceinline__ uint64_t lp_steps(uint64_t v, bool down) {
+  v = lp_step<D>(v, down);
+  if constexpr (D > 1) v = lp_steps<D / 2>(v, down);
+  return v;
+}
+// a wavefront's 64 keys, the largest in lane 0
+__device__ __forceinline__ uint64_t lp_sort(uint64_t v) {
+  v = lp_steps<1>(v, (threadIdx.x & 2) == 0);
+  v = lp_steps<2>(v, (threadIdx.x & 4) == 0);
+  v = lp_steps<4>(v, (threadIdx.x & 8) == 0);
+  v = lp_steps<8>(v, (threadIdx.x & 16) == 0);
+  v = lp_steps<16>(v, (threadIdx.x & 32) == 0);
+  return lp_steps<32>(v, true);
+}
+// the 64 largest of two sorted 64, sorted
+__device__ __forceinline__ uint64_t lp_merge(uint64_t a, uint64_t b) {
+  return lp_steps<32>(max(a, __shfl(b, 63 - (threadIdx.x & 63), 64)), true);
+}
+// The 64 best of the n keys collected, sorted, in every wavefront (0: none): each sorts its share, then they are merged.
+__device__ __forceinline__ uint64_t lp_best64(LpShared &sh, int n) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  uint64_t v = 0;
+  for (int at = 64 * w; at < n; at += kLpThreads) {
+    const uint64_t more = lp_sort(at + lane < n ? sh.keys[at + lane] : 0);
+    v = at == 64 * w ? more : lp_merge(v, more);
+  }
+  __syncthreads();
+  sh.best[threadIdx.x] = v;
+  __syncthreads();
+  v = sh.best[lane];
+  for (int i = 1; i < kLpThreads / 64 && 64 * i < n; i++) v = lp_merge(v, sh.best[64 * i + lane]);
+  return v;
+}
+
 // the sums of the whole workgroup, in every thread
 __device__ __forceinline__ LpStats lp_block_stats(LpStats v, LpShared &sh, float c) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const LpStats o{__shfl_xor(v.m, d, 64), __shfl_xor(v.s, d, 64), __shfl_xor(v.w, d, 64)};
-    v = lp_join(v, o, c);
-  }
+  // first the largest, then everything in terms of it: one exponential a lane
+  float m = v.m;
+  m = fmaxf(m, lp_across<1>(m));
+  m = fmaxf(m, lp_across<2>(m));
+  m = fmaxf(m, lp_across<4>(m));
+  m = fmaxf(m, lp_across<8>(m));
+  m = fmaxf(m, lp_across<16>(m));
+  m = fmaxf(m, lp_across<32>(m));
+  v = lp_join(v, LpStats{m, 0.f, 0.f}, c);
+  v.s += lp_across<1>(v.s), v.w += lp_across<1>(v.w);
+  v.s += lp_across<2>(v.s), v.w += lp_across<2>(v.w);
+  v.s += lp_across<4>(v.s), v.w += lp_across<4>(v.w);
+  v.s += lp_across<8>(v.s), v.w += lp_across<8>(v.w);
+  v.s += lp_across<16>(v.s), v.w += lp_across<16>(v.w);
+  v.s += lp_across<32>(v.s), v.w += lp_across<32>(v.w);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) sh.stats[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -79,75 +153,61 @@ __device__ __forceinline__ LpStats lp_block_stats(LpStats v, LpShared &sh, float
   return v;
 }
 
-// sh.bound = the k-th largest of the threads' keys (0: none), if that is more than it was
+// sh.bound = the k-th best of 64 groups' best keys (0: fewer than k groups have one), if that is more than it was
 __device__ __forceinline__ void lp_raise_bound(uint64_t best, int k, LpShared &sh) {
-  const uint64_t mine = best ? best : threadIdx.x;     // (a key of a value is larger than any thread's number)
-  sh.best[threadIdx.x] = mine;
   __syncthreads();
-  int larger = 0;
-#pragma unroll 8
-  for (int i = 0; i < kLpThreads; i++) larger += sh.best[i] > mine;
-  if (larger == k - 1 && best > sh.bound) sh.bound = best;
+  sh.best[threadIdx.x] = best;
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    uint64_t v = sh.best[threadIdx.x];
+#pragma unroll
+    for (int i = 1; i < kLpThreads / 64; i++) v = max(v, sh.best[64 * i + threadIdx.x]);
+    v = lp_sort(v);
+    if ((int)threadIdx.x == k - 1 && v > sh.bound) sh.bound = v;
+  }
   __syncthreads();
 }
 
-// keeps the k best of the keys collected, in order
+// The k best of the keys collected stay, in order.
 __device__ __forceinline__ void lp_keep_best(int k, LpShared &sh) {
   __syncthreads();
   const int n = sh.count;
-  constexpr int kPer = kLpRoom / kLpThreads;
-  uint64_t mine[kPer];
-  int rank[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; i++) {
-    const int at = i * kLpThreads + threadIdx.x;
-    mine[i] = at < n ? sh.keys[at] : 0;
-    rank[i] = 0;
-  }
-  for (int j = 0; j < n; j++) {
-    const uint64_t other = sh.keys[j];
-#pragma unroll
-    for (int i = 0; i < kPer; i++) {
-      if (i * kLpThreads >= n) break;
-      rank[i] += other > mine[i];
-    }
-  }
+  const uint64_t v = lp_best64(sh, n);
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kPer; i++)
-    if (mine[i] && rank[i] < k) {
-      sh.keys[rank[i]] = mine[i];
-      if (rank[i] == k - 1) sh.bound = mine[i];
-    }
+  if ((int)threadIdx.x < k) {
+    sh.keys[threadIdx.x] = v;
+    if ((int)threadIdx.x == k - 1 && v) sh.bound = v;
+  }
   if (threadIdx.x == 0) sh.count = min(n, k);
   __syncthreads();
 }
 
-// Adds to the collected keys what beats the bound of N keys a thread; key(i) is 0 where there is none, best the largest.
+// Adds the keys of a thread that reach the bound to those collected; key(i) is 0 where there is none, worth(i) says cheaply that it may.
+template <int N, typename Worth, typename Key>
+__device__ __forceinline__ void lp_push(Worth worth, Key key, uint64_t bound, LpShared &sh) {
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    if (!worth(i)) continue;
+    const uint64_t v = key(i);
+    if (v && v >= bound) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kLpRoom) sh.keys[at] = v;
+    }
+  }
+}
+
+// One chunk when the keys may come in rising order: where they do not fit, those before are cut to the best, the bound is raised by the
+// chunk's own, and what reaches it then is at most k groups' keys.
 template <int N, typename Key>
-__device__ __forceinline__ void lp_collect(Key key, uint64_t best, bool first, int k, LpShared &sh) {
-  if (first) lp_raise_bound(best, k, sh);
+__device__ __forceinline__ void lp_push_careful(Key key, uint64_t best, int k, LpShared &sh) {
   for (int again = 0; again < 2; again++) {
+    __syncthreads();
     const int before = sh.count;
     const uint64_t bound = sh.bound;
     __syncthreads();
-    if (best >= bound && best) {
-#pragma unroll
-      for (int i = 0; i < N; i++) {
-        const uint64_t v = key(i);
-        if (v && v >= bound) {
-          const int at = atomicAdd(&sh.count, 1);
-          if (at < kLpRoom) sh.keys[at] = v;
-        }
-      }
-    }
+    lp_push<N>([](int) { return true; }, key, bound, sh);
     __syncthreads();
-    const int n = sh.count;
-    if (n <= kLpRoom) {
-      if (n > kLpRoom - 32 * N) lp_keep_best(k, sh);   // (k threads' keys have to fit beside what is there)
-      return;
-    }
-    // too many: what was there is cut to the best, and the bound raised by this chunk's own
+    if (sh.count <= kLpRoom) return;
     __syncthreads();
     if (threadIdx.x == 0) sh.count = before;
     lp_keep_best(k, sh);
@@ -155,8 +215,8 @@ __device__ __forceinline__ void lp_collect(Key key, uint64_t best, bool first, i
   }
 }
 
-// the row's results from its sums and the keys kept
-__device__ __forceinline__ void lp_write(const LpArgs &a, int row, float token_logit, const LpStats v, const LpShared &sh) {
+// the row's results from its sums and its best keys, in order in the first wavefront
+__device__ __forceinline__ void lp_write(const LpArgs &a, int row, float token_logit, const LpStats v, uint64_t key) {
   const float log_s = logf(v.s);
   const bool none = v.m == -INFINITY && v.s == 0.f;    // no token is possible: log 0, and nothing to be uncertain about
   if (threadIdx.x == 0) {
@@ -164,7 +224,6 @@ __device__ __forceinline__ void lp_write(const LpArgs &a, int row, float token_l
     a.entropy[row] = none ? 0.f : log_s - 0.6931471805599453f * (v.w / v.s);
   }
   if ((int)threadIdx.x < a.k) {
-    const uint64_t key = (int)threadIdx.x < sh.count ? sh.keys[threadIdx.x] : 0;
     const size_t at = (size_t)row * a.k + threadIdx.x;
     a.top_ids[at] = key ? (int32_t)~(uint32_t)key : -1;
     a.top_logprobs[at] = none ? -INFINITY : key ? (lp_value(key) - v.m) * a.inv_temp - log_s : NAN;
@@ -178,9 +237,50 @@ __device__ __forceinline__ float lp_token_logit(const LpArgs &a, int row, bool b
   return bf16 ? bf16_to_f32(((const uint16_t *)a.logits)[at]) : ((const float *)a.logits)[at];
 }
 
+// a thread's values of a chunk
+template <bool BF16>
+struct LpChunk {
+  static constexpr int E = BF16 ? 8 : 4, N = E * kLpVectors;         // of a vector; in all
+  v4i raw[kLpVectors];
+  __device__ __forceinline__ static int vector(int c0, int u) { return c0 + u * kLpThreads + (int)threadIdx.x; }
+  // the vectors from c0 on that lie in the row and before v1 whole (0 for the others)
+  __device__ __forceinline__ void load(const uint8_t *aligned, int c0, int v1, int lead, int V) {
+#pragma unroll
+    for (int u = 0; u < kLpVectors; u++) {
+      const int v = vector(c0, u), e0 = v * E - lead;
+      raw[u] = (v4i){0, 0, 0, 0};
+      if (v < v1 && e0 >= 0 && e0 + E <= V) raw[u] = *(const v4i *)(aligned + (size_t)v * 16);
+    }
+  }
+  __device__ __forceinline__ void values(const uint8_t *aligned, int c0, int v1, int lead, int V, float (&x)[N]) const {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const uint32_t w = (uint32_t)raw[i / E][BF16 ? i % E / 2 : i % E];
+      x[i] = __uint_as_float(BF16 ? (i & 1 ? w & 0xffff0000u : w << 16) : w);
+    }
+    if (c0 * E - lead >= 0 && c0 + kLpThreads * kLpVectors <= v1 && (c0 + kLpThreads * kLpVectors) * E - lead <= V) return;
+#pragma unroll
+    for (int u = 0; u < kLpVectors; u++) {             // a chunk at an end of the row or the segment
+      const int v = vector(c0, u), e0 = v * E - lead;
+      if (v < v1 && e0 >= 0 && e0 + E <= V) continue;
+#pragma unroll
+      for (int i = 0; i < E; i++) {
+        const bool there = v < v1 && e0 + i >= 0 && e0 + i < V;
+        x[u * E + i] = !there ? -INFINITY : BF16 ? bf16_to_f32(((const uint16_t *)aligned)[(size_t)v * E + i]) : ((const float *)aligned)[(size_t)v * E + i];
+      }
+    }
+  }
+  // value i as a key; 0: not of this row and segment, or no number
+  __device__ __forceinline__ static uint64_t key(const float (&x)[N], int i, int c0, int v1, int lead, int V) {
+    const int v = vector(c0, i / E), e = v * E - lead + i % E;
+    return v < v1 && e >= 0 && e < V && x[i] == x[i] ? lp_key(x[i], (uint32_t)e) : 0;
+  }
+};
+
 template <bool BF16>
 __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(const LpArgs a) {
-  constexpr int E = BF16 ? 8 : 4, N = E * kLpVectors;  // elements of a vector; of a thread's share of a chunk
+  typedef LpChunk<BF16> Chunk;
+  constexpr int E = Chunk::E, N = Chunk::N, kChunk = kLpThreads * kLpVectors;
   __shared__ LpShared sh;
   const int row = blockIdx.x / a.n_seg, seg = blockIdx.x % a.n_seg, tid = threadIdx.x;
   const uint8_t *base = (const uint8_t *)a.logits + (size_t)row * a.row_stride * (16 / E);
@@ -188,73 +288,100 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(const LpArgs
   const int lead = (int)((uintptr_t)base % 16) / (16 / E);
   const uint8_t *aligned = base - lead * (16 / E);
   const int n_vec = (a.V + lead + E - 1) / E, v0 = seg * a.seg_vectors, v1 = min(v0 + a.seg_vectors, n_vec);
+  Chunk chunk;
+  chunk.load(aligned, v0, v1, lead, a.V);
   const float token_logit = a.n_seg == 1 && tid == 0 ? lp_token_logit(a, row, BF16) : 0.f;
   if (tid == 0) {
     sh.bound = 0;
     sh.count = 0;
   }
-  __syncthreads();
   LpStats st{-INFINITY, 0.f, 0.f};
-  bool first = true;
-  for (int c0 = v0; c0 < v1; c0 += kLpThreads * kLpVectors) {
+  uint64_t bound = 0;
+  float bound_value = -INFINITY;
+  for (int c0 = v0; c0 < v1; c0 += kChunk) {
     float x[N];
+    chunk.values(aligned, c0, v1, lead, a.V, x);
+    chunk.load(aligned, c0 + kChunk, v1, lead, a.V);   // the next one while this one is worked on
+    float most = x[0];
 #pragma unroll
-    for (int u = 0; u < kLpVectors; u++) {
-      const int v = c0 + u * kLpThreads + tid, e0 = v * E - lead;
-      v4i raw = (v4i){0, 0, 0, 0};
-      const bool whole = v < v1 && e0 >= 0 && e0 + E <= a.V;
-      if (whole) raw = *(const v4i *)(aligned + (size_t)v * 16);
-#pragma unroll
-      for (int i = 0; i < E; i++) {
-        float f;
-        if (BF16) f = bf16_to_f32((uint16_t)((uint32_t)raw[i / 2] >> (16 * (i & 1))));
-        else f = __uint_as_float((uint32_t)raw[i & 3]);
-        x[u * E + i] = whole ? f : -INFINITY;
-      }
-      if (!whole && v < v1) {
-#pragma unroll
-        for (int i = 0; i < E; i++)
-          if (e0 + i >= 0 && e0 + i < a.V)
-            x[u * E + i] = BF16 ? bf16_to_f32(((const uint16_t *)aligned)[(size_t)v * E + i]) : ((const float *)aligned)[(size_t)v * E + i];
-      }
-    }
-    float most = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < N; i++) most = fmaxf(most, x[i]);
+    for (int i = 1; i + 1 < N; i += 2) most = fmaxf(fmaxf(most, x[i]), x[i + 1]);
+    most = fmaxf(most, x[N - 1]);
     if (most > st.m) {
-      const float d = st.m == -INFINITY ? -1e4f : fmaxf((st.m - most) * a.c, -1e4f), f = exp2f(d);
+      const float d = st.m == -INFINITY ? -1e4f : fmaxf((st.m - most) * a.c, -1e4f), f = __builtin_amdgcn_exp2f(d);
       st.w = f * (st.w + d * st.s);
       st.s *= f;
       st.m = most;
     }
-    // (the difference first: c times a logit of the type's lowest value, as masks use it, would be -inf)
-    const float base = st.m == -INFINITY ? 0.f : st.m;
+    // (x - m) c; where m is a mask of the type's lowest value m c would be -inf, so there the difference comes first
+    const bool low = st.m < -1e37f && st.m > -INFINITY;
+    if (__builtin_expect(__any(low), 0)) {
+      const float m = st.m == -INFINITY ? 0.f : st.m;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      const float t = (x[i] - base) * a.c, e = __builtin_amdgcn_exp2f(t);
-      st.s += e;
-      st.w = fmaf(e, fmaxf(t, -1000.f), st.w);         // (0 times -inf where a logit is -inf)
+      for (int i = 0; i < N; i++) {
+        const float t = (x[i] - m) * a.c, e = __builtin_amdgcn_exp2f(t);
+        st.s += e;
+        st.w = fmaf(e, fmaxf(t, -1000.f), st.w);       // (0 times -inf where a logit is -inf)
+      }
+    } else {
+      const float off = st.m == -INFINITY ? 0.f : st.m * a.c;
+      float s2 = 0.f, w2 = 0.f;                        // two sums at a time: each waits for its last addition
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        const float t = fmaf(x[i], a.c, -off), e = __builtin_amdgcn_exp2f(t);
+        const float t2 = fmaf(x[i + 1], a.c, -off), e2 = __builtin_amdgcn_exp2f(t2);
+        st.s += e;
+        s2 += e2;
+        st.w = fmaf(e, fmaxf(t, -1000.f), st.w);
+        w2 = fmaf(e2, fmaxf(t2, -1000.f), w2);
+      }
+      st.s += s2;
+      st.w += w2;
     }
     if (a.k) {
-      const float bound = sh.bound ? lp_value(sh.bound) : -INFINITY;
-      if (__syncthreads_or(first || most >= bound)) {
-        const auto key = [&](int i) -> uint64_t {
-          const int e = (c0 + (i / E) * kLpThreads + tid) * E - lead + i % E;
-          const bool there = c0 + (i / E) * kLpThreads + tid < v1 && e >= 0 && e < a.V && x[i] == x[i];
-          return there ? lp_key(x[i], (uint32_t)e) : 0;
-        };
-        uint64_t best = 0;
+      if (c0 == v0) {
+        int at = N;                                    // the first place of the largest value
 #pragma unroll
-        for (int i = 0; i < N; i++) best = max(best, key(i));
-        lp_collect<N>(key, best, first, a.k, sh);
-        first = false;
+        for (int i = N - 1; i >= 0; i--) at = x[i] == most ? i : at;
+        const int v = Chunk::vector(c0, at / E), e = v * E - lead + at % E;
+        lp_raise_bound(at < N && v < v1 && e >= 0 && e < a.V ? lp_key(most, (uint32_t)e) : 0, a.k, sh);
+        bound = sh.bound;
+        bound_value = bound ? lp_value(bound) : -INFINITY;
+      }
+      if (most >= bound_value) lp_push<N>([&](int i) { return x[i] >= bound_value; }, [&](int i) { return Chunk::key(x, i, c0, v1, lead, a.V); }, bound, sh);
+      // After 3 and 8 chunks what is collected gives a better bound, so that fewer keys come from those that follow.
+      const int turn = (c0 - v0) / kChunk;
+      if ((turn == 2 || turn == 7) && c0 + 2 * kChunk < v1) {
+        __syncthreads();
+        if (sh.count <= kLpRoom) {
+          lp_keep_best(a.k, sh);
+          bound = sh.bound;
+          bound_value = bound ? lp_value(bound) : -INFINITY;
+        }
       }
     }
   }
-  st = lp_block_stats(st, sh, a.c);
-  if (a.k) lp_keep_best(a.k, sh);
+  st = lp_block_stats(st, sh, a.c);                    // (ends behind a barrier)
+  uint64_t key = 0;
+  if (a.k) {
+    __syncthreads();
+    if (__builtin_expect(sh.count > kLpRoom, 0)) {     // rising values: once more, with care
+      __syncthreads();
+      if (tid == 0) sh.count = 0;
+      for (int c0 = v0; c0 < v1; c0 += kChunk) {
+        float x[N];
+        chunk.load(aligned, c0, v1, lead, a.V);
+        chunk.values(aligned, c0, v1, lead, a.V, x);
+        uint64_t best = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++) best = max(best, Chunk::key(x, i, c0, v1, lead, a.V));
+        lp_push_careful<N>([&](int i) { return Chunk::key(x, i, c0, v1, lead, a.V); }, best, a.k, sh);
+      }
+      __syncthreads();
+    }
+    key = lp_best64(sh, sh.count);
+  }
   if (a.n_seg == 1) {
-    lp_write(a, row, token_logit, st, sh);
+    lp_write(a, row, token_logit, st, key);
     return;
   }
   const size_t part = (size_t)row * a.n_seg + seg;
@@ -263,37 +390,40 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(const LpArgs
     a.part_stats[part * 3 + 1] = st.s;
     a.part_stats[part * 3 + 2] = st.w;
   }
-  if (tid < a.k) a.part_keys[part * a.k + tid] = tid < sh.count ? sh.keys[tid] : 0;
+  if (tid < a.k) a.part_keys[part * a.k + tid] = key;
 }
 
+// A row's segments: the sums, and of their sorted keys those that reach the k-th best of the segments' first ones.
 __global__ __launch_bounds__(kLpThreads) void token_logprobs_join_kernel(const LpArgs a, int bf16) {
   constexpr int N = kLpSegments * MOE_MAX_TOPK / kLpThreads;
   __shared__ LpShared sh;
   const int row = blockIdx.x, tid = threadIdx.x;
+  uint64_t keys[N], first = 0;
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const int at = i * kLpThreads + tid;
+    keys[i] = at < a.n_seg * a.k ? a.part_keys[(size_t)row * a.n_seg * a.k + at] : 0;
+  }
+  LpStats st{-INFINITY, 0.f, 0.f};
+  if (tid < a.n_seg) {
+    const float *p = a.part_stats + ((size_t)row * a.n_seg + tid) * 3;
+    st = {p[0], p[1], p[2]};
+    if (a.k) first = a.part_keys[((size_t)row * a.n_seg + tid) * a.k];
+  }
   const float token_logit = tid == 0 ? lp_token_logit(a, row, bf16) : 0.f;
   if (tid == 0) {
     sh.bound = 0;
     sh.count = 0;
   }
-  __syncthreads();
-  LpStats st{-INFINITY, 0.f, 0.f};
-  if (tid < a.n_seg) {
-    const float *p = a.part_stats + ((size_t)row * a.n_seg + tid) * 3;
-    st = {p[0], p[1], p[2]};
-  }
   st = lp_block_stats(st, sh, a.c);
+  uint64_t key = 0;
   if (a.k) {
-    uint64_t keys[N], best = 0;
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-      const int at = i * kLpThreads + tid;
-      keys[i] = at < a.n_seg * a.k ? a.part_keys[(size_t)row * a.n_seg * a.k + at] : 0;
-      best = max(best, keys[i]);
-    }
-    lp_collect<N>([&](int i) { return keys[i]; }, best, true, a.k, sh);
-    lp_keep_best(a.k, sh);
+    lp_raise_bound(first, a.k, sh);                    // (every key is of a lane of its own: 64 segments at most)
+    lp_push<N>([](int) { return true; }, [&](int i) { return keys[i]; }, sh.bound, sh);
+    __syncthreads();
+    key = lp_best64(sh, sh.count);
   }
-  lp_write(a, row, token_logit, st, sh);
+  lp_write(a, row, token_logit, st, key);
 }
 
 // Segments of a row: enough workgroups for the chip, but none of less than a vector a thread.
