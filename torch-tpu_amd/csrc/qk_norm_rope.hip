@@ -6,10 +6,11 @@
 //
 // One rounding at the end: to bf16, or to e4m3 after the division by the head's scale.
 // It is bound by bytes, so a value is read once and written once.  A lane holds 8 neighbouring elements of a head, D/8 lanes a head
-// (rounded up to a power of two); the sum of squares is a butterfly over those lanes, and the partner of an (i, i + R/2) pair comes
+// (rounded up to a power of two); the sum of squares is taken over those lanes, and the partner of an (i, i + R/2) pair comes
 // from the lane R/16 further as the two bf16 that the register holds.  A lane's angles and weights are the same for every head, so it
 // takes several heads of a token where there are tokens enough to fill the chip.
 #include "moe_common.h"
+#include "lanes.h"
 #include "../../include/moe_hip.h"
 
 namespace moe {
@@ -26,7 +27,7 @@ struct RopeArgs {
   const int64_t *slots;
   const float *k_scale, *v_scale;
   float eps;
-  int T, Hq, Hkv, D, R, P, page_log2, weights_bf16, interleaved, cache_fp8, heads_per_group, groups_per_token;
+  int T, Hq, Hkv, D, R, P, page_log2, weights_bf16, interleaved, cache_fp8, groups_per_token;
 };
 
 __device__ __forceinline__ void load_weight(const void *w, int is_bf16, int e, float *out) {
@@ -52,6 +53,12 @@ __device__ __forceinline__ v2i pack8_fp8(const float *v) {
   hi = __builtin_amdgcn_cvt_pk_fp8_f32(fp8_range(v[6]), fp8_range(v[7]), hi, true);
   return (v2i){lo, hi};
 }
+__device__ __forceinline__ v2i scaled_fp8(const float *v, float scale) {
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) y[i] = v[i] / scale;
+  return pack8_fp8(y);
+}
 __device__ __forceinline__ v4i pack8_bf16(const float *v) {
   return (v4i){(int)pack2_bf16(v[0], v[1]), (int)pack2_bf16(v[2], v[3]), (int)pack2_bf16(v[4], v[5]), (int)pack2_bf16(v[6], v[7])};
 }
@@ -63,7 +70,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const RopeArgs a) {
   if (t >= a.T) return;                                // (whole groups of LPH lanes, which is what the shuffles reach)
   const int part = (int)(group % a.groups_per_token), L = threadIdx.x % LPH, e = 8 * L;
   const bool live = e < a.D;
-  const int heads = a.Hq + 2 * a.Hkv, h0 = part * a.heads_per_group, h1 = min(h0 + a.heads_per_group, heads);
+  const int heads = a.Hq + 2 * a.Hkv;
   const int pos = a.positions[t];
   const bool placed = pos >= 0 && pos < a.P;
   const int64_t slot = a.slots ? a.slots[t] : -1;
@@ -86,72 +93,95 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const RopeArgs a) {
   }
   const int lane = threadIdx.x & 63;
   const int other = turned && !a.interleaved ? (second ? lane - step : lane + step) : lane;
-  const int eo = e + 8 * (other - lane);
   const uint16_t *src = a.qkv + t * a.row_stride + e;
+  const v4i none = (v4i){0, 0, 0, 0};
 
-  for (int h = h0; h < h1; h++) {
-    const v4i raw = live ? *(const v4i *)(src + (size_t)h * a.D) : (v4i){0, 0, 0, 0};
-    const int kind = h < a.Hq ? 0 : h < a.Hq + a.Hkv ? 1 : 2;
-    float y[8];
+  // Of a query or key head: y = r (x w cos + x' w' sin), where x' and w' are the pair's other value and weight and r is 1 over the
+  // root mean square.  w cos and w' sin are the same for all heads of a kind: formed once.
+  float wc[8], ws[8];
+  const auto factors = [&](const void *w) {
+    float w1[8], w2[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) w1[i] = w2[i] = 1.f;
+    if (w && live) {
+      load_weight(w, a.weights_bf16, e, w1);
+      load_weight(w, a.weights_bf16, e + 8 * (other - lane), w2);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) wc[i] = w1[i] * c[i], ws[i] = (a.interleaved ? w1[i ^ 1] : w2[i]) * s[i];
+  };
+  const auto turn = [&](const v4i raw, bool normed, float (&y)[8]) {
+    float x[8], z[8];
+    float r = 1.f;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      y[2 * i] = bf16_to_f32((uint16_t)((uint32_t)raw[i] & 0xffff));
-      y[2 * i + 1] = bf16_to_f32((uint16_t)((uint32_t)raw[i] >> 16));
+      const uint32_t o = a.interleaved ? (uint32_t)raw[i] : (uint32_t)__shfl(raw[i], other, 64);
+      x[2 * i] = bf16_to_f32((uint16_t)((uint32_t)raw[i] & 0xffff));
+      x[2 * i + 1] = bf16_to_f32((uint16_t)((uint32_t)raw[i] >> 16));
+      const float lo = bf16_to_f32((uint16_t)(o & 0xffff)), hi = bf16_to_f32((uint16_t)(o >> 16));
+      z[2 * i] = a.interleaved ? hi : lo;
+      z[2 * i + 1] = a.interleaved ? lo : hi;
     }
-    if (kind < 2) {
-      float z[8];                                      // the pair's other value
+    if (normed) {
+      float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const uint32_t o = (uint32_t)__shfl(raw[i], other, 64);
-        z[2 * i] = bf16_to_f32((uint16_t)(o & 0xffff));
-        z[2 * i + 1] = bf16_to_f32((uint16_t)(o >> 16));
-      }
-      const void *w = kind == 0 ? a.q_weight : a.k_weight;
-      if (w) {
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) sum = fmaf(y[i], y[i], sum);
-#pragma unroll
-        for (int d = 1; d < LPH; d <<= 1) sum += __shfl_xor(sum, d, 64);
-        const float r = 1.0f / sqrtf(sum / (float)a.D + a.eps);
-        float w1[8], w2[8];
-        if (live) {
-          load_weight(w, a.weights_bf16, e, w1);
-          load_weight(w, a.weights_bf16, eo, w2);
-#pragma unroll
-          for (int i = 0; i < 8; i++) y[i] = y[i] * r * w1[i], z[i] = z[i] * r * w2[i];
-        }
-      }
-      float o[8];
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const float p = a.interleaved ? y[i ^ 1] : z[i];
-        o[i] = turned ? y[i] * c[i] + p * s[i] : y[i];
-      }
-#pragma unroll
-      for (int i = 0; i < 8; i++) y[i] = o[i];
+      for (int i = 0; i < 8; i++) sum = fmaf(x[i], x[i], sum);
+      r = 1.0f / sqrtf(lane_sum<LPH>(sum) / (float)a.D + a.eps);
     }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float o = x[i] * wc[i];
+      y[i] = r * (turned ? fmaf(z[i], ws[i], o) : o);
+    }
+  };
+  const auto place = [&](uint8_t *cache, int64_t block_bytes, int kh) {
+    const int64_t within = ((slot & ((1 << a.page_log2) - 1)) * a.Hkv + kh) * (int64_t)a.D + e;
+    return cache + (slot >> a.page_log2) * block_bytes + within * (a.cache_fp8 ? 1 : 2);
+  };
+
+  // Heads part, part + stride, ...: groups side by side read and write heads side by side.
+  const int stride = a.groups_per_token;
+  int h = part;
+  float y[8];
+  v4i raw = live && h < heads ? *(const v4i *)(src + (size_t)h * a.D) : none;
+  const auto next = [&]() {                            // the next head is asked for before this one is worked on
+    const v4i now = raw;
+    h += stride;
+    if (h < heads && live) raw = *(const v4i *)(src + (size_t)h * a.D);
+    return now;
+  };
+  if (h < a.Hq) factors(a.q_weight);
+  while (h < a.Hq) {
+    uint16_t *at = a.q_out + (t * a.Hq + h) * a.D + e;
+    turn(next(), a.q_weight != nullptr, y);
+    if (live) *(v4i *)at = placed ? pack8_bf16(y) : none;
+  }
+  if (h < a.Hq + a.Hkv) factors(a.k_weight);
+  while (h < a.Hq + a.Hkv) {
+    const int kh = h - a.Hq;
+    turn(next(), a.k_weight != nullptr, y);
     if (!live) continue;
-    if (kind == 0) {
-      *(v4i *)(a.q_out + (t * a.Hq + h) * a.D + e) = placed ? pack8_bf16(y) : (v4i){0, 0, 0, 0};
+    if (a.k_out) *(v4i *)(a.k_out + (t * a.Hkv + kh) * a.D + e) = placed ? pack8_bf16(y) : none;
+    if (!a.k_cache || !stored) continue;
+    uint8_t *at = place(a.k_cache, a.k_block_bytes, kh);
+    if (a.cache_fp8) *(v2i *)at = scaled_fp8(y, a.k_scale ? a.k_scale[kh] : 1.0f);
+    else *(v4i *)at = pack8_bf16(y);
+  }
+  while (h < heads) {
+    const int kh = h - a.Hq - a.Hkv;
+    const v4i now = next();
+    if (!live || !a.v_cache || !stored) continue;
+    uint8_t *at = place(a.v_cache, a.v_block_bytes, kh);
+    if (!a.cache_fp8) {
+      *(v4i *)at = now;
       continue;
     }
-    const int kh = kind == 1 ? h - a.Hq : h - a.Hq - a.Hkv;
-    if (a.k_out && kind == 1) *(v4i *)(a.k_out + (t * a.Hkv + kh) * a.D + e) = placed ? pack8_bf16(y) : (v4i){0, 0, 0, 0};
-    uint8_t *cache = kind == 1 ? a.k_cache : a.v_cache;
-    if (!cache || !stored) continue;
-    const int64_t block_bytes = kind == 1 ? a.k_block_bytes : a.v_block_bytes;
-    const int64_t within = ((slot & ((1 << a.page_log2) - 1)) * a.Hkv + kh) * (int64_t)a.D + e;
-    uint8_t *at = cache + (slot >> a.page_log2) * block_bytes + within * (a.cache_fp8 ? 1 : 2);
-    if (a.cache_fp8) {
-      const float *scale = kind == 1 ? a.k_scale : a.v_scale;
-      const float sc = scale ? scale[kh] : 1.0f;
 #pragma unroll
-      for (int i = 0; i < 8; i++) y[i] = y[i] / sc;
-      *(v2i *)at = pack8_fp8(y);
-    } else {
-      *(v4i *)at = kind == 1 ? pack8_bf16(y) : raw;
+    for (int i = 0; i < 4; i++) {
+      y[2 * i] = bf16_to_f32((uint16_t)((uint32_t)now[i] & 0xffff));
+      y[2 * i + 1] = bf16_to_f32((uint16_t)((uint32_t)now[i] >> 16));
     }
+    *(v2i *)at = scaled_fp8(y, a.v_scale ? a.v_scale[kh] : 1.0f);
   }
 }
 
@@ -187,7 +217,11 @@ extern "C" int moe_qk_norm_rope(void *stream, const void *qkv_bf16, int64_t row_
   RopeArgs a{(const uint16_t *)qkv_bf16, row_stride, positions, cos_sin, q_weight, k_weight, (uint16_t *)q_out_bf16, (uint16_t *)k_out_bf16,
              (uint8_t *)k_cache, (uint8_t *)v_cache, k_block_stride * wide, v_block_stride * wide,
              cached ? (int64_t)n_blocks * page_size : 0, cached ? slots : nullptr, k_scale, v_scale, eps, T, Hq, Hkv, D, R, P,
-             cached ? __builtin_ctz(page_size) : 0, weight_dtype == MOE_DTYPE_BF16, interleaved ? 1 : 0, wide == 1, 1, (int)heads};
+             cached ? __builtin_ctz(page_size) : 0, weight_dtype == MOE_DTYPE_BF16, interleaved ? 1 : 0, wide == 1, (int)heads};
+  // a group's heads: one while the chip is not full of groups, then as many as keep it so
+  const int64_t share = (int64_t)T * heads / 32768;
+  const int64_t most = share < 1 ? 1 : share > 10 ? 10 : share;
+  a.groups_per_token = (int)((heads + most - 1) / most);
   const int lph = D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32;
   const int64_t groups = (int64_t)T * a.groups_per_token, blocks = (groups + 256 / lph - 1) / (256 / lph);
   if (blocks > 0x7fffffff) return MOE_E_SHAPE;

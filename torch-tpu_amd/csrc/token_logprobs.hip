@@ -15,6 +15,7 @@
 #include <math.h>
 #include "moe_common.h"
 #include "moe_layout.h"
+#include "lanes.h"
 #include "../../include/moe_hip.h"
 
 namespace moe {
@@ -65,31 +66,10 @@ struct LpShared {
   int count;
 };
 
-// the value of lane ^ D, without a trip through LDS
-template <int D>
-__device__ __forceinline__ uint32_t lp_across(uint32_t v) {
-  typedef uint32_t v2u __attribute__((ext_vector_type(2)));
-  if (D == 1) return __builtin_amdgcn_update_dpp(v, v, 0xb1, 0xf, 0xf, false);         // quad_perm 1 0 3 2
-  if (D == 2) return __builtin_amdgcn_update_dpp(v, v, 0x4e, 0xf, 0xf, false);         // quad_perm 2 3 0 1
-  if (D == 4) {                                                                        // from 4 lanes up and down in a row
-    const uint32_t up = __builtin_amdgcn_update_dpp(v, v, 0x104, 0xf, 0x5, false);
-    return __builtin_amdgcn_update_dpp(up, v, 0x114, 0xf, 0xa, false);
-  }
-  if (D == 8) return __builtin_amdgcn_update_dpp(v, v, 0x128, 0xf, 0xf, false);        // row rotated by 8
-  const v2u r = D == 16 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
-  return (threadIdx.x & D) ? r[0] : r[1];
-}
-template <int D>
-__device__ __forceinline__ uint64_t lp_across(uint64_t v) {
-  return (uint64_t)lp_across<D>((uint32_t)(v >> 32)) << 32 | lp_across<D>((uint32_t)v);
-}
-template <int D>
-__device__ __forceinline__ float lp_across(float v) { return __uint_as_float(lp_across<D>(__float_as_uint(v))); }
-
 // a step of a sorting network: lanes D apart, the larger value to the lower lane where `down`
 template <int D>
 __device__ __forceinline__ uint64_t lp_step(uint64_t v, bool down) {
-  const uint64_t o = lp_across<D>(v);
+  const uint64_t o = lane_xor<D>(v);
   return (((threadIdx.x & D) == 0) == down) == (v > o) ? v : o;
 }
 template <int D>
@@ -131,19 +111,19 @@ __device__ __forceinline__ uint64_t lp_best64(LpShared &sh, int n) {
 __device__ __forceinline__ LpStats lp_block_stats(LpStats v, LpShared &sh, float c) {
   // first the largest, then everything in terms of it: one exponential a lane
   float m = v.m;
-  m = fmaxf(m, lp_across<1>(m));
-  m = fmaxf(m, lp_across<2>(m));
-  m = fmaxf(m, lp_across<4>(m));
-  m = fmaxf(m, lp_across<8>(m));
-  m = fmaxf(m, lp_across<16>(m));
-  m = fmaxf(m, lp_across<32>(m));
+  m = fmaxf(m, lane_xor<1>(m));
+  m = fmaxf(m, lane_xor<2>(m));
+  m = fmaxf(m, lane_xor<4>(m));
+  m = fmaxf(m, lane_xor<8>(m));
+  m = fmaxf(m, lane_xor<16>(m));
+  m = fmaxf(m, lane_xor<32>(m));
   v = lp_join(v, LpStats{m, 0.f, 0.f}, c);
-  v.s += lp_across<1>(v.s), v.w += lp_across<1>(v.w);
-  v.s += lp_across<2>(v.s), v.w += lp_across<2>(v.w);
-  v.s += lp_across<4>(v.s), v.w += lp_across<4>(v.w);
-  v.s += lp_across<8>(v.s), v.w += lp_across<8>(v.w);
-  v.s += lp_across<16>(v.s), v.w += lp_across<16>(v.w);
-  v.s += lp_across<32>(v.s), v.w += lp_across<32>(v.w);
+  v.s += lane_xor<1>(v.s), v.w += lane_xor<1>(v.w);
+  v.s += lane_xor<2>(v.s), v.w += lane_xor<2>(v.w);
+  v.s += lane_xor<4>(v.s), v.w += lane_xor<4>(v.w);
+  v.s += lane_xor<8>(v.s), v.w += lane_xor<8>(v.w);
+  v.s += lane_xor<16>(v.s), v.w += lane_xor<16>(v.w);
+  v.s += lane_xor<32>(v.s), v.w += lane_xor<32>(v.w);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) sh.stats[threadIdx.x >> 6] = v;
   __syncthreads();
