@@ -9,6 +9,7 @@
 #include <type_traits>
 #include "moe_common.h"
 #include "moe_layout.h"
+#include "lanes.h"
 #include "../../include/moe_hip.h"
 
 namespace moe {
@@ -82,13 +83,9 @@ __device__ __forceinline__ void attn_walk(const AttnArgs &a, Segment segment) {
     total += units;
     if (units > 0) longest = max(longest, (mine.kv + UNIT - 1) / UNIT);
   }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    total += __shfl_xor(total, d, 64);
-    longest = max(longest, __shfl_xor(longest, d, 64));
-  }
-  total = __builtin_amdgcn_readfirstlane(total);
-  longest = __builtin_amdgcn_readfirstlane(longest);
+  int upto = lane_sum_upto(total);                     // (with up to 64 requests: the line's length up to each)
+  total = __builtin_amdgcn_readlane(upto, 63);
+  longest = __builtin_amdgcn_readfirstlane(lane_max(longest));
   // An equal share for every workgroup, but of one long tile no more than pays: n units cut into stretches of x take x steps of a unit, then
   // a join of n / x parts, least at x = sqrt(n cut), cut the time of a part over that of a unit.  (One token over 32767 keys: 28, 23.5 and
   // 26 us with stretches of 2, 4 and 8 units; over 1000 keys 14.8 and 17.8 us with 2 and 4.)
@@ -106,12 +103,7 @@ __device__ __forceinline__ void attn_walk(const AttnArgs &a, Segment segment) {
       if (b0 + lane < a.B) mine = attn_request(a, b0 + lane);
       else mine.n = 0;
       units = attn_head_units<ROWS, UNIT>(a, mine) * a.Hkv;
-    }
-    int upto = units;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(upto, d, 64);
-      if (lane >= d) upto += o;
+      upto = lane_sum_upto(units);
     }
     const uint64_t past = __ballot(start < before + upto);
     if (past) {
@@ -244,7 +236,7 @@ struct AttnState {
 
 // The products' operands come from LDS some hundred cycles after they are asked for, a group of matrix instructions takes 32 to 64: operands
 // are asked for AHEAD groups before their use, and the order written here is kept (left to itself the compiler asks
-// and waits in turn; 64 keys of 32 rows then took 2.3 us, half of it such waits).
+// and waits in turn: 683 instead of 728 TFLOP/s with 2042 rows of a chunk over 8190 keys).
 __device__ __forceinline__ void in_this_order() { __builtin_amdgcn_sched_barrier(0); }
 __device__ __forceinline__ void made_here(v4f &x) { asm volatile("" : "+v"(x)); }      // (products are moved freely otherwise)
 
@@ -294,9 +286,12 @@ __device__ __forceinline__ void attn_scores(const uint8_t *at, const v8bf (&q)[N
 template <int NQ>
 struct AttnSight {
   uint64_t mask[NQ];                   // without masks: the last key seen
-  __device__ __forceinline__ bool sees(const AttnArgs &a, const AttnRequest &r, int qc, int key) const {
-    const int i = key - r.prefix;
-    return a.masks ? i < 0 || (key < r.kv && i < 64 && (mask[qc] >> (i & 63) & 1)) : key <= (int)mask[qc];
+  // bit k: query qc sees key first_key + k
+  __device__ __forceinline__ uint64_t from(const AttnArgs &a, const AttnRequest &r, int qc, int first_key) const {
+    const auto first = [](int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; };
+    if (!a.masks) return first((int)mask[qc] + 1 - first_key);
+    const int i = first_key - r.prefix;                // the first key's bit
+    return first(r.kv - first_key) & (i >= 64 ? 0ull : i >= 0 ? mask[qc] >> i : i > -64 ? mask[qc] << -i | first(-i) : ~0ull);
   }
 };
 
@@ -306,11 +301,13 @@ __device__ __forceinline__ void attn_hide(const AttnArgs &a, const AttnRequest &
                                           v4f (&s)[KT][NQ]) {
   const int g4 = 4 * ((threadIdx.x & 63) >> 4);
 #pragma unroll
-  for (int kt = 0; kt < KT; kt++)
+  for (int qc = 0; qc < NQ; qc++) {
+    const uint64_t seen = sight.from(a, r, qc, first_key) >> g4;
 #pragma unroll
-    for (int qc = 0; qc < NQ; qc++)
+    for (int kt = 0; kt < KT; kt++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) s[kt][qc][i] = sight.sees(a, r, qc, first_key + 16 * kt + g4 + i) ? s[kt][qc][i] * c : -INFINITY;
+      for (int i = 0; i < 4; i++) s[kt][qc][i] = seen >> (16 * kt + i) & 1 ? s[kt][qc][i] * c : -INFINITY;
+  }
 }
 
 // 16 bytes of the cache -> operands of 8 bf16: themselves, or two of e4m3 codes
@@ -348,7 +345,7 @@ __device__ __forceinline__ void attn_add_no_numbers(const AttnArgs &a, const Att
     const uint8_t *row = attn_row<DT * (FP8 ? 16 : 32)>(a, a.v_cache, a.v_block_bytes, attn_block(a, table, key), kh, key);
     bool sees[NQ];
 #pragma unroll
-    for (int qc = 0; qc < NQ; qc++) sees[qc] = sight.sees(a, r, qc, key);
+    for (int qc = 0; qc < NQ; qc++) sees[qc] = sight.from(a, r, qc, key) & 1;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
 #pragma unroll
@@ -363,14 +360,14 @@ __device__ __forceinline__ void attn_add_no_numbers(const AttnArgs &a, const Att
 }
 
 // a lane's queries as the scores' second operand: element j of step s is d = 32 s + 8 g + j, or with e4m3 keys, of which a lane reads
-// 16 at a time, d = 64 (s / 2) + 16 g + 8 (s % 2) + j
-template <int NQ, int D, bool FP8>
+// 16 at a time, d = 64 (s / 2) + 16 g + 8 (s % 2) + j.  Its 16s of rows lie STEP apart.
+template <int NQ, int D, bool FP8, int STEP = 16>
 __device__ __forceinline__ void attn_queries(const AttnArgs &a, const AttnRequest &r, int kh, int first_row, v8bf (&q)[NQ][D / 32],
                                              AttnSight<NQ> &sight) {
   const int lane = threadIdx.x & 63, g = lane >> 4;
 #pragma unroll
   for (int qc = 0; qc < NQ; qc++) {
-    const int row = min(first_row + 16 * qc + (lane & 15), r.n * a.G - 1), j = row / a.G, h = kh * a.G + row - j * a.G;
+    const int row = min(first_row + STEP * qc + (lane & 15), r.n * a.G - 1), j = row / a.G, h = kh * a.G + row - j * a.G;
     const uint16_t *src = a.q + (size_t)(r.t0 + j) * a.q_stride + (size_t)h * D;
 #pragma unroll
     for (int s = 0; s < D / 32; s++) q[qc][s] = *(const v8bf *)(src + (FP8 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g));
@@ -401,7 +398,8 @@ __device__ __forceinline__ void attn_store(const AttnArgs &a, const AttnRequest 
 }
 
 // ---- few rows: the four wavefronts take the keys in turn --------------------------------------------------------------
-// Up to 64 rows to a cached key the cache's bytes bound it.  A wavefront takes 32 keys of a unit of 128 by itself: keys go
+// Up to 16 rows to a cached key the cache's bytes bound it (64 requests, up to 8192 keys, bf16: 135 us, 4.9 TB/s, what a large copy reaches;
+// one request of 32767: 23.6 us, of which 14 are its bytes and the rest the chain of launch, lengths, tables, a tile's end and the join).  A wavefront takes 32 keys of a unit of 128 by itself: keys go
 // from memory straight into operand registers, values through LDS that no other wavefront touches, so nothing waits at a
 // barrier, and the next keys and values are asked for before the present ones are worked on.  The wavefronts' results meet in
 // LDS at the end of a tile.
@@ -578,13 +576,14 @@ __device__ __forceinline__ void attn_put_values(uint8_t *at, const v4i (&raw)[NU
 
 // ---- more rows: the wavefronts take the rows, and share the keys ---------------------------------------------------------
 // Up to about 128 rows to a cached key both the bytes and the products count.  A workgroup stages 64 keys and values at a time in
-// LDS, two stages of them, and every wavefront takes its rows past all of them, one barrier a stage.  The bytes of the stages after
-// that wait in registers, of two stages where there are enough (a stage takes less time than the way to memory).
+// LDS, two stages of them, and every wavefront takes its 16s of rows (in turn, so that a tile that is not full keeps all at work) past all of them, one barrier a stage.  The bytes of the stage after
+// that wait in registers (of two stages after it: no faster).  32 trees of up to 16 tokens over up to 8001 e4m3 keys: 71 us, 2.35 TB/s and
+// 354 TFLOP/s; without the work on the stages 54, without the stages 56: two workgroups to a compute unit overlap the two in part, and
+// LDS and registers hold no third.
 template <int D, bool FP8, int NQ>
 __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const AttnArgs a) {
   constexpr int ROWS = 64 * NQ, UNIT = 64, DT = D / 16, LD = 2 * D + 32, STAGE = 2 * UNIT * LD;
   constexpr int BYTES = FP8 ? D : 2 * D, TPR = 4, NU = BYTES / (16 * TPR);           // a row's threads; a thread's 16-byte pieces of its row
-  constexpr int SETS = NQ == 1 ? 2 : 1;
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
   __shared__ int any_odd;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c16 = lane & 15;
@@ -595,84 +594,84 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const AttnArgs a) {
     const int last = c1 - 1;
     const int stage_row = attn_stage_row<FP8, TPR>(tid / TPR), piece = tid % TPR;
     uint8_t *const stage_at = lds + stage_row * LD + (FP8 ? 32 : 16) * piece;
-    v4i kr[SETS][NU], vr[SETS][NU];
+    v4i kr[NU], vr[NU];
     int block;                                         // of the unit that is asked for next
     const auto key_of = [&](int unit) { return min(min(unit, last) * UNIT + stage_row, r.kv - 1); };
-    const auto ask = [&](int unit, v4i (&k)[NU], v4i (&v)[NU]) {
+    const auto ask = [&](int unit) {
       const uint8_t *ka = attn_row<BYTES>(a, a.k_cache, a.k_block_bytes, block, kh, key_of(unit)) + 16 * piece;
       const uint8_t *va = attn_row<BYTES>(a, a.v_cache, a.v_block_bytes, block, kh, key_of(unit)) + 16 * piece;
 #pragma unroll
       for (int u = 0; u < NU; u++) {
-        k[u] = *(const v4i *)(ka + 16 * TPR * u);
-        v[u] = *(const v4i *)(va + 16 * TPR * u);
+        kr[u] = *(const v4i *)(ka + 16 * TPR * u);
+        vr[u] = *(const v4i *)(va + 16 * TPR * u);
       }
       block = attn_block(a, table, key_of(unit + 1));
     };
-    const auto put = [&](int unit, const v4i (&k)[NU], const v4i (&v)[NU]) {
-      attn_put<FP8, TPR, NU>(stage_at + (unit & 1) * STAGE, k);
-      attn_put_values<FP8, TPR, NU>(stage_at + (unit & 1) * STAGE + UNIT * LD, v, (unit + 1) * UNIT > clear,
+    const auto put = [&](int unit) {
+      attn_put<FP8, TPR, NU>(stage_at + (unit & 1) * STAGE, kr);
+      attn_put_values<FP8, TPR, NU>(stage_at + (unit & 1) * STAGE + UNIT * LD, vr, (unit + 1) * UNIT > clear,
                                     unit * UNIT + stage_row < r.kv, &any_odd);
     };
     if (tid == 0) any_odd = 0;
     block = attn_block(a, table, key_of(c0));
-    ask(c0, kr[0], vr[0]);
-    if (SETS == 2) ask(c0 + 1, kr[SETS - 1], vr[SETS - 1]);
-    __syncthreads();
-    put(c0, kr[0], vr[0]);
-    ask(c0 + SETS, kr[0], vr[0]);
-    __syncthreads();
-    // a stage: `work` on it, the next one's bytes from registers to LDS, the one's after those asked for
-    const auto stages = [&](auto work) {
-      const auto step = [&](int c, v4i (&k)[NU], v4i (&v)[NU]) {
-        work(c, lds + (c & 1) * STAGE);
-        put(c + 1, k, v);
-        ask(c + 1 + SETS, k, v);
-        __syncthreads();
-      };
-      if (SETS == 1) {
-        for (int c = c0; c < c1; c++) step(c, kr[0], vr[0]);
-      } else {
-        for (int c = c0; c < c1; c += 2) {
-          step(c, kr[SETS - 1], vr[SETS - 1]);
-          if (c + 1 < c1) step(c + 1, kr[0], vr[0]);
-        }
-      }
+    const auto begin = [&] {
+      ask(c0);
+      __syncthreads();
+      put(c0);
+      ask(c0 + 1);
+      __syncthreads();
     };
-    if (m_tile * ROWS + 16 * NQ * w < r.n * a.G) {
-      v8bf q[NQ][D / 32];
-      AttnSight<NQ> sight;
-      attn_queries<NQ, D, false>(a, r, kh, m_tile * ROWS + 16 * NQ * w, q, sight);
-      AttnState<NQ, DT> st;
+    // the next stage's bytes from registers to LDS, the one's after those asked for
+    const auto end_stage = [&](int c) {
+      put(c + 1);
+      ask(c + 2);
+      __syncthreads();
+    };
+    const auto take = [&](auto sixteens) {
+      constexpr int N = decltype(sixteens)::value, AHEAD = N == 2 && !FP8 ? 2 : 3;     // (as the registers allow)
+      v8bf q[N][D / 32];
+      AttnSight<N> sight;
+      attn_queries<N, D, false, 64>(a, r, kh, m_tile * ROWS + 16 * w, q, sight);
+      AttnState<N, DT> st;
       st.clear();
-      stages([&](int c, const uint8_t *stage) {
+      begin();
+      for (int c = c0; c < c1; c++) {
+        const uint8_t *stage = lds + (c & 1) * STAGE;
         const bool edge = (c + 1) * UNIT > clear;
-        v4f s[4][NQ];
-        attn_scores<3, 4, LD>(stage + c16 * LD + 16 * g, q, s);
+        v4f s[4][N];
+        attn_scores<AHEAD, 4, LD>(stage + c16 * LD + 16 * g, q, s);
         const uint8_t *read_at = stage + UNIT * LD + (4 * g + c16 / 4) * LD + 8 * (c16 % 4);
-        v8bf p[2][NQ], va[2 * DT];
+        v8bf p[2][N], va[2 * DT];
 #pragma unroll
-        for (int i = 0; i < 3; i++) va[i] = attn_values<LD>(read_at, i);
+        for (int i = 0; i < AHEAD; i++) va[i] = attn_values<LD>(read_at, i);
         float scl = scale;
         if (__builtin_expect(edge, 0)) {
           attn_hide(a, r, sight, c * UNIT, scale, s);
           scl = 1.f;
         }
         st.template softmax<4>(s, scl, edge || c == c0, p);
-        attn_add_values<3, 2, LD>(st, read_at, p, va);
-      });
+        attn_add_values<AHEAD, 2, LD>(st, read_at, p, va);
+        end_stage(c);
+      }
       if (__builtin_expect(any_odd, 0)) {
         const int from = max(c0, clear / UNIT) * UNIT;          // the first unit whose values were looked at
-        attn_add_no_numbers<NQ, DT, FP8>(a, r, sight, table, kh, from, c1 * UNIT - from, st);
+        attn_add_no_numbers<N, DT, FP8>(a, r, sight, table, kh, from, c1 * UNIT - from, st);
       }
 #pragma unroll
-      for (int qc = 0; qc < NQ; qc++) {
+      for (int qc = 0; qc < N; qc++) {
         const float l = over_groups(st.l[qc], true);
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
-          attn_store<ROWS, D>(a, r, kh, m_tile, 16 * NQ * w + 16 * qc + c16, 16 * dt + 4 * g, whole, part, st.o[dt][qc], st.m[qc], l);
+          attn_store<ROWS, D>(a, r, kh, m_tile, 16 * w + 64 * qc + c16, 16 * dt + 4 * g, whole, part, st.o[dt][qc], st.m[qc], l);
       }
-    } else {                                           // a wavefront without rows only helps with the bytes
-      stages([](int, const uint8_t *) {});
+    };
+    // the tile's 16s of rows go to the wavefronts in turn, so that a tile that is not full still keeps all of them at work
+    const int rows = r.n * a.G - m_tile * ROWS - 16 * w;
+    if (NQ == 2 && rows > 64) take(std::integral_constant<int, NQ>());
+    else if (rows > 0) take(std::integral_constant<int, 1>());
+    else {                                             // a wavefront without rows only helps with the bytes
+      begin();
+      for (int c = c0; c < c1; c++) end_stage(c);
     }
     __syncthreads();
   });
@@ -730,24 +729,28 @@ __global__ __launch_bounds__(512, 2) void attn_pairs_kernel(const AttnArgs a) {
 
     if (tid == 0) any_odd = 0;
     block = attn_block(a, table, key_of(c0));
-    ask(a.k_cache, a.k_block_bytes, block, c0, kr);
-    ask(a.v_cache, a.v_block_bytes, block, c0, vr);
-    block = block_v = attn_block(a, table, key_of(c0 + 1));
-    put_keys(c0);
-    ask(a.k_cache, a.k_block_bytes, block, c0 + 1, kr);
-    block = attn_block(a, table, key_of(c0 + 2));
-    __syncthreads();
-    if (late) {                                        // slot 0
-      stage(c0);
+    const auto begin = [&] {
+      ask(a.k_cache, a.k_block_bytes, block, c0, kr);
+      ask(a.v_cache, a.v_block_bytes, block, c0, vr);
+      block = block_v = attn_block(a, table, key_of(c0 + 1));
+      put_keys(c0);
+      ask(a.k_cache, a.k_block_bytes, block, c0 + 1, kr);
+      block = attn_block(a, table, key_of(c0 + 2));
       __syncthreads();
-    }
-    if (m_tile * ROWS + 16 * NQ * w < r.n * a.G) {
-      v8bf q[NQ][X];
-      AttnSight<NQ> sight;
-      attn_queries<NQ, D, false>(a, r, kh, m_tile * ROWS + 16 * NQ * w, q, sight);
-      AttnState<NQ, DT> st;
+      if (late) {                                        // slot 0
+        stage(c0);
+        __syncthreads();
+      }
+    };
+    const auto take = [&](auto sixteens) {
+      constexpr int N = decltype(sixteens)::value;
+      v8bf q[N][X];
+      AttnSight<N> sight;
+      attn_queries<N, D, false, 128>(a, r, kh, m_tile * ROWS + 16 * w, q, sight);
+      AttnState<N, DT> st;
       st.clear();
-      v4f s[4][NQ];
+      begin();
+      v4f s[4][N];
       attn_scores<4, 4, LD>(lds + (c0 & 1) * HALF + c16 * LD + 16 * g, q, s);
       __syncthreads();
       for (int c = c0; c < c1; c++) {
@@ -758,7 +761,7 @@ __global__ __launch_bounds__(512, 2) void attn_pairs_kernel(const AttnArgs a) {
           attn_hide(a, r, sight, c * UNIT, scale, s);
           scl = 1.f;
         }
-        v8bf p[2][NQ], v[2 * DT];
+        v8bf p[2][N], v[2 * DT];
         st.template softmax<4>(s, scl, edge || c == c0, p);
         __syncthreads();
         attn_scores<4, 4, LD>(lds + ((c + 1) & 1) * HALF + c16 * LD + 16 * g, q, s);       // (past the last unit: of no use)
@@ -771,16 +774,21 @@ __global__ __launch_bounds__(512, 2) void attn_pairs_kernel(const AttnArgs a) {
       if (!late) __syncthreads();
       if (__builtin_expect(any_odd, 0)) {
         const int from = max(c0, clear / UNIT) * UNIT;          // the first unit whose values were looked at
-        attn_add_no_numbers<NQ, DT, FP8>(a, r, sight, table, kh, from, c1 * UNIT - from, st);
+        attn_add_no_numbers<N, DT, FP8>(a, r, sight, table, kh, from, c1 * UNIT - from, st);
       }
 #pragma unroll
-      for (int qc = 0; qc < NQ; qc++) {
+      for (int qc = 0; qc < N; qc++) {
         const float l = over_groups(st.l[qc], true);
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
-          attn_store<ROWS, D>(a, r, kh, m_tile, 16 * NQ * w + 16 * qc + c16, 16 * dt + 4 * g, whole, part, st.o[dt][qc], st.m[qc], l);
+          attn_store<ROWS, D>(a, r, kh, m_tile, 16 * w + 128 * qc + c16, 16 * dt + 4 * g, whole, part, st.o[dt][qc], st.m[qc], l);
       }
-    } else {                                           // a wavefront without rows only helps with the bytes
+    };
+    const int rows = r.n * a.G - m_tile * ROWS - 16 * w;           // the 16s of rows in turn, as above
+    if (rows > 128) take(std::integral_constant<int, NQ>());
+    else if (rows > 0) take(std::integral_constant<int, 1>());
+    else {                                             // a wavefront without rows only helps with the bytes
+      begin();
       __syncthreads();
       for (int c = c0; c < c1; c++) {
         stage(c + late);
@@ -826,15 +834,31 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
   float m = -INFINITY, l = 0.f;
   v4f o = (v4f){0.f, 0.f, 0.f, 0.f};
   if (row < r.n * a.G) {
-#pragma unroll 8
-    for (int w = w0 + split; w <= w1; w += SPLIT) {
-      const size_t at = part(w);
-      const float pm = a.part_ml[at * 2], pl = a.part_ml[at * 2 + 1], top = fmaxf(m, pm);
-      const v4f po = *(const v4f *)(a.part_o + at * D + d);
-      const float fo = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top), fp = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(pm - top);
-      m = top;
-      l = l * fo + pl * fp;
-      o = o * fo + po * fp;
+    for (int first = w0 + split; first <= w1; first += 4 * SPLIT) {      // four parts asked for at a time (eight: slower where there are four)
+      float pm[4], pl[4];
+      v4f po[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const size_t at = part(min(first + i * SPLIT, w1));
+        pm[i] = a.part_ml[at * 2], pl[i] = a.part_ml[at * 2 + 1];
+        po[i] = *(const v4f *)(a.part_o + at * D + d);
+      }
+      const float before = m;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if (first + i * SPLIT > w1) pm[i] = -INFINITY, pl[i] = 0.f, po[i] = (v4f){0.f, 0.f, 0.f, 0.f};
+        m = fmaxf(m, pm[i]);
+      }
+      const float top = m == -INFINITY ? 0.f : m;      // (nothing seen so far: weights of 0, not of -inf + inf)
+      const float f = __builtin_amdgcn_exp2f(before - top);
+      l *= f;
+      o *= f;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float w = __builtin_amdgcn_exp2f(pm[i] - top);
+        l += pl[i] * w;
+        o += po[i] * w;
+      }
     }
   }
   if (SPLIT > 1) {
@@ -858,15 +882,33 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
 }
 
 // ---- which kernel -------------------------------------------------------------------------------------------------------
-// By the rows to a cached key that a request has on average.
+// By the rows to a cached key that a request has on average, and by whether there is work for large tiles at all.  Measured, in us, 4 cache
+// heads of 128, bf16 (e4m3); B requests of n tokens, 8 query heads a cache head, L keys:
+//   rows  B x n x L            16 rows    64           128          256
+//   8     64 x 1 x 8192        135 (81)
+//   24    64 x 3 x 8192        134 (73)   123 (70)     126 (78)                     (16: with two 16s of rows a wavefront)
+//   48    64 x 6 x 8192                   127 (76)     130 (92)     126 (110)
+//   96    32 x 12 x 8192                  141 (116)    139 (104)    133 (117)
+//   192   16 x 24 x 8192                  164          106          95
+//   512   16 x 64 x 8192                  221          176          162
+//   512   4 x 64 x 2048                   38 (39)      55 (54)      54 (55)
+//   512   1 x 64 x 8192                   42 (43)      85 (85)      54 (55)
+//   512   16 x 64 x 512                   29           37           37
+//   512   4 x 64 x 8192                   70 (73)      78 (79)      74 (75)
+//   2048  4 x 256 x 512, causal           54           42           43
+//   400   1 x 400 x 2048, causal, no shared heads
+//                                         29           33           37
+// Large tiles read a key for more rows, small ones are more stretches at work and fewer, smaller parts to join.  Up to so many products of
+// row and key (with the table's width, as the lengths are on the device) the latter counts.  16 rows: two workgroups to a compute unit
+// for e4m3, whose loads are half as long (256 requests of 2048 keys: 90 us with 512 workgroups, 105 with 256; bf16 146 and 141).
 struct AttnPlan {
   int rows, groups;                    // rows of a tile; workgroups, a multiple of 8
   float cut;
 };
-static AttnPlan attn_plan(int T, int Hq, int Hkv, int B, int cache_dtype) {
+static AttnPlan attn_plan(int T, int Hq, int Hkv, int B, int cache_dtype, bool trees, int64_t keys) {
   const int64_t rows = B > 0 ? ((int64_t)T * (Hq / Hkv) + B - 1) / B : 1;
   if (rows <= 16) return {16, cache_dtype == MOE_DTYPE_FP8 ? 512 : 256, 0.0625f};
-  if (rows <= 64) return {64, 512, 0.125f};
+  if (rows <= 64 || (int64_t)T * Hq <= (trees ? 20000000 : 8000000) / (keys > 0 ? keys : 1)) return {64, 512, 0.125f};
   if (rows <= 128) return {128, 512, 0.125f};
   return {256, 256, 0.25f};
 }
@@ -876,7 +918,7 @@ static AttnPlan attn_plan(int T, int Hq, int Hkv, int B, int cache_dtype) {
 extern "C" size_t moe_tree_attention_workspace_bytes(int T, int Hq, int Hkv, int D, int B, int cache_dtype) {
   using namespace moe;
   if (T < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || D < 1 || B < 0 || (cache_dtype != MOE_DTYPE_BF16 && cache_dtype != MOE_DTYPE_FP8)) return 0;
-  const AttnPlan plan = attn_plan(T, Hq, Hkv, B, cache_dtype);
+  const AttnPlan plan = attn_plan(T, Hq, Hkv, B, cache_dtype, false, 1ll << 31);      // (shorter caches need no more)
   const size_t rows = plan.rows, parts = 2 * plan.groups;
   return align_up(parts * rows * D * 4, 256) + align_up(parts * rows * 8, 256) + plan.groups * 32;
 }
@@ -905,7 +947,7 @@ extern "C" int moe_tree_attention(void *stream, const void *q_bf16, int64_t q_st
   if ((uintptr_t)workspace % 256) return MOE_E_ALIGN;
   if (workspace_bytes < moe_tree_attention_workspace_bytes(T, Hq, Hkv, D, B, cache_dtype)) return MOE_E_WORKSPACE;
   const int fp8 = cache_dtype == MOE_DTYPE_FP8, wide = fp8 ? 1 : 2;
-  const AttnPlan plan = attn_plan(T, Hq, Hkv, B, cache_dtype);
+  const AttnPlan plan = attn_plan(T, Hq, Hkv, B, cache_dtype, masks != nullptr, (int64_t)table_width * page_size);
   // the line's length at most, in units
   if (((int64_t)T * (Hq / Hkv) / plan.rows + B) * Hkv * (((int64_t)table_width * page_size + 63) / 64) >= (1ll << 31)) return MOE_E_SHAPE;
   const size_t parts = 2 * plan.groups;
