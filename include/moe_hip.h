@@ -404,7 +404,8 @@ int moe_router_logits(void *stream, const void *x_bf16, int T, int H, const void
  * fit its table row or the batch's T rows, when a tree has more than 64 tokens, or when the pages needed by it and the requests before it are more than
  * there are; the others are granted.  Outputs: cu_tokens [B + 1]; positions [T] int32 (a tree's token: cached
  * length + depth); slots [T]; masks [T] with parents (without: causal order, masks not written); kv_lens [B] = lens +
- * counts.  Rows of no request get -1 / -1 / 0.  B <= MOE_MAX_REQUESTS.
+ * counts.  Rows of no request get -1 / -1 / 0.  B <= MOE_MAX_REQUESTS.  A caller that keeps fewer tokens than it brought puts the pages
+ * that its lens no longer reach back on the stack.
  */
 int moe_cache_plan(void *stream, int32_t *block_tables, int64_t table_stride, int B, int table_width, const int32_t *lens,
                    const int32_t *counts, const int32_t *free_blocks, int n_free_max, const int32_t *n_free, int page_size,

@@ -61,3 +61,54 @@ def test_the_command_runs(example, monkeypatch, capsys):
     monkeypatch.setattr("sys.argv", ["tree_decode.py", "--requests", "2", "--steps", "4", "--cache", "fp8"])
     example.main()
     assert capsys.readouterr().out.count("mean log probability") == 2
+
+
+def test_a_captured_step_replays_as_it_runs(pkg, example):
+    """Plan, projections, rotation, attention, MoE layers and log probabilities in one graph: new lengths and tokens go in by copies."""
+    print("captured step", flush=True)
+    g = torch.Generator().manual_seed(8)
+    model = example.Decoder(seed=2)
+    B, n = 3, 5
+    cache = example.Cache(model, B)
+    example.prefill(model, cache, [torch.randint(model.vocab, (k,), generator=g).tolist() for k in (40, 3, 17)])
+    full, tables = cache.lens.clone(), cache.tables.clone()
+    text = [(k.clone(), v.clone()) for k, v in cache.layers]
+    counts = torch.full((B,), n, dtype=torch.int32, device="cuda:0")
+    tokens = torch.zeros(B * n, dtype=torch.int64, device="cuda:0")
+    parents = torch.zeros(B * n, dtype=torch.int32, device="cuda:0")
+
+    def step():
+        plan = pkg.cache_plan(cache.tables, cache.lens, counts, cache.free, cache.n_free, cache.page, B * n, parents)
+        logits = model.forward(tokens, plan, cache)
+        return [x for x in plan] + list(pkg.token_logprobs(logits, tokens, top_k=3))
+
+    inputs = [(full - k, torch.randint(model.vocab, (B * n,), generator=g), torch.tensor(tree * B, dtype=torch.int32))
+              for k, tree in ((0, [-1, 0, 0, 1, 1]), (1, [-1, 0, 1, 2, 3]), (2, [-1, -1, 0, 0, 3]))]
+
+    def put(lens, some, above):
+        cache.lens.copy_(lens)
+        tokens.copy_(some)
+        parents.copy_(above)
+        cache.tables.copy_(tables)
+        for (k, v), (k0, v0) in zip(cache.layers, text):
+            k.copy_(k0)
+            v.copy_(v0)
+
+    want = []
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for x in inputs:
+            put(*x)
+            want.append([y.clone() for y in step()])
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    put(*inputs[0])
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in (1, 0, 2, 2, 1):
+        put(*inputs[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        for k, (x, y) in enumerate(zip(got, want[i])):
+            assert torch.equal(x, y), (i, k)
