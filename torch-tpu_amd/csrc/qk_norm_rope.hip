@@ -220,9 +220,10 @@ extern "C" int moe_qk_norm_rope(void *stream, const void *qkv_bf16, int64_t row_
              (uint8_t *)k_cache, (uint8_t *)v_cache, k_block_stride * wide, v_block_stride * wide,
              cached ? (int64_t)n_blocks * page_size : 0, cached ? slots : nullptr, k_scale, v_scale, eps, T, Hq, Hkv, D, R, P,
              cached ? __builtin_ctz(page_size) : 0, weight_dtype == MOE_DTYPE_BF16, interleaved ? 1 : 0, wide == 1, (int)heads};
-  // A group's heads: one while the chip is not full of groups, then as many as leave 8192 of them (2500 tokens of 40 heads, e4m3: 15.4 us, 18.1
-  // with 32768 groups; 6000 tokens, bf16: 26 and 31), at most 10 (16384 tokens: 5, 10, 20 heads take 80, 72, 75 to 81).
-  const int64_t share = (int64_t)T * heads / 8192;
+  // A group's heads: one while the chip is not full of groups, then as many as leave 16384 of them (6000 tokens of 40 heads: 26 us, 31 with
+  // 32768; 2500 into an e4m3 cache 16.6 and 18.1, 15.6 with 8192, which takes 613 tokens of 64-element heads from 4.8 to 6.1), at most 10 (16384
+  // tokens: 5, 10, 20 heads take 80, 72, 75 to 81).
+  const int64_t share = (int64_t)T * heads / 16384;
   const int64_t most = share < 1 ? 1 : share > 10 ? 10 : share;
   a.groups_per_token = (int)((heads + most - 1) / most);
   const int lph = D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32;
