@@ -439,6 +439,9 @@ int moe_qk_norm_rope(void *stream, const void *qkv_bf16, int64_t row_stride, int
  * workspace: moe_tree_attention_workspace_bytes(...) bytes, 256-byte aligned.
  */
 size_t moe_tree_attention_workspace_bytes(int T, int Hq, int Hkv, int D, int B, int cache_dtype);
+/* Rows (a token and one of a cache head's query heads) of a tile of the kernel that such a call runs: 16, 64, 128 or 256; 0 for a shape
+ * that moe_tree_attention refuses.  trees: masks are given. */
+int moe_tree_attention_tile_rows(int T, int Hq, int Hkv, int B, int cache_dtype, int trees, int table_width, int page_size);
 int moe_tree_attention(void *stream, const void *q_bf16, int64_t q_stride, int T, int Hq, int Hkv, int D, const void *k_cache,
                        const void *v_cache, int cache_dtype, int n_blocks, int64_t k_block_stride, int64_t v_block_stride,
                        int page_size, const int32_t *block_tables, int64_t table_stride, int table_width, const int32_t *kv_lens,

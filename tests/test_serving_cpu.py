@@ -155,3 +155,18 @@ def test_no_kernel_spills(source, tmp_path):
     assert sizes, "no kernel found"
     spills = {n: b for n, b in sizes.items() if b}
     assert not spills, f"kernels spill to scratch: {spills}"
+
+
+@pytest.mark.parametrize("T,Hq,Hkv,B,trees,room,rows", [
+    (64, 32, 4, 64, False, 8192, 16), (128, 32, 4, 64, True, 8192, 16), (64, 32, 32, 1, True, 131072, 64), (384, 32, 4, 64, True, 8192, 64),
+    (768, 32, 4, 64, True, 32768, 128), (512, 32, 4, 32, True, 32768, 128), (512, 32, 4, 32, True, 1024, 64), (1024, 32, 4, 16, True, 32768, 256),
+    (2042, 32, 8, 2, False, 8192, 256), (200, 32, 8, 2, False, 1024, 64), (0, 4, 2, 0, False, 0, 16)])
+def test_tile_rows_by_rows_and_room(pkg, T, Hq, Hkv, B, trees, room, rows):
+    for dtype in (1, 2):
+        assert lib().moe_tree_attention_tile_rows(T, Hq, Hkv, B, dtype, trees, room // 16, 16) == rows
+
+
+def test_tile_rows_of_refused_shapes(pkg):
+    for bad in ((-1, 4, 2, 1, 1, 0, 4, 16), (1, 4, 3, 1, 1, 0, 4, 16), (1, 0, 1, 1, 1, 0, 4, 16), (1, 4, 2, 4097, 1, 0, 4, 16), (1, 4, 2, 1, 0, 0, 4, 16),
+                (1, 4, 2, 1, 1, 0, -1, 16), (1, 4, 2, 1, 1, 0, 4, 24), (1, 4, 2, 1, 1, 0, 4, 2048)):
+        assert lib().moe_tree_attention_tile_rows(*bad) == 0, bad

@@ -72,6 +72,7 @@ SIGNATURES = {
                                  c_void_p, c_void_p, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int64,
                                  c_int64, c_int, c_void_p, c_void_p, c_void_p]),
     "moe_tree_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    "moe_tree_attention_tile_rows": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "moe_tree_attention": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int64,
                                    c_int64, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int, c_void_p, c_float, c_void_p,
                                    c_void_p, c_void_p, c_void_p, c_void_p, c_size_t]),

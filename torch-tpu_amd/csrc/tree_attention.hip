@@ -927,6 +927,14 @@ extern "C" size_t moe_tree_attention_workspace_bytes(int T, int Hq, int Hkv, int
   return align_up(parts * rows * D * 4, 256) + align_up(parts * rows * 8, 256) + plan.groups * 32;
 }
 
+extern "C" int moe_tree_attention_tile_rows(int T, int Hq, int Hkv, int B, int cache_dtype, int trees, int table_width, int page_size) {
+  using namespace moe;
+  if (T < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || B < 0 || B > MOE_MAX_REQUESTS || (cache_dtype != MOE_DTYPE_BF16 && cache_dtype != MOE_DTYPE_FP8) ||
+      table_width < 0 || page_size < 1 || page_size > MOE_MAX_PAGE || (page_size & (page_size - 1)))
+    return 0;
+  return attn_plan(T, Hq, Hkv, B, cache_dtype, trees != 0, (int64_t)table_width * page_size).rows;
+}
+
 extern "C" int moe_tree_attention(void *stream, const void *q_bf16, int64_t q_stride, int T, int Hq, int Hkv, int D,
                                   const void *k_cache, const void *v_cache, int cache_dtype, int n_blocks, int64_t k_block_stride,
                                   int64_t v_block_stride, int page_size, const int32_t *block_tables, int64_t table_stride,
