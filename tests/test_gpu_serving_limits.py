@@ -1,0 +1,80 @@
+"""The serving step's operators at the limits of what they accept."""
+import pytest
+import torch
+
+import serving_plain as plain
+from test_gpu_serving import say
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------ token_logprobs
+def log_probabilities(x, tokens, k, temperature):
+    """float64, distances from the maximum first, so that nothing cancels -> (logprobs, entropy, top_logprobs, top_ids)."""
+    x = x.double()
+    d = (x - x.amax(-1, keepdim=True)) / temperature
+    e = d.exp()
+    s = e.sum(-1, keepdim=True)
+    lp = d - s.log()
+    entropy = s.log()[:, 0] - (e * d.clamp(min=-1000)).sum(-1) / s[:, 0]
+    ids = x.sort(dim=-1, descending=True, stable=True).indices[:, :k]
+    return lp.gather(1, tokens[:, None])[:, 0], entropy, lp.gather(1, ids), ids
+
+
+def check_sharp(pkg, dev, x, k, temperature, tokens):
+    """A logarithm is off by roundings of its own size, and by those of the sum it comes from: V / 256 + 32 additions one after the other,
+    and exponentials of up to -30 (smaller ones add nothing) whose exponents went through four roundings.  None of it grows with the logits."""
+    say("token_logprobs", tuple(x.shape), x.dtype, "temperature", temperature)
+    said = pkg.token_logprobs(x.to(dev), tokens.to(dev), top_k=k, temperature=temperature)
+    lp, ent, tops, ids = log_probabilities(x, tokens, k, temperature)
+    sums = (x.shape[1] / 256 + 32 + 30 * 4) * plain.U32
+
+    def close(got, want, most):
+        got = got.double().cpu()
+        beyond = want.abs() > 3.3e38                     # more than float32 holds
+        assert bool((got[beyond] < -3.3e38).all())
+        worst = ((got - want).abs() / most)[~beyond]
+        assert worst.numel() == 0 or float(worst.max()) <= 1, f"{float(worst.max())} of the bound"
+    assert said.top_ids.cpu().tolist() == ids.tolist()
+    close(said.logprobs, lp, sums + 8 * plain.U32 * lp.abs())
+    close(said.top_logprobs, tops, sums + 8 * plain.U32 * tops.abs())
+    close(said.entropy, ent, sums * (1 + 2 * ent))
+    assert bool((said.logprobs <= sums).all()) and bool((said.top_logprobs <= sums).all())
+
+
+SHAPES = [(3, 5000), (2, 131072), (1100, 517)]           # in segments, in one piece; short rows
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("T,V", SHAPES)
+@pytest.mark.parametrize("temperature", [1e-3, 1e-5, 1e-6, 1e-8, 1e-20, 1e-29])
+def test_logprobs_at_small_temperatures(pkg, dev, temperature, T, V, bf16):
+    """One token dominates, or several equal ones do, in different threads and segments."""
+    g = torch.Generator().manual_seed(V)
+    x = (10 + 18 * torch.rand(T, V, generator=g)).to(torch.bfloat16 if bf16 else torch.float32)
+    x[0, V // 3] = 29.7
+    x[1, 0] = x[1, 300] = x[1, V // 2 + 1] = x[1, V - 1] = 29.3
+    tokens = torch.randint(0, V, (T,), generator=g)
+    tokens[0], tokens[1] = V // 3, V - 1
+    check_sharp(pkg, dev, x, 5, temperature, tokens)
+
+
+@pytest.mark.parametrize("T,V", SHAPES)
+@pytest.mark.parametrize("far", [300.0, 1e4, -1e4, 1e6])
+def test_logprobs_of_logits_far_from_zero(pkg, dev, far, T, V):
+    g = torch.Generator().manual_seed(V)
+    x = far + torch.randn(T, V, generator=g)
+    check_sharp(pkg, dev, x, 5, 1.0, torch.randint(0, V, (T,), generator=g))
+
+
+@pytest.mark.parametrize("T,V", SHAPES)
+@pytest.mark.parametrize("temperature", [1.0, 2.0])
+def test_logprobs_of_the_largest_logits(pkg, dev, temperature, T, V):
+    """Tokens forced by the type's highest value."""
+    x = torch.randn(T, V, generator=torch.Generator().manual_seed(V)).to(torch.bfloat16)
+    top = torch.finfo(torch.bfloat16).max
+    x[0, V // 3] = top
+    x[1, 1] = x[1, 400] = x[1, V - 1] = top
+    x[1, 2:100] = 1e38
+    x[2 % T] = top
+    check_sharp(pkg, dev, x, 5, temperature, torch.full((T,), V - 1))

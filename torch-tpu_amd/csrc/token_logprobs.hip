@@ -60,6 +60,13 @@ __device__ __forceinline__ LpStats lp_join(const LpStats a, const LpStats b, flo
   return {m, a.s * fa + b.s * fb, fa * (a.w + da * a.s) + fb * (b.w + db * b.s)};
 }
 
+// Exponents t = (x - m) c cost one instruction as fma(x, c, -off), off = m c rounded: they are then all off by the same shift, m c - off, which
+// an fma gives exactly and which goes out of the sums when m changes and at the end.  Where m c is so large that the shift is not
+// small (a low temperature, a mask of the type's lowest value) the difference comes first, and there is no shift.
+constexpr float kLpFar = 65536.f;                      // (a shift of 2^-9 at the most)
+__device__ __forceinline__ bool lp_near(float m, float c) { return fabsf(m * c) < kLpFar; }
+__device__ __forceinline__ float lp_shift(float m, float c) { return lp_near(m, c) ? fmaf(m, c, -(m * c)) : 0.f; }
+
 struct LpShared {
   LpStats stats[kLpThreads / 64];
   uint64_t best[kLpThreads];
@@ -289,18 +296,18 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(const LpArgs
     for (int i = 1; i + 1 < N; i += 2) most = fmaxf(fmaxf(most, x[i]), x[i + 1]);
     most = fmaxf(most, x[N - 1]);
     if (most > st.m) {
-      const float d = st.m == -INFINITY ? -1e4f : fmaxf((st.m - most) * a.c, -1e4f), f = __builtin_amdgcn_exp2f(d);
+      const float d = st.m == -INFINITY ? -1e4f : fmaxf((st.m - most) * a.c, -1e4f) + (lp_shift(most, a.c) - lp_shift(st.m, a.c));
+      const float f = __builtin_amdgcn_exp2f(d);
       st.w = f * (st.w + d * st.s);
       st.s *= f;
       st.m = most;
     }
-    // (x - m) c; where m is a mask of the type's lowest value m c would be -inf, so there the difference comes first
-    const bool low = st.m < -1e37f && st.m > -INFINITY;
-    if (__builtin_expect(__any(low), 0)) {
-      const float m = st.m == -INFINITY ? 0.f : st.m;
+    const bool far = st.m > -INFINITY && !lp_near(st.m, a.c);
+    if (__builtin_expect(__any(far), 0)) {
+      const float m = st.m == -INFINITY ? 0.f : st.m, shift = lp_shift(st.m, a.c);
 #pragma unroll
       for (int i = 0; i < N; i++) {
-        const float t = (x[i] - m) * a.c, e = __builtin_amdgcn_exp2f(t);
+        const float t = fmaf(x[i] - m, a.c, shift), e = __builtin_amdgcn_exp2f(t);
         st.s += e;
         st.w = fmaf(e, fmaxf(t, -1000.f), st.w);       // (0 times -inf where a logit is -inf)
       }
@@ -342,6 +349,9 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(const LpArgs
       }
     }
   }
+  const float shift = lp_shift(st.m, a.c), unshift = __builtin_amdgcn_exp2f(-shift);
+  st.w = unshift * (st.w - shift * st.s);
+  st.s *= unshift;
   st = lp_block_stats(st, sh, a.c);                    // (ends behind a barrier)
   uint64_t key = 0;
   if (a.k) {
