@@ -285,6 +285,8 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(const LpArgs
     sh.count = 0;
   }
   LpStats st{-INFINITY, 0.f, 0.f};
+  float off = 0.f, shift = 0.f;                        // of st.m
+  bool far = false;
   uint64_t bound = 0;
   float bound_value = -INFINITY;
   for (int c0 = v0; c0 < v1; c0 += kChunk) {
@@ -296,15 +298,17 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(const LpArgs
     for (int i = 1; i + 1 < N; i += 2) most = fmaxf(fmaxf(most, x[i]), x[i + 1]);
     most = fmaxf(most, x[N - 1]);
     if (most > st.m) {
-      const float d = st.m == -INFINITY ? -1e4f : fmaxf((st.m - most) * a.c, -1e4f) + (lp_shift(most, a.c) - lp_shift(st.m, a.c));
+      const float now = lp_shift(most, a.c), d = st.m == -INFINITY ? -1e4f : fmaxf((st.m - most) * a.c, -1e4f) + (now - shift);
       const float f = __builtin_amdgcn_exp2f(d);
       st.w = f * (st.w + d * st.s);
       st.s *= f;
       st.m = most;
+      shift = now;
+      off = most * a.c;
+      far = !lp_near(most, a.c);
     }
-    const bool far = st.m > -INFINITY && !lp_near(st.m, a.c);
     if (__builtin_expect(__any(far), 0)) {
-      const float m = st.m == -INFINITY ? 0.f : st.m, shift = lp_shift(st.m, a.c);
+      const float m = st.m == -INFINITY ? 0.f : st.m;
 #pragma unroll
       for (int i = 0; i < N; i++) {
         const float t = fmaf(x[i] - m, a.c, shift), e = __builtin_amdgcn_exp2f(t);
@@ -312,7 +316,6 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(const LpArgs
         st.w = fmaf(e, fmaxf(t, -1000.f), st.w);       // (0 times -inf where a logit is -inf)
       }
     } else {
-      const float off = st.m == -INFINITY ? 0.f : st.m * a.c;
       float s2 = 0.f, w2 = 0.f;                        // two sums at a time: each waits for its last addition
 #pragma unroll
       for (int i = 0; i < N; i += 2) {
@@ -349,7 +352,7 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(const LpArgs
       }
     }
   }
-  const float shift = lp_shift(st.m, a.c), unshift = __builtin_amdgcn_exp2f(-shift);
+  const float unshift = __builtin_amdgcn_exp2f(-shift);
   st.w = unshift * (st.w - shift * st.s);
   st.s *= unshift;
   st = lp_block_stats(st, sh, a.c);                    // (ends behind a barrier)
