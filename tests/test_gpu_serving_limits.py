@@ -1,9 +1,11 @@
 """The serving step's operators at the limits of what they accept."""
+import math
+
 import pytest
 import torch
 
 import serving_plain as plain
-from test_gpu_serving import say
+from test_gpu_serving import STEPS, Step, say
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +80,21 @@ def test_logprobs_of_the_largest_logits(pkg, dev, temperature, T, V):
     x[1, 2:100] = 1e38
     x[2 % T] = top
     check_sharp(pkg, dev, x, 5, temperature, torch.full((T,), V - 1))
+
+
+# ------------------------------------------------------------------------------------------------ tree_attention
+@pytest.mark.parametrize("step", [s for s in STEPS if len(s[1]) > 2], ids=lambda s: s[0])
+def test_attention_of_a_part_of_a_batch(pkg, dev, step):
+    """The last requests of a batch by slices of its tensors: the rows before theirs are rows of no request."""
+    _, reqs, Hq, Hkv, D, page, fp8, as_tree = step
+    say("tree_attention part of", step)
+    s = Step(len(reqs) * 7 + Hq, reqs, Hq, Hkv, D, page, fp8, as_tree, spare_rows=3)
+    a = s.args(dev)
+    skip = len(reqs) - 2
+    out = torch.full_like(a["q"], 7.0)
+    out, lse = pkg.tree_attention(**{**a, "kv_lens": a["kv_lens"][skip:], "cu_tokens": a["cu_tokens"][skip:], "block_tables": a["block_tables"][skip:]},
+                                  out=out, return_lse=True)
+    s.tables, s.lens, first = s.tables[skip:], s.lens[skip:], s.cu[skip]
+    s.cu = s.cu[skip:]
+    s.check(out, lse)
+    assert first > 0 and bool((out[:first] == 0).all()) and bool((lse[:first] == -math.inf).all())

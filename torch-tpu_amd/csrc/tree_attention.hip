@@ -825,7 +825,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
       if (r.prefix < 0)
         for (int j = 0; j < r.n; j++) nothing(r.t0 + j);
     }
-    for (int t = min(max(a.cu[a.B], 0), a.T) + (int)blockIdx.x; t < a.T; t += gridDim.x) nothing(t);
+    const int first = min(max(a.cu[0], 0), a.T), end = min(max(a.cu[a.B], 0), a.T);
+    for (int t = blockIdx.x; t < first; t += gridDim.x) nothing(t);
+    for (int t = end + (int)blockIdx.x; t < a.T; t += gridDim.x) nothing(t);
     return;
   }
   const int *rec = a.records + 8 * blockIdx.x;
