@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import serving_plain as plain
-from test_gpu_serving import STEPS, Step, say
+from test_gpu_serving import STEPS, Step, ints, say
 
 pytestmark = pytest.mark.gpu
 
@@ -98,3 +98,12 @@ def test_attention_of_a_part_of_a_batch(pkg, dev, step):
     s.cu = s.cu[skip:]
     s.check(out, lse)
     assert first > 0 and bool((out[:first] == 0).all()) and bool((lse[:first] == -math.inf).all())
+
+
+def test_attention_of_no_request(pkg, dev):
+    say("tree_attention of no request")
+    for cached in (torch.zeros(3, 16, 2, 64, dtype=torch.bfloat16, device=dev), torch.zeros(0, 16, 2, 64, dtype=torch.bfloat16, device=dev)):
+        for first in (0, 2):
+            out, lse = pkg.tree_attention(torch.ones(5, 4, 64, dtype=torch.bfloat16, device=dev), cached, cached, ints([], dev).view(0, 4), ints([], dev),
+                                          ints([first], dev), out=torch.full((5, 4, 64), 7.0, dtype=torch.bfloat16, device=dev), return_lse=True)
+            assert bool((out == 0).all()) and bool((lse == -math.inf).all())

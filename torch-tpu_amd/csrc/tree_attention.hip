@@ -954,8 +954,8 @@ extern "C" int moe_tree_attention(void *stream, const void *q_bf16, int64_t q_st
   if (k_block_stride >= (1ll << 31) || v_block_stride >= (1ll << 31) || row >= (1 << 22)) return MOE_E_SHAPE;
   if (q_stride % 8 || k_block_stride % 16 || v_block_stride % 16) return MOE_E_ALIGN;
   if (T == 0) return MOE_OK;
-  if (B == 0 || !q_bf16 || !out_bf16 || !kv_lens || !cu_tokens || !workspace) return MOE_E_NULL;
-  if (table_width && n_blocks && (!block_tables || !k_cache || !v_cache)) return MOE_E_NULL;
+  if (!q_bf16 || !out_bf16 || !cu_tokens || !workspace || (B && !kv_lens)) return MOE_E_NULL;
+  if (B && table_width && n_blocks && (!block_tables || !k_cache || !v_cache)) return MOE_E_NULL;
   for (const void *p : {q_bf16, k_cache, v_cache, (const void *)out_bf16})
     if ((uintptr_t)p % 16) return MOE_E_ALIGN;
   if ((uintptr_t)workspace % 256) return MOE_E_ALIGN;
