@@ -82,6 +82,28 @@ def test_logprobs_of_the_largest_logits(pkg, dev, temperature, T, V):
     check_sharp(pkg, dev, x, 5, temperature, torch.full((T,), V - 1))
 
 
+# ------------------------------------------------------------------------------------------------ cache_plan
+def test_plan_of_tensors_side_by_side_in_memory(pkg, dev):
+    """One allocation for all, results right before and after what is read, lengths between the rows of the table: nothing overlaps."""
+    say("cache_plan in one allocation")
+    tables, lens, counts, free, T = [[4, -1, -1], [6, 1, -1]], [3, 7], [2, 4], [0, 2, 3, 5], 6
+    want = plain.plan(tables, lens, counts, free, 4, 4, T, None)
+    mem = torch.full((64,), -9, dtype=torch.int32, device=dev)
+    rows = mem[:32].view(2, 16)
+    rows[:, :3] = ints(tables, dev)
+    mem[4:6], mem[6:8], mem[32:36], mem[36] = ints(lens, dev), ints(counts, dev), ints(free, dev), 4
+    at = lambda i: mem.data_ptr() + 4 * i
+    slots = torch.zeros(T, dtype=torch.int64, device=dev)
+    kv, cu, left, pos = 8, 10, 37, 38                     # kv_lens right behind counts, the count left right behind the stack's
+    rc = pkg._lib.lib.moe_cache_plan(torch.cuda.current_stream().cuda_stream, at(0), 16, 2, 3, at(4), at(6), at(32), 4, at(36), 4, None, T, at(cu), at(pos),
+                                     slots.data_ptr(), None, at(kv), at(left))
+    torch.cuda.synchronize()
+    assert rc == 0
+    assert (rows[:, :3].tolist(), mem[cu:cu + 3].tolist(), mem[pos:pos + T].tolist(), slots.tolist(), mem[kv:kv + 2].tolist(), int(mem[left])) == (
+        want[0], want[1], want[2], want[3], want[5], want[6])
+    assert mem[4:8].tolist() == lens + counts and mem[32:37].tolist() == free + [4]
+
+
 # ------------------------------------------------------------------------------------------------ tree_attention
 @pytest.mark.parametrize("step", [s for s in STEPS if len(s[1]) > 2], ids=lambda s: s[0])
 def test_attention_of_a_part_of_a_batch(pkg, dev, step):

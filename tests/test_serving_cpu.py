@@ -40,6 +40,22 @@ def test_cache_plan_refusals(pkg):
     assert call(left=fake) == E_MODE          # the count read and the count written are one
 
 
+def test_cache_plan_refuses_results_over_what_it_reads(pkg):
+    """Every workgroup reads the lengths while another writes results already: lengths updated in place would be a race."""
+    read = dict(lens=8, counts=8, free=16, n_free=4, parents=16)
+    written = dict(cu=12, pos=16, slots=32, masks=32, kv=8, left=4, tables=4 * (8 + 6))
+    names = ["tables", "stride", "B", "W", "lens", "counts", "free", "F", "n_free", "page", "parents", "T", "cu", "pos", "slots", "masks", "kv", "left"]
+    at = {n: 0x10000 + 0x1000 * i for i, n in enumerate([*read, *written])}
+
+    def call(**moved):
+        a = {**dict(stride=8, B=2, W=6, F=4, page=16, T=4), **{n: ctypes.c_void_p(p) for n, p in {**at, **moved}.items()}}
+        return lib().moe_cache_plan(None, *[a[n] for n in names])
+    for r, size in read.items():
+        for w, wide in written.items():
+            for moved in (at[r], at[r] + size - 4, at[r] - wide + 4):             # at its start, on its last value, its first value under the last result
+                assert call(**{w: moved}) == E_MODE, (r, w, moved - at[r])
+
+
 def test_qk_norm_rope_refusals(pkg):
     names = ["qkv", "stride", "T", "Hq", "Hkv", "D", "pos", "cs", "P", "R", "pairs", "qw", "kw", "wt", "eps", "q", "k", "kc", "vc", "ct", "blocks",
              "ks", "vs", "page", "slots", "kscale", "vscale"]

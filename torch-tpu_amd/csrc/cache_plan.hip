@@ -168,7 +168,25 @@ extern "C" int moe_cache_plan(void *stream, int32_t *block_tables, int64_t table
   if (!cu_tokens || !n_free || !n_free_out) return MOE_E_NULL;
   if (B && (!lens || !counts || !kv_lens || (table_width && !block_tables))) return MOE_E_NULL;
   if ((n_free_max && !free_blocks) || (T && (!positions || !slots || (parents && !masks)))) return MOE_E_NULL;
-  if (n_free == n_free_out) return MOE_E_MODE;        // every workgroup reads the one while the first writes the other
+  // Every workgroup reads all lengths, the stack and its count while others write already: what is written has to lie apart from what is read.
+  struct Range {
+    const void *at;
+    int64_t bytes;
+    bool meets(const Range &o) const {
+      return bytes > 0 && o.bytes > 0 && (uintptr_t)at < (uintptr_t)o.at + o.bytes && (uintptr_t)o.at < (uintptr_t)at + bytes;
+    }
+  };
+  const Range read[] = {{lens, 4ll * B}, {counts, 4ll * B}, {free_blocks, 4ll * n_free_max}, {n_free, 4}, {parents, parents ? 4ll * T : 0}};
+  const Range written[] = {{cu_tokens, 4ll * (B + 1)}, {positions, 4ll * T}, {slots, 8ll * T}, {masks, parents ? 8ll * T : 0}, {kv_lens, 4ll * B},
+                           {n_free_out, 4}};
+  const Range table{block_tables, B ? 4 * ((B - 1) * table_stride + table_width) : 0};
+  for (const Range &r : read) {
+    for (const Range &w : written)
+      if (w.meets(r)) return MOE_E_MODE;
+    if (table.meets(r))                                // (something may lie between the rows)
+      for (int b = 0; b < B; b++)
+        if (Range{block_tables + b * table_stride, 4ll * table_width}.meets(r)) return MOE_E_MODE;
+  }
   PlanArgs a{block_tables, table_stride, lens, counts, free_blocks, n_free, T ? parents : nullptr, B, table_width, n_free_max,
              __builtin_ctz(page_size), T, cu_tokens, positions, kv_lens, n_free_out, slots, masks};
   const int64_t rows = ((int64_t)B + 3) / 4, fill = ((int64_t)T + 2047) / 2048;
