@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import serving_plain as plain
+from test_gpu_attention_tiles import attend, with_room
 from test_gpu_serving import STEPS, Step, ints, say
 
 pytestmark = pytest.mark.gpu
@@ -129,3 +130,30 @@ def test_attention_of_no_request(pkg, dev):
             out, lse = pkg.tree_attention(torch.ones(5, 4, 64, dtype=torch.bfloat16, device=dev), cached, cached, ints([], dev).view(0, 4), ints([], dev),
                                           ints([first], dev), out=torch.full((5, 4, 64), 7.0, dtype=torch.bfloat16, device=dev), return_lse=True)
             assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+
+
+def ramp(s, of_key):
+    """Every value of request b's i-th key is of_key(i)."""
+    page = s.k.shape[1]
+    for b, l in enumerate(s.lens):
+        for i in range(l):
+            s.k[s.tables[b][i // page], i % page] = torch.tensor(float(of_key(i))).to(s.kind)
+
+
+LONG = [(16, [(2600, 1), (2400, 2)], 8, 2), (64, [(2600, 8)], 8, 1), (128, [(2600, 16), (2300, 16)], 8, 1), (256, [(2600, 32)], 8, 1)]
+
+
+@pytest.mark.parametrize("rows,reqs,Hq,Hkv", LONG)
+@pytest.mark.parametrize("size,rise", [(1e25, 39.0), (1e30, 39.0), (1e30, 10.0), (2e34, 39.0), (2e34, 0.0)])
+def test_attention_of_large_values(pkg, dev, size, rise, rows, reqs, Hq, Hkv):
+    """Values near the type's largest, and keys here and there that outscore the ones before them by `rise`: the weighted mean is a
+    number, and so is everything on the way to it while the values' size times the number of keys is one."""
+    say("tree_attention of values around", size, "rise", rise)
+    s = Step(12, reqs, Hq, Hkv, 64, 16, False, True)
+    s = with_room(s) if rows > 16 else s
+    s.v = (s.v.float() * size).to(torch.bfloat16)
+    s.q[:] = 2
+    ramp(s, lambda i: rise / 16 if i // 128 % 2 and i % 32 == 5 else 0)          # a score is 64 products, 2 k / 8 each
+    out, lse = attend(pkg, dev, s, rows)
+    assert bool(out.isfinite().all())
+    s.check(out, lse)

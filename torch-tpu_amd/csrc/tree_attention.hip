@@ -150,9 +150,11 @@ __device__ __forceinline__ void attn_walk(const AttnArgs &a, Segment segment) {
 // Scores are formed transposed, S^T = K Q^T, so that a lane holds for ONE query (lane % 16) the keys 4 g + i, g = lane / 16, of two
 // tiles of 16.  Those eight are at once the lane's operand of O^T = V^T P^T, if the reduction runs over the keys in that
 // order: no probability changes its lane.  V^T comes from row-major values in LDS by the transposing read.
-// p = 2^(s c - m): m is the maximum of a tile's first keys and follows it later only where sums exceed 2^60: in between p, the
-// sums and the output merely have another exponent, nothing is lost, and no maximum is formed nor anything rescaled.  p is rounded to bf16 for the product (what the matrix cores take; an error of 2^-9 of each term, as the
-// output's own rounding); its sum is taken before that, in fp32.
+// p = 2^(s c - m): m lies kLag above the maximum of a tile's first keys and follows it later only where a lane's probabilities add up to more than 1, so
+// that in between no maximum is formed nor anything rescaled.  The largest p is between about 2^-kLag and 1: sums of p v are no larger
+// than the softmax's own before its division, and they lose what is smaller than 2^(kLag - 126).  p is rounded to bf16 for the product (what
+// the matrix cores take; an error of 2^-9 of each term, as the output's own rounding); its sum is taken before that, in fp32.
+constexpr float kLag = 16.f;                           // (scores that outgrow the first keys' by 11 raise m, a few times a tile at the most)
 __device__ __forceinline__ float over_groups(float v, bool sum) {
   v2u r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   v = sum ? __uint_as_float(r[0]) + __uint_as_float(r[1]) : fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -173,7 +175,7 @@ struct AttnState {
       for (int dt = 0; dt < DT; dt++) o[dt][qc] = (v4f){0.f, 0.f, 0.f, 0.f};
     }
   }
-  // lets m follow the largest of KT tiles' scores
+  // lets m follow the largest of KT tiles' scores (a little more is left alone)
   template <int KT>
   __device__ __forceinline__ void raise(const v4f (&s)[KT][NQ], float c) {
     float top[NQ];
@@ -189,7 +191,7 @@ struct AttnState {
     if (__builtin_expect(__any(grown), 0)) {
 #pragma unroll
       for (int qc = 0; qc < NQ; qc++) {
-        const float t = over_groups(top[qc], false), now = t > m[qc] + 8.f ? t : m[qc];
+        const float t = over_groups(top[qc], false), now = t > m[qc] - kLag + 8.f ? t + kLag : m[qc];
         const float f = now == m[qc] ? 1.f : __builtin_amdgcn_exp2f(m[qc] - now);
         m[qc] = now;
         l[qc] *= f;
@@ -208,7 +210,7 @@ struct AttnState {
       weigh<KT>(s, c, p, sum);
       bool far = false;
 #pragma unroll
-      for (int qc = 0; qc < NQ; qc++) far |= sum[qc] > 0x1p60f;
+      for (int qc = 0; qc < NQ; qc++) far |= sum[qc] > 1.f;
       if (__builtin_expect(rise || !__any(far), 1)) break;
       rise = true;
     }
