@@ -435,7 +435,7 @@ int moe_qk_norm_rope(void *stream, const void *qkv_bf16, int64_t row_stride, int
  * q [T, Hq, D] bf16 (rows q_stride apart), query head h on cache head h / (Hq / Hkv); scores scale * q.k (times k_scale
  * of the head), out [T, Hq, D] bf16 (times v_scale), lse [T, Hq] fp32 or NULL = log of the sum of exponentials.
  * A row that sees no key, of a refused request (kv_lens < n) or of no request: out 0, lse -inf.
- * D 64 or 128; masks cover requests of at most 64 new tokens, without masks there is no limit.  Scales are positive.
+ * D 64 or 128; masks cover requests of at most 64 new tokens, without masks there is no limit.  Scales may have any sign.
  * (T Hq / (16 Hkv) + B) Hkv table_width page_size / 64 below 2^31.
  * workspace: moe_tree_attention_workspace_bytes(...) bytes, 256-byte aligned.
  */

@@ -132,12 +132,33 @@ def test_attention_of_no_request(pkg, dev):
             assert bool((out == 0).all()) and bool((lse == -math.inf).all())
 
 
+TILES = [(16, [(300, 1), (180, 2), (256, 1)], 8, 2), (64, [(300, 8)], 8, 1), (128, [(300, 16), (288, 16)], 8, 1), (256, [(300, 32)], 8, 1)]
+
+
 def ramp(s, of_key):
     """Every value of request b's i-th key is of_key(i)."""
     page = s.k.shape[1]
     for b, l in enumerate(s.lens):
         for i in range(l):
             s.k[s.tables[b][i // page], i % page] = torch.tensor(float(of_key(i))).to(s.kind)
+
+
+@pytest.mark.parametrize("rows,reqs,Hq,Hkv", TILES)
+@pytest.mark.parametrize("slope", [0.3, -0.3])
+@pytest.mark.parametrize("how", ["scale", "k_scale", "both"])
+def test_attention_with_negative_scales(pkg, dev, how, slope, rows, reqs, Hq, Hkv):
+    """Scores far apart, rising or falling along the keys."""
+    say("tree_attention", how, "negative, slope", slope)
+    s = Step(11, reqs, Hq, Hkv, 64, 16, how != "scale", True)
+    s = with_room(s) if rows > 16 else s
+    s.q[:] = 2
+    ramp(s, lambda i: (i - 200) * slope)
+    if how != "k_scale":
+        s.scale = -s.scale
+    if how != "scale":
+        s.ks = -torch.linspace(0.7, 1.0, Hkv)
+        s.vs = -s.vs
+    s.check(*attend(pkg, dev, s, rows, scale=s.scale))
 
 
 LONG = [(16, [(2600, 1), (2400, 2)], 8, 2), (64, [(2600, 8)], 8, 1), (128, [(2600, 16), (2300, 16)], 8, 1), (256, [(2600, 32)], 8, 1)]

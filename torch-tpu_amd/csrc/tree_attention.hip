@@ -362,17 +362,21 @@ __device__ __forceinline__ void attn_add_no_numbers(const AttnArgs &a, const Att
 }
 
 // a lane's queries as the scores' second operand: element j of step s is d = 32 s + 8 g + j, or with e4m3 keys, of which a lane reads
-// 16 at a time, d = 64 (s / 2) + 16 g + 8 (s % 2) + j.  Its 16s of rows lie STEP apart.
+// 16 at a time, d = 64 (s / 2) + 16 g + 8 (s % 2) + j.  Its 16s of rows lie STEP apart.  Of the scores' factor the queries take the
+// sign, so that the largest score is the largest product.
 template <int NQ, int D, bool FP8, int STEP = 16>
-__device__ __forceinline__ void attn_queries(const AttnArgs &a, const AttnRequest &r, int kh, int first_row, v8bf (&q)[NQ][D / 32],
+__device__ __forceinline__ void attn_queries(const AttnArgs &a, const AttnRequest &r, int kh, int first_row, float factor, v8bf (&q)[NQ][D / 32],
                                              AttnSight<NQ> &sight) {
-  const int lane = threadIdx.x & 63, g = lane >> 4;
+  const int lane = threadIdx.x & 63, g = lane >> 4, flip = factor < 0.f ? (int)0x80008000 : 0;
 #pragma unroll
   for (int qc = 0; qc < NQ; qc++) {
     const int row = min(first_row + STEP * qc + (lane & 15), r.n * a.G - 1), j = row / a.G, h = kh * a.G + row - j * a.G;
     const uint16_t *src = a.q + (size_t)(r.t0 + j) * a.q_stride + (size_t)h * D;
 #pragma unroll
-    for (int s = 0; s < D / 32; s++) q[qc][s] = *(const v8bf *)(src + (FP8 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g));
+    for (int s = 0; s < D / 32; s++) {
+      const v4i w = *(const v4i *)(src + (FP8 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g));
+      q[qc][s] = __builtin_bit_cast(v8bf, w ^ flip);
+    }
     sight.mask[qc] = a.masks ? (uint64_t)a.masks[r.t0 + j] : (uint64_t)(r.prefix + j);
   }
 }
@@ -416,10 +420,10 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(const AttnArgs a) {
   const uint8_t *read_at = values + (4 * g + c16 / 4) * LD + 8 * (c16 % 4);
   attn_walk<ROWS, UNIT>(a, [&](const AttnRequest r, int b, int kh, int m_tile, int c0, int c1, bool whole, int part) {
     const int32_t *table = a.tables + (size_t)b * a.table_stride;
-    const float scale = a.scale * (a.k_scale ? a.k_scale[kh] : 1.f) * 1.4426950408889634f;
+    const float factor = a.scale * (a.k_scale ? a.k_scale[kh] : 1.f) * 1.4426950408889634f, scale = fabsf(factor);
     v8bf q[NQ][D / 32];
     AttnSight<NQ> sight;
-    attn_queries<NQ, D, FP8>(a, r, kh, m_tile * ROWS, q, sight);
+    attn_queries<NQ, D, FP8>(a, r, kh, m_tile * ROWS, factor, q, sight);
     const int clear = a.masks ? r.prefix : r.prefix + m_tile * ROWS / a.G + 1;      // keys below it are seen by every row
     AttnState<NQ, DT> st;
     st.clear();
@@ -592,7 +596,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const AttnArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c16 = lane & 15;
   attn_walk<ROWS, UNIT>(a, [&](const AttnRequest r, int b, int kh, int m_tile, int c0, int c1, bool whole, int part) {
     const int32_t *table = a.tables + (size_t)b * a.table_stride;
-    const float scale = a.scale * (a.k_scale ? a.k_scale[kh] : 1.f) * 1.4426950408889634f;
+    const float factor = a.scale * (a.k_scale ? a.k_scale[kh] : 1.f) * 1.4426950408889634f, scale = fabsf(factor);
     const int clear = a.masks ? r.prefix : r.prefix + m_tile * ROWS / a.G + 1;      // keys below it are seen by every row
     const int last = c1 - 1;
     const int stage_row = attn_stage_row<FP8, TPR>(tid / TPR), piece = tid % TPR;
@@ -634,7 +638,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const AttnArgs a) {
       constexpr int N = decltype(sixteens)::value, AHEAD = N == 2 && !FP8 ? 2 : 3;     // (as the registers allow)
       v8bf q[N][D / 32];
       AttnSight<N> sight;
-      attn_queries<N, D, false, 64>(a, r, kh, m_tile * ROWS + 16 * w, q, sight);
+      attn_queries<N, D, false, 64>(a, r, kh, m_tile * ROWS + 16 * w, factor, q, sight);
       AttnState<N, DT> st;
       st.clear();
       begin();
@@ -702,7 +706,7 @@ __global__ __launch_bounds__(512, 2) void attn_pairs_kernel(const AttnArgs a) {
   const int late = __builtin_amdgcn_readfirstlane(w) >> 2;
   attn_walk<ROWS, UNIT>(a, [&](const AttnRequest r, int b, int kh, int m_tile, int c0, int c1, bool whole, int part) {
     const int32_t *table = a.tables + (size_t)b * a.table_stride;
-    const float scale = a.scale * (a.k_scale ? a.k_scale[kh] : 1.f) * 1.4426950408889634f;
+    const float factor = a.scale * (a.k_scale ? a.k_scale[kh] : 1.f) * 1.4426950408889634f, scale = fabsf(factor);
     const int clear = a.masks ? r.prefix : r.prefix + m_tile * ROWS / a.G + 1;      // keys below it are seen by every row
     const int last = c1 - 1;
     const int i = tid / TPR, piece = tid % TPR, stage_row = attn_stage_row<FP8, TPR>(i);
@@ -752,7 +756,7 @@ __global__ __launch_bounds__(512, 2) void attn_pairs_kernel(const AttnArgs a) {
       constexpr int N = decltype(sixteens)::value;
       v8bf q[N][X];
       AttnSight<N> sight;
-      attn_queries<N, D, false, 128>(a, r, kh, m_tile * ROWS + 16 * w, q, sight);
+      attn_queries<N, D, false, 128>(a, r, kh, m_tile * ROWS + 16 * w, factor, q, sight);
       AttnState<N, DT> st;
       st.clear();
       begin();

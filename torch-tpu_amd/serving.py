@@ -68,7 +68,7 @@ def tree_attention(q, k_cache, v_cache, block_tables, kv_lens, cu_tokens, masks=
     [T] int64 from cache_plan), or without masks one token or a causal chunk.
 
     q [T, Hq, D] bf16, D 64 or 128, Hq a multiple of the cache's heads; caches [blocks, page, heads, D] bf16 or e4m3 (with the
-    scales of qk_norm_rope); kv_lens [B] and cu_tokens [B + 1] from the plan; scale defaults to D ** -0.5.
+    scales of qk_norm_rope); kv_lens [B] and cu_tokens [B + 1] from the plan; scale, of any sign, defaults to D ** -0.5.
     Returns out [T, Hq, D] bf16, or (out, lse [T, Hq] float32).  A row that sees no key is 0, its lse -inf."""
     o, lse = _ops.tree_attention.default(q, k_cache, v_cache, block_tables, kv_lens, cu_tokens, masks, scale, k_scale, v_scale, out, return_lse)
     return (o, lse) if return_lse else o
