@@ -392,7 +392,7 @@ int moe_router_logits(void *stream, const void *x_bf16, int T, int H, const void
  *              *_block_stride elements apart (both may lie in one allocation).  page_size: a power of two.
  *   slot       block * page_size + place in the page, int64; -1: none.
  *   tokens     of all requests one after another: request b holds rows [cu_tokens[b], cu_tokens[b + 1]), cu_tokens [B + 1] ascending.  Rows
- *              before cu_tokens[0] and from cu_tokens[B] on belong to no request.
+ *              before cu_tokens[0] and from cu_tokens[B] on belong to no request.  (Where it descends results are undefined, but every launch ends.)
  *   tree       parents [T] int32: of a drafted token, the place of its parent among its own request's (before its own), -1 for
  *              one that follows the cached text directly.  masks [T] int64: bit i = sees its request's token i.
  */

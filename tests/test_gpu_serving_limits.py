@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import serving_plain as plain
-from test_gpu_attention_tiles import attend, with_room
+from test_gpu_attention_tiles import ROOM, attend, tile_rows, with_room
 from test_gpu_serving import STEPS, Step, ints, say
 
 pytestmark = pytest.mark.gpu
@@ -130,6 +130,23 @@ def test_attention_of_no_request(pkg, dev):
             out, lse = pkg.tree_attention(torch.ones(5, 4, 64, dtype=torch.bfloat16, device=dev), cached, cached, ints([], dev).view(0, 4), ints([], dev),
                                           ints([first], dev), out=torch.full((5, 4, 64), 7.0, dtype=torch.bfloat16, device=dev), return_lse=True)
             assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+
+
+@pytest.mark.parametrize("rows,n,Hq,B", [(16, 64, 4, 70), (64, 64, 8, 8), (128, 64, 13, 8), (256, 64, 32, 8)])
+@pytest.mark.parametrize("as_tree", [True, False])
+def test_attention_ends_where_cu_tokens_descends(pkg, dev, as_tree, rows, n, Hq, B):
+    """Every second request claims all rows: more work than the batch can have.  The results are undefined, but the call ends, writes inside
+    its results only, and the next one is right."""
+    say("tree_attention with descending cu_tokens", rows, n)
+    s = with_room(Step(5, [(900, n)] + [(700, 0)] * (B - 1), Hq, 1, 64, 16, False, as_tree))
+    a, T = s.args(dev), s.T
+    mem = torch.full((T + 8, Hq, 64), 7.0, dtype=torch.bfloat16, device=dev)
+    bad = ints([0, T] * B, dev)[:B + 1].contiguous()
+    assert tile_rows(pkg, s) == rows
+    pkg.tree_attention(**{**a, "cu_tokens": bad, "kv_lens": ints([ROOM] * B, dev)}, out=mem[4:4 + T])
+    torch.cuda.synchronize()
+    assert bool((mem[:4] == 7).all()) and bool((mem[4 + T:] == 7).all())
+    s.check(*attend(pkg, dev, s, rows))
 
 
 TILES = [(16, [(300, 1), (180, 2), (256, 1)], 8, 2), (64, [(300, 8)], 8, 1), (128, [(300, 16), (288, 16)], 8, 1), (256, [(300, 32)], 8, 1)]

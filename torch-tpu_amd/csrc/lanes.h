@@ -37,15 +37,15 @@ __device__ __forceinline__ float lane_sum(float v) {
   return v;
 }
 
-// the sum of a wavefront's lanes 0 .. this one
-__device__ __forceinline__ int lane_sum_upto(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);                      // from 1, 2, 4, 8 lanes down in a row of 16
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);                      // a row's last lane to the next row
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);                      // lane 31 to the upper half
-  return v;
+// the sum of a wavefront's lanes 0 .. this one, 2^32 - 1 where it is more
+__device__ __forceinline__ uint32_t lane_sum_upto(uint32_t v) {
+  const auto add = [](uint32_t a, int b) { return __builtin_elementwise_add_sat(a, (uint32_t)b); };
+  v = add(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));               // from 1, 2, 4, 8 lanes down in a row of 16
+  v = add(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
+  v = add(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
+  v = add(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
+  v = add(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));               // a row's last lane to the next row
+  return add(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));            // lane 31 to the upper half
 }
 // the largest over a wavefront
 __device__ __forceinline__ int lane_max(int v) {

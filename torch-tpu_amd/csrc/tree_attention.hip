@@ -36,6 +36,7 @@ struct AttnArgs {
   float *part_o, *part_ml;             // [2 groups][rows][D]; [2 groups][rows][2]
   int32_t *records;                    // [groups][8]: of the tile that begins in a stretch and goes on: last stretch, the
                                        // request's first row and rows, head, tile, part
+  uint32_t most_units;                 // the line's length at most
 };
 
 // ---- who does what ----------------------------------------------------------------------------------------------------
@@ -70,30 +71,34 @@ __device__ __forceinline__ int attn_head_units(const AttnArgs &a, const AttnRequ
 
 // A workgroup's way along its stretch: calls segment(request, head, tile, units c0 .. c1 of the tile's u, part) for each piece.
 // Every wavefront adds the line up for itself, 64 requests at a time, and finds its first request among them: one trip to
-// memory and no barrier stand in front of the work.  (The host has seen to it that the line's length fits an int.)
+// memory and no barrier stand in front of the work.  The host has seen to it that the line's length fits an int where cu_tokens ascends;
+// where it does not, requests share rows and the line may have any length: a longer one than the host allowed for is taken for empty, so that
+// no index wraps and every walk ends.
 template <int ROWS, int UNIT, typename Segment>
 __device__ __forceinline__ void attn_walk(const AttnArgs &a, Segment segment) {
   const int lane = threadIdx.x & 63;
   AttnRequest mine{0, 0, 0, -1};
-  int units = 0, total = 0, longest = 0;
+  int units = 0, longest = 0;
+  uint32_t upto = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     if (b0 + lane < a.B) mine = attn_request(a, b0 + lane);
     else mine.n = 0;
     units = attn_head_units<ROWS, UNIT>(a, mine) * a.Hkv;
-    total += units;
+    upto = __builtin_elementwise_add_sat(upto, (uint32_t)units);
     if (units > 0) longest = max(longest, (mine.kv + UNIT - 1) / UNIT);
   }
-  int upto = lane_sum_upto(total);                     // (with up to 64 requests: the line's length up to each)
-  total = __builtin_amdgcn_readlane(upto, 63);
+  upto = lane_sum_upto(upto);                          // (with up to 64 requests: the line's length up to each)
+  int total = __builtin_amdgcn_readlane(upto, 63);
+  if ((uint32_t)total > a.most_units) total = 0;
   longest = __builtin_amdgcn_readfirstlane(lane_max(longest));
   // An equal share for every workgroup, but of one long tile no more than pays: n units cut into stretches of x take x steps of a unit, then
   // a join of n / x parts, least at x = sqrt(n cut), cut the time of a part over that of a unit.  (One token over 32767 keys: 28, 23.5 and
   // 26 us with stretches of 2, 4 and 8 units; over 1000 keys 14.8 and 17.8 us with 2 and 4.)
-  const int even = (total + a.groups - 1) / a.groups, least = __builtin_amdgcn_readfirstlane((int)ceilf(sqrtf((float)longest * a.cut)));
+  const int even = (int)(((uint32_t)total + a.groups - 1) / (uint32_t)a.groups), least = __builtin_amdgcn_readfirstlane((int)ceilf(sqrtf((float)longest * a.cut)));
   const int per = max(max(even, least), 1);
   // Neighbouring stretches, whose tiles have keys in common, on one XCD and so behind one L2: workgroups go to the eight XCDs in turn.
-  const int eighth = ((total + per - 1) / per + 7) / 8, wg = blockIdx.x, place = wg < 8 * eighth ? wg % 8 * eighth + wg / 8 : wg;
-  const int start = (int)min((int64_t)place * per, (int64_t)total), end = min(start + per, total);
+  const int eighth = (int)(((uint32_t)total + per - 1) / (uint32_t)per + 7) / 8, wg = blockIdx.x, place = wg < 8 * eighth ? wg % 8 * eighth + wg / 8 : wg;
+  const int start = (int)min((int64_t)place * per, (int64_t)total), end = start + min(per, total - start);
   if (threadIdx.x == 0) a.records[8 * place] = -1;
   if (start >= end) return;
   int b = 0, before = 0;
@@ -105,11 +110,11 @@ __device__ __forceinline__ void attn_walk(const AttnArgs &a, Segment segment) {
       units = attn_head_units<ROWS, UNIT>(a, mine) * a.Hkv;
       upto = lane_sum_upto(units);
     }
-    const uint64_t past = __ballot(start < before + upto);
+    const uint64_t past = __ballot(start < before + (int)upto);
     if (past) {
       const int l = __builtin_ctzll(past);
       b = b0 + l;
-      before += __builtin_amdgcn_readlane(upto - units, l);
+      before += __builtin_amdgcn_readlane((int)upto - units, l);
       r = {__builtin_amdgcn_readlane(mine.t0, l), __builtin_amdgcn_readlane(mine.n, l), __builtin_amdgcn_readlane(mine.kv, l),
            __builtin_amdgcn_readlane(mine.prefix, l)};
       break;
@@ -968,14 +973,14 @@ extern "C" int moe_tree_attention(void *stream, const void *q_bf16, int64_t q_st
   if (workspace_bytes < moe_tree_attention_workspace_bytes(T, Hq, Hkv, D, B, cache_dtype)) return MOE_E_WORKSPACE;
   const int fp8 = cache_dtype == MOE_DTYPE_FP8, wide = fp8 ? 1 : 2;
   const AttnPlan plan = attn_plan(T, Hq, Hkv, B, cache_dtype, masks != nullptr, (int64_t)table_width * page_size);
-  // the line's length at most, in units
-  if (((int64_t)T * (Hq / Hkv) / plan.rows + B) * Hkv * (((int64_t)table_width * page_size + 63) / 64) >= (1ll << 31)) return MOE_E_SHAPE;
+  const int64_t most_units = ((int64_t)T * (Hq / Hkv) / plan.rows + B) * Hkv * (((int64_t)table_width * page_size + 63) / 64);
+  if (most_units >= (1ll << 31)) return MOE_E_SHAPE;
   const size_t parts = 2 * plan.groups;
   AttnArgs a{(const uint16_t *)q_bf16, q_stride, T, Hq, Hkv, Hq / Hkv, B, n_blocks, __builtin_ctz(page_size), n_blocks ? table_width : 0,
              (const uint8_t *)k_cache, (const uint8_t *)v_cache, (uint32_t)(k_block_stride * wide), (uint32_t)(v_block_stride * wide), table_stride,
              block_tables, kv_lens, cu_tokens, masks, scale, k_scale, v_scale, (uint16_t *)out_bf16, lse, plan.groups, plan.cut, (float *)workspace,
              (float *)((uint8_t *)workspace + align_up(parts * plan.rows * D * 4, 256)),
-             (int32_t *)((uint8_t *)workspace + align_up(parts * plan.rows * D * 4, 256) + align_up(parts * plan.rows * 8, 256))};
+             (int32_t *)((uint8_t *)workspace + align_up(parts * plan.rows * D * 4, 256) + align_up(parts * plan.rows * 8, 256)), (uint32_t)most_units};
   hipStream_t st = (hipStream_t)stream;
   using std::integral_constant;
   const auto run = [&](auto dim, auto narrow) {
