@@ -195,3 +195,40 @@ def test_attention_of_large_values(pkg, dev, size, rise, rows, reqs, Hq, Hkv):
     out, lse = attend(pkg, dev, s, rows)
     assert bool(out.isfinite().all())
     s.check(out, lse)
+
+
+# ------------------------------------------------------------------------------------------------ the registered ops
+def test_schemas_say_what_is_written_and_shared(pkg, dev):
+    """torch's own check of a schema: which arguments are written, and which results share memory with them or each other."""
+    from torch.library import opcheck
+    ops = torch.ops.my_ops
+    check = lambda op, args, kwargs=None: opcheck(op.default, args, kwargs or {}, test_utils="test_schema")
+    s = Step(21, [(60, 9), (7, 3)], 8, 2, 128, 16, False, True)
+    a = s.args(dev)
+    del a["k_scale"], a["v_scale"]
+    check(ops.tree_attention, (), a)
+    check(ops.tree_attention, (), {**a, "out": torch.zeros_like(a["q"]), "return_lse": True})
+    for parents in (None, ints([-1, 0, 0, -1, 0], dev)):
+        check(ops.cache_plan, (ints([[3, -1], [1, -1]], dev), ints([5, 2], dev), ints([3, 2], dev), ints([0, 2], dev), ints([2], dev), 4, 5, parents))
+    x = torch.randn(3, 8 * 64, device=dev).to(torch.bfloat16)
+    rope = (x, ints([0, 1, 2], dev), torch.randn(8, 64, device=dev), 4, 2)
+    check(ops.qk_norm_rope, rope)
+    k, v = (torch.zeros(2, 16, 2, 64, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    check(ops.qk_norm_rope, rope, dict(k_cache=k, v_cache=v, slots=ints([0, 1, 2], dev, torch.int64), out=torch.zeros(3, 4, 64, dtype=torch.bfloat16, device=dev)))
+    check(ops.token_logprobs, (torch.randn(3, 50, device=dev), ints([1, 2, 3], dev, torch.int64), 4, 1.0))
+
+
+def test_results_of_inputs_with_gradients_warn_in_backward(pkg, dev):
+    """The operators have no gradient: a backward pass through them says so instead of going past them silently."""
+    s = Step(21, [(60, 9), (7, 3)], 8, 2, 128, 16, False, True)
+    a = s.args(dev)
+    a["q"].requires_grad_()
+    w = torch.ones(64, device=dev, requires_grad=True)
+    x = torch.randn(3, 8 * 64, device=dev).to(torch.bfloat16)
+    results = [pkg.tree_attention(**a), pkg.tree_attention(**a, out=torch.zeros_like(a["q"])),
+               *pkg.qk_norm_rope(x, ints([0, 1, 2], dev), torch.randn(8, 64, device=dev), 4, 2, w, w),
+               pkg.token_logprobs(torch.randn(3, 50, device=dev, requires_grad=True), ints([1, 2, 3], dev, torch.int64)).logprobs]
+    for r in results:
+        assert r.requires_grad
+        with pytest.warns(UserWarning, match="autograd kernel was not registered"):
+            r.sum().backward()

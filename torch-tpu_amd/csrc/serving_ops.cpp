@@ -252,16 +252,18 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor &logits, 
 
 }  // namespace
 
+// What a schema says of memory: (a!) is written, a result (a) is that tensor where it is handed over, results with the same letter share an
+// allocation.  (A result marked as written, (a!), would drop out of autograd: backward would not warn that there is no gradient.)
 TORCH_LIBRARY_FRAGMENT(my_ops, m) {
   m.def("cache_plan(Tensor(a!) block_tables, Tensor lens, Tensor counts, Tensor free_blocks, Tensor n_free, int page_size, "
-        "int max_tokens, Tensor? parents=None) -> (Tensor, Tensor, Tensor, Tensor?, Tensor, Tensor)");
+        "int max_tokens, Tensor? parents=None) -> (Tensor(b), Tensor(b), Tensor(b), Tensor(b)?, Tensor(b), Tensor(b))");
   m.def("qk_norm_rope(Tensor qkv, Tensor positions, Tensor cos_sin, int n_heads, int n_kv_heads, Tensor? q_weight=None, "
         "Tensor? k_weight=None, float eps=1e-6, bool interleaved=False, Tensor(a!)? k_cache=None, Tensor(b!)? v_cache=None, "
-        "Tensor? slots=None, Tensor? k_scale=None, Tensor? v_scale=None, Tensor(c!)? out=None) -> (Tensor, Tensor?)");
+        "Tensor? slots=None, Tensor? k_scale=None, Tensor? v_scale=None, Tensor(c!)? out=None) -> (Tensor(c), Tensor?)");
   m.def("tree_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor kv_lens, Tensor cu_tokens, "
         "Tensor? masks=None, float? scale=None, Tensor? k_scale=None, Tensor? v_scale=None, Tensor(a!)? out=None, "
-        "bool return_lse=False) -> (Tensor, Tensor?)");
-  m.def("token_logprobs(Tensor logits, Tensor tokens, int top_k=0, float temperature=1.0) -> (Tensor, Tensor, Tensor, Tensor)");
+        "bool return_lse=False) -> (Tensor(a), Tensor?)");
+  m.def("token_logprobs(Tensor logits, Tensor tokens, int top_k=0, float temperature=1.0) -> (Tensor(a), Tensor(a), Tensor(a), Tensor(a))");
 }
 
 TORCH_LIBRARY_IMPL(my_ops, CompositeExplicitAutograd, m) {
