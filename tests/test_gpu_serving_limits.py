@@ -6,7 +6,7 @@ import torch
 
 import serving_plain as plain
 from test_gpu_attention_tiles import ROOM, attend, tile_rows, with_room
-from test_gpu_serving import STEPS, Step, ints, say
+from test_gpu_serving import STEPS, Step, check_rows, ints, say
 
 pytestmark = pytest.mark.gpu
 
@@ -195,6 +195,21 @@ def test_attention_of_large_values(pkg, dev, size, rise, rows, reqs, Hq, Hkv):
     out, lse = attend(pkg, dev, s, rows)
     assert bool(out.isfinite().all())
     s.check(out, lse)
+
+
+# ------------------------------------------------------------------------------------------------ qk_norm_rope
+@pytest.mark.parametrize("T,Hq,Hkv,D,R,pairs", [(5, 6, 2, 128, 64, True), (33, 8, 8, 96, 96, False), (613, 4, 3, 64, 64, False), (2049, 32, 4, 128, 128, False),
+                                               (70, 3, 1, 256, 128, True)])
+def test_norm_rope_of_many_tokens_without_a_cache(pkg, dev, T, Hq, Hkv, D, R, pairs):
+    say("qk_norm_rope without a cache", T, Hq, Hkv, D)
+    g = torch.Generator().manual_seed(T)
+    x = torch.randn(T, (Hq + 2 * Hkv) * D, generator=g).to(torch.bfloat16)
+    pos = torch.randint(-1, 41, (T,), generator=g).to(torch.int32)               # -1 and 40: no such places
+    cs, w = torch.randn(40, R, generator=g), [(1 + 0.3 * torch.randn(D, generator=g)).to(torch.bfloat16) for _ in range(2)]
+    q, k = pkg.qk_norm_rope(x.to(dev), pos.to(dev), cs.to(dev), Hq, Hkv, w[0].to(dev), w[1].to(dev), 1e-5, pairs)
+    heads = x.view(T, Hq + 2 * Hkv, D)
+    check_rows(q, plain.norm_rope(heads[:, :Hq], w[0], 1e-5, pos, cs, pairs), "q")
+    check_rows(k, plain.norm_rope(heads[:, Hq:Hq + Hkv], w[1], 1e-5, pos, cs, pairs), "k")
 
 
 # ------------------------------------------------------------------------------------------------ the registered ops
