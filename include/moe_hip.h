@@ -401,9 +401,11 @@ int moe_router_logits(void *stream, const void *x_bf16, int T, int H, const void
  * What one step needs, from lengths: request b holds lens[b] cached tokens and brings counts[b] new ones (0: idle).
  * New pages come from the top of the stack free_blocks[0 .. n_free), request by request, and are appended to
  * block_tables [B, table_width] (rows table_stride apart); n_free_out is what is left of the stack.  Nothing that
- * is written may overlap lens, counts, free_blocks, n_free or parents (MOE_E_MODE): lengths are not updated in place.  A request is refused - kv_lens 0, its rows' positions and slots -1, masks 0, its table untouched - when its tokens do not
- * fit its table row or the batch's T rows, when a tree has more than 64 tokens, or when the pages needed by it and the requests before it are more than
- * there are; the others are granted.  Outputs: cu_tokens [B + 1]; positions [T] int32 (a tree's token: cached
+ * is written may overlap lens, counts, free_blocks, n_free or parents (MOE_E_MODE): lengths are not updated in place.
+ * A request is refused - kv_lens 0, its rows' positions and slots -1, masks 0, its table untouched - when its tokens do not fit its table row, when
+ * they and those of the requests before it are more than the batch's T rows, when a tree has more than 64 tokens, or when the pages needed
+ * by it and by the requests before it that fit are more than there are.  Requests before it count there whether they were granted or not: once the rows
+ * are exceeded every later request is refused (one without tokens too), once the pages are every later one that needs any.  Outputs: cu_tokens [B + 1]; positions [T] int32 (a tree's token: cached
  * length + depth); slots [T]; masks [T] with parents (without: causal order, masks not written); kv_lens [B] = lens +
  * counts.  Rows of no request get -1 / -1 / 0.  B <= MOE_MAX_REQUESTS.  A caller that keeps fewer tokens than it brought puts the pages
  * that its lens no longer reach back on the stack.

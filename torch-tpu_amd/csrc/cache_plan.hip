@@ -1,8 +1,9 @@
 // Bookkeeping of a paged cache for one step, on the GPU and in one launch: which new pages each request gets, where its new
 // tokens' keys and values go, their positions, and which of a tree's drafted tokens each of them sees.
 //
-//   need_b = pages(len_b + n_b) - pages(len_b);  upto_b = need_0 + ... + need_b
-//   a request is granted its step when its tokens fit its table row and the batch's rows, and upto_b <= the free pages left;
+//   need_b = pages(len_b + n_b) - pages(len_b), 0 where the tokens do not fit;  upto_b = need_0 + ... + need_b
+//   a request is granted its step when its tokens fit its table row and the batch's rows, and upto_b <= the free pages: what
+//   requests before it need and bring counts, granted or not
 //   its i-th new page is free[n_free - 1 - (upto_b - need_b + i)]
 //
 // What bounds it is the launch and a chain of dependent reads (lengths -> sums -> free pages -> stores), not bytes, so it

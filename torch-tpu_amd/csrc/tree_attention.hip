@@ -409,8 +409,8 @@ __device__ __forceinline__ void attn_store(const AttnArgs &a, const AttnRequest 
 }
 
 // ---- few rows: the four wavefronts take the keys in turn --------------------------------------------------------------
-// Up to 16 rows to a cached key the cache's bytes bound it (64 requests, up to 8192 keys, bf16: 135 us, 4.9 TB/s, what a large copy reaches;
-// one request of 32767: 23.6 us, of which 14 are its bytes and the rest the chain of launch, lengths, tables, a tile's end and the join).  A wavefront takes 32 keys of a unit of 128 by itself: keys go
+// Up to 16 rows to a cached key the cache's bytes bound it (64 requests, up to 8192 keys, bf16: 134 us, 4.9 TB/s, what a large copy reaches;
+// one request of 32767: 23.4 us, of which 14 are its bytes and the rest the chain of launch, lengths, tables, a tile's end and the join).  A wavefront takes 32 keys of a unit of 128 by itself: keys go
 // from memory straight into operand registers, values through LDS that no other wavefront touches, so nothing waits at a
 // barrier, and the next keys and values are asked for before the present ones are worked on.  The wavefronts' results meet in
 // LDS at the end of a tile.
@@ -546,9 +546,10 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(const AttnArgs a) {
 }
 
 // ---- staging in LDS (the two kernels below) ---------------------------------------------------------------------------
-// Rows of a stage are 32 bytes longer than their values: operands are read without bank conflicts then (counted: none).  TPR
+// Rows of a stage are 32 bytes longer than their values, so that reads of operands spread over the banks.  TPR
 // threads write a row, 16 bytes of it at a time; which row thread group i takes is chosen so that the rows of one write fall into different
-// banks as well: four rows 4 apart, or of bytes widened to 32 apart 0, 1, 8 and 9.
+// banks as well: four rows 4 apart, or of bytes widened to 32 apart 0, 1, 8 and 9.  Counted: no conflicts in the kernel of many rows on
+// a bf16 cache; in the one of 128 rows on an e4m3 cache 2.7 of 10.1 million cycles at which LDS is read or written.
 template <bool FP8, int TPR>
 __device__ __forceinline__ int attn_stage_row(int i) {
   if (FP8) return TPR == 4 ? (i & ~15) | (i & 1) | (i & 2) << 2 | (i >> 1 & 6) : i;
@@ -589,9 +590,9 @@ __device__ __forceinline__ void attn_put_values(uint8_t *at, const v4i (&raw)[NU
 // Up to about 128 rows to a cached key both the bytes and the products count.  A workgroup stages 64 keys and values at a time in
 // LDS, two stages of them, and every wavefront takes its rows past all of them, one barrier a stage; 16s of rows go to the wavefronts in turn, so that
 // a tile that is not full keeps all at work (57 requests of about 145 rows: 108 us, 117 with neighbouring 16s together).  The bytes of the stage after
-// that wait in registers (of two stages after it: no faster).  32 trees of up to 16 tokens over up to 8001 e4m3 keys: 71 us, 2.35 TB/s and
-// 354 TFLOP/s; without the work on the stages 54, without the stages 56: two workgroups to a compute unit overlap the two in part, and
-// LDS and registers hold no third.
+// that wait in registers (of two stages after it: no faster).  32 trees of up to 16 tokens over up to 8001 e4m3 keys: 69.5 us, 2.4 TB/s and
+// 361 TFLOP/s; without the work on the stages 54, without the stages 56: two workgroups to a compute unit overlap the two in part, and
+// LDS and registers hold no third.  (Codes are widened before they go to LDS, so an e4m3 cache has the stages of a bf16 one.)
 template <int D, bool FP8, int NQ>
 __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const AttnArgs a) {
   constexpr int ROWS = 64 * NQ, UNIT = 64, DT = D / 16, LD = 2 * D + 32, STAGE = 2 * UNIT * LD;
@@ -698,9 +699,10 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const AttnArgs a) {
 // A barrier ends a slot.  While it weighs unit c a wavefront also stages its share of the keys of c + 1 and the values of c, the
 // second group's a unit further on, so that each stage is whole a slot before the first group needs it and is written when the second
 // group has left it (two stages of each).  The 16s of rows go to the wavefronts in turn here too.
-// Two chunks of 1021 tokens over 8190 keys: 224 to 238 us, 843 to 893 TFLOP/s where a large product alone reaches 1254; without the reads of
-// operands from LDS 5 % less, without the exponentials 5 to 8 %, without staging 10 to 17 %: every slot is full of instructions.
-// 16 trees of up to 64 tokens over up to 12288 keys: 123 us, 600 TFLOP/s (tiles that are not full, and a join of 11 us).
+// Two chunks of 1021 tokens over 8190 keys: 219 to 238 us, 843 to 913 TFLOP/s where a large product alone reaches 1254; without the reads of
+// operands from LDS 5 % less, without the exponentials 5 to 8 %, without staging 10 to 17 %.  Counted for a SIMD: the matrix cores are busy 196
+// thousand clocks, the vector unit 220 thousand, of about 460 thousand: the two still add up more than they overlap.
+// 16 trees of up to 64 tokens over up to 12288 keys: 119 to 124 us, 600 to 622 TFLOP/s (tiles that are not full, and a join of 12 us).
 template <int D, bool FP8, int NQ>
 __global__ __launch_bounds__(512, 2) void attn_pairs_kernel(const AttnArgs a) {
   constexpr int ROWS = 128 * NQ, UNIT = 64, DT = D / 16, X = D / 32, LD = 2 * D + 32, HALF = UNIT * LD;
@@ -916,8 +918,16 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
 //   400   1 x 400 x 2048, causal, no shared heads
 //                                         29           33           37
 // Large tiles read a key for more rows, small ones are more stretches at work and fewer, smaller parts to join.  Up to so many products of
-// row and key (with the table's width, as the lengths are on the device) the latter counts.  16 rows: two workgroups to a compute unit
+// row and key the latter counts.  16 rows: two workgroups to a compute unit
 // for e4m3, whose loads are half as long (256 requests of 2048 keys: 90 us with 512 workgroups, 105 with 256; bf16 146 and 141).
+// Lengths are on the device, so the rule takes the table's width for them, and the average over all B requests for a request's rows.  Where these
+// mislead it the call is right, but slower, us:
+//   4 x 64 x 2048 with a table of 8192: 42 (38 in tiles of 64 rows); 1 x 64 x 8192 with one of 131072: 54 (43)
+//   4 x 64 x 2048 beside 252 idle requests: 72;  511 x 1 x 1000 and a prompt of 512 in one call: 1613 (206 and 42 in two), 255 x 1 x 2048 and one
+//   of 1024: 530.  (16 rows for the prompt: as many passes over its keys, and the walk)
+// The walk along the line takes its time too: a piece of a causal request adds up all tiles of the request (attn_head_units), so that a prompt of 8192
+// tokens from its start takes 1610 us of which 760 are the walk's, and requests without tokens are passed one by one (two single tokens over
+// 2048 keys: 17, with 4000 idle requests between them 54).
 struct AttnPlan {
   int rows, groups;                    // rows of a tile; workgroups, a multiple of 8
   float cut;

@@ -7,7 +7,8 @@
     said = token_logprobs(logits, tokens, top_k=8)
 
 The functions are thin: the operators of the same names in torch.ops.my_ops check, allocate and launch (csrc/serving_ops.cpp).
-Everything stays on the device, so that a step can be captured into a graph.  Inference only.
+Everything stays on the device, so that a step can be captured into a graph.  Inference only: a backward pass through them warns and
+gives no gradient.
 """
 from __future__ import annotations
 
@@ -43,8 +44,9 @@ def cache_plan(block_tables, lens, counts, free_blocks, n_free, page_size: int, 
     free_blocks [F] int32 with n_free [1] int32 of them free, taken from the top; page_size a power of two up to 1024;
     max_tokens rows of the batch; parents [max_tokens] int32: each drafted token's parent among its request's tokens,
     -1 for none (trees of at most 64 tokens), or None: every request's tokens follow one another.
-    A request that finds no room - in its table row, the batch, or the free pages left by those before it - is refused: kv_lens 0,
-    slots -1."""
+    A request that finds no room - in its table row, the batch's rows, or the free pages - is refused: kv_lens 0, slots -1.
+    It still counts against the rows and pages of those after it: once the rows are exceeded all later requests are
+    refused, once the pages are all later ones that need any."""
     return CachePlan(*_ops.cache_plan.default(block_tables, lens, counts, free_blocks, n_free, page_size, max_tokens, parents))
 
 
