@@ -62,6 +62,7 @@ extern "C" {
 #define MOE_MAX_TOPK    32
 #define MOE_MAX_REQUESTS 4096   /* requests of one step of the paged cache */
 #define MOE_MAX_PAGE    1024    /* tokens of a cache page (a power of two) */
+#define MOE_MAX_BIASES  2047    /* biased tokens of a request */
 
 /*
  * Library version and the gfx target it was built for.  The version changes whenever a caller built against an
@@ -462,6 +463,38 @@ size_t moe_token_logprobs_workspace_bytes(int T, int V, int k, int logits_dtype)
 int moe_token_logprobs(void *stream, const void *logits, int logits_dtype, int64_t row_stride, int T, int V, const int64_t *tokens,
                        int k, float temperature, float *logprobs, float *entropy, float *top_logprobs, int32_t *top_ids,
                        void *workspace, size_t workspace_bytes);
+
+/*
+ * Between two blocks: u = x rsqrt(mean(x^2) + eps) post_weight (x itself without a post_weight), h = residual + scale gate u, y =
+ * h rsqrt(mean(h^2) + eps) weight.  x [T, H] bf16, residual [T, H] of residual_dtype or NULL (0), weights [H] of weight_dtype or NULL (y:
+ * weights of 1), gate of gate_dtype or NULL (1), its value of row t and column c at t gate_row_stride + c gate_col_stride, of which either
+ * may be 0 and the second at most 1.  y [T, H] bf16 from the h before its rounding; residual_out [T, H] of residual_dtype = h, or NULL.  Rows at any
+ * distance.  y and residual_out may each take the place of x or residual, row on row; otherwise nothing written may lie over what is read (MOE_E_MODE).
+ * H at most 32768; 16384 where H, a distance or a pointer does not divide into 16 bytes.
+ */
+int moe_residual_norm(void *stream, const void *x_bf16, int64_t x_stride, int T, int H, const void *residual, int residual_dtype,
+                      int64_t residual_stride, const void *weight, const void *post_weight, int weight_dtype, const void *gate,
+                      int gate_dtype, int64_t gate_row_stride, int64_t gate_col_stride, float scale, float eps, void *y_bf16,
+                      int64_t y_stride, void *residual_out, int64_t residual_out_stride);
+
+/*
+ * What requests ask of their logits [T, V] (fp32 or bf16, rows row_stride apart), -> out in the same type, which may be logits itself.
+ * Request b has rows [cu_tokens[b], cu_tokens[b + 1]) (cu_tokens NULL: row b, B = T) and a history [B, L] int32 (rows history_stride apart) of
+ * history_lens[b] tokens (NULL: L), the first prompt_lens[b] of them its prompt (NULL: none).  With tokens [T] int64 a row's history goes on with the
+ * tokens of its request that its mask names (masks [T] int64, up to 64 tokens a request; NULL: those up to its own).  Of a
+ * token that was generated n times (history after the prompt, and path), or heard in the prompt only:
+ *   x = x > 0 ? x / repetition[b] : x repetition[b];  x -= frequency[b] n + presence[b] (n > 0);   (fp32 [B], NULL: 1, 0, 0)
+ * Then bias[b][i] is added to token bias_ids[b][i], i < n_bias (of equal ids the last counts), and what allowed does not
+ * name becomes -inf: bit v % 32 of word v / 32 of row allowed_rows[t] (NULL: t, n_allowed = T) of allowed [n_allowed][ceil(V / 32)]; a row
+ * outside [0, n_allowed): everything is allowed.  fp32, one rounding.  Ids outside [0, V) are passed over; rows of no request pass
+ * as they are.  L + T below 2^20, n_bias at most MOE_MAX_BIASES.
+ */
+int moe_adjust_logits(void *stream, const void *logits, int dtype, int64_t row_stride, int T, int V, const int32_t *cu_tokens, int B,
+                      const int32_t *history, int64_t history_stride, int L, const int32_t *history_lens, const int32_t *prompt_lens,
+                      const int64_t *tokens, const int64_t *masks, const float *repetition, const float *frequency,
+                      const float *presence, const int32_t *bias_ids, int64_t bias_ids_stride, const float *bias, int64_t bias_stride,
+                      int n_bias, const int32_t *allowed, int64_t allowed_stride, int n_allowed, const int32_t *allowed_rows,
+                      void *out, int64_t out_stride);
 
 #ifdef __cplusplus
 }

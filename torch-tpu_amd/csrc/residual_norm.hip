@@ -1,0 +1,243 @@
+// What stands between two blocks of a decoder, in one pass over its rows:
+//
+//   u = x                                            the block's output
+//   u = u rsqrt(mean(u^2) + eps) post_weight         (with a post_weight)
+//   h = residual + scale gate u                      the residual stream
+//   y = h rsqrt(mean(h^2) + eps) weight              the next block's input
+//
+// Bound by bytes: every value is read once and written once, so a row stays in the registers of the wavefronts that share it, sums of
+// squares are added over lanes by data-parallel moves and over wavefronts in LDS, and y is formed from the h in registers, before
+// its rounding.  All of it in fp32 with one rounding to each output.
+#include "moe_common.h"
+#include "lanes.h"
+#include "../../include/moe_hip.h"
+
+namespace moe {
+
+struct NormArgs {
+  const uint16_t *x;
+  int64_t x_stride;
+  const void *residual;
+  int64_t residual_stride;
+  const void *weight, *post_weight, *gate;
+  int64_t gate_row, gate_col;          // strides, of which either may be 0: the same for all rows, for all columns
+  uint16_t *y;
+  void *h;
+  int64_t y_stride, h_stride;
+  float scale, eps, over_h;            // 1 / H
+  int T, H, residual_f32, weight_f32, gate_f32;
+};
+
+// N neighbouring values, N = 8 on 16 bytes
+template <int N>
+__device__ __forceinline__ void norm_load(const void *base, int64_t at, bool f32, float (&v)[N]) {
+  if (f32) {
+    const float *p = (const float *)base + at;
+    if constexpr (N == 8) {
+      const v4f a = *(const v4f *)p, b = *(const v4f *)(p + 4);
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
+    } else {
+      v[0] = *p;
+    }
+  } else {
+    const uint16_t *p = (const uint16_t *)base + at;
+    if constexpr (N == 8) {
+      const v4i w = *(const v4i *)p;
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[2 * i] = __uint_as_float((uint32_t)w[i] << 16), v[2 * i + 1] = __uint_as_float((uint32_t)w[i] & 0xffff0000u);
+    } else {
+      v[0] = bf16_to_f32(*p);
+    }
+  }
+}
+template <int N>
+__device__ __forceinline__ void norm_store(void *base, int64_t at, bool f32, const float (&v)[N]) {
+  if (f32) {
+    float *p = (float *)base + at;
+    if constexpr (N == 8) {
+      *(v4f *)p = (v4f){v[0], v[1], v[2], v[3]};
+      *(v4f *)(p + 4) = (v4f){v[4], v[5], v[6], v[7]};
+    } else {
+      *p = v[0];
+    }
+  } else {
+    uint16_t *p = (uint16_t *)base + at;
+    if constexpr (N == 8) *(v4i *)p = (v4i){(int)pack2_bf16(v[0], v[1]), (int)pack2_bf16(v[2], v[3]), (int)pack2_bf16(v[4], v[5]), (int)pack2_bf16(v[6], v[7])};
+    else *p = (uint16_t)pack2_bf16(v[0], 0.f);
+  }
+}
+
+// The sum over the WAVES wavefronts of a row; `turn` names the sum, so that a second one needs no barrier of its own.
+template <int WAVES>
+__device__ __forceinline__ float row_sum(float v, int turn) {
+  v = lane_sum<64>(v);
+  if constexpr (WAVES > 1) {
+    __shared__ float sh[2][WAVES];
+    if ((threadIdx.x & 63) == 0) sh[turn][threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < WAVES; i++) v += sh[turn][i];
+  }
+  return v;
+}
+
+// A row to WAVES wavefronts, P pieces of N values to a lane.  One wavefront a row: four rows to a workgroup.
+template <int WAVES, int P, int N>
+__global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) void residual_norm_kernel(const NormArgs a) {
+  constexpr int ROWS = WAVES > 1 ? 1 : 4, LANES = 64 * WAVES;
+  const int64_t t = (int64_t)blockIdx.x * ROWS + (WAVES > 1 ? 0 : threadIdx.x >> 6);
+  if (t >= a.T) return;                                // (whole wavefronts, and no barrier where there are several rows)
+  const int lane = WAVES > 1 ? threadIdx.x : threadIdx.x & 63;
+  float u[P][N], h[P][N], w[N > 1 ? P : 1][N];
+  const auto place = [&](int p) { return (p * LANES + lane) * N; };
+  const auto live = [&](int p) { return place(p) < a.H; };
+  // one by one, many pieces to a lane: weights are read where they are used, or they would not fit beside the row
+  const auto weights = [&](const void *from, int p) -> float (&)[N] {
+    float (&to)[N] = w[N > 1 ? p : 0];
+#pragma unroll
+    for (int i = 0; i < N; i++) to[i] = 1.f;
+    if (from && live(p)) norm_load<N>(from, place(p), a.weight_f32, to);
+    return to;
+  };
+#pragma unroll
+  for (int p = 0; p < P; p++) {
+    const int e = place(p);
+#pragma unroll
+    for (int i = 0; i < N; i++) u[p][i] = h[p][i] = 0.f;
+    if (!live(p)) continue;
+    norm_load<N>(a.x, t * a.x_stride + e, false, u[p]);
+    if (a.residual) norm_load<N>(a.residual, t * a.residual_stride + e, a.residual_f32, h[p]);
+  }
+  if (a.post_weight) {
+    float sum = 0.f;
+#pragma unroll
+    for (int p = 0; p < P; p++)
+#pragma unroll
+      for (int i = 0; i < N; i++) sum = fmaf(u[p][i], u[p][i], sum);
+    if (N > 1) {
+#pragma unroll
+      for (int p = 0; p < P; p++) weights(a.post_weight, p);
+    }
+    const float r = 1.0f / sqrtf(row_sum<WAVES>(sum, 0) * a.over_h + a.eps);
+#pragma unroll
+    for (int p = 0; p < P; p++) {
+      const float (&by)[N] = N > 1 ? w[N > 1 ? p : 0] : weights(a.post_weight, p);
+#pragma unroll
+      for (int i = 0; i < N; i++) u[p][i] *= r * by[i];
+    }
+  }
+  if (a.gate) {
+#pragma unroll
+    for (int p = 0; p < P; p++) {
+      if (!live(p)) continue;
+      float g[N];
+      if (a.gate_col) {
+        norm_load<N>(a.gate, t * a.gate_row + place(p), a.gate_f32, g);
+      } else {
+        const float one = a.gate_f32 ? ((const float *)a.gate)[t * a.gate_row] : bf16_to_f32(((const uint16_t *)a.gate)[t * a.gate_row]);
+#pragma unroll
+        for (int i = 0; i < N; i++) g[i] = one;
+      }
+#pragma unroll
+      for (int i = 0; i < N; i++) u[p][i] *= g[i];
+    }
+  }
+  float sum = 0.f;
+#pragma unroll
+  for (int p = 0; p < P; p++) {
+    if (N > 1) weights(a.weight, p);                   // (before the wait for the sum)
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      h[p][i] = fmaf(a.scale, u[p][i], h[p][i]);
+      sum = fmaf(h[p][i], h[p][i], sum);
+    }
+    if (live(p) && a.h) norm_store<N>(a.h, t * a.h_stride + place(p), a.residual_f32, h[p]);
+  }
+  const float r = 1.0f / sqrtf(row_sum<WAVES>(sum, 1) * a.over_h + a.eps);
+#pragma unroll
+  for (int p = 0; p < P; p++) {
+    if (!live(p)) continue;
+    const float (&by)[N] = N > 1 ? w[N > 1 ? p : 0] : weights(a.weight, p);
+#pragma unroll
+    for (int i = 0; i < N; i++) h[p][i] *= r * by[i];
+    norm_store<N>(a.y, t * a.y_stride + place(p), false, h[p]);
+  }
+}
+
+// Whether rows of `bytes` bytes, T of them `stride` bytes apart, share memory with others; the same rows do not count.
+static bool rows_clash(const void *a, int64_t a_stride, int64_t a_bytes, const void *b, int64_t b_stride, int64_t b_bytes, int64_t T) {
+  if (!a || !b || T == 0) return false;
+  const uint8_t *p = (const uint8_t *)a, *q = (const uint8_t *)b;
+  if (p == q && (T == 1 || a_stride == b_stride) && a_bytes == b_bytes) return false;
+  if (p + (T - 1) * a_stride + a_bytes <= q || q + (T - 1) * b_stride + b_bytes <= p) return false;
+  if (T == 1 || a_stride != b_stride || a_stride <= 0) return true;
+  const int64_t off = ((q - p) % a_stride + a_stride) % a_stride;
+  return off < a_bytes || a_stride - off < b_bytes;
+}
+
+}  // namespace moe
+
+extern "C" int moe_residual_norm(void *stream, const void *x_bf16, int64_t x_stride, int T, int H, const void *residual, int residual_dtype,
+                                 int64_t residual_stride, const void *weight, const void *post_weight, int weight_dtype, const void *gate,
+                                 int gate_dtype, int64_t gate_row_stride, int64_t gate_col_stride, float scale, float eps, void *y_bf16,
+                                 int64_t y_stride, void *residual_out, int64_t residual_out_stride) {
+  using namespace moe;
+  for (const int t : {residual_dtype, weight_dtype, gate_dtype})
+    if (t != MOE_DTYPE_F32 && t != MOE_DTYPE_BF16) return MOE_E_MODE;
+  if (T < 0 || H < 1 || H > 32768 || x_stride < H || y_stride < H || (residual && residual_stride < H) || (residual_out && residual_out_stride < H) ||
+      !(eps >= 0.f))
+    return MOE_E_SHAPE;
+  if (gate && (gate_row_stride < 0 || gate_col_stride < 0 || gate_col_stride > 1 || (gate_row_stride && gate_col_stride && gate_row_stride < H)))
+    return MOE_E_SHAPE;
+  if (T == 0) return MOE_OK;
+  if (!x_bf16 || !y_bf16) return MOE_E_NULL;
+  const int64_t rb = residual_dtype == MOE_DTYPE_F32 ? 4 : 2, wb = weight_dtype == MOE_DTYPE_F32 ? 4 : 2, gb = gate_dtype == MOE_DTYPE_F32 ? 4 : 2;
+  for (const void *p : {x_bf16, (const void *)y_bf16})
+    if ((uintptr_t)p % 2) return MOE_E_ALIGN;
+  if ((uintptr_t)residual % rb || (uintptr_t)residual_out % rb || (uintptr_t)weight % wb || (uintptr_t)post_weight % wb || (uintptr_t)gate % gb)
+    return MOE_E_ALIGN;
+  // What is written lies over nothing that is read, but a row may take the place of the row that it comes from.
+  const int64_t xs = 2 * x_stride, ys = 2 * y_stride, rs = rb * residual_stride, hs = rb * residual_out_stride, row = 2ll * H, wide = rb * H;
+  const int64_t gate_rows = gate_row_stride ? T : 1, gate_row = gb * (gate_col_stride ? H : 1);
+  const auto over = [&](const void *p, int64_t stride, int64_t bytes) {
+    if (rows_clash(p, stride, bytes, x_bf16, xs, row, T) || rows_clash(p, stride, bytes, residual, rs, wide, T)) return true;
+    for (const void *w : {weight, post_weight})
+      if (w && (const uint8_t *)p < (const uint8_t *)w + wb * H && (const uint8_t *)w < (const uint8_t *)p + (T - 1) * stride + bytes) return true;
+    return gate && (const uint8_t *)p < (const uint8_t *)gate + (gate_rows - 1) * gate_row_stride * gb + gate_row &&
+           (const uint8_t *)gate < (const uint8_t *)p + (T - 1) * stride + bytes;
+  };
+  if (over(y_bf16, ys, row) || (residual_out && (over(residual_out, hs, wide) || residual_out == y_bf16 || rows_clash(residual_out, hs, wide, y_bf16, ys, row, T))))
+    return MOE_E_MODE;
+  NormArgs a{(const uint16_t *)x_bf16, x_stride, residual, residual_stride, weight, post_weight, gate, gate_row_stride, gate_col_stride,
+             (uint16_t *)y_bf16, residual_out, y_stride, residual_out_stride, scale, eps, 1.0f / (float)H, T, H,
+             residual_dtype == MOE_DTYPE_F32, weight_dtype == MOE_DTYPE_F32, gate_dtype == MOE_DTYPE_F32};
+  // 8 values at a time where every row begins on 16 bytes of them, else one.
+  bool whole = H % 8 == 0 && x_stride % 8 == 0 && y_stride % 8 == 0 && (!residual || residual_stride % 8 == 0) &&
+               (!residual_out || residual_out_stride % 8 == 0) && (!gate || !gate_col_stride || gate_row_stride % 8 == 0);
+  for (const void *p : {x_bf16, (const void *)y_bf16, residual, (const void *)residual_out, weight, post_weight, gate_col_stride ? gate : nullptr})
+    whole = whole && (uintptr_t)p % 16 == 0;
+  if (!whole && H > 16384) return MOE_E_ALIGN;          // (a row of single values would not fit the registers)
+  hipStream_t st = (hipStream_t)stream;
+  const unsigned grid = (unsigned)T;
+#define RUN(W, P, N) residual_norm_kernel<W, P, N><<<W == 1 ? (grid + 3) / 4 : grid, W == 1 ? 256 : 64 * W, 0, st>>>(a)
+  if (whole) {
+    const int pieces = H / 8;
+    if (pieces <= 64) RUN(1, 1, 8);
+    else if (pieces <= 128) RUN(2, 1, 8);
+    else if (pieces <= 256) RUN(4, 1, 8);
+    else if (pieces <= 512) RUN(4, 2, 8);
+    else if (pieces <= 1024) RUN(8, 2, 8);
+    else if (pieces <= 2048) RUN(16, 2, 8);
+    else RUN(16, 4, 8);
+  } else {
+    if (H <= 256) RUN(1, 4, 1);
+    else if (H <= 1024) RUN(4, 4, 1);
+    else if (H <= 2048) RUN(4, 8, 1);
+    else if (H <= 8192) RUN(16, 8, 1);
+    else RUN(16, 16, 1);
+  }
+#undef RUN
+  return (int)hipGetLastError();
+}

@@ -1,5 +1,5 @@
 // Operators of a serving step around the MoE layer in the namespace my_ops: cache_plan, qk_norm_rope, tree_attention,
-// token_logprobs (include/moe_hip.h has their definitions).  Plain host C++ on the C ABI, as my_ops.cpp: at decode sizes
+// token_logprobs, residual_norm, adjust_logits (include/moe_hip.h has their definitions).  Plain host C++ on the C ABI, as my_ops.cpp: at decode sizes
 // a call's checks and allocations in Python would take longer than its kernel.  Results are allocated here where
 // the caller hands none over; the current device's current stream is used; argument errors through TORCH_CHECK.
 // Inference only: none of them records a gradient.
@@ -250,6 +250,133 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor &logits, 
   return {lp, entropy, top, ids};
 }
 
+int float_kind(const Tensor &t, const char *name) {
+  TORCH_CHECK(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, name, " must be float32 or bfloat16");
+  return t.scalar_type() == at::kFloat ? MOE_DTYPE_F32 : MOE_DTYPE_BF16;
+}
+void need_matrix(const Tensor &t, const char *name, int64_t rows, int64_t cols, const Tensor &like) {
+  need_gpu(t, name, like);
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == cols, name, " must be [", rows, ", ", cols, "], got ", t.sizes());
+  need_rows(t, name);
+}
+
+std::tuple<Tensor, Tensor> residual_norm(const Tensor &x, const OptTensor &residual, const OptTensor &weight, const OptTensor &post_weight,
+                                         const OptTensor &gate, double scale, double eps, const OptTensor &out,
+                                         const OptTensor &residual_out) {
+  TORCH_CHECK(x.dim() == 2 && x.scalar_type() == at::kBFloat16, "x must be [tokens, width] bfloat16");
+  need_gpu(x, "x", x);
+  need_rows(x, "x");
+  const int64_t T = x.size(0), H = x.size(1);
+  int residual_kind = MOE_DTYPE_BF16, weight_kind = MOE_DTYPE_BF16, gate_kind = MOE_DTYPE_BF16;
+  if (residual) {
+    need_matrix(*residual, "residual", T, H, x);
+    residual_kind = float_kind(*residual, "residual");
+  } else if (residual_out) {
+    residual_kind = float_kind(*residual_out, "residual_out");
+  }
+  for (const auto &[w, name] : {std::pair<const OptTensor &, const char *>(weight, "weight"), {post_weight, "post_weight"}})
+    if (w) {
+      weight_kind = float_kind(*w, name);
+      need_vector(*w, name, w->scalar_type(), H, x);
+    }
+  TORCH_CHECK(!weight || !post_weight || weight->scalar_type() == post_weight->scalar_type(), "weight and post_weight must have the same dtype");
+  int64_t gate_row = 0, gate_col = 0;
+  if (gate) {
+    need_gpu(*gate, "gate", x);
+    gate_kind = float_kind(*gate, "gate");
+    TORCH_CHECK((gate->dim() == 1 && gate->size(0) == H) ||
+                    (gate->dim() == 2 && (gate->size(0) == T || gate->size(0) == 1) && (gate->size(1) == H || gate->size(1) == 1)),
+                "gate must be [width], or [tokens or 1, width or 1], got ", gate->sizes());
+    const int64_t rows = gate->dim() == 2 ? gate->size(0) : 1, cols = gate->size(-1);
+    TORCH_CHECK(cols == 1 || gate->stride(-1) == 1, "gate must have contiguous rows");
+    gate_col = cols > 1 ? 1 : 0;
+    gate_row = rows > 1 ? gate->stride(0) : 0;
+  }
+  c10::DeviceGuard guard(x.device());
+  const auto result = [&](const OptTensor &given, const char *name, at::ScalarType kind) {
+    if (!given) return at::empty({T, H}, x.options().dtype(kind));
+    need_matrix(*given, name, T, H, x);
+    TORCH_CHECK(given->scalar_type() == kind, name, " must be ", kind, ", got ", given->scalar_type());
+    return *given;
+  };
+  const Tensor y = result(out, "out", at::kBFloat16), h = result(residual_out, "residual_out", residual_kind == MOE_DTYPE_F32 ? at::kFloat : at::kBFloat16);
+  check_rc(moe_residual_norm(current_stream(x), x.data_ptr(), row_stride(x), fits_int(T, "tokens"), fits_int(H, "width"),
+                             data_or_null<void>(residual), residual_kind, residual ? row_stride(*residual) : 0, data_or_null<void>(weight),
+                             data_or_null<void>(post_weight), weight_kind, data_or_null<void>(gate), gate_kind, gate_row, gate_col, (float)scale,
+                             (float)eps, y.data_ptr(), row_stride(y), h.data_ptr(), row_stride(h)),
+           "residual_norm");
+  return {y, h};
+}
+
+Tensor adjust_logits(const Tensor &logits, const OptTensor &cu_tokens, const OptTensor &history, const OptTensor &history_lens,
+                     const OptTensor &prompt_lens, const OptTensor &tokens, const OptTensor &masks, const OptTensor &repetition,
+                     const OptTensor &frequency, const OptTensor &presence, const OptTensor &bias_ids, const OptTensor &bias,
+                     const OptTensor &allowed, const OptTensor &allowed_rows, const OptTensor &out) {
+  TORCH_CHECK(logits.dim() == 2, "logits must be [tokens, vocabulary]");
+  const int kind = float_kind(logits, "logits");
+  need_gpu(logits, "logits", logits);
+  need_rows(logits, "logits");
+  const int64_t T = logits.size(0), V = logits.size(1);
+  if (cu_tokens) {
+    TORCH_CHECK(cu_tokens->dim() == 1 && cu_tokens->size(0) > 0, "cu_tokens must hold requests + 1 values");
+    need_vector(*cu_tokens, "cu_tokens", at::kInt, cu_tokens->size(0), logits);
+  }
+  const int64_t B = cu_tokens ? cu_tokens->size(0) - 1 : T;
+  int64_t L = 0;
+  if (history) {
+    TORCH_CHECK(history->dim() == 2 && history->scalar_type() == at::kInt, "history must be [requests, tokens] int32");
+    L = history->size(1);
+    need_matrix(*history, "history", B, L, logits);
+  }
+  TORCH_CHECK(history.has_value() || (!history_lens && !prompt_lens), "history_lens and prompt_lens belong to a history");
+  if (history_lens) need_vector(*history_lens, "history_lens", at::kInt, B, logits);
+  if (prompt_lens) need_vector(*prompt_lens, "prompt_lens", at::kInt, B, logits);
+  if (tokens) need_vector(*tokens, "tokens", at::kLong, T, logits);
+  TORCH_CHECK(tokens.has_value() || !masks, "masks belong to tokens");
+  if (masks) need_vector(*masks, "masks", at::kLong, T, logits);
+  if (repetition) need_vector(*repetition, "repetition", at::kFloat, B, logits);
+  if (frequency) need_vector(*frequency, "frequency", at::kFloat, B, logits);
+  if (presence) need_vector(*presence, "presence", at::kFloat, B, logits);
+  TORCH_CHECK(bias_ids.has_value() == bias.has_value(), "bias_ids and bias belong together");
+  int64_t n_bias = 0;
+  if (bias_ids) {
+    TORCH_CHECK(bias_ids->dim() == 2 && bias_ids->scalar_type() == at::kInt, "bias_ids must be [requests, biases] int32");
+    TORCH_CHECK(bias->scalar_type() == at::kFloat, "bias must be float32");
+    n_bias = bias_ids->size(1);
+    need_matrix(*bias_ids, "bias_ids", B, n_bias, logits);
+    need_matrix(*bias, "bias", B, n_bias, logits);
+  }
+  TORCH_CHECK(allowed.has_value() || !allowed_rows, "allowed_rows belong to allowed");
+  int64_t n_allowed = 0;
+  if (allowed) {
+    TORCH_CHECK(allowed->dim() == 2 && allowed->scalar_type() == at::kInt, "allowed must be [rows, vocabulary / 32] int32");
+    n_allowed = allowed->size(0);
+    need_matrix(*allowed, "allowed", n_allowed, (V + 31) / 32, logits);
+    if (allowed_rows) need_vector(*allowed_rows, "allowed_rows", at::kInt, T, logits);
+    else TORCH_CHECK(n_allowed == T, "allowed without allowed_rows must have a row for each of logits");
+  }
+  c10::DeviceGuard guard(logits.device());
+  Tensor x;
+  if (out) {
+    need_matrix(*out, "out", T, V, logits);
+    TORCH_CHECK(out->scalar_type() == logits.scalar_type(), "out must have the dtype of logits");
+    x = *out;
+  } else {
+    x = at::empty({T, V}, logits.options());
+  }
+  check_rc(moe_adjust_logits(current_stream(logits), logits.data_ptr(), kind, row_stride(logits), fits_int(T, "tokens"), fits_int(V, "vocabulary"),
+                             data_or_null<int32_t>(cu_tokens), fits_int(B, "requests"), data_or_null<int32_t>(history),
+                             history ? row_stride(*history) : 0, fits_int(L, "history"), data_or_null<int32_t>(history_lens),
+                             data_or_null<int32_t>(prompt_lens), data_or_null<int64_t>(tokens), data_or_null<int64_t>(masks),
+                             data_or_null<float>(repetition), data_or_null<float>(frequency), data_or_null<float>(presence),
+                             data_or_null<int32_t>(bias_ids), bias_ids ? row_stride(*bias_ids) : 0, data_or_null<float>(bias),
+                             bias ? row_stride(*bias) : 0, fits_int(n_bias, "biases"), data_or_null<int32_t>(allowed),
+                             allowed ? row_stride(*allowed) : 0, fits_int(n_allowed, "allowed"), data_or_null<int32_t>(allowed_rows), x.data_ptr(),
+                             row_stride(x)),
+           "adjust_logits");
+  return x;
+}
+
 }  // namespace
 
 // What a schema says of memory: (a!) is written, a result (a) is that tensor where it is handed over, results with the same letter share an
@@ -264,6 +391,11 @@ TORCH_LIBRARY_FRAGMENT(my_ops, m) {
         "Tensor? masks=None, float? scale=None, Tensor? k_scale=None, Tensor? v_scale=None, Tensor(a!)? out=None, "
         "bool return_lse=False) -> (Tensor(a), Tensor?)");
   m.def("token_logprobs(Tensor logits, Tensor tokens, int top_k=0, float temperature=1.0) -> (Tensor(a), Tensor(a), Tensor(a), Tensor(a))");
+  m.def("residual_norm(Tensor x, Tensor? residual=None, Tensor? weight=None, Tensor? post_weight=None, Tensor? gate=None, "
+        "float scale=1.0, float eps=1e-6, Tensor(a!)? out=None, Tensor(b!)? residual_out=None) -> (Tensor(a), Tensor(b))");
+  m.def("adjust_logits(Tensor logits, Tensor? cu_tokens=None, Tensor? history=None, Tensor? history_lens=None, Tensor? prompt_lens=None, "
+        "Tensor? tokens=None, Tensor? masks=None, Tensor? repetition=None, Tensor? frequency=None, Tensor? presence=None, "
+        "Tensor? bias_ids=None, Tensor? bias=None, Tensor? allowed=None, Tensor? allowed_rows=None, Tensor(a!)? out=None) -> Tensor(a)");
 }
 
 TORCH_LIBRARY_IMPL(my_ops, CompositeExplicitAutograd, m) {
@@ -271,4 +403,6 @@ TORCH_LIBRARY_IMPL(my_ops, CompositeExplicitAutograd, m) {
   m.impl("qk_norm_rope", qk_norm_rope);
   m.impl("tree_attention", tree_attention);
   m.impl("token_logprobs", token_logprobs);
+  m.impl("residual_norm", residual_norm);
+  m.impl("adjust_logits", adjust_logits);
 }

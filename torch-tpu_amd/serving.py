@@ -81,3 +81,30 @@ def token_logprobs(logits, tokens, top_k: int = 0, temperature: float = 1.0) -> 
     entropy, and its top_k <= 32 most likely tokens (equal logits: the lower index first).  -inf logits are masked tokens;
     a row of nothing else gives -inf and entropy 0; a token outside [0, V) gives -inf; NaN or +inf in a row give NaN."""
     return TokenLogprobs(*_ops.token_logprobs.default(logits, tokens, top_k, temperature))
+
+
+def residual_norm(x, residual=None, weight=None, post_weight=None, gate=None, scale: float = 1.0, eps: float = 1e-6, out=None,
+                  residual_out=None):
+    """What stands between two blocks, in one pass: a norm of the block's output, its gate, the residual, a norm for the next block.
+
+    u = x rsqrt(mean(x^2) + eps) post_weight (x itself without a post_weight);  h = residual + scale gate u;
+    y = h rsqrt(mean(h^2) + eps) weight.  x [T, H] bf16; residual [T, H] bf16 or float32 (None: 0); weights [H] bf16 or float32 (both alike);
+    gate bf16 or float32, [H] or [T or 1, H or 1].  Rows at any distance.  Returns (y [T, H] bf16, h in the residual's dtype).
+    out and residual_out may each be x or the residual itself; other overlaps are refused.  H up to 32768 (16384 where rows do not
+    begin on 16 bytes)."""
+    return _ops.residual_norm.default(x, residual, weight, post_weight, gate, scale, eps, out, residual_out)
+
+
+def adjust_logits(logits, cu_tokens=None, history=None, history_lens=None, prompt_lens=None, tokens=None, masks=None, repetition=None,
+                  frequency=None, presence=None, bias_ids=None, bias=None, allowed=None, allowed_rows=None, out=None):
+    """Penalties for repeated tokens, biases of single ones and grammar masks on logits [T, V] (float32 or bf16), in one pass.
+
+    Rows belong to requests by cu_tokens [B + 1] from cache_plan (None: a row each).  history [B, L] int32 holds each request's
+    history_lens [B] tokens (None: L), the first prompt_lens [B] of them its prompt (None: none); with tokens [T] int64 a row's history
+    goes on with those that its mask names (masks [T] from cache_plan; None: those up to its own).  Of a token generated n times or
+    heard in the prompt: x / repetition where x > 0, else x repetition; then - frequency n - presence (where n > 0); [B] float32
+    each.  Then + bias [B, N] float32 of the tokens bias_ids [B, N] int32 (of equal ids the last counts; N <= 2047), and -inf where
+    allowed [M, ceil(V / 32)] int32 has no bit for the token in the row's grammar, allowed_rows [T] int32 (None: its own; -1: none).
+    Ids outside [0, V) are passed over.  Returns out, a new tensor unless given; logits itself may be given."""
+    return _ops.adjust_logits.default(logits, cu_tokens, history, history_lens, prompt_lens, tokens, masks, repetition, frequency, presence,
+                                      bias_ids, bias, allowed, allowed_rows, out)
