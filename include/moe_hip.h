@@ -51,6 +51,7 @@ extern "C" {
 #define MOE_DTYPE_F32   0
 #define MOE_DTYPE_BF16  1
 #define MOE_DTYPE_FP8   2      /* e4m3fn: the caches of the attention entry points */
+#define MOE_DTYPE_FP4   3      /* e2m1fn, two to a byte, with powers of two: likewise */
 
 #define MOE_ROUTE_SOFTMAX 0   /* select on logits; weights = softmax over all experts      */
 #define MOE_ROUTE_SIGMOID 1   /* scores = sigmoid(logit); select on scores + bias          */
@@ -432,6 +433,18 @@ int moe_qk_norm_rope(void *stream, const void *qkv_bf16, int64_t row_stride, int
                      const int64_t *slots, const float *k_scale, const float *v_scale);
 
 /*
+ * The same into a cache in 4 bits (its layout: moe_window_attention): of 32 neighbouring elements of a key or value the power of two is the least that
+ * brings all of them to 7 or below, its byte goes to k_scale / v_scale [n_blocks, page_size, Hkv, D / 32] (blocks *_scale_block_stride bytes apart);
+ * the codes are the nearest (ties to even, 6 at most).  A NaN or an infinity among the 32: byte 255, all of them read as NaN.
+ * D a multiple of 32, the caches' block strides (in elements) too.
+ */
+int moe_qk_norm_rope_fp4(void *stream, const void *qkv_bf16, int64_t row_stride, int T, int Hq, int Hkv, int D,
+                         const int32_t *positions, const float *cos_sin, int P, int R, int interleaved, const void *q_weight,
+                         const void *k_weight, int weight_dtype, float eps, void *q_out_bf16, void *k_cache, void *v_cache, int n_blocks,
+                         int64_t k_block_stride, int64_t v_block_stride, int page_size, const int64_t *slots, void *k_scale, void *v_scale,
+                         int64_t k_scale_block_stride, int64_t v_scale_block_stride);
+
+/*
  * Attention of the new tokens over the cache, which holds their own keys and values too (moe_qk_norm_rope has stored
  * them).  Of request b's kv_lens[b] keys the last n = cu_tokens[b + 1] - cu_tokens[b] are the new tokens'; every new token sees all
  * before them, and of the new ones those of its mask (masks NULL: itself and the ones before it).
@@ -451,6 +464,27 @@ int moe_tree_attention(void *stream, const void *q_bf16, int64_t q_stride, int T
                        int page_size, const int32_t *block_tables, int64_t table_stride, int table_width, const int32_t *kv_lens,
                        const int32_t *cu_tokens, int B, const int64_t *masks, float scale, const float *k_scale,
                        const float *v_scale, void *out_bf16, float *lse, void *workspace, size_t workspace_bytes);
+
+/*
+ * moe_tree_attention where a token sees a window of the text and its first tokens, and over a cache in 4 bits.
+ *
+ *   window W, sinks S   the keys that a token may see by moe_tree_attention's rules, numbered from 0 in the cache's order: it sees the last
+ *                       W and the first S of them.  W 0: all.  Pages of which no token sees a key are not read.
+ *   MOE_DTYPE_FP4       caches [n_blocks, page_size, Hkv, D / 2] bytes: element 2 i in the low 4 bits of byte i, 2 i + 1 in the high ones; codes 0 to 7 are 0,
+ *                       0.5, 1, 1.5, 2, 3, 4, 6, with bit 3 their negatives.  k_scale / v_scale [n_blocks, page_size, Hkv, D / 32] bytes: an element
+ *                       times 2^(byte - 127) of its 32 neighbours is its value (255: NaN), blocks *_scale_block_stride bytes apart.  The
+ *                       caches' block strides count elements, as ever, and divide by 32.
+ *   MOE_DTYPE_BF16, _FP8  k_scale / v_scale are fp32 of each head or NULL, their strides unused.
+ * Everything else as moe_tree_attention; the workspace is moe_tree_attention_workspace_bytes of the same arguments.
+ */
+int moe_window_attention_tile_rows(int T, int Hq, int Hkv, int B, int cache_dtype, int trees, int table_width, int page_size, int window,
+                                   int sinks);
+int moe_window_attention(void *stream, const void *q_bf16, int64_t q_stride, int T, int Hq, int Hkv, int D, const void *k_cache,
+                         const void *v_cache, int cache_dtype, int n_blocks, int64_t k_block_stride, int64_t v_block_stride,
+                         int page_size, const int32_t *block_tables, int64_t table_stride, int table_width, const int32_t *kv_lens,
+                         const int32_t *cu_tokens, int B, const int64_t *masks, float scale, const void *k_scale, const void *v_scale,
+                         int64_t k_scale_block_stride, int64_t v_scale_block_stride, int window, int sinks, void *out_bf16, float *lse,
+                         void *workspace, size_t workspace_bytes);
 
 /*
  * logits [T, V] fp32 or bf16 (rows row_stride apart) divided by temperature: logprobs [T] of tokens [T] int64, entropy [T]

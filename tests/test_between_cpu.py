@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import between_plain as plain
-from test_serving_cpu import E_ALIGN, E_MODE, E_NULL, E_SHAPE, fake, lib, odd, test_no_kernel_spills as no_kernel_spills
+from test_serving_cpu import E_ALIGN, E_MODE, E_NULL, E_SHAPE, E_WS, fake, lib, odd, test_no_kernel_spills as no_kernel_spills
 
 at = lambda n: ctypes.c_void_p(0x100000 * n)
 
@@ -92,3 +92,83 @@ def test_plain_adjust_logits_by_hand():
     # the path of the second drafted token: itself and the first
     out, _ = plain.adjust_logits(x.repeat(3, 1), [0, 3], None, None, None, [0, 2, 3], [1, 3, 4], [2.0], None, None, None, None, None, None)
     assert out[:, [0, 2, 3]].tolist() == [[1.0, 2.0, 1.0], [1.0, 1.0, 1.0], [2.0, 2.0, 0.5]]
+
+
+def test_window_attention_refusals(pkg):
+    names = ["q", "qs", "T", "Hq", "Hkv", "D", "kc", "vc", "ct", "blocks", "ks", "vs", "page", "bt", "bts", "W", "lens", "cu", "B", "masks", "scale",
+             "kscale", "vscale", "kss", "vss", "window", "sinks", "out", "lse", "ws", "wsb"]
+    ws = lib().moe_tree_attention_workspace_bytes(4, 8, 2, 128, 3, 3)
+    assert ws > 0 and ws % 256 == 0
+    good = dict(q=fake, qs=1024, T=4, Hq=8, Hkv=2, D=128, kc=fake, vc=fake, ct=3, blocks=5, ks=16 * 256, vs=16 * 256, page=16, bt=fake, bts=4, W=4,
+                lens=fake, cu=fake, B=3, masks=None, scale=0.1, kscale=fake, vscale=fake, kss=128, vss=128, window=5, sinks=1, out=fake, lse=None, ws=fake, wsb=ws)
+
+    def call(**other):
+        a = {**good, **other}
+        return lib().moe_window_attention(None, *[a[n] for n in names])
+    for bad in (dict(T=-1), dict(Hkv=3), dict(D=96), dict(B=5000), dict(page=12), dict(qs=1000), dict(bts=3), dict(ks=128), dict(kss=127), dict(vss=127),
+                dict(kss=1 << 31), dict(window=-1), dict(sinks=-1), dict(blocks=-1)):
+        assert call(**bad) == E_SHAPE, bad
+    for bad in (dict(q=odd), dict(kc=odd), dict(out=odd), dict(ks=16 * 256 + 16), dict(ws=odd)):
+        assert call(**bad) == E_ALIGN, bad
+    assert call(ct=0) == E_MODE and call(ct=4) == E_MODE
+    assert call(wsb=ws - 1) == E_WS
+    for name in ("q", "kc", "vc", "bt", "lens", "cu", "out", "ws", "kscale", "vscale"):
+        assert call(**{name: None}) == E_NULL, name
+    assert call(T=0, q=None, out=None) == 0
+    rows = lambda *a: lib().moe_window_attention_tile_rows(*a)
+    assert rows(64, 32, 4, 64, 3, 0, 512, 16, 0, 0) == 16 and rows(2042, 32, 8, 2, 1, 0, 512, 16, 0, 0) == 256 and rows(200, 32, 8, 2, 1, 0, 8192, 16, 500, 4) == 64
+    for bad in ((-1, 4, 2, 1, 1, 0, 4, 16, 1, 0), (1, 4, 2, 1, 4, 0, 4, 16, 1, 0), (1, 4, 2, 1, 1, 0, 4, 16, -1, 0), (1, 4, 2, 1, 1, 0, 4, 16, 1, -1)):
+        assert rows(*bad) == 0
+
+
+def test_store_in_four_bits_refusals(pkg):
+    names = ["qkv", "stride", "T", "Hq", "Hkv", "D", "pos", "cs", "P", "R", "pairs", "qw", "kw", "wt", "eps", "q", "kc", "vc", "blocks",
+             "ks", "vs", "page", "slots", "kscale", "vscale", "kss", "vss"]
+    good = dict(qkv=fake, stride=8 * 128, T=2, Hq=4, Hkv=2, D=128, pos=fake, cs=fake, P=10, R=128, pairs=0, qw=fake, kw=fake, wt=1, eps=1e-6, q=fake,
+                kc=fake, vc=fake, blocks=3, ks=16 * 256, vs=16 * 256, page=16, slots=fake, kscale=fake, vscale=fake, kss=128, vss=128)
+
+    def call(**other):
+        a = {**good, **other}
+        return lib().moe_qk_norm_rope_fp4(None, *[a[n] for n in names])
+    for bad in (dict(T=-1), dict(D=0), dict(page=24), dict(ks=100), dict(kss=127), dict(vss=0)):
+        assert call(**bad) == E_SHAPE, bad
+    for bad in (dict(D=112, stride=1024, R=96), dict(ks=16 * 256 + 8), dict(kc=odd)):
+        assert call(**bad) == E_ALIGN, bad
+    for name in ("qkv", "pos", "q", "kc", "vc", "slots", "kscale", "vscale"):
+        assert call(**{name: None}) == E_NULL, name
+    assert call(T=0, qkv=None, pos=None, q=None) == 0
+
+
+def test_ops_refuse_caches_that_do_not_fit(pkg):
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)
+    bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="GPU"):
+        pkg.tree_attention(bf(2, 4, 64), bf(3, 16, 2, 64), bf(3, 16, 2, 64), i32(1, 3), i32(1), i32(2), window=4)
+
+
+def test_no_window_kernel_spills(tmp_path):
+    no_kernel_spills("window_attention.hip", tmp_path)
+
+
+def test_four_bits_by_hand():
+    import window_plain as window
+    x = torch.zeros(32, dtype=torch.float64)
+    x[:6] = torch.tensor([7.0, -6.9, 5.0, 0.25, 0.75, -0.24])
+    codes, powers = window.encode(x)
+    assert powers.tolist() == [127] and codes.tolist()[:3] == [0xf7, 0x06, 0x82]      # 5 and 0.25 are ties: to 4 and 0; -0.24 to -0
+    assert window.decode(codes, powers).tolist()[:6] == [6.0, -6.0, 4.0, 0.0, 1.0, 0.0]
+    x[0] = 7.5
+    codes, powers = window.encode(x)
+    assert powers.tolist() == [128] and window.decode(codes, powers).tolist()[:3] == [8.0, -6.0, 4.0]
+
+
+def test_plain_window_by_hand():
+    import window_plain as window
+    q, k = torch.zeros(2, 1, 4), torch.zeros(2, 4, 1, 4).double()
+    v = torch.arange(8.0)[:, None].expand(8, 4).reshape(2, 4, 1, 4).double()
+    # rows see 0 .. 4 and 0 .. 5; of these the last two and the first one
+    out, lse, _ = window.attention(q, k, v, [[0, 1]], [6], [0, 2], None, 1.0, 2, 1)
+    assert torch.allclose(out[:, 0, 0], torch.tensor([(0 + 3 + 4) / 3, (0 + 4 + 5) / 3]).double()) and torch.allclose(lse, torch.tensor(3.0).double().log())
+    # a tree whose second token does not see the first
+    out, _, _ = window.attention(q, k, v, [[0, 1]], [6], [0, 2], [0b01, 0b10], 1.0, 2, 0)
+    assert torch.allclose(out[:, 0, 0], torch.tensor([(3 + 4) / 2, (3 + 5) / 2]).double())

@@ -79,6 +79,13 @@ SIGNATURES = {
     "moe_token_logprobs_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "moe_token_logprobs": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_int, c_float, c_void_p, c_void_p,
                                    c_void_p, c_void_p, c_void_p, c_size_t]),
+    "moe_qk_norm_rope_fp4": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
+                                     c_void_p, c_void_p, c_int, c_float, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int,
+                                     c_void_p, c_void_p, c_void_p, c_int64, c_int64]),
+    "moe_window_attention_tile_rows": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "moe_window_attention": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int64,
+                                     c_int64, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int, c_void_p, c_float, c_void_p,
+                                     c_void_p, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_size_t]),
     "moe_residual_norm": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int, c_void_p,
                                   c_int, c_int64, c_int64, c_float, c_float, c_void_p, c_int64, c_void_p, c_int64]),
     "moe_adjust_logits": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_int, c_void_p, c_int64, c_int, c_void_p,

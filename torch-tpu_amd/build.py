@@ -16,7 +16,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmoe_hip.so")
 PROBE_LIB = os.path.join(HERE, "libmoe_bench_probe.so")
 SOURCES = ["route.hip", "permute.hip", "quant_reduce.hip", "gemm_fp8.hip", "dense_small.hip", "decode_prep.hip", "router_front.hip",
-           "cache_plan.hip", "qk_norm_rope.hip", "tree_attention.hip", "token_logprobs.hip", "residual_norm.hip",
+           "cache_plan.hip", "qk_norm_rope.hip", "tree_attention.hip", "window_attention.hip", "token_logprobs.hip", "residual_norm.hip",
            "adjust_logits.hip", "capi.hip"]
 PROBE_SOURCES = ["probe.hip"]
 SHIM_LIB = os.path.join(HERE, "libmy_ops_torch.so")

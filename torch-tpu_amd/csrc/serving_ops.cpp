@@ -8,6 +8,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <optional>
 #include <tuple>
 
@@ -74,23 +75,41 @@ class Pieces {
 struct Cache {
   int dtype, n_blocks, page, heads, dim;
   int64_t k_stride, v_stride;
+  int64_t k_scale_stride, v_scale_stride;      // of a cache in 4 bits
 };
-// K and V caches [n_blocks, page_size, Hkv, D]: the last three dimensions contiguous, blocks at any distance
+// K and V caches [n_blocks, page_size, Hkv, D]: the last three dimensions contiguous, blocks at any distance.  In 4 bits two elements are one of
+// float4_e2m1fn_x2, and the scales are caches of their own, [n_blocks, page_size, Hkv, D / 32] float8_e8m0fnu.
 Cache cache_of(const Tensor &k, const Tensor &v, const OptTensor &k_scale, const OptTensor &v_scale, const Tensor &like) {
   TORCH_CHECK(k.dim() == 4 && v.dim() == 4, "k_cache and v_cache must be [n_blocks, page_size, heads, head_dim]");
   TORCH_CHECK(k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type(), "k_cache and v_cache must have the same shape and dtype");
-  TORCH_CHECK(k.scalar_type() == at::kBFloat16 || k.scalar_type() == at::kFloat8_e4m3fn, "the caches must be bfloat16 or float8_e4m3fn");
+  const bool fp4 = k.scalar_type() == at::kFloat4_e2m1fn_x2;
+  TORCH_CHECK(k.scalar_type() == at::kBFloat16 || k.scalar_type() == at::kFloat8_e4m3fn || fp4,
+              "the caches must be bfloat16, float8_e4m3fn or float4_e2m1fn_x2");
   need_gpu(k, "k_cache", like);
   need_gpu(v, "v_cache", like);
   const int64_t row = k.size(1) * k.size(2) * k.size(3);
   for (const Tensor *t : {&k, &v})
     TORCH_CHECK(t->numel() == 0 || t->size(0) == 0 || t->select(0, 0).is_contiguous(), "a block of a cache must be contiguous");
+  if (fp4) {
+    TORCH_CHECK(k_scale && v_scale, "a float4_e2m1fn_x2 cache needs k_scale and v_scale");
+    TORCH_CHECK(k.size(3) % 16 == 0, "a float4_e2m1fn_x2 cache must hold heads of a multiple of 32 elements");
+    for (const auto &[s, name] : {std::pair<const Tensor &, const char *>(*k_scale, "k_scale"), {*v_scale, "v_scale"}}) {
+      need_gpu(s, name, like);
+      TORCH_CHECK(s.scalar_type() == at::kFloat8_e8m0fnu, name, " of a float4_e2m1fn_x2 cache must be float8_e8m0fnu");
+      TORCH_CHECK(s.sizes() == at::IntArrayRef({k.size(0), k.size(1), k.size(2), k.size(3) / 16}), name,
+                  " must be [n_blocks, page_size, heads, head_dim / 32], got ", s.sizes());
+      TORCH_CHECK(s.numel() == 0 || s.size(0) == 0 || s.select(0, 0).is_contiguous(), "a block of ", name, " must be contiguous");
+    }
+    const auto stride = [&](const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2) * t.size(3); };
+    return {MOE_DTYPE_FP4, fits_int(k.size(0), "n_blocks"), fits_int(k.size(1), "page_size"), fits_int(k.size(2), "heads"),
+            fits_int(2 * k.size(3), "head_dim"), 2 * stride(k), 2 * stride(v), stride(*k_scale), stride(*v_scale)};
+  }
   const bool fp8 = k.scalar_type() == at::kFloat8_e4m3fn;
   TORCH_CHECK(fp8 || (!k_scale && !v_scale), "k_scale and v_scale belong to a float8_e4m3fn cache");
   if (k_scale) need_vector(*k_scale, "k_scale", at::kFloat, k.size(2), like);
   if (v_scale) need_vector(*v_scale, "v_scale", at::kFloat, k.size(2), like);
   return {fp8 ? MOE_DTYPE_FP8 : MOE_DTYPE_BF16, fits_int(k.size(0), "n_blocks"), fits_int(k.size(1), "page_size"),
-          fits_int(k.size(2), "heads"), fits_int(k.size(3), "head_dim"), k.size(0) > 1 ? k.stride(0) : row, v.size(0) > 1 ? v.stride(0) : row};
+          fits_int(k.size(2), "heads"), fits_int(k.size(3), "head_dim"), k.size(0) > 1 ? k.stride(0) : row, v.size(0) > 1 ? v.stride(0) : row, 0, 0};
 }
 
 std::tuple<Tensor, Tensor, Tensor, OptTensor, Tensor, Tensor> cache_plan(const Tensor &block_tables, const Tensor &lens,
@@ -152,7 +171,7 @@ std::tuple<Tensor, OptTensor> qk_norm_rope(const Tensor &qkv, const Tensor &posi
   TORCH_CHECK(!q_weight || !k_weight || q_weight->scalar_type() == k_weight->scalar_type(), "q_weight and k_weight must have the same dtype");
   TORCH_CHECK(k_cache.has_value() == v_cache.has_value() && k_cache.has_value() == slots.has_value(),
               "k_cache, v_cache and slots belong together");
-  Cache c{MOE_DTYPE_BF16, 0, 1, (int)n_kv_heads, (int)D, n_kv_heads * D, n_kv_heads * D};
+  Cache c{MOE_DTYPE_BF16, 0, 1, (int)n_kv_heads, (int)D, n_kv_heads * D, n_kv_heads * D, 0, 0};
   if (k_cache) {
     c = cache_of(*k_cache, *v_cache, k_scale, v_scale, qkv);
     TORCH_CHECK(c.heads == n_kv_heads && c.dim == D, "the caches must hold ", n_kv_heads, " heads of ", D);
@@ -172,6 +191,16 @@ std::tuple<Tensor, OptTensor> qk_norm_rope(const Tensor &qkv, const Tensor &posi
   }
   OptTensor k;
   if (!k_cache) k = at::empty({T, n_kv_heads, D}, qkv.options());
+  if (c.dtype == MOE_DTYPE_FP4) {
+    check_rc(moe_qk_norm_rope_fp4(current_stream(qkv), qkv.data_ptr(), row_stride(qkv), fits_int(T, "tokens"), (int)n_heads, (int)n_kv_heads,
+                                  fits_int(D, "head_dim"), positions.data_ptr<int32_t>(), cos_sin.data_ptr<float>(),
+                                  fits_int(cos_sin.size(0), "positions"), fits_int(cos_sin.size(1), "rotated dimensions"), interleaved,
+                                  data_or_null<void>(q_weight), data_or_null<void>(k_weight), wt, (float)eps, q.data_ptr(), k_cache->data_ptr(),
+                                  v_cache->data_ptr(), c.n_blocks, c.k_stride, c.v_stride, c.page, data_or_null<int64_t>(slots),
+                                  k_scale->data_ptr(), v_scale->data_ptr(), c.k_scale_stride, c.v_scale_stride),
+             "qk_norm_rope");
+    return {q, OptTensor()};
+  }
   check_rc(moe_qk_norm_rope(current_stream(qkv), qkv.data_ptr(), row_stride(qkv), fits_int(T, "tokens"), (int)n_heads, (int)n_kv_heads,
                             fits_int(D, "head_dim"), positions.data_ptr<int32_t>(), cos_sin.data_ptr<float>(),
                             fits_int(cos_sin.size(0), "positions"), fits_int(cos_sin.size(1), "rotated dimensions"), interleaved,
@@ -186,7 +215,7 @@ std::tuple<Tensor, OptTensor> qk_norm_rope(const Tensor &qkv, const Tensor &posi
 std::tuple<Tensor, OptTensor> tree_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &block_tables,
                                              const Tensor &kv_lens, const Tensor &cu_tokens, const OptTensor &masks,
                                              std::optional<double> scale, const OptTensor &k_scale, const OptTensor &v_scale,
-                                             const OptTensor &out, bool return_lse) {
+                                             const OptTensor &out, bool return_lse, std::optional<int64_t> window, int64_t sinks) {
   TORCH_CHECK(q.dim() == 3 && q.scalar_type() == at::kBFloat16, "q must be [tokens, heads, head_dim] bfloat16");
   need_gpu(q, "q", q);
   const int64_t T = q.size(0), Hq = q.size(1), D = q.size(2);
@@ -200,6 +229,8 @@ std::tuple<Tensor, OptTensor> tree_attention(const Tensor &q, const Tensor &k_ca
   need_vector(kv_lens, "kv_lens", at::kInt, B, q);
   need_vector(cu_tokens, "cu_tokens", at::kInt, B + 1, q);
   if (masks) need_vector(*masks, "masks", at::kLong, T, q);
+  TORCH_CHECK(!window || *window > 0, "window must be positive");
+  TORCH_CHECK(sinks >= 0 && (window || sinks == 0), "sinks must not be negative, and belong to a window");
   c10::DeviceGuard guard(q.device());
   Tensor o;
   if (out) {
@@ -215,6 +246,18 @@ std::tuple<Tensor, OptTensor> tree_attention(const Tensor &q, const Tensor &k_ca
   const int t = fits_int(T, "tokens"), h = fits_int(Hq, "heads"), b = fits_int(B, "requests");
   const size_t need = moe_tree_attention_workspace_bytes(t, h, c.heads, c.dim, b, c.dtype);
   const Tensor ws = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
+  if (window || c.dtype == MOE_DTYPE_FP4) {
+    const int64_t most = 0x7fffffff;               // (no text is longer)
+    check_rc(moe_window_attention(current_stream(q), q.data_ptr(), T > 1 ? q.stride(0) : Hq * D, t, h, c.heads, c.dim, k_cache.data_ptr(),
+                                  v_cache.data_ptr(), c.dtype, c.n_blocks, c.k_stride, c.v_stride, c.page, block_tables.data_ptr<int32_t>(),
+                                  row_stride(block_tables), fits_int(block_tables.size(1), "table width"), kv_lens.data_ptr<int32_t>(),
+                                  cu_tokens.data_ptr<int32_t>(), b, data_or_null<int64_t>(masks), (float)scale.value_or(1.0 / std::sqrt((double)D)),
+                                  data_or_null<void>(k_scale), data_or_null<void>(v_scale), c.k_scale_stride, c.v_scale_stride,
+                                  (int)std::min(window.value_or(0), most), (int)std::min(sinks, most), o.data_ptr(), data_or_null<float>(lse),
+                                  ws.data_ptr(), need),
+             "tree_attention");
+    return {o, lse};
+  }
   check_rc(moe_tree_attention(current_stream(q), q.data_ptr(), T > 1 ? q.stride(0) : Hq * D, t, h, c.heads, c.dim, k_cache.data_ptr(),
                               v_cache.data_ptr(), c.dtype, c.n_blocks, c.k_stride, c.v_stride, c.page, block_tables.data_ptr<int32_t>(),
                               row_stride(block_tables), fits_int(block_tables.size(1), "table width"), kv_lens.data_ptr<int32_t>(),
@@ -380,16 +423,16 @@ Tensor adjust_logits(const Tensor &logits, const OptTensor &cu_tokens, const Opt
 }  // namespace
 
 // What a schema says of memory: (a!) is written, a result (a) is that tensor where it is handed over, results with the same letter share an
-// allocation.  (A result marked as written, (a!), would drop out of autograd: backward would not warn that there is no gradient.)
+// allocation.  (qk_norm_rope writes the scales of a cache in 4 bits only.  A result marked as written, (a!), would drop out of autograd: backward would not warn that there is no gradient.)
 TORCH_LIBRARY_FRAGMENT(my_ops, m) {
   m.def("cache_plan(Tensor(a!) block_tables, Tensor lens, Tensor counts, Tensor free_blocks, Tensor n_free, int page_size, "
         "int max_tokens, Tensor? parents=None) -> (Tensor(b), Tensor(b), Tensor(b), Tensor(b)?, Tensor(b), Tensor(b))");
   m.def("qk_norm_rope(Tensor qkv, Tensor positions, Tensor cos_sin, int n_heads, int n_kv_heads, Tensor? q_weight=None, "
         "Tensor? k_weight=None, float eps=1e-6, bool interleaved=False, Tensor(a!)? k_cache=None, Tensor(b!)? v_cache=None, "
-        "Tensor? slots=None, Tensor? k_scale=None, Tensor? v_scale=None, Tensor(c!)? out=None) -> (Tensor(c), Tensor?)");
+        "Tensor? slots=None, Tensor(d!)? k_scale=None, Tensor(e!)? v_scale=None, Tensor(c!)? out=None) -> (Tensor(c), Tensor?)");
   m.def("tree_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor kv_lens, Tensor cu_tokens, "
         "Tensor? masks=None, float? scale=None, Tensor? k_scale=None, Tensor? v_scale=None, Tensor(a!)? out=None, "
-        "bool return_lse=False) -> (Tensor(a), Tensor?)");
+        "bool return_lse=False, int? window=None, int sinks=0) -> (Tensor(a), Tensor?)");
   m.def("token_logprobs(Tensor logits, Tensor tokens, int top_k=0, float temperature=1.0) -> (Tensor(a), Tensor(a), Tensor(a), Tensor(a))");
   m.def("residual_norm(Tensor x, Tensor? residual=None, Tensor? weight=None, Tensor? post_weight=None, Tensor? gate=None, "
         "float scale=1.0, float eps=1e-6, Tensor(a!)? out=None, Tensor(b!)? residual_out=None) -> (Tensor(a), Tensor(b))");

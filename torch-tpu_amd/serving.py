@@ -58,21 +58,27 @@ def qk_norm_rope(qkv, positions, cos_sin, n_heads: int, n_kv_heads: int, q_weigh
     cosines, then R/2 sines of each position's angles, R <= D a multiple of 16; weights [D] bf16 or float32, None: that
     side is not normalised.  Pairs (i, i + R/2), or neighbours with interleaved.
     With caches [blocks, page, n_kv_heads, D] (bf16, or e4m3 with optional scales [n_kv_heads] that values are divided by)
-    and slots [T] int64: stores keys and values, returns q [T, n_heads, D].  Without: returns (q, k)."""
+    and slots [T] int64: stores keys and values, returns q [T, n_heads, D].  Without: returns (q, k).
+    Caches in 4 bits are float4_e2m1fn_x2 [blocks, page, n_kv_heads, D / 2] (two elements to a byte, the first in the low bits), their scales
+    float8_e8m0fnu [blocks, page, n_kv_heads, D / 32], written beside them: the power of two of 32 neighbouring elements, the least that
+    brings them to 7 or below (the largest code is 6).  D a multiple of 32."""
     q, k = _ops.qk_norm_rope.default(qkv, positions, cos_sin, n_heads, n_kv_heads, q_weight, k_weight, eps, interleaved, k_cache, v_cache,
                                      slots, k_scale, v_scale, out)
     return q if k is None else (q, k)
 
 
 def tree_attention(q, k_cache, v_cache, block_tables, kv_lens, cu_tokens, masks=None, scale=None, k_scale=None, v_scale=None, out=None,
-                   return_lse: bool = False):
+                   return_lse: bool = False, window=None, sinks: int = 0):
     """Attention of the new tokens over the paged cache that holds them too: a tree of drafted tokens of each request (masks
     [T] int64 from cache_plan), or without masks one token or a causal chunk.
 
     q [T, Hq, D] bf16, D 64 or 128, Hq a multiple of the cache's heads; caches [blocks, page, heads, D] bf16 or e4m3 (with the
-    scales of qk_norm_rope); kv_lens [B] and cu_tokens [B + 1] from the plan; scale, of any sign, defaults to D ** -0.5.
+    scales of qk_norm_rope), or in 4 bits as qk_norm_rope writes them; kv_lens [B] and cu_tokens [B + 1] from the plan; scale, of any sign, defaults to
+    D ** -0.5.  window: of the keys that a row may see by these rules, in the cache's order, it sees the last `window` and the first
+    `sinks`; pages that none of a request's rows sees are not read (their table entries may be anything).
     Returns out [T, Hq, D] bf16, or (out, lse [T, Hq] float32).  A row that sees no key is 0, its lse -inf."""
-    o, lse = _ops.tree_attention.default(q, k_cache, v_cache, block_tables, kv_lens, cu_tokens, masks, scale, k_scale, v_scale, out, return_lse)
+    o, lse = _ops.tree_attention.default(q, k_cache, v_cache, block_tables, kv_lens, cu_tokens, masks, scale, k_scale, v_scale, out, return_lse,
+                                       window, sinks)
     return (o, lse) if return_lse else o
 
 
