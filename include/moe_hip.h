@@ -63,7 +63,7 @@ extern "C" {
 #define MOE_MAX_TOPK    32
 #define MOE_MAX_REQUESTS 4096   /* requests of one step of the paged cache */
 #define MOE_MAX_PAGE    1024    /* tokens of a cache page (a power of two) */
-#define MOE_MAX_BIASES  2047    /* biased tokens of a request */
+#define MOE_MAX_BIASES  1023    /* biased tokens of a request */
 
 /*
  * Library version and the gfx target it was built for.  The version changes whenever a caller built against an

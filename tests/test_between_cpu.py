@@ -46,7 +46,7 @@ def test_adjust_logits_refusals(pkg):
     def call(**other):
         a = {**good, **other}
         return lib().moe_adjust_logits(None, *[a[n] for n in names])
-    for bad in (dict(T=-1), dict(V=0), dict(B=-1), dict(L=-1), dict(nb=-1), dict(nb=2048, bis=3000, bvs=3000), dict(xs=999), dict(os=999), dict(na=-1), dict(cu=None),
+    for bad in (dict(T=-1), dict(V=0), dict(B=-1), dict(L=-1), dict(nb=-1), dict(nb=1024, bis=3000, bvs=3000), dict(xs=999), dict(os=999), dict(na=-1), dict(cu=None),
                 dict(hs=49), dict(bis=4), dict(bvs=4), dict(als=31), dict(rows=None), dict(L=(1 << 20) - 4, hs=1 << 20)):
         assert call(**bad) == E_SHAPE, bad
     assert call(dt=2) == E_MODE

@@ -90,7 +90,7 @@ class Case:
     ([40, 1], 333, 50, False, False, dict(biases=2, spare=2, gap=1)), ([1] * 33, 1001, 30, True, False, dict(masked="rows")),
     ([5, 6], 513, 20, True, True, dict(penalties="repetition")), ([5, 6], 514, 20, False, True, dict(penalties="frequency")),
     ([4], 515, 20, True, True, dict(penalties="presence", biases=1)), ([4, 4], 516, 20, True, True, dict(penalties=None, biases=7, masked="own")),
-    ([2], 24600, 5, False, False, dict(biases=2047)), ([0, 0], 40, 4, True, False, dict(spare=5)), ([300], 60, 8, True, False, {})])
+    ([2], 24600, 5, False, False, dict(biases=1023)), ([0, 0], 40, 4, True, False, dict(spare=5)), ([300], 60, 8, True, False, {})])
 def test_equals_the_plain_form(pkg, dev, counts, V, L, bf16, tree, how):
     say("adjust_logits", len(counts), "requests", V, L, "bf16" if bf16 else "f32", tree, how)
     c = Case(V + L, counts, V, L, bf16, tree, **how)

@@ -7,9 +7,15 @@
 //        -> -inf unless the grammar allows the token
 //
 // fp32, one rounding at the end.  Bound by bytes: logits once in, once out.  A workgroup takes a segment of the vocabulary for some rows.  It
-// counts the history's tokens that lie in the segment in LDS, so that no counter per vocabulary entry exists in memory and histories, which are short
-// beside the vocabulary, are read again by each segment.  Most tokens are touched by nothing: a bit of each says so, and their values pass
-// as they are.
+// counts the history's tokens that lie in the segment in LDS, so that no counter per vocabulary entry exists in memory, and a bit per token
+// says which were touched.  A row streams through registers, is stored as it is (but for what its grammar forbids) without waiting for the
+// counts, and the threads that stored the few touched values then store those once more.
+// Rows of 131072 fp32 values, 64 of them with up to 8192 tokens of history: 28 us, 14 without the histories (2.4 and 4.8 TB/s); 1290 rows of 100003
+// bf16 values, 128 requests' trees, every other row with a grammar: 157 us, 104 with neither (3.3 and 5.0 TB/s).  What histories cost is the
+// comparisons of every token in every segment and the counting, about 25 instructions a token; LDS atomics of all lanes instead of a branch: 32 us,
+// 32 KB segments: 30 and 200 us, 8 KB: 32 and 167.
+#include <math.h>
+#include <type_traits>
 #include "moe_common.h"
 #include "../../include/moe_hip.h"
 
@@ -41,36 +47,105 @@ constexpr uint32_t kOnce = 2, kHeard = 1, kBiasShift = 21, kCounts = (1u << kBia
 
 template <int SEG>
 struct LogitTable {
-  uint32_t count[SEG + 8];             // of token first - 8 + i: a group of 16 bytes may begin up to 7 tokens before the segment
+  uint32_t count[SEG + 8];             // of token first - 8 + i: a group of 16 bytes may begin up to 7 tokens before the segment.  (Those of
+                                       // ids below 0 and beyond the vocabulary are never read.)
   uint32_t touched[SEG / 32 + 2];
+  __device__ __forceinline__ void touch(uint32_t place) { atomicOr(&touched[place >> 5], 1u << (place & 31)); }
+  __device__ __forceinline__ void add(int64_t place, uint32_t what) {
+    if (place < 0 || place >= SEG + 8) return;
+    atomicAdd(&count[place], what);
+    touch(place);
+  }
 };
 
-template <int SEG>
-__device__ __forceinline__ void note(LogitTable<SEG> &s, int64_t place, uint32_t what) {
-  if (place < 0 || place >= SEG + 8) return;
-  atomicAdd(&s.count[place], what);
-  atomicOr(&s.touched[place >> 5], 1u << (place & 31));
-}
+typedef uint16_t __attribute__((aligned(1))) any_u16;
 
-template <int SEG, bool BF16>
+// BYTES of a row to a workgroup: BYTES / 16 groups of 16 bytes, P of them to a thread.  MANY: several rows, of which the next one is on its way
+// while one is worked on.
+template <int BYTES, bool BF16, bool MANY>
 __global__ __launch_bounds__(256) void adjust_logits_kernel(const LogitArgs a) {
-  constexpr int N = BF16 ? 8 : 4, E = BF16 ? 2 : 4;    // values of 16 bytes; bytes of one
-  __shared__ LogitTable<SEG> s;
-  const int tid = threadIdx.x;
+  constexpr int N = BF16 ? 8 : 4, E = BF16 ? 2 : 4, SEG = BYTES / E;             // values of 16 bytes; bytes of one
+  constexpr int P = BYTES / 4096, ALL = (1 << N) - 1;
+  struct Group {
+    uint32_t w[4], let;                // let: the grammar's bits for its values
+  };
+  __shared__ __attribute__((aligned(16))) LogitTable<SEG> s;
+  const int tid = threadIdx.x, lane = tid & 63;
   const int seg = blockIdx.x % a.segments;
-  const int64_t first = (int64_t)seg * SEG;            // the segment's first token, for a row that begins on 16 bytes
+  const int first = seg * SEG, from = first - 8;       // the segment's first token, for a row that begins on 16 bytes; the first counter's
   const int t0 = (int)(blockIdx.x / a.segments) * a.rows, t1 = min(t0 + a.rows, a.T);
+
+  // A row's groups begin on 16 bytes of memory: where the row does not, the first one begins `before` values earlier.  Of most segments all
+  // groups lie within the row (inside); of the others some have values before or behind it, which are taken value by value.
+  const auto row_in = [&](int t) { return (const uint8_t *)a.in + t * a.in_stride * E; };
+  const auto before_of = [&](int t) { return (int)((uintptr_t)row_in(t) % 16) / E; };
+  const auto inside_of = [&](int before) { return first >= before && first - before + SEG <= a.V; };
+  const auto token_of = [&](int p, int before) { return first + (p * 256 + tid) * N - before; };
+  const auto grammar_of = [&](int t) { return !a.allowed ? -1 : a.allowed_row ? a.allowed_row[t] : t; };
+  const auto words_of = [&](int grammar) { return grammar >= 0 && grammar < a.allowed_rows ? (const uint32_t *)a.allowed + grammar * a.allowed_stride : nullptr; };
+  const int last_bits = (a.V + 31) / 32 * 4 - 2;       // a row of the grammar's last two bytes
+  const auto bits_at = [&](const uint32_t *words, int v) {
+    const int at = min(v >> 3, last_bits);
+    return (uint32_t)*(const any_u16 *)((const uint8_t *)words + at) >> (v - 8 * at) & ALL;
+  };
+  const auto load = [&](int t, const uint32_t *words, Group *g) {
+    const uint8_t *in = row_in(t);
+    const int before = before_of(t);
+    const bool inside = inside_of(before);
+#pragma unroll
+    for (int p = 0; p < P; p++) {
+      const int v = token_of(p, before);
+      g[p].let = ALL;
+      if (inside || (v >= 0 && v + N <= a.V)) {
+        const v4i raw = *(const v4i *)(in + (uint32_t)(v * E));
+#pragma unroll
+        for (int i = 0; i < 4; i++) g[p].w[i] = (uint32_t)raw[i];
+      }
+    }
+    if (words) {
+#pragma unroll
+      for (int p = 0; p < P; p++) {
+        const int v = token_of(p, before);
+        if (inside || (v >= 0 && v + N <= a.V)) g[p].let = bits_at(words, v);
+      }
+    }
+  };
+  const auto store = [&](uint8_t *out, int v, bool same, const uint32_t (&w)[4]) {
+    if (same) {
+      *(v4i *)(out + (uint32_t)(v * E)) = (v4i){(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; k++) {
+        if (BF16) ((uint16_t *)out)[(uint32_t)(v + k)] = (uint16_t)(w[k / 2] >> (16 * (k & 1)));
+        else ((uint32_t *)out)[(uint32_t)(v + k)] = w[k];
+      }
+    }
+  };
+
   int b = -1, begin = 0, end = 0;                      // the request whose history is counted, its rows
   uint64_t path = 0;                                   // the tokens of the tree that are counted
+  uint32_t drafted = ~0u;                              // lane i: the counter of the request's token i
+  float rep = 1.f, less = 1.f, freq = 0.f, pres = 0.f; // less: 1 / rep
+  bool counts = false;
+  Group now[P], next[MANY ? P : 1];
+  const uint32_t *words = words_of(grammar_of(t0)), *next_words = nullptr;
+  int next_grammar = MANY && t0 + 1 < t1 ? grammar_of(t0 + 1) : -1;
+  uint64_t next_mask = a.masks ? (uint64_t)a.masks[t0] : 0;
+  load(t0, words, now);
   for (int t = t0; t < t1; t++) {
+    // What the next rows need is asked for here: nothing below waits for a trip to memory that begins with this row, but its request's
+    // history where a new one begins.
+    const uint64_t mask = next_mask;
+    if (MANY && a.masks && t + 1 < t1) next_mask = (uint64_t)a.masks[t + 1];
     bool fresh = false;
     if (a.cu) {
       if (b < 0 || t >= end) {                         // the last request that begins at t or before
-        int lo = 0, hi = a.B;
+        int lo = 0, hi = a.B;                          // 64 places at a time
         while (lo < hi) {
-          const int mid = (lo + hi + 1) / 2;
-          if (a.cu[mid] <= t) lo = mid;
-          else hi = mid - 1;
+          const int step = (hi - lo + 63) / 64, at = lo + (1 + lane) * step;
+          const int past = __popcll(__ballot(at <= hi && a.cu[min(at, hi)] <= t));
+          hi = min(lo + (past + 1) * step - 1, hi);
+          lo += past * step;
         }
         fresh = true;
         b = lo < a.B && a.cu[lo] <= t ? lo : a.B;
@@ -82,114 +157,179 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const LogitArgs a) {
       b = t, begin = t, end = t + 1;
     }
     const bool none = b >= a.B;                        // a row of no request passes as it is
-    const float rep = !none && a.repetition ? a.repetition[b] : 1.f, freq = !none && a.frequency ? a.frequency[b] : 0.f,
-                pres = !none && a.presence ? a.presence[b] : 0.f;
-    const bool counts = rep != 1.f || freq != 0.f || pres != 0.f;
+    // The history's first tokens are asked for together with its length and the penalties: one trip to memory.
+    const int32_t *ids = a.history + (none ? 0 : b * a.history_stride);
+    const bool heard = fresh && !none && a.history && a.L > 0;
+    // (Four neighbours to a lane: histories are read by every segment, and single values took more loads than the logits.)
+    v4i asked_for = {-1, -1, -1, -1};
+    int len = 0, asked = 0;
+    const bool whole = (uintptr_t)ids % 16 == 0;
+    const auto ask = [&](int i0) {
+      const int i = i0 + 4 * tid;
+      if (whole && i + 4 <= a.L) {
+        asked_for = *(const v4i *)(ids + i);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) asked_for[j] = i + j < a.L ? ids[i + j] : -1;
+      }
+    };
     if (fresh) {
-      __syncthreads();
-      for (int i = tid; i < SEG + 8; i += 256) s.count[i] = 0;
+      if (heard) ask(0);
+      rep = !none && a.repetition ? a.repetition[b] : 1.f;
+      freq = !none && a.frequency ? a.frequency[b] : 0.f;
+      pres = !none && a.presence ? a.presence[b] : 0.f;
+      len = heard && a.history_lens ? min(a.history_lens[b], a.L) : a.L;
+      asked = heard && a.prompt_lens ? min(a.prompt_lens[b], len) : 0;
+      drafted = !none && a.tokens && a.masks && tid < 64 && begin + tid < end ? (uint32_t)(a.tokens[begin + tid] - from) : ~0u;
+    }
+    if (MANY && t + 1 < t1) {
+      next_words = words_of(next_grammar);
+      load(t + 1, next_words, next);
+      if (t + 2 < t1) next_grammar = grammar_of(t + 2);
+    }
+
+    // The row as it is, but for what its grammar forbids: this waits for nothing but the row.
+    const uint8_t *in = row_in(t);
+    uint8_t *out = (uint8_t *)a.out + t * a.out_stride * E;
+    const int before = before_of(t);
+    const bool same = (uintptr_t)out % 16 == (uintptr_t)in % 16, moved = a.out != a.in, inside = inside_of(before);
+    if (none) words = nullptr;
+#pragma unroll
+    for (int p = 0; p < P; p++) {
+      const int v = token_of(p, before);
+      uint32_t (&w)[4] = now[p].w;
+      if (inside || (v >= 0 && v + N <= a.V)) {
+        if (words) {
+          const uint32_t let = now[p].let;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            if (BF16) {
+              const uint32_t keep = ((uint32_t)((int)(let << (31 - 2 * i)) >> 31) & 0xffffu) | ((uint32_t)((int)(let << (30 - 2 * i)) >> 31) & 0xffff0000u);
+              w[i] = (w[i] & keep) | (0xff80ff80u & ~keep);
+            } else {
+              w[i] = let >> i & 1 ? w[i] : 0xff800000u;
+            }
+          }
+        } else {
+          now[p].let = ALL;
+        }
+        if (moved || words) store(out, v, same, w);
+      } else {
+        for (int k = max(v, 0); k < min(v + N, a.V); k++) {
+          const bool may = !words || words[k >> 5] >> (k & 31) & 1;
+          if (BF16) ((uint16_t *)out)[k] = may ? ((const uint16_t *)in)[k] : 0xff80;
+          else ((uint32_t *)out)[k] = may ? ((const uint32_t *)in)[k] : 0xff800000u;
+        }
+      }
+    }
+
+    if (fresh) {
+      less = 1.0f / rep;
+      counts = rep != 1.f || freq != 0.f || pres != 0.f;
+      path = 0;
+      for (int i = tid; i < SEG / 4 + 2; i += 256) *(v4i *)&s.count[4 * i] = (v4i){0, 0, 0, 0};
       for (int i = tid; i < SEG / 32 + 2; i += 256) s.touched[i] = 0;
       __syncthreads();
       if (!none && a.n_bias) {
         for (int i = tid; i < a.n_bias; i += 256) {
-          const int64_t place = (int64_t)a.bias_ids[b * a.bias_ids_stride + i] - first + 8;
-          if (place < 0 || place >= SEG + 8) continue;
+          const uint32_t place = (uint32_t)(a.bias_ids[b * a.bias_ids_stride + i] - from);
+          if (place >= SEG + 8) continue;
           atomicMax(&s.count[place], (uint32_t)(i + 1) << kBiasShift);
-          atomicOr(&s.touched[place >> 5], 1u << (place & 31));
+          s.touch(place);
         }
         __syncthreads();
       }
-      if (!none && counts && a.history) {
-        const int len = min(max(a.history_lens ? a.history_lens[b] : a.L, 0), a.L), asked = a.prompt_lens ? a.prompt_lens[b] : 0;
-        for (int i = tid; i < len; i += 256) {
-          const int64_t place = (int64_t)a.history[b * a.history_stride + i] - first + 8;
-          if (place < 0 || place >= SEG + 8) continue;
-          if (i < asked) atomicOr(&s.count[place], kHeard);
-          else atomicAdd(&s.count[place], kOnce);
-          atomicOr(&s.touched[place >> 5], 1u << (place & 31));
+      if (heard && counts) {
+        for (int i = 0; i < len; i += 1024) {
+          const v4i id = asked_for;
+          if (i + 1024 < len) ask(i + 1024);           // (on their way while these are counted)
+            const bool said = i >= asked && i + 1024 <= len, prompt = i + 1024 <= asked;       // (elsewhere threads differ)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const uint32_t place = (uint32_t)(id[j] - from);
+              if (place >= SEG + 8) continue;
+              const int at = i + 4 * tid + j;
+              const uint64_t here = __ballot(true);
+              if ((said || prompt) && __popcll(here) > 40) {     // a text that repeats itself: so many additions at one address take as many turns
+                const uint64_t like = __ballot(place == (uint32_t)__builtin_amdgcn_readfirstlane(place));
+                if (like >> lane & 1) {
+                  if (lane == __builtin_ctzll(like)) {
+                    if (prompt) atomicOr(&s.count[place], kHeard);
+                    else atomicAdd(&s.count[place], (uint32_t)__popcll(like) * kOnce);
+                    s.touch(place);
+                  }
+                  continue;
+                }
+              }
+              if (said || (at >= asked && at < len)) atomicAdd(&s.count[place], kOnce);
+              else if (at < asked) atomicOr(&s.count[place], kHeard);
+              s.touch(place);
+            }
         }
       }
-      path = 0;
       if (!none && counts && a.tokens && !a.masks)     // what stands before the row
-        for (int i = begin + tid; i < t; i += 256) note<SEG>(s, a.tokens[i] - first + 8, kOnce);
+        for (int i = begin + tid; i < t; i += 256) s.add(a.tokens[i] - from, kOnce);
     }
     if (!none && counts && a.tokens) {
       if (a.masks) {
-        const uint64_t mask = (uint64_t)a.masks[t];
-        if (tid < 64 && begin + tid < end) {
-          const int was = path >> tid & 1, is = mask >> tid & 1;
-          if (was != is) note<SEG>(s, a.tokens[begin + tid] - first + 8, is ? kOnce : 0u - kOnce);
+        const int was = path >> lane & 1, is = mask >> lane & 1;
+        if (drafted < SEG + 8 && was != is) {
+          atomicAdd(&s.count[drafted], is ? kOnce : 0u - kOnce);
+          s.touch(drafted);
         }
         path = mask;
       } else if (tid == 0) {
-        note<SEG>(s, a.tokens[t] - first + 8, kOnce);
+        s.add(a.tokens[t] - from, kOnce);
       }
     }
     __syncthreads();
-    // Groups of 16 bytes of memory: a row that does not begin on one has its first group `before` values earlier.
-    const uint8_t *in = (const uint8_t *)a.in + t * a.in_stride * E;
-    uint8_t *out = (uint8_t *)a.out + t * a.out_stride * E;
-    const int before = (int)((uintptr_t)in % 16) / E;
-    const bool same = (uintptr_t)out % 16 == (uintptr_t)in % 16;
-    const int grammar = a.allowed && !none ? (a.allowed_row ? a.allowed_row[t] : t) : -1;
-    const uint32_t *words = grammar >= 0 && grammar < a.allowed_rows ? (const uint32_t *)a.allowed + grammar * a.allowed_stride : nullptr;
-    const int last_word = (a.V - 1) / 32;
-    for (int i = tid; i < SEG / N; i += 256) {
-      const int64_t v0 = first + (int64_t)i * N - before;
-      if (v0 >= a.V) break;
-      const int from = v0 < 0 ? (int)-v0 : 0, upto = v0 + N > a.V ? (int)(a.V - v0) : N;     // the group's values that are the row's
-      if (from >= upto) continue;
-      const bool full = from == 0 && upto == N;
-      uint32_t raw[N];
-      if (full) {
-        const v4i w = *(const v4i *)(in + v0 * E);
-#pragma unroll
-        for (int k = 0; k < N; k++) raw[k] = BF16 ? (uint32_t)w[k / 2] >> (16 * (k & 1)) & 0xffff : (uint32_t)w[k];
-      } else {
-#pragma unroll
-        for (int k = 0; k < N; k++) raw[k] = k >= from && k < upto ? (BF16 ? (uint32_t)((const uint16_t *)in)[v0 + k] : ((const uint32_t *)in)[v0 + k]) : 0;
+
+    // The touched values, each by the thread that has just stored it.
+    const auto adjusted = [&](float x, uint32_t c) {
+      if (c & kCounts) {
+        const float n = (float)((c & kCounts) >> 1);
+        x = x * (x > 0.f ? less : rep) - (n > 0.f ? fmaf(freq, n, pres) : 0.f);
       }
-      const int at = i * N - before + 8;               // the first one's counter
-      const uint32_t hit = (uint32_t)(((uint64_t)s.touched[(at >> 5) + 1] << 32 | s.touched[at >> 5]) >> (at & 31)) & ((1u << N) - 1);
-      uint32_t let = (1u << N) - 1;
-      if (words) {
-        const int64_t w0 = v0 + from;
-        const int w = (int)(w0 >> 5);
-        let = (uint32_t)(((uint64_t)words[min(w + 1, last_word)] << 32 | words[w]) >> (w0 & 31)) << from & ((1u << N) - 1);
-      }
-      if (hit) {
+      if (c >> kBiasShift) x += a.bias[b * a.bias_stride + (c >> kBiasShift) - 1];
+      return x;
+    };
+    if (!none && (counts || a.n_bias)) {
+      uint32_t hit[P];
 #pragma unroll
-        for (int k = 0; k < N; k++) {
-          if (!(hit >> k & 1)) continue;
-          const uint32_t c = s.count[at + k];
-          float x = BF16 ? bf16_to_f32((uint16_t)raw[k]) : __uint_as_float(raw[k]);
-          if (c & kCounts) {
-            x = x > 0.f ? x / rep : x * rep;
-            const float n = (float)((c & kCounts) >> 1);
-            x = x - freq * n - (n > 0.f ? pres : 0.f);
+      for (int p = 0; p < P; p++) {
+        const int at = (p * 256 + tid) * N - before + 8;         // the first one's counter
+        const uint32_t lo = s.touched[at >> 5], hi = s.touched[(at >> 5) + 1];
+        hit[p] = __builtin_amdgcn_alignbit(hi, lo, at & 31) & ALL;
+      }
+#pragma unroll
+      for (int p = 0; p < P; p++) {
+        const int v = token_of(p, before), at = (p * 256 + tid) * N - before + 8;
+        if (inside || (v >= 0 && v + N <= a.V)) {
+          const v4i w = {(int)now[p].w[0], (int)now[p].w[1], (int)now[p].w[2], (int)now[p].w[3]};
+          uint32_t left = hit[p] & now[p].let;
+          while (left) {                               // (few, if any: a wavefront passes as often as one of its lanes has hits)
+            const int k = __builtin_ctz(left);
+            left &= left - 1;
+            const int word = BF16 ? k >> 1 : k;
+            const uint32_t low = word & 1 ? w[1] : w[0], high = word & 1 ? w[3] : w[2], one = word & 2 ? high : low;
+            const float x = adjusted(BF16 ? __uint_as_float(one >> (16 * (k & 1)) << 16) : __uint_as_float(one), s.count[at + k]);
+            if (BF16) ((uint16_t *)out)[(uint32_t)(v + k)] = (uint16_t)pack2_bf16(x, 0.f);
+            else ((float *)out)[(uint32_t)(v + k)] = x;
           }
-          if (c >> kBiasShift) x += a.bias[b * a.bias_stride + (c >> kBiasShift) - 1];
-          raw[k] = BF16 ? f32_to_bf16(x) : __float_as_uint(x);
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < N; k++)
-        if (!(let >> k & 1)) raw[k] = BF16 ? 0xff80u : 0xff800000u;
-      if (full && same) {
-        v4i w;
-#pragma unroll
-        for (int k = 0; k < 4; k++) w[k] = BF16 ? (int)(raw[N / 4 * k] | raw[N / 4 * k + 1] << 16) : (int)raw[k];
-        *(v4i *)(out + v0 * E) = w;
-      } else {
-#pragma unroll
-        for (int k = 0; k < N; k++) {
-          if (k < from || k >= upto) continue;
-          if (BF16) ((uint16_t *)out)[v0 + k] = (uint16_t)raw[k];
-          else ((uint32_t *)out)[v0 + k] = raw[k];
+        } else if (hit[p]) {
+          for (int k = max(-v, 0); k < N && v + k < a.V; k++) {
+            if (!s.count[at + k] || (words && !(words[(v + k) >> 5] >> ((v + k) & 31) & 1))) continue;
+            const float x = adjusted(BF16 ? bf16_to_f32(((const uint16_t *)in)[v + k]) : ((const float *)in)[v + k], s.count[at + k]);
+            if (BF16) ((uint16_t *)out)[v + k] = (uint16_t)pack2_bf16(x, 0.f);
+            else ((float *)out)[v + k] = x;
+          }
         }
       }
     }
-    __syncthreads();
+#pragma unroll
+    for (int p = 0; p < P; p++) now[p] = next[MANY ? p : 0];
+    words = next_words;
+    if (MANY) __syncthreads();
   }
 }
 
@@ -203,7 +343,7 @@ extern "C" int moe_adjust_logits(void *stream, const void *logits, int dtype, in
                                  void *out, int64_t out_stride) {
   using namespace moe;
   if (dtype != MOE_DTYPE_F32 && dtype != MOE_DTYPE_BF16) return MOE_E_MODE;
-  if (T < 0 || V < 1 || B < 0 || L < 0 || n_bias < 0 || n_bias > MOE_MAX_BIASES || row_stride < V || out_stride < V || n_allowed < 0 ||
+  if (T < 0 || V < 1 || V >= (1 << 30) || B < 0 || L < 0 || n_bias < 0 || n_bias > MOE_MAX_BIASES || row_stride < V || out_stride < V || n_allowed < 0 ||
       (!cu_tokens && B != T) || (int64_t)L + T >= (1 << 20))
     return MOE_E_SHAPE;
   if ((history && history_stride < L) || (n_bias && (bias_ids_stride < n_bias || bias_stride < n_bias)) ||
@@ -216,15 +356,30 @@ extern "C" int moe_adjust_logits(void *stream, const void *logits, int dtype, in
   const uint8_t *i0 = (const uint8_t *)logits, *o0 = (const uint8_t *)out;
   if (!(i0 == o0 && (row_stride == out_stride || T == 1)) && i0 < o0 + ((T - 1) * out_stride + V) * e && o0 < i0 + ((T - 1) * row_stride + V) * e)
     return MOE_E_MODE;
-  constexpr int SEG = 8192;
   const int rows = B > 0 ? (T + B - 1) / B : 1;
-  LogitArgs a{logits, out, row_stride, out_stride, T, V, B, L, dtype == MOE_DTYPE_BF16, rows < 16 ? rows : 16, (V + 7 + SEG - 1) / SEG, cu_tokens,
+  LogitArgs a{logits, out, row_stride, out_stride, T, V, B, L, dtype == MOE_DTYPE_BF16, rows < 4 ? rows : 4, 0, cu_tokens,
               history, history_stride, history_lens, prompt_lens, tokens, masks, repetition, frequency, presence, bias_ids, bias_ids_stride, bias,
               bias_stride, n_bias, allowed, allowed_stride, n_allowed, allowed_rows};
-  const int64_t blocks = (int64_t)a.segments * ((T + a.rows - 1) / a.rows);
-  if (blocks > 0x7fffffff) return MOE_E_SHAPE;
   hipStream_t st = (hipStream_t)stream;
-  if (a.bf16) adjust_logits_kernel<SEG, true><<<(unsigned)blocks, 256, 0, st>>>(a);
-  else adjust_logits_kernel<SEG, false><<<(unsigned)blocks, 256, 0, st>>>(a);
-  return (int)hipGetLastError();
+  // (rows that begin on 16 bytes need no room for the values before)
+  const int64_t wide = (uintptr_t)logits % 16 == 0 && (T == 1 || row_stride * e % 16 == 0) ? V : (int64_t)V + 16 / e - 1;
+  const auto run = [&](auto bytes) {
+    constexpr int BYTES = decltype(bytes)::value;
+    a.segments = (int)((wide * e + BYTES - 1) / BYTES);
+    const int64_t blocks = (int64_t)a.segments * ((T + a.rows - 1) / a.rows);
+    if (blocks > 0x7fffffff) return MOE_E_SHAPE;
+    const unsigned n = (unsigned)blocks;
+    if (a.rows > 1) {
+      if (a.bf16) adjust_logits_kernel<BYTES, true, true><<<n, 256, 0, st>>>(a);
+      else adjust_logits_kernel<BYTES, false, true><<<n, 256, 0, st>>>(a);
+    } else {
+      if (a.bf16) adjust_logits_kernel<BYTES, true, false><<<n, 256, 0, st>>>(a);
+      else adjust_logits_kernel<BYTES, false, false><<<n, 256, 0, st>>>(a);
+    }
+    return (int)hipGetLastError();
+  };
+  using std::integral_constant;
+  const int64_t work = (int64_t)((T + a.rows - 1) / a.rows) * V * e;
+  if (work < (1 << 20)) return run(integral_constant<int, 4096>());
+  return run(integral_constant<int, 16384>());
 }

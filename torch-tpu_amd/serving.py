@@ -109,7 +109,7 @@ def adjust_logits(logits, cu_tokens=None, history=None, history_lens=None, promp
     history_lens [B] tokens (None: L), the first prompt_lens [B] of them its prompt (None: none); with tokens [T] int64 a row's history
     goes on with those that its mask names (masks [T] from cache_plan; None: those up to its own).  Of a token generated n times or
     heard in the prompt: x / repetition where x > 0, else x repetition; then - frequency n - presence (where n > 0); [B] float32
-    each.  Then + bias [B, N] float32 of the tokens bias_ids [B, N] int32 (of equal ids the last counts; N <= 2047), and -inf where
+    each.  Then + bias [B, N] float32 of the tokens bias_ids [B, N] int32 (of equal ids the last counts; N <= 1023), and -inf where
     allowed [M, ceil(V / 32)] int32 has no bit for the token in the row's grammar, allowed_rows [T] int32 (None: its own; -1: none).
     Ids outside [0, V) are passed over.  Returns out, a new tensor unless given; logits itself may be given."""
     return _ops.adjust_logits.default(logits, cu_tokens, history, history_lens, prompt_lens, tokens, masks, repetition, frequency, presence,
