@@ -26,8 +26,7 @@ def test_residual_norm_refusals(pkg):
         assert call(**bad) == E_MODE, bad
     for bad in (dict(x=None), dict(y=None)):
         assert call(**bad) == E_NULL, bad
-    for bad in (dict(x=ctypes.c_void_p(0x100001)), dict(res=ctypes.c_void_p(0x200002), rt=0), dict(gate=ctypes.c_void_p(0x500002), gt=0),
-                dict(H=16385, xs=20000, ys=20000, rs=20000, hs=20000, gr=20000), dict(H=20000, xs=20001, ys=20000, rs=20000, hs=20000, gr=20000)):
+    for bad in (dict(x=ctypes.c_void_p(0x100001)), dict(res=ctypes.c_void_p(0x200002), rt=0), dict(gate=ctypes.c_void_p(0x500002), gt=0)):
         assert call(**bad) == E_ALIGN, bad
     row = lambda p, n: ctypes.c_void_p(p.value + 2 * n)
     # over what is read, but not row on row

@@ -40,7 +40,7 @@ def check(a, got, scale, eps):
     (13, 520, False, "full", True, "both", True, 1.0), (4, 1024, True, "token", False, "weight", True, 2.0), (33, 1999, True, "token", False, "both", False, 0.7),
     (6, 2048, False, "one", False, "both", False, 1.0), (2, 4096, True, "column", True, "both", True, 1.0), (3, 4104, False, "full", False, "post", True, 1.0),
     (2, 8192, False, None, False, "both", False, 1.0), (2, 8200, True, "column", False, "both", False, 1.0), (3, 8193, False, "full", False, "both", False, 1.0),
-    (1, 16384, False, "row", False, "both", False, 1.0), (2, 16383, True, "full", True, "both", False, 1.0), (2, 32768, True, "column", False, "both", True, 1.0),
+    (1, 16384, False, "row", False, "both", False, 1.0), (2, 16383, True, "full", True, "both", False, 1.0), (2, 32768, True, "column", False, "both", True, 1.0), (2, 32761, False, "full", True, "both", False, 1.0),
     (1030, 255, False, "token", True, "both", False, 1.0), (613, 1000, False, None, False, "weight", False, 1.0), (0, 128, False, None, False, "both", False, 1.0)])
 def test_equals_the_plain_form(pkg, dev, T, H, wide, gate, gate_f32, weights, weights_f32, scale):
     say("residual_norm", T, H, wide, gate, weights)

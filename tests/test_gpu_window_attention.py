@@ -155,6 +155,51 @@ def test_windows_in_larger_tiles(pkg, dev, rows, cache, reqs, Hq, Hkv, D, as_tre
     s.check(out, lse)
 
 
+@pytest.mark.parametrize("D,Hq,Hkv", [(128, 8, 4), (64, 6, 2), (64, 16, 8)])
+@pytest.mark.parametrize("W,sinks", [(None, 0), (70, 3)])
+def test_two_heads_to_a_workgroup(pkg, dev, D, Hq, Hkv, W, sinks):
+    """Single tokens of many requests over a 4-bit cache: neighbouring heads' keys are read together."""
+    say("tree_attention, 4 bits, two heads", D, Hq, Hkv, W)
+    g = torch.Generator().manual_seed(D + Hkv)
+    reqs = [(int(n), 1) for n in torch.randint(0, 700, (130 // Hkv + 30,), generator=g)] + [(-1, 1), (0, 0), (1500, 1), (5, 1)]
+    s = Step(D, reqs, Hq, Hkv, D, 16, "fp4", False, W, sinks, spare_rows=2)
+    assert len(reqs) * Hkv >= 128 and s.rows(pkg) == 16
+    out, lse = pkg.tree_attention(**s.args(dev), return_lse=True)
+    torch.cuda.synchronize()
+    s.check(out, lse)
+    assert torch.equal(out, pkg.tree_attention(**s.args(dev)))
+
+
+@pytest.mark.parametrize("cache,reqs,Hq,Hkv,D,W,sinks", [
+    # a tile to each workgroup or several, parts of one, and lengths too different for either
+    ("bf16", [(400 + b, 1) for b in range(100)], 8, 4, 64, 200, 4), ("bf16", [(300, 1)] * 260, 4, 2, 128, 100, 0), ("fp8", [(900, 1)] * 3, 4, 2, 64, 500, 1),
+    ("fp4", [(90 * b, 1) for b in range(70)], 2, 1, 64, 600, 0), ("bf16", [(2000, 1), (100, 1)], 2, 1, 64, 1900, 7),
+    # prompts: more tiles than lanes, and many requests with tiles of their own
+    ("bf16", [(0, 1500), (700, 900)], 8, 2, 64, 300, 4), ("fp4", [(100, 2500)], 2, 2, 64, None, 0), ("fp4", [(13 * b, 40 + b) for b in range(70)], 4, 1, 64, 64, 2),
+    ("fp8", [(500, 200), (0, 3), (40, 700)], 16, 1, 128, 90, 0), ("fp4", [(0, 1100), (3, 1), (-1, 4), (90, 600)], 3, 1, 64, None, 0)])
+def test_ways_along_the_line(pkg, dev, cache, reqs, Hq, Hkv, D, W, sinks):
+    say("tree_attention, lines of", len(reqs), "requests", cache, W)
+    for room in (None, 131072):                          # (another room, another tile)
+        s = Step(len(reqs) + D, reqs, Hq, Hkv, D, 64, cache, False, W, sinks)
+        if room:
+            one_request_in_room(s, room)
+        out, lse = pkg.tree_attention(**s.args(dev), return_lse=True)
+        torch.cuda.synchronize()
+        s.check(out, lse)
+        assert torch.equal(out, pkg.tree_attention(**s.args(dev)))
+
+
+@pytest.mark.parametrize("cu", [[0, 5, 3, 9], [9, 0, 9, 2], [0, 9, 0, 9], [-4, 20, 1, 3]])
+def test_every_walk_ends(pkg, dev, cu):
+    """cu_tokens that do not ascend: results are undefined, but the launch ends."""
+    say("tree_attention in a window, cu_tokens", cu)
+    for W, cache in ((20, "bf16"), (None, "fp4")):
+        s = Step(2, [(300, 3), (200, 3), (64, 3)], 8, 2, 64, 16, cache, False, W)
+        pkg.tree_attention(**s.args(dev, cu_tokens=ints(cu, dev)))
+        pkg.tree_attention(**s.args(dev, kv_lens=ints([2 ** 31 - 1, -5, 7], dev)))
+    torch.cuda.synchronize()
+
+
 @pytest.mark.parametrize("cache", ["bf16", "fp8", "fp4"])
 @pytest.mark.parametrize("as_tree", [False, True])
 def test_scores_that_grow_along_a_window(pkg, dev, cache, as_tree):

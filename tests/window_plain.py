@@ -54,14 +54,15 @@ def attention(q, k, v, tables, kv_lens, cu, masks, scale, window=None, sinks=0):
         p = S - n
         may = torch.zeros(n, S, dtype=torch.bool)
         may[:, :p] = True
-        for j in range(n):
-            for i in range(n):
-                may[j, p + i] = bool(masks[t0 + j] >> i & 1) if masks is not None else i <= j
+        if masks is None:
+            may[:, p:] = torch.ones(n, n, dtype=torch.bool).tril()
+        else:
+            may[:, p:] = torch.tensor([[m >> i & 1 == 1 for i in range(n)] for m in masks[t0:t1]])
         if window is not None:
             number = may.long().cumsum(1) - 1
             may &= (number >= may.sum(1, keepdim=True) - window) | (number < sinks)
-        used = [s for s in range(S) if bool(may[:, s].any())]            # (the table may hold nothing for the others)
-        at = torch.tensor([tables[b][s // page] * page + s % page for s in used], dtype=torch.long)
+        used = may.any(0).nonzero()[:, 0]                                # (the table may hold nothing for the others)
+        at = torch.tensor(tables[b], dtype=torch.long)[used // page] * page + used % page
         K, V, sees = k.flatten(0, 1)[at], v.flatten(0, 1)[at], may[:, used]
         for h in range(Hkv):
             x = torch.einsum("ngd,sd->ngs", q[t0:t1, h * G:(h + 1) * G].double(), K[:, h].nan_to_num(0.0, 0.0, 0.0)) * scale

@@ -99,7 +99,7 @@ __device__ __forceinline__ int attn_head_units(const AttnArgs &a, const AttnRequ
 // memory and no barrier stand in front of the work.  The host has seen to it that the line's length fits an int where cu_tokens ascends;
 // where it does not, requests share rows and the line may have any length: a longer one than the host allowed for is taken for empty, so that
 // no index wraps and every walk ends.
-template <int ROWS, int UNIT, bool LOCAL, typename Segment>
+template <int ROWS, int UNIT, typename Segment>
 __device__ __forceinline__ void attn_walk(const AttnArgs &a, Segment segment) {
   const int lane = threadIdx.x & 63;
   AttnRequest mine{0, 0, 0, -1};
@@ -108,9 +108,9 @@ __device__ __forceinline__ void attn_walk(const AttnArgs &a, Segment segment) {
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     if (b0 + lane < a.B) mine = attn_request(a, b0 + lane);
     else mine.n = 0;
-    units = attn_head_units<ROWS, UNIT, LOCAL>(a, mine) * a.Hkv;
+    units = attn_head_units<ROWS, UNIT, false>(a, mine) * a.Hkv;
     upto = __builtin_elementwise_add_sat(upto, (uint32_t)units);
-    if (units > 0) longest = max(longest, LOCAL ? attn_reach<ROWS, UNIT, LOCAL>(a, mine, (mine.n * a.G - 1) / ROWS).units : (mine.kv + UNIT - 1) / UNIT);
+    if (units > 0) longest = max(longest, (mine.kv + UNIT - 1) / UNIT);
   }
   upto = lane_sum_upto(upto);                          // (with up to 64 requests: the line's length up to each)
   int total = __builtin_amdgcn_readlane(upto, 63);
@@ -132,7 +132,7 @@ __device__ __forceinline__ void attn_walk(const AttnArgs &a, Segment segment) {
     if (a.B > 64) {
       if (b0 + lane < a.B) mine = attn_request(a, b0 + lane);
       else mine.n = 0;
-      units = attn_head_units<ROWS, UNIT, LOCAL>(a, mine) * a.Hkv;
+      units = attn_head_units<ROWS, UNIT, false>(a, mine) * a.Hkv;
       upto = lane_sum_upto(units);
     }
     const uint64_t past = __ballot(start < before + (int)upto);
@@ -147,20 +147,20 @@ __device__ __forceinline__ void attn_walk(const AttnArgs &a, Segment segment) {
     before += __builtin_amdgcn_readlane(upto, 63);
   }
   for (int at = start;;) {
-    const int head = attn_head_units<ROWS, UNIT, LOCAL>(a, r);
+    const int head = attn_head_units<ROWS, UNIT, false>(a, r);
     if (at >= before + head * a.Hkv) {
       before += head * a.Hkv;
       r = attn_request(a, ++b);
       continue;
     }
     const int kh = (at - before) / head, in_head = at - before - kh * head;
-    int m = 0, u = LOCAL ? attn_reach<ROWS, UNIT, LOCAL>(a, r, 0).units : (r.kv + UNIT - 1) / UNIT, first = 0;
+    int m = 0, u = (r.kv + UNIT - 1) / UNIT, first = 0;
     if (a.masks || r.n == 1) {
       m = in_head / u;
       first = m * u;
     } else {
       for (;; m++) {
-        u = attn_reach<ROWS, UNIT, LOCAL>(a, r, m).units;
+        u = attn_reach<ROWS, UNIT, false>(a, r, m).units;
         if (in_head < first + u) break;
         first += u;
       }
@@ -174,6 +174,173 @@ __device__ __forceinline__ void attn_walk(const AttnArgs &a, Segment segment) {
     at += c1 - c0;
     if (at >= end) break;
   }
+}
+
+// The same for LOCAL kernels.  With a window most tiles are equally long, and lengths may be alike without one: where all tiles filled up to the longest
+// one's length are not more than an eighth longer, the line has every tile at that length, and stretches are whole tiles or a tile's equal parts, so that
+// none holds the end of one tile and the beginning of the next and, of whole tiles, nothing is left to join (two chunks of 1021 tokens
+// in a window of 1024: 89 us with stretches across tiles, 73 so; 64 single tokens: 42 and 34).
+template <int ROWS, int UNIT, int HEADS, typename Segment>
+__device__ __forceinline__ void attn_walk_local(const AttnArgs &a, Segment segment) {
+  const int lane = threadIdx.x & 63, heads = a.Hkv / HEADS;
+  const auto tiles_of = [&](const AttnRequest &r) { return r.n <= 0 || r.prefix < 0 ? 0 : (r.n * a.G + ROWS - 1) / ROWS; };
+  const auto alike = [&](const AttnRequest &r) { return a.masks || r.n == 1; };        // all tiles of the request
+  struct Tiles {
+    int units, longest;                // of all tiles of a request for a head; of the longest of them
+  };
+  // of a request that all lanes hold, a tile to a lane
+  const auto sum_of = [&](const AttnRequest &r) {
+    const int tiles = tiles_of(r);
+    if (alike(r)) {
+      const int u = tiles ? attn_reach<ROWS, UNIT, true>(a, r, 0).units : 0;
+      return Tiles{tiles * u, u};
+    }
+    int sum = 0, most = 0;
+    for (int m = 0; m < tiles; m += 64) {
+      const int u = m + lane < tiles ? attn_reach<ROWS, UNIT, true>(a, r, m + lane).units : 0;
+      sum += __builtin_amdgcn_readlane(lane_sum_upto((uint32_t)u), 63);
+      most = max(most, u);
+    }
+    return Tiles{sum, __builtin_amdgcn_readfirstlane(lane_max(most))};
+  };
+  const auto of_lane = [&](const AttnRequest &r, int l) {
+    return AttnRequest{__builtin_amdgcn_readlane(r.t0, l), __builtin_amdgcn_readlane(r.n, l), __builtin_amdgcn_readlane(r.kv, l), __builtin_amdgcn_readlane(r.prefix, l)};
+  };
+  // of 64 requests, one to a lane: the units of each one's tiles (a lane by itself, or all of them for one request after the other if that
+  // takes fewer turns)
+  const auto head_units = [&](const AttnRequest &r) {
+    const int tiles = tiles_of(r), turns = alike(r) ? 1 : tiles;
+    const int most = __builtin_amdgcn_readfirstlane(lane_max(turns)), together = __builtin_amdgcn_readlane(lane_sum_upto((uint32_t)(turns + 63) / 64), 63);
+    Tiles t{0, 0};
+    if (most <= 2 * together) {
+      if (alike(r)) {
+        t.longest = tiles ? attn_reach<ROWS, UNIT, true>(a, r, 0).units : 0;
+        t.units = tiles * t.longest;
+      } else {
+        for (int m = 0; m < tiles; m++) {
+          const int u = attn_reach<ROWS, UNIT, true>(a, r, m).units;
+          t.units += u;
+          t.longest = max(t.longest, u);
+        }
+      }
+      return t;
+    }
+    for (uint64_t todo = __ballot(tiles > 0); todo; todo &= todo - 1) {
+      const int l = __builtin_ctzll(todo);
+      const Tiles its = sum_of(of_lane(r, l));
+      if (lane == l) t = its;
+    }
+    return t;
+  };
+  const auto request = [&](int b) { return b < a.B ? attn_request(a, b) : AttnRequest{0, 0, 0, -1}; };
+
+  AttnRequest mine{0, 0, 0, -1};
+  int units = 0, longest = 0;
+  uint32_t upto = 0, tiles = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    mine = request(b0 + lane);
+    const Tiles its = head_units(mine);
+    units = its.units * heads;
+    longest = max(longest, its.longest);
+    upto = __builtin_elementwise_add_sat(upto, (uint32_t)units);
+    tiles = __builtin_elementwise_add_sat(tiles, (uint32_t)(tiles_of(mine) * heads));
+  }
+  upto = lane_sum_upto(upto);                          // (with up to 64 requests: the line's length up to each)
+  int total = __builtin_amdgcn_readlane(upto, 63);
+  if ((uint32_t)total > a.most_units) total = 0;
+  tiles = __builtin_amdgcn_readlane(lane_sum_upto(tiles), 63);
+  longest = __builtin_amdgcn_readfirstlane(lane_max(longest));
+  const int even = (int)(((uint32_t)total + a.groups - 1) / (uint32_t)a.groups), least = max(__builtin_amdgcn_readfirstlane((int)ceilf(sqrtf((float)longest * a.cut))), 1);
+  int per = max(max(even, least), 1), filled = 0;      // filled: the length of every tile on the line, or 0: their own
+  if (total > 0 && (uint64_t)tiles * (uint64_t)longest * 8 <= (uint64_t)total * 9) {
+    const uint32_t groups = (uint32_t)a.groups;
+    if (tiles >= groups) {                             // some tiles to each workgroup, if few of these go without
+      const uint32_t each = (tiles + groups - 1) / groups;
+      if ((uint64_t)tiles * 8 >= (uint64_t)groups * each * 7) filled = longest, per = longest * (int)each;
+    } else {                                           // a tile to some workgroups
+      const int share = (int)(groups / tiles), most = max(longest / least, 1), pieces = min(share, most);
+      if (most < share || tiles * (uint32_t)pieces * 8 >= groups * 7) {
+        per = (longest + pieces - 1) / pieces;
+        filled = per * ((longest + per - 1) / per);
+      }
+    }
+    if ((uint64_t)tiles * (uint64_t)filled > 0x7fffffffull) filled = 0, per = max(even, least);
+  }
+  if (filled) {
+    total = (int)tiles * filled;
+    units = tiles_of(mine) * heads * filled;
+    upto = lane_sum_upto((uint32_t)units);
+  }
+  // Neighbouring stretches on one XCD, as above.
+  const int eighth = (int)(((uint32_t)total + per - 1) / (uint32_t)per + 7) / 8, wg = blockIdx.x, place = wg < 8 * eighth ? wg % 8 * eighth + wg / 8 : wg;
+  const int start = (int)min((int64_t)place * per, (int64_t)total), end = start + min(per, total - start);
+  if (threadIdx.x == 0) a.records[8 * place] = -1;
+  if (start >= end) return;
+  int b = 0, before = 0;
+  AttnRequest r{};
+  for (int b0 = 0;; b0 += 64) {                        // (ends: start < total)
+    if (a.B > 64) {
+      mine = request(b0 + lane);
+      units = filled ? tiles_of(mine) * heads * filled : head_units(mine).units * heads;
+      upto = lane_sum_upto((uint32_t)units);
+    }
+    const uint64_t past = __ballot(start < before + (int)upto);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      b = b0 + l;
+      before += __builtin_amdgcn_readlane((int)upto - units, l);
+      r = of_lane(mine, l);
+      break;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  int head = filled ? tiles_of(r) * filled : sum_of(r).units;
+  for (int at = start;;) {
+    if (at >= before + head * heads) {
+      before += head * heads;
+      r = attn_request(a, ++b);
+      head = filled ? tiles_of(r) * filled : sum_of(r).units;
+      continue;
+    }
+    const int kh = (at - before) / head, in_head = at - before - kh * head;
+    int m = 0, u = 0, slots = filled, first = 0;
+    if (filled || alike(r)) {
+      if (!filled) slots = attn_reach<ROWS, UNIT, true>(a, r, 0).units;
+      m = in_head / slots;
+      first = m * slots;
+      u = attn_reach<ROWS, UNIT, true>(a, r, m).units;
+    } else {
+      for (;; m += 64) {                               // (ends: the tiles' units add up to more than in_head)
+        const int own = m + lane < tiles_of(r) ? attn_reach<ROWS, UNIT, true>(a, r, m + lane).units : 0;
+        const int so_far = first + (int)lane_sum_upto((uint32_t)own);
+        const uint64_t past = __ballot(in_head < so_far);
+        if (past) {
+          const int l = __builtin_ctzll(past);
+          m += l;
+          u = slots = __builtin_amdgcn_readlane(own, l);
+          first = __builtin_amdgcn_readlane(so_far, l) - u;
+          break;
+        }
+        first = __builtin_amdgcn_readlane(so_far, 63);
+      }
+    }
+    const int c0 = in_head - first, c1 = min(u, c0 + (end - at));
+    if (c0 < u) {                                      // (behind it the tile is filled up)
+      if (threadIdx.x == 0 && c0 == 0 && c1 < u) {
+        int32_t *rec = a.records + 8 * place;
+        rec[0] = (at + u - 1) / per, rec[1] = r.t0, rec[2] = r.n, rec[3] = kh, rec[4] = m, rec[5] = at > start;
+      }
+      segment(r, b, kh, m, c0, c1, c0 == 0 && c1 == u, 2 * place + (at - c0 > start ? 1 : 0));
+    }
+    at += min(slots - c0, end - at);
+    if (at >= end) break;
+  }
+}
+// LOCAL or not
+template <int ROWS, int UNIT, bool LOCAL, int HEADS, typename Segment>
+__device__ __forceinline__ void attn_go(const AttnArgs &a, Segment segment) {
+  if constexpr (LOCAL) attn_walk_local<ROWS, UNIT, HEADS>(a, segment);
+  else attn_walk<ROWS, UNIT>(a, segment);
 }
 
 // ---- softmax and products of 32 keys ----------------------------------------------------------------------------------
@@ -507,18 +674,20 @@ __device__ __forceinline__ void attn_store(const AttnArgs &a, const AttnRequest 
 // from memory straight into operand registers, values through LDS that no other wavefront touches, so nothing waits at a
 // barrier, and the next keys and values are asked for before the present ones are worked on.  The wavefronts' results meet in
 // LDS at the end of a tile.
-template <int D, int C, bool LOCAL, int NQ>
+template <int D, int C, bool LOCAL, int NQ, int HEADS>
 __global__ __launch_bounds__(256, 2) void attn_keys_kernel(const AttnArgs a) {
-  constexpr int ROWS = 16 * NQ, UNIT = 128, DT = D / 16, LD = 2 * D + 32;
+  constexpr int ROWS = 16 * NQ, SHARE = 4 / HEADS, UNIT = 32 * SHARE, DT = D / 16, LD = 2 * D + 32;
   using Piece = AttnPiece<C, C == MOE_DTYPE_FP4 ? D / 8 : 16>;
   constexpr int E = Piece::E, P = D / (4 * E);         // a lane's pieces of a key
   constexpr int kValues = 4 * 32 * LD, kMerge = 4 * DT * NQ * 64 * 16;
   __shared__ __attribute__((aligned(16))) uint8_t lds[kValues > kMerge ? kValues : kMerge];
   __shared__ float sh_m[4][ROWS], sh_l[4][ROWS];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c16 = lane & 15;
+  const int of_head = w % HEADS, part_of_unit = w / HEADS;
   uint8_t *values = lds + w * 32 * LD;
   const uint8_t *read_at = values + (4 * g + c16 / 4) * LD + 8 * (c16 % 4);
-  attn_walk<ROWS, UNIT, LOCAL>(a, [&](const AttnRequest r, int b, int kh, int m_tile, int c0, int c1, bool whole, int part) {
+  attn_go<ROWS, UNIT, LOCAL, HEADS>(a, [&](const AttnRequest r, int b, int first_head, int m_tile, int c0, int c1, bool whole, int part) {
+    const int kh = first_head * HEADS + of_head;
     const int32_t *table = a.tables + (size_t)b * a.table_stride;
     const float factor = a.scale * (a.k_scale ? a.k_scale[kh] : 1.f) * 1.4426950408889634f, scale = fabsf(factor);
     v8bf q[NQ][D / 32];
@@ -532,7 +701,7 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(const AttnArgs a) {
     Piece kr[2][P], vr[2][P];
     uint32_t kp[2], vp[2];                             // their powers of two
     int block[2];
-    const auto key_of = [&](int unit, int kt) { return min(reach.unit(unit) * UNIT + 32 * w + 16 * kt + c16, r.kv - 1); };
+    const auto key_of = [&](int unit, int kt) { return min(reach.unit(unit) * UNIT + 32 * part_of_unit + 16 * kt + c16, r.kv - 1); };
     const auto blocks = [&](int unit) {
 #pragma unroll
       for (int kt = 0; kt < 2; kt++) block[kt] = attn_block(a, table, key_of(unit, kt));
@@ -555,7 +724,7 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(const AttnArgs a) {
     bool sure = true;                                  // the next keys may be the first that a row sees
     blocks(min(c0 + 1, c1 - 1));
     for (int c = c0; c < c1; c++) {
-      const int key0 = reach.unit(c) * UNIT + 32 * w;
+      const int key0 = reach.unit(c) * UNIT + 32 * part_of_unit;
       v4f s[2][NQ];
 #pragma unroll
       for (int kt = 0; kt < 2; kt++)
@@ -627,21 +796,21 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(const AttnArgs a) {
 #pragma unroll
     for (int qc = 0; qc < NQ; qc++) {
       const int row = 16 * qc + c16;
-      float m = sh_m[0][row], l = 0.f, f[4];
+      float m = sh_m[of_head][row], l = 0.f, f[SHARE];
 #pragma unroll
-      for (int i = 1; i < 4; i++) m = fmaxf(m, sh_m[i][row]);
+      for (int i = 1; i < SHARE; i++) m = fmaxf(m, sh_m[of_head + HEADS * i][row]);
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        f[i] = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(sh_m[i][row] - m);
-        l += sh_l[i][row] * f[i];
+      for (int i = 0; i < SHARE; i++) {
+        f[i] = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(sh_m[of_head + HEADS * i][row] - m);
+        l += sh_l[of_head + HEADS * i][row] * f[i];
       }
 #pragma unroll
-      for (int x = 0; x < DT / 4; x++) {
-        const int dt = w * (DT / 4) + x;
+      for (int x = 0; x < DT / SHARE; x++) {
+        const int dt = part_of_unit * (DT / SHARE) + x;
         v4f o = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 4; i++) o += *(const v4f *)(lds + (((size_t)i * DT + dt) * NQ + qc) * 1024 + lane * 16) * f[i];
-        attn_store<ROWS, D>(a, r, kh, m_tile, row, 16 * dt + 4 * g, whole, part, o, m, l);
+        for (int i = 0; i < SHARE; i++) o += *(const v4f *)(lds + (((size_t)(of_head + HEADS * i) * DT + dt) * NQ + qc) * 1024 + lane * 16) * f[i];
+        attn_store<ROWS, D>(a, r, kh, m_tile, row, 16 * dt + 4 * g, whole, part * HEADS + of_head, o, m, l);
       }
     }
     __syncthreads();
@@ -704,7 +873,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const AttnArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
   __shared__ int any_odd;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c16 = lane & 15;
-  attn_walk<ROWS, UNIT, LOCAL>(a, [&](const AttnRequest r, int b, int kh, int m_tile, int c0, int c1, bool whole, int part) {
+  attn_go<ROWS, UNIT, LOCAL, 1>(a, [&](const AttnRequest r, int b, int kh, int m_tile, int c0, int c1, bool whole, int part) {
     const int32_t *table = a.tables + (size_t)b * a.table_stride;
     const float factor = a.scale * (a.k_scale ? a.k_scale[kh] : 1.f) * 1.4426950408889634f, scale = fabsf(factor);
     const int clear = a.masks ? r.prefix : r.prefix + m_tile * ROWS / a.G + 1;      // keys below it are seen by every row
@@ -752,7 +921,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const AttnArgs a) {
       __syncthreads();
     };
     const auto take = [&](auto sixteens) {
-      constexpr int N = decltype(sixteens)::value, AHEAD = N == 2 && C == MOE_DTYPE_BF16 ? 2 : 3;     // (as the registers allow)
+      constexpr int N = decltype(sixteens)::value, AHEAD = N == 2 && C == MOE_DTYPE_BF16 ? (LOCAL ? 1 : 2) : 3;     // (as the registers allow)
       v8bf q[N][D / 32];
       AttnSight<N, LOCAL> sight;
       attn_queries<N, D, 8, LOCAL, 64>(a, r, kh, m_tile * ROWS + 16 * w, factor, q, sight);
@@ -825,7 +994,7 @@ __global__ __launch_bounds__(512, 2) void attn_pairs_kernel(const AttnArgs a) {
   __shared__ int any_odd;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c16 = lane & 15;
   const int late = __builtin_amdgcn_readfirstlane(w) >> 2;
-  attn_walk<ROWS, UNIT, LOCAL>(a, [&](const AttnRequest r, int b, int kh, int m_tile, int c0, int c1, bool whole, int part) {
+  attn_go<ROWS, UNIT, LOCAL, 1>(a, [&](const AttnRequest r, int b, int kh, int m_tile, int c0, int c1, bool whole, int part) {
     const int32_t *table = a.tables + (size_t)b * a.table_stride;
     const float factor = a.scale * (a.k_scale ? a.k_scale[kh] : 1.f) * 1.4426950408889634f, scale = fabsf(factor);
     const int clear = a.masks ? r.prefix : r.prefix + m_tile * ROWS / a.G + 1;      // keys below it are seen by every row
@@ -971,13 +1140,15 @@ __global__ __launch_bounds__(512, 2) void attn_pairs_kernel(const AttnArgs a) {
 struct AttnPlan {
   int rows, groups;                    // rows of a tile; workgroups, a multiple of 8
   float cut;
+  int heads;                           // cache heads of a workgroup (of 16 rows)
 };
 inline AttnPlan attn_plan(int T, int Hq, int Hkv, int B, int cache_dtype, bool trees, int64_t keys) {
   const int64_t rows = B > 0 ? ((int64_t)T * (Hq / Hkv) + B - 1) / B : 1;
-  if (rows <= 16) return {16, cache_dtype == MOE_DTYPE_BF16 ? 256 : 512, 0.0625f};
-  if (rows <= 64 || (int64_t)T * Hq <= (trees ? 20000000 : 8000000) / (keys > 0 ? keys : 1)) return {64, 512, 0.125f};
-  if (rows <= 128) return {128, 512, 0.125f};
-  return {256, 256, 0.25f};
+  const int heads = Hkv % 2 == 0 && (int64_t)B * Hkv >= 128 ? 2 : 1;
+  if (rows <= 16) return {16, cache_dtype == MOE_DTYPE_BF16 ? 256 : 512, 0.0625f, cache_dtype == MOE_DTYPE_FP4 ? heads : 1};
+  if (rows <= 64 || (int64_t)T * Hq <= (trees ? 20000000 : 8000000) / (keys > 0 ? keys : 1)) return {64, 512, 0.125f, 1};
+  if (rows <= 128) return {128, 512, 0.125f, 1};
+  return {256, 256, 0.25f, 1};
 }
 // the keys that a row sees at most, where there is room for so many
 inline int64_t attn_seen(int64_t room, int window, int sinks) {
@@ -1023,8 +1194,8 @@ inline int attn_arguments(const void *q_bf16, int64_t q_stride, int T, int Hq, i
   a = AttnArgs{(const uint16_t *)q_bf16, q_stride, T, Hq, Hkv, Hq / Hkv, B, n_blocks, __builtin_ctz(page_size), n_blocks ? table_width : 0,
                (const uint8_t *)k_cache, (const uint8_t *)v_cache, (uint32_t)(k_block_stride * bits / 8), (uint32_t)(v_block_stride * bits / 8), table_stride,
                block_tables, kv_lens, cu_tokens, masks, scale, four ? nullptr : (const float *)k_scale, four ? nullptr : (const float *)v_scale,
-               (uint16_t *)out_bf16, lse, p.groups, p.cut, (float *)workspace, (float *)(ws + align_up(parts * p.rows * D * 4, 256)),
-               (int32_t *)(ws + align_up(parts * p.rows * D * 4, 256) + align_up(parts * p.rows * 8, 256)), (uint32_t)most_units,
+               (uint16_t *)out_bf16, lse, p.groups, p.cut, (float *)workspace, (float *)(ws + align_up(parts * p.rows * p.heads * D * 4, 256)),
+               (int32_t *)(ws + align_up(parts * p.rows * p.heads * D * 4, 256) + align_up(parts * p.rows * p.heads * 8, 256)), (uint32_t)most_units,
                window ? window : 0x7fffffff, sinks, four ? (const uint8_t *)k_scale : nullptr, four ? (const uint8_t *)v_scale : nullptr,
                (uint32_t)k_scale_stride, (uint32_t)v_scale_stride};
   plan = p;
@@ -1034,7 +1205,10 @@ inline int attn_arguments(const void *q_bf16, int64_t q_stride, int T, int Hq, i
 // The main launch of a plan's kernel.  (The join, which knows nothing of the cache, is launched by attn_join.)
 template <int D, int C, bool LOCAL>
 void attn_main(const AttnArgs &a, const AttnPlan &plan, hipStream_t st) {
-  if (plan.rows == 16) attn_keys_kernel<D, C, LOCAL, 1><<<a.groups, 256, 0, st>>>(a);
+  if (plan.rows == 16 && plan.heads == 1) attn_keys_kernel<D, C, LOCAL, 1, 1><<<a.groups, 256, 0, st>>>(a);
+  else if (plan.rows == 16) {
+    if constexpr (C == MOE_DTYPE_FP4) attn_keys_kernel<D, C, LOCAL, 1, 2><<<a.groups, 256, 0, st>>>(a);
+  }
   else if (plan.rows == 64) attn_rows_kernel<D, C, LOCAL, 1><<<a.groups, 256, 0, st>>>(a);
   else if (plan.rows == 128) attn_rows_kernel<D, C, LOCAL, 2><<<a.groups, 256, 0, st>>>(a);
   else attn_pairs_kernel<D, C, LOCAL, 2><<<a.groups, 512, 0, st>>>(a);

@@ -6,7 +6,7 @@ namespace moe {
 // ---- joining ------------------------------------------------------------------------------------------------------------
 // Row blocks of the tile that began in stretch blockIdx.x and went on in later ones: the parts in the stretches' order.  A row is taken by
 // SPLIT groups of D / 4 lanes, each a share of the parts, which meet in LDS.  Rows of no request and of refused ones become 0.
-template <int ROWS, int D, int SPLIT>
+template <int ROWS, int D, int SPLIT, int HEADS>
 __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
   constexpr int lanes = D / 4, per_block = 256 / (lanes * SPLIT);
   __shared__ v4f sh_o[256];
@@ -32,9 +32,11 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
   const int w1 = rec[0], kh = rec[3], m_tile = rec[4], side = rec[5], w0 = blockIdx.x;
   const AttnRequest r{rec[1], rec[2], 0, 0};
   if (w1 <= w0) return;
-  const int in_tile = blockIdx.y * per_block + group / SPLIT, row = m_tile * ROWS + in_tile;
-  if (m_tile * ROWS + (int)blockIdx.y * per_block >= r.n * a.G) return;
-  const auto part = [&](int w) { return (size_t)(2 * w + (w == w0 ? side : 0)) * ROWS + in_tile; };
+  constexpr int blocks = ROWS / per_block;             // of a head
+  const int of_head = blockIdx.y / blocks, first_row = blockIdx.y % blocks * per_block;
+  const int in_tile = first_row + group / SPLIT, row = m_tile * ROWS + in_tile;
+  if (m_tile * ROWS + first_row >= r.n * a.G) return;
+  const auto part = [&](int w) { return ((size_t)(2 * w + (w == w0 ? side : 0)) * HEADS + of_head) * ROWS + in_tile; };
   float m = -INFINITY, l = 0.f;
   v4f o = (v4f){0.f, 0.f, 0.f, 0.f};
   if (row < r.n * a.G) {
@@ -82,21 +84,23 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
       o += sh_o[tid + i * lanes] * f;
     }
   }
-  attn_store<ROWS, D>(a, r, kh, m_tile, in_tile, d, true, 0, o, m, l);
+  attn_store<ROWS, D>(a, r, kh * HEADS + of_head, m_tile, in_tile, d, true, 0, o, m, l);
 }
 
 void attn_join(const AttnArgs &a, const AttnPlan &plan, int D, hipStream_t st) {
   using std::integral_constant;
   const auto run = [&](auto dim) {
     constexpr int Dc = decltype(dim)::value;
-    const auto join = [&](auto rows, auto split) {
-      constexpr int R = decltype(rows)::value, S = decltype(split)::value;
-      attn_join_kernel<R, Dc, S><<<dim3(a.groups, R * Dc * S / 1024 + 1), 256, 0, st>>>(a);
+    const auto join = [&](auto rows, auto split, auto heads) {
+      constexpr int R = decltype(rows)::value, S = decltype(split)::value, H = decltype(heads)::value;
+      attn_join_kernel<R, Dc, S, H><<<dim3(a.groups, R * H * Dc * S / 1024 + 1), 256, 0, st>>>(a);
     };
-    if (plan.rows == 16) join(integral_constant<int, 16>(), integral_constant<int, 8>());
-    else if (plan.rows == 64) join(integral_constant<int, 64>(), integral_constant<int, 2>());
-    else if (plan.rows == 128) join(integral_constant<int, 128>(), integral_constant<int, 1>());
-    else join(integral_constant<int, 256>(), integral_constant<int, 1>());
+    constexpr integral_constant<int, 1> one{};
+    if (plan.rows == 16 && plan.heads == 1) join(integral_constant<int, 16>(), integral_constant<int, 8>(), one);
+    else if (plan.rows == 16) join(integral_constant<int, 16>(), integral_constant<int, 8>(), integral_constant<int, 2>());
+    else if (plan.rows == 64) join(integral_constant<int, 64>(), integral_constant<int, 2>(), one);
+    else if (plan.rows == 128) join(integral_constant<int, 128>(), one, one);
+    else join(integral_constant<int, 256>(), one, one);
   };
   if (D == 64) run(integral_constant<int, 64>());
   else run(integral_constant<int, 128>());
@@ -108,7 +112,7 @@ extern "C" size_t moe_tree_attention_workspace_bytes(int T, int Hq, int Hkv, int
   using namespace moe;
   if (T < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || D < 1 || B < 0 || cache_dtype < MOE_DTYPE_BF16 || cache_dtype > MOE_DTYPE_FP4) return 0;
   const AttnPlan plan = attn_plan(T, Hq, Hkv, B, cache_dtype, false, 1ll << 31);      // (shorter caches need no more)
-  const size_t rows = plan.rows, parts = 2 * plan.groups;
+  const size_t rows = (size_t)plan.rows * plan.heads, parts = 2 * plan.groups;
   return align_up(parts * rows * D * 4, 256) + align_up(parts * rows * 8, 256) + plan.groups * 32;
 }
 

@@ -96,8 +96,7 @@ def residual_norm(x, residual=None, weight=None, post_weight=None, gate=None, sc
     u = x rsqrt(mean(x^2) + eps) post_weight (x itself without a post_weight);  h = residual + scale gate u;
     y = h rsqrt(mean(h^2) + eps) weight.  x [T, H] bf16; residual [T, H] bf16 or float32 (None: 0); weights [H] bf16 or float32 (both alike);
     gate bf16 or float32, [H] or [T or 1, H or 1].  Rows at any distance.  Returns (y [T, H] bf16, h in the residual's dtype).
-    out and residual_out may each be x or the residual itself; other overlaps are refused.  H up to 32768 (16384 where rows do not
-    begin on 16 bytes)."""
+    out and residual_out may each be x or the residual itself; other overlaps are refused.  H up to 32768."""
     return _ops.residual_norm.default(x, residual, weight, post_weight, gate, scale, eps, out, residual_out)
 
 
