@@ -1,10 +1,10 @@
 """A small decoder with drafted token trees on one GPU: the paged-cache operators around the FP8 MoE layer.
 
-    python examples/tree_decode.py [--requests 4] [--steps 16] [--cache fp8]
+    python examples/tree_decode.py [--requests 4] [--steps 16] [--cache fp8 | fp4] [--window 64 --sinks 4] [--repetition 1.2]
 
 Each step takes every request's last token and a small tree of guesses for what follows it, runs them all in one pass
-(cache_plan, then per layer: products, qk_norm_rope into the cache, tree_attention, the MoE layer; token_logprobs on the logits),
-and keeps the guesses that the model itself would have chosen.  The guesses are what the model answered the last time it saw a
+(cache_plan, then per layer: products, qk_norm_rope into the cache, tree_attention, residual_norm, the MoE layer; adjust_logits where there is a
+penalty, token_logprobs on the logits), and keeps the guesses that the model itself would have chosen.  The guesses are what the model answered the last time it saw a
 token, at first what its output layer makes of the token's embedding alone.  Weights are random, so the text means nothing; what is shown is how many tokens come out of a step.
 """
 import argparse
@@ -20,7 +20,10 @@ pkg = load_package()
 
 
 class Decoder:
-    def __init__(self, layers=2, hidden=512, heads=8, kv_heads=2, head_dim=64, experts=8, top_k=2, inter=256, vocab=2048, device="cuda:0", seed=0):
+    def __init__(self, layers=2, hidden=512, heads=8, kv_heads=2, head_dim=64, experts=8, top_k=2, inter=256, vocab=2048, device="cuda:0", seed=0,
+                 window=None, sinks=0):
+        """window: every other layer, from the first on, sees the last `window` tokens and the first `sinks`."""
+        self.views = [dict(window=window, sinks=sinks) if window and i % 2 == 0 else {} for i in range(layers)]
         self.heads, self.kv_heads, self.head_dim, self.hidden, self.vocab = heads, kv_heads, head_dim, hidden, vocab
         g = torch.Generator().manual_seed(seed)
 
@@ -45,25 +48,20 @@ class Decoder:
 
     def guesses(self):
         """-> the four likeliest tokens after each token of the vocabulary, as far as its embedding says."""
-        logits = pkg.mm_bf16(self.norm(self.embedding), self.output)
+        logits = pkg.mm_bf16(pkg.residual_norm(self.embedding)[0], self.output)
         return pkg.token_logprobs(logits, torch.arange(self.vocab, device=logits.device), top_k=4).top_ids.tolist()
-
-    @staticmethod
-    def norm(x):
-        x = x.float()
-        return (x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-6)).to(torch.bfloat16)
 
     def forward(self, tokens, plan, cache):
         """tokens [T] of the plan's rows -> logits [T, vocab] bf16."""
-        x = self.embedding[tokens.clamp(min=0)]
-        for layer, (k_cache, v_cache) in zip(self.layers, cache.layers):
-            qkv = pkg.mm_bf16(self.norm(x), layer["qkv"])
+        y, x = pkg.residual_norm(self.embedding[tokens.clamp(min=0)])
+        for layer, view, (k_cache, v_cache), (k_scale, v_scale) in zip(self.layers, self.views, cache.layers, cache.scales):
+            qkv = pkg.mm_bf16(y, layer["qkv"])
             q = pkg.qk_norm_rope(qkv, plan.positions, self.cos_sin, self.heads, self.kv_heads, layer["q_norm"], layer["k_norm"],
-                                 k_cache=k_cache, v_cache=v_cache, slots=plan.slots)
-            o = pkg.tree_attention(q, k_cache, v_cache, cache.tables, plan.kv_lens, plan.cu_tokens, plan.masks)
-            x = x + pkg.mm_bf16(o.flatten(1), layer["o"])
-            x = x + layer["moe"](self.norm(x))
-        return pkg.mm_bf16(self.norm(x), self.output)
+                                 k_cache=k_cache, v_cache=v_cache, slots=plan.slots, k_scale=k_scale, v_scale=v_scale)
+            o = pkg.tree_attention(q, k_cache, v_cache, cache.tables, plan.kv_lens, plan.cu_tokens, plan.masks, k_scale=k_scale, v_scale=v_scale, **view)
+            y, x = pkg.residual_norm(pkg.mm_bf16(o.flatten(1), layer["o"]), x)
+            y, x = pkg.residual_norm(layer["moe"](y), x)
+        return pkg.mm_bf16(y, self.output)
 
 
 class Cache:
@@ -73,11 +71,19 @@ class Cache:
         device = model.embedding.device
         blocks = requests * pages_each
         shape = (blocks, page, model.kv_heads, model.head_dim)
-        self.page, self.layers = page, [(torch.zeros(shape, device=device).to(dtype), torch.zeros(shape, device=device).to(dtype)) for _ in model.layers]
+        def zeros(dtype, per):                           # `per` elements to one of dtype
+            if dtype not in (torch.float4_e2m1fn_x2, torch.float8_e8m0fnu):
+                return torch.zeros(shape, device=device).to(dtype)
+            return torch.zeros(*shape[:3], shape[3] // per, dtype=torch.uint8, device=device).view(dtype)
+
+        four = dtype == torch.float4_e2m1fn_x2             # a cache in 4 bits has powers of two beside it
+        self.page, self.layers = page, [(zeros(dtype, 2), zeros(dtype, 2)) for _ in model.layers]
+        self.scales = [(zeros(torch.float8_e8m0fnu, 32), zeros(torch.float8_e8m0fnu, 32)) if four else (None, None) for _ in model.layers]
         self.tables = torch.zeros(requests, pages_each, dtype=torch.int32, device=device)
         self.free = torch.arange(blocks, dtype=torch.int32, device=device)
         self.n_free = torch.full((1,), blocks, dtype=torch.int32, device=device)
         self.lens = torch.zeros(requests, dtype=torch.int32, device=device)
+        self.text = torch.zeros(requests, pages_each * page, dtype=torch.int32, device=device)        # the tokens whose keys are cached
 
     def plan(self, counts, max_tokens, parents=None):
         p = pkg.cache_plan(self.tables, self.lens, counts, self.free, self.n_free, self.page, max_tokens, parents)
@@ -86,17 +92,17 @@ class Cache:
         self.n_free = p.n_free
         return p
 
-    def keep(self, plan, kept):
+    def keep(self, plan, kept, tokens):
         """kept[b]: the rows of the step that stay, in text order.  Their keys and values move up behind the cached text (their angles
         are already those of their depth), and pages that nothing needs any more go back on the stack."""
         rows = [(b, self.lens[b].item() + i, row) for b, some in enumerate(kept) for i, row in enumerate(some)]
         if rows:
             b, place, row = (torch.tensor(x, device=self.lens.device) for x in zip(*rows))
             to = self.tables[b, place // self.page].long() * self.page + place % self.page
-            for pair in self.layers:
-                for cache in pair:
-                    flat = cache.view(torch.uint8).flatten(0, 1)
-                    flat[to] = flat[plan.slots[row]]
+            for cache in [c for pair in self.layers + self.scales for c in pair if c is not None]:
+                flat = cache.view(torch.uint8).flatten(0, 1)
+                flat[to] = flat[plan.slots[row]]
+            self.text[b, place] = tokens[row].int()
         had = (plan.kv_lens + self.page - 1) // self.page
         self.lens = self.lens + torch.tensor([len(k) for k in kept], dtype=torch.int32, device=self.lens.device)
         column = torch.arange(self.tables.shape[1], device=self.lens.device)
@@ -106,7 +112,7 @@ class Cache:
         self.n_free = self.n_free + back.numel()
 
 
-def prefill(model, cache, prompts):
+def prefill(model, cache, prompts, repetition=None):
     """prompts: a list of token lists -> each request's most likely next token."""
     device = model.embedding.device
     counts = torch.tensor([len(p) for p in prompts], dtype=torch.int32, device=device)
@@ -114,11 +120,16 @@ def prefill(model, cache, prompts):
     plan = cache.plan(counts, tokens.numel())
     logits = model.forward(tokens, plan, cache)
     cache.lens = plan.kv_lens
+    for b, p in enumerate(prompts):
+        cache.text[b, :len(p)] = torch.tensor(p, dtype=torch.int32)
     last = (plan.cu_tokens[1:] - 1).long()
-    return pkg.token_logprobs(logits[last], tokens[last], top_k=1).top_ids[:, 0].tolist()
+    logits = logits[last]
+    if repetition is not None:
+        logits = pkg.adjust_logits(logits, history=cache.text, history_lens=cache.lens, repetition=repetition)
+    return pkg.token_logprobs(logits, tokens[last], top_k=1).top_ids[:, 0].tolist()
 
 
-def step(model, cache, trees):
+def step(model, cache, trees, repetition=None):
     """trees[b]: (tokens, parents) of request b, the first token the last one chosen, the others guesses.  -> per request the
     tokens chosen after it and their log probabilities; the best continuations of every token that was run."""
     device = model.embedding.device
@@ -128,6 +139,9 @@ def step(model, cache, trees):
     parents = torch.tensor([p for _, above in trees for p in above], dtype=torch.int32, device=device)
     plan = cache.plan(counts, tokens.numel(), parents)
     logits = model.forward(tokens, plan, cache)
+    if repetition is not None:                             # each token under what its request has said and its own path through the tree
+        logits = pkg.adjust_logits(logits, plan.cu_tokens, history=cache.text, history_lens=cache.lens, tokens=tokens, masks=plan.masks,
+                                   repetition=repetition)
     # each guess under the logits of the token before it, and the best continuations of every token
     best = pkg.token_logprobs(logits, tokens, top_k=4)
     start = plan.cu_tokens[:-1].repeat_interleave(counts)
@@ -147,7 +161,7 @@ def step(model, cache, trees):
         chosen.append(said)
         kept.append(path)
         first += len(tree)
-    cache.keep(plan, kept)
+    cache.keep(plan, kept, tokens)
     return chosen, dict(zip(flat, top))
 
 
@@ -165,13 +179,16 @@ def draft(token, answers, width=2, depth=3):
     return tokens, parents
 
 
-def generate(model, cache, prompts, steps):
-    """-> per request the first token (prefill's), and the (token, log probability) list of what followed it in `steps` steps."""
-    first = last = prefill(model, cache, prompts)
+def generate(model, cache, prompts, steps, repetition=None):
+    """-> per request the first token (prefill's), and the (token, log probability) list of what followed it in `steps` steps.
+    repetition: a penalty for tokens that a request has had before, of all requests alike."""
+    if repetition is not None:
+        repetition = torch.full((len(prompts),), float(repetition), device=cache.lens.device)
+    first = last = prefill(model, cache, prompts, repetition)
     last, text, answers = list(last), [[] for _ in prompts], model.guesses()
     for _ in range(steps):
         trees = [draft(t, answers) for t in last]
-        chosen, seen = step(model, cache, trees)
+        chosen, seen = step(model, cache, trees, repetition)
         for token, top in seen.items():
             answers[token] = top
         for b, said in enumerate(chosen):
@@ -184,13 +201,16 @@ def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--requests", type=int, default=4)
     ap.add_argument("--steps", type=int, default=16)
-    ap.add_argument("--cache", choices=["bf16", "fp8"], default="bf16")
+    ap.add_argument("--cache", choices=["bf16", "fp8", "fp4"], default="bf16")
+    ap.add_argument("--window", type=int, help="every other layer sees the last so many tokens")
+    ap.add_argument("--sinks", type=int, default=0, help="and the first so many")
+    ap.add_argument("--repetition", type=float, help="a penalty above 1 for tokens that a request has had")
     args = ap.parse_args()
     g = torch.Generator().manual_seed(1)
-    dtype = torch.bfloat16 if args.cache == "bf16" else torch.float8_e4m3fn
-    model = Decoder()
+    dtype = dict(bf16=torch.bfloat16, fp8=torch.float8_e4m3fn, fp4=torch.float4_e2m1fn_x2)[args.cache]
+    model = Decoder(window=args.window, sinks=args.sinks)
     prompts = [torch.randint(model.vocab, (5 + 3 * b,), generator=g).tolist() for b in range(args.requests)]
-    _, text = generate(model, Cache(model, args.requests, dtype=dtype), prompts, args.steps)
+    _, text = generate(model, Cache(model, args.requests, dtype=dtype), prompts, args.steps, args.repetition)
     for b, said in enumerate(text):
         print(f"request {b}: {len(said)} tokens in {args.steps} steps, mean log probability {sum(lp for _, lp in said) / len(said):.3f}")
 
