@@ -188,3 +188,38 @@ def test_cu_tokens_out_of_order_end(pkg, dev):
         a["cu_tokens"].copy_(torch.tensor(cu))
         pkg.adjust_logits(**a)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("counts,V,L,bf16,tree,how", [
+    # large enough for segments of 32 KB, and of 64 KB where single rows have long histories
+    ([1] * 40, 60001, 700, True, False, dict(masked="rows")), ([1] * 36, 131072, 4200, False, False, dict(biases=3)), ([3, 16, 5, 1], 100003, 500, True, True, dict(masked="own")),
+    ([1] * 70, 130001, 4100, True, False, {}), ([7, 1], 262145, 60, False, True, {})])
+def test_large_vocabularies(pkg, dev, counts, V, L, bf16, tree, how):
+    say("adjust_logits, large", len(counts), V, L, bf16)
+    c = Case(V + L, counts, V, L, bf16, tree, **how)
+    got = pkg.adjust_logits(**c.args(dev))
+    torch.cuda.synchronize()
+    c.check(got)
+
+
+def test_texts_that_repeat_themselves(pkg, dev):
+    """Thousands of equal tokens, of two in turn, of none; counted exactly."""
+    x = torch.zeros(4, 9000, device=dev)
+    history = torch.zeros(4, 5000, dtype=torch.int32, device=dev)
+    history[0], history[1], history[2], history[3] = 7, 8191, -1, 8999
+    history[1, ::2] = 3
+    lens = torch.tensor([5000, 4999, 5000, 4097], dtype=torch.int32, device=dev)
+    prompt = torch.tensor([0, 1030, 5, 4096], dtype=torch.int32, device=dev)
+    one = torch.ones(4, device=dev)
+    y = pkg.adjust_logits(x, history=history, history_lens=lens, prompt_lens=prompt, frequency=one)
+    want = torch.zeros(4, 9000)
+    want[0, 7], want[1, 3], want[1, 8191], want[3, 8999] = -5000, -1985, -1984, -1
+    assert torch.equal(y.cpu(), want)
+
+
+def test_tokens_beyond_32_bits_are_no_tokens(pkg, dev):
+    x = torch.zeros(2, 50, device=dev)
+    tokens = torch.tensor([(1 << 32) + 3, -(1 << 40)], device=dev)
+    cu = torch.tensor([0, 2], dtype=torch.int32, device=dev)
+    for masks in (None, torch.tensor([1, 3], device=dev)):
+        assert not pkg.adjust_logits(x, cu, tokens=tokens, masks=masks, presence=torch.ones(1, device=dev)).any()

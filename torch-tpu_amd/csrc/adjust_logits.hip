@@ -10,10 +10,10 @@
 // counts the history's tokens that lie in the segment in LDS, so that no counter per vocabulary entry exists in memory, and a bit per token
 // says which were touched.  A row streams through registers, is stored as it is (but for what its grammar forbids) without waiting for the
 // counts, and the threads that stored the few touched values then store those once more.
-// Rows of 131072 fp32 values, 64 of them with up to 8192 tokens of history: 28 us, 14 without the histories (2.4 and 4.8 TB/s); 1290 rows of 100003
-// bf16 values, 128 requests' trees, every other row with a grammar: 157 us, 104 with neither (3.3 and 5.0 TB/s).  What histories cost is the
-// comparisons of every token in every segment and the counting, about 25 instructions a token; LDS atomics of all lanes instead of a branch: 32 us,
-// 32 KB segments: 30 and 200 us, 8 KB: 32 and 167.
+// 64 rows of 131072 fp32 values with up to 8192 tokens of history: 24 us, 14 without the histories (2.8 and 4.9 TB/s); 1290 rows of 100003
+// bf16 values, 128 requests' trees, every other row with a grammar: 156 us, 104 with neither (3.3 and 5.0 TB/s).  What histories cost is the
+// comparisons of every token in every segment and the counting, about 25 instructions a token.  (LDS atomics of all lanes instead of a branch: slower; a list of
+// the touched tokens in place of the bits: 30 and 180 us.)
 #include <math.h>
 #include <type_traits>
 #include "moe_common.h"
@@ -62,10 +62,10 @@ typedef uint16_t __attribute__((aligned(1))) any_u16;
 
 // BYTES of a row to a workgroup: BYTES / 16 groups of 16 bytes, P of them to a thread.  MANY: several rows, of which the next one is on its way
 // while one is worked on.
-template <int BYTES, bool BF16, bool MANY>
-__global__ __launch_bounds__(256) void adjust_logits_kernel(const LogitArgs a) {
+template <int BYTES, int THREADS, bool BF16, bool MANY>
+__global__ __launch_bounds__(THREADS) void adjust_logits_kernel(const LogitArgs a) {
   constexpr int N = BF16 ? 8 : 4, E = BF16 ? 2 : 4, SEG = BYTES / E;             // values of 16 bytes; bytes of one
-  constexpr int P = BYTES / 4096, ALL = (1 << N) - 1;
+  constexpr int P = BYTES / (16 * THREADS), ALL = (1 << N) - 1;
   struct Group {
     uint32_t w[4], let;                // let: the grammar's bits for its values
   };
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const LogitArgs a) {
   const auto row_in = [&](int t) { return (const uint8_t *)a.in + t * a.in_stride * E; };
   const auto before_of = [&](int t) { return (int)((uintptr_t)row_in(t) % 16) / E; };
   const auto inside_of = [&](int before) { return first >= before && first - before + SEG <= a.V; };
-  const auto token_of = [&](int p, int before) { return first + (p * 256 + tid) * N - before; };
+  const auto token_of = [&](int p, int before) { return first + (p * THREADS + tid) * N - before; };
   const auto grammar_of = [&](int t) { return !a.allowed ? -1 : a.allowed_row ? a.allowed_row[t] : t; };
   const auto words_of = [&](int grammar) { return grammar >= 0 && grammar < a.allowed_rows ? (const uint32_t *)a.allowed + grammar * a.allowed_stride : nullptr; };
   const int last_bits = (a.V + 31) / 32 * 4 - 2;       // a row of the grammar's last two bytes
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const LogitArgs a) {
       const int v = token_of(p, before);
       g[p].let = ALL;
       if (inside || (v >= 0 && v + N <= a.V)) {
-        const v4i raw = *(const v4i *)(in + (uint32_t)(v * E));
+        const v4i raw = *(const v4i *)(in + (uint32_t)v * (uint32_t)E);
 #pragma unroll
         for (int i = 0; i < 4; i++) g[p].w[i] = (uint32_t)raw[i];
       }
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const LogitArgs a) {
   };
   const auto store = [&](uint8_t *out, int v, bool same, const uint32_t (&w)[4]) {
     if (same) {
-      *(v4i *)(out + (uint32_t)(v * E)) = (v4i){(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+      *(v4i *)(out + (uint32_t)v * (uint32_t)E) = (v4i){(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
     } else {
 #pragma unroll
       for (int k = 0; k < N; k++) {
@@ -180,7 +180,8 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const LogitArgs a) {
       pres = !none && a.presence ? a.presence[b] : 0.f;
       len = heard && a.history_lens ? min(a.history_lens[b], a.L) : a.L;
       asked = heard && a.prompt_lens ? min(a.prompt_lens[b], len) : 0;
-      drafted = !none && a.tokens && a.masks && tid < 64 && begin + tid < end ? (uint32_t)(a.tokens[begin + tid] - from) : ~0u;
+      const int64_t draft = !none && a.tokens && a.masks && tid < 64 && begin + tid < end ? a.tokens[begin + tid] - from : -1;
+      drafted = draft >= 0 && draft < SEG + 8 ? (uint32_t)draft : ~0u;
     }
     if (MANY && t + 1 < t1) {
       next_words = words_of(next_grammar);
@@ -227,11 +228,11 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const LogitArgs a) {
       less = 1.0f / rep;
       counts = rep != 1.f || freq != 0.f || pres != 0.f;
       path = 0;
-      for (int i = tid; i < SEG / 4 + 2; i += 256) *(v4i *)&s.count[4 * i] = (v4i){0, 0, 0, 0};
-      for (int i = tid; i < SEG / 32 + 2; i += 256) s.touched[i] = 0;
+      for (int i = tid; i < SEG / 4 + 2; i += THREADS) *(v4i *)&s.count[4 * i] = (v4i){0, 0, 0, 0};
+      for (int i = tid; i < SEG / 32 + 2; i += THREADS) s.touched[i] = 0;
       __syncthreads();
       if (!none && a.n_bias) {
-        for (int i = tid; i < a.n_bias; i += 256) {
+        for (int i = tid; i < a.n_bias; i += THREADS) {
           const uint32_t place = (uint32_t)(a.bias_ids[b * a.bias_ids_stride + i] - from);
           if (place >= SEG + 8) continue;
           atomicMax(&s.count[place], (uint32_t)(i + 1) << kBiasShift);
@@ -240,10 +241,10 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const LogitArgs a) {
         __syncthreads();
       }
       if (heard && counts) {
-        for (int i = 0; i < len; i += 1024) {
+        for (int i = 0; i < len; i += 4 * THREADS) {
           const v4i id = asked_for;
-          if (i + 1024 < len) ask(i + 1024);           // (on their way while these are counted)
-            const bool said = i >= asked && i + 1024 <= len, prompt = i + 1024 <= asked;       // (elsewhere threads differ)
+          if (i + 4 * THREADS < len) ask(i + 4 * THREADS);           // (on their way while these are counted)
+            const bool said = i >= asked && i + 4 * THREADS <= len, prompt = i + 4 * THREADS <= asked;       // (elsewhere threads differ)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
               const uint32_t place = (uint32_t)(id[j] - from);
@@ -268,12 +269,12 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const LogitArgs a) {
         }
       }
       if (!none && counts && a.tokens && !a.masks)     // what stands before the row
-        for (int i = begin + tid; i < t; i += 256) s.add(a.tokens[i] - from, kOnce);
+        for (int i = begin + tid; i < t; i += THREADS) s.add(a.tokens[i] - from, kOnce);
     }
     if (!none && counts && a.tokens) {
       if (a.masks) {
         const int was = path >> lane & 1, is = mask >> lane & 1;
-        if (drafted < SEG + 8 && was != is) {
+        if (drafted != ~0u && was != is) {
           atomicAdd(&s.count[drafted], is ? kOnce : 0u - kOnce);
           s.touch(drafted);
         }
@@ -297,13 +298,13 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const LogitArgs a) {
       uint32_t hit[P];
 #pragma unroll
       for (int p = 0; p < P; p++) {
-        const int at = (p * 256 + tid) * N - before + 8;         // the first one's counter
+        const int at = (p * THREADS + tid) * N - before + 8;         // the first one's counter
         const uint32_t lo = s.touched[at >> 5], hi = s.touched[(at >> 5) + 1];
         hit[p] = __builtin_amdgcn_alignbit(hi, lo, at & 31) & ALL;
       }
 #pragma unroll
       for (int p = 0; p < P; p++) {
-        const int v = token_of(p, before), at = (p * 256 + tid) * N - before + 8;
+        const int v = token_of(p, before), at = (p * THREADS + tid) * N - before + 8;
         if (inside || (v >= 0 && v + N <= a.V)) {
           const v4i w = {(int)now[p].w[0], (int)now[p].w[1], (int)now[p].w[2], (int)now[p].w[3]};
           uint32_t left = hit[p] & now[p].let;
@@ -363,23 +364,32 @@ extern "C" int moe_adjust_logits(void *stream, const void *logits, int dtype, in
   hipStream_t st = (hipStream_t)stream;
   // (rows that begin on 16 bytes need no room for the values before)
   const int64_t wide = (uintptr_t)logits % 16 == 0 && (T == 1 || row_stride * e % 16 == 0) ? V : (int64_t)V + 16 / e - 1;
-  const auto run = [&](auto bytes) {
-    constexpr int BYTES = decltype(bytes)::value;
+  const auto run = [&](auto bytes, auto threads) {
+    constexpr int BYTES = decltype(bytes)::value, TH = decltype(threads)::value;
     a.segments = (int)((wide * e + BYTES - 1) / BYTES);
     const int64_t blocks = (int64_t)a.segments * ((T + a.rows - 1) / a.rows);
     if (blocks > 0x7fffffff) return MOE_E_SHAPE;
     const unsigned n = (unsigned)blocks;
-    if (a.rows > 1) {
-      if (a.bf16) adjust_logits_kernel<BYTES, true, true><<<n, 256, 0, st>>>(a);
-      else adjust_logits_kernel<BYTES, false, true><<<n, 256, 0, st>>>(a);
+    const auto launch = [&](auto many) {
+      constexpr bool M = decltype(many)::value;
+      if (a.bf16) adjust_logits_kernel<BYTES, TH, true, M><<<n, TH, 0, st>>>(a);
+      else adjust_logits_kernel<BYTES, TH, false, M><<<n, TH, 0, st>>>(a);
+    };
+    if constexpr (TH <= 512) {
+      if (a.rows > 1) launch(std::integral_constant<bool, true>());
+      else launch(std::integral_constant<bool, false>());
     } else {
-      if (a.bf16) adjust_logits_kernel<BYTES, true, false><<<n, 256, 0, st>>>(a);
-      else adjust_logits_kernel<BYTES, false, false><<<n, 256, 0, st>>>(a);
+      launch(std::integral_constant<bool, false>());
     }
     return (int)hipGetLastError();
   };
   using std::integral_constant;
   const int64_t work = (int64_t)((T + a.rows - 1) / a.rows) * V * e;
-  if (work < (1 << 20)) return run(integral_constant<int, 4096>());
-  return run(integral_constant<int, 16384>());
+  // Few values: segments of 8 KB, so that the whole chip takes part (a row of 131072 bf16 values 7.2 us, 9.7 with 16 KB).  Else of 32 KB: fewer segments read
+  // the histories again, more workgroups share the chip (64 rows of 131072 bf16 values with 8192 tokens of history: 16.8 us, 19.5 with 16 KB, 29 with
+  // 8; 64 of 100003 with 2000, half of them masked: 14.6, 15.5, 19.6).  Long histories of single rows are read by even fewer segments of 64 KB (15.0
+  // and 15.6; fp32 23.8, 25.7 with 32 KB, 28 with 16; of several rows, which wait for each other, 210 and 156).
+  if (work < (2 << 20)) return run(integral_constant<int, 8192>(), integral_constant<int, 512>());
+  if (a.rows == 1 && history && L >= 4096 && work >= (16 << 20)) return run(integral_constant<int, 65536>(), integral_constant<int, 1024>());
+  return run(integral_constant<int, 32768>(), integral_constant<int, 512>());
 }
