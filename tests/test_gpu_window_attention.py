@@ -99,7 +99,8 @@ def one_request_in_room(s, room):
 
 
 LARGE = [
-    (64, [(50, 8), (0, 7), (129, 5), (64, 1), (10, 0), (31, 9)], 16, 2, True), (64, [(0, 10), (90, 5), (5, 1), (300, 9)], 8, 1, False),
+    (64, [(50, 4), (0, 3), (129, 2), (64, 1), (10, 0), (31, 5)], 16, 2, True), (64, [(0, 4), (90, 5), (5, 1), (300, 4)], 8, 1, False),
+    (128, [(50, 8), (0, 7), (129, 5), (64, 1), (10, 0), (31, 9)], 16, 2, True), (128, [(0, 10), (90, 5), (5, 1), (300, 9)], 8, 1, False),
     (128, [(50, 16), (0, 7), (129, 13), (64, 1), (200, 16), (33, 30)], 16, 2, True), (128, [(0, 150), (63, 65), (64, 64)], 3, 3, False),
     (256, [(50, 64), (0, 33), (129, 20), (10, 0), (64, 64), (7, 13)], 16, 2, True), (256, [(0, 150), (90, 65), (33, 1), (100, 129)], 8, 2, False),
     (256, [(1500, 64), (1391, 61), (1280, 33)], 8, 2, True),

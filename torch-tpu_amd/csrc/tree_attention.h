@@ -84,13 +84,13 @@ __device__ __forceinline__ AttnReach attn_reach(const AttnArgs &a, const AttnReq
   const int skip = max(lowest - first, 0);
   return {upto - skip, first, skip, r.prefix + j1 + 1 - a.window};
 }
-template <int ROWS, int UNIT, bool LOCAL>
+template <int ROWS, int UNIT>
 __device__ __forceinline__ int attn_head_units(const AttnArgs &a, const AttnRequest &r) {
   if (r.n <= 0 || r.prefix < 0) return 0;
   const int tiles = (r.n * a.G + ROWS - 1) / ROWS;
-  if (a.masks || r.n == 1) return tiles * attn_reach<ROWS, UNIT, LOCAL>(a, r, 0).units;
+  if (a.masks || r.n == 1) return tiles * attn_reach<ROWS, UNIT, false>(a, r, 0).units;
   int sum = 0;
-  for (int m = 0; m < tiles; m++) sum += attn_reach<ROWS, UNIT, LOCAL>(a, r, m).units;
+  for (int m = 0; m < tiles; m++) sum += attn_reach<ROWS, UNIT, false>(a, r, m).units;
   return sum;
 }
 
@@ -108,7 +108,7 @@ __device__ __forceinline__ void attn_walk(const AttnArgs &a, Segment segment) {
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     if (b0 + lane < a.B) mine = attn_request(a, b0 + lane);
     else mine.n = 0;
-    units = attn_head_units<ROWS, UNIT, false>(a, mine) * a.Hkv;
+    units = attn_head_units<ROWS, UNIT>(a, mine) * a.Hkv;
     upto = __builtin_elementwise_add_sat(upto, (uint32_t)units);
     if (units > 0) longest = max(longest, (mine.kv + UNIT - 1) / UNIT);
   }
@@ -132,7 +132,7 @@ __device__ __forceinline__ void attn_walk(const AttnArgs &a, Segment segment) {
     if (a.B > 64) {
       if (b0 + lane < a.B) mine = attn_request(a, b0 + lane);
       else mine.n = 0;
-      units = attn_head_units<ROWS, UNIT, false>(a, mine) * a.Hkv;
+      units = attn_head_units<ROWS, UNIT>(a, mine) * a.Hkv;
       upto = lane_sum_upto(units);
     }
     const uint64_t past = __ballot(start < before + (int)upto);
@@ -147,7 +147,7 @@ __device__ __forceinline__ void attn_walk(const AttnArgs &a, Segment segment) {
     before += __builtin_amdgcn_readlane(upto, 63);
   }
   for (int at = start;;) {
-    const int head = attn_head_units<ROWS, UNIT, false>(a, r);
+    const int head = attn_head_units<ROWS, UNIT>(a, r);
     if (at >= before + head * a.Hkv) {
       before += head * a.Hkv;
       r = attn_request(a, ++b);
@@ -179,7 +179,8 @@ __device__ __forceinline__ void attn_walk(const AttnArgs &a, Segment segment) {
 // The same for LOCAL kernels.  With a window most tiles are equally long, and lengths may be alike without one: where all tiles filled up to the longest
 // one's length are not more than an eighth longer, the line has every tile at that length, and stretches are whole tiles or a tile's equal parts, so that
 // none holds the end of one tile and the beginning of the next and, of whole tiles, nothing is left to join (two chunks of 1021 tokens
-// in a window of 1024: 89 us with stretches across tiles, 73 so; 64 single tokens: 42 and 34).
+// in a window of 1024, 32 query heads: 84 us with stretches across tiles, 59 so; 64 single tokens: 42.6 and 41.4).  A lane adds up
+// a tile of a causal request, 64 at once.
 template <int ROWS, int UNIT, int HEADS, typename Segment>
 __device__ __forceinline__ void attn_walk_local(const AttnArgs &a, Segment segment) {
   const int lane = threadIdx.x & 63, heads = a.Hkv / HEADS;
@@ -674,6 +675,9 @@ __device__ __forceinline__ void attn_store(const AttnArgs &a, const AttnRequest 
 // from memory straight into operand registers, values through LDS that no other wavefront touches, so nothing waits at a
 // barrier, and the next keys and values are asked for before the present ones are worked on.  The wavefronts' results meet in
 // LDS at the end of a tile.
+// In 4 bits a head's key is 64 bytes or 32, half a line of memory or less, so that one head's keys alone come at 2.6 to 2.9 TB/s.  With HEADS = 2 a
+// workgroup reads two neighbouring heads' keys at the same time, a pair of wavefronts (SHARE) to each: 4.0 TB/s (256 requests of up to 8192 keys: 261 us with
+// one head, 174 with two).
 template <int D, int C, bool LOCAL, int NQ, int HEADS>
 __global__ __launch_bounds__(256, 2) void attn_keys_kernel(const AttnArgs a) {
   constexpr int ROWS = 16 * NQ, SHARE = 4 / HEADS, UNIT = 32 * SHARE, DT = D / 16, LD = 2 * D + 32;
@@ -864,7 +868,8 @@ __device__ __forceinline__ void attn_put_values(uint8_t *at, const Piece (&raw)[
 // a tile that is not full keeps all at work (57 requests of about 145 rows: 108 us, 117 with neighbouring 16s together).  The bytes of the stage after
 // that wait in registers (of two stages after it: no faster).  32 trees of up to 16 tokens over up to 8001 e4m3 keys: 69.5 us, 2.4 TB/s and
 // 361 TFLOP/s; without the work on the stages 54, without the stages 56: two workgroups to a compute unit overlap the two in part, and
-// LDS and registers hold no third.  (Codes are widened before they go to LDS, so an e4m3 cache has the stages of a bf16 one.)
+// LDS and registers hold no third.  (Codes are widened before they go to LDS, so an e4m3 cache has the stages of a bf16 one, and a 4-bit
+// cache too: the same trees over half the bytes take 63 us and a join of 5 to 8, bound by the products, the widening and the stages.)
 template <int D, int C, bool LOCAL, int NQ>
 __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const AttnArgs a) {
   constexpr int ROWS = 64 * NQ, UNIT = 64, DT = D / 16, LD = 2 * D + 32, STAGE = 2 * UNIT * LD;
@@ -921,7 +926,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const AttnArgs a) {
       __syncthreads();
     };
     const auto take = [&](auto sixteens) {
-      constexpr int N = decltype(sixteens)::value, AHEAD = N == 2 && C == MOE_DTYPE_BF16 ? (LOCAL ? 1 : 2) : 3;     // (as the registers allow)
+      constexpr int N = decltype(sixteens)::value, AHEAD = N == 2 && C == MOE_DTYPE_BF16 ? (LOCAL ? 1 : 2) : 3;     // (as the registers allow: 2 of LOCAL spills)
       v8bf q[N][D / 32];
       AttnSight<N, LOCAL> sight;
       attn_queries<N, D, 8, LOCAL, 64>(a, r, kh, m_tile * ROWS + 16 * w, factor, q, sight);
@@ -985,6 +990,8 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const AttnArgs a) {
 // operands from LDS 5 % less, without the exponentials 5 to 8 %, without staging 10 to 17 %.  Counted for a SIMD: the matrix cores are busy 196
 // thousand clocks, the vector unit 220 thousand, of about 460 thousand: the two still add up more than they overlap.
 // 16 trees of up to 64 tokens over up to 12288 keys: 119 to 124 us, 600 to 622 TFLOP/s (tiles that are not full, and a join of 12 us).
+// LOCAL: the chunks in a window of 1024 58 us, 520 TFLOP/s of what the rows see (tiles of 64 tokens over 17 units for 16 units' worth of keys, then
+// the way to the first unit); the trees over a 4-bit cache in a window of 4095 75 us and a join of 10.5.
 template <int D, int C, bool LOCAL, int NQ>
 __global__ __launch_bounds__(512, 2) void attn_pairs_kernel(const AttnArgs a) {
   constexpr int ROWS = 128 * NQ, UNIT = 64, DT = D / 16, X = D / 32, LD = 2 * D + 32, HALF = UNIT * LD;
@@ -1137,6 +1144,12 @@ __global__ __launch_bounds__(512, 2) void attn_pairs_kernel(const AttnArgs a) {
 // The walk along the line takes its time too: a piece of a causal request adds up all tiles of the request (attn_head_units), so that a prompt of 8192
 // tokens from its start takes 1610 us of which 760 are the walk's, and requests without tokens are passed one by one (two single tokens over
 // 2048 keys: 17, with 4000 idle requests between them 54).
+// 4 bits: keys are cheaper to read than to unpack, so that tiles of 128 pay from 33 rows on (32 requests over 8001 keys, 64 and 128 rows a tile: 59 and 59 us
+// at 32 rows, 66 and 64 at 48, 76 and 69 at 64).  Of single tokens two heads to a workgroup where each still finds a tile to itself,
+// from 128 tiles of a head on (64 requests 62 and 56 us with one and two heads, 256 requests 261 and 174; one request of 32767 keys 18.5 and
+// 23), and 512 workgroups (64 requests: 75 us with 256).
+// With a window a tile's keys are at most the window's, which the rule takes for `keys`; the table above holds as it is (16 rows in bf16, 64 requests in
+// a window of 1024: 41.6 us with 256 workgroups, 45.5 with 512; 16 x 64 tokens in one of 1024, 64, 128 and 256 rows: 46, 49 and 52; 32 x 64: 84, 63 and 61).
 struct AttnPlan {
   int rows, groups;                    // rows of a tile; workgroups, a multiple of 8
   float cut;
@@ -1146,7 +1159,7 @@ inline AttnPlan attn_plan(int T, int Hq, int Hkv, int B, int cache_dtype, bool t
   const int64_t rows = B > 0 ? ((int64_t)T * (Hq / Hkv) + B - 1) / B : 1;
   const int heads = Hkv % 2 == 0 && (int64_t)B * Hkv >= 128 ? 2 : 1;
   if (rows <= 16) return {16, cache_dtype == MOE_DTYPE_BF16 ? 256 : 512, 0.0625f, cache_dtype == MOE_DTYPE_FP4 ? heads : 1};
-  if (rows <= 64 || (int64_t)T * Hq <= (trees ? 20000000 : 8000000) / (keys > 0 ? keys : 1)) return {64, 512, 0.125f, 1};
+  if (rows <= (cache_dtype == MOE_DTYPE_FP4 ? 32 : 64) || (int64_t)T * Hq <= (trees ? 20000000 : 8000000) / (keys > 0 ? keys : 1)) return {64, 512, 0.125f, 1};
   if (rows <= 128) return {128, 512, 0.125f, 1};
   return {256, 256, 0.25f, 1};
 }
