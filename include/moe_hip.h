@@ -436,7 +436,7 @@ int moe_qk_norm_rope(void *stream, const void *qkv_bf16, int64_t row_stride, int
  * The same into a cache in 4 bits (its layout: moe_window_attention): of 32 neighbouring elements of a key or value the power of two is the least that
  * brings all of them to 7 or below, its byte goes to k_scale / v_scale [n_blocks, page_size, Hkv, D / 32] (blocks *_scale_block_stride bytes apart);
  * the codes are the nearest (ties to even, 6 at most).  A NaN or an infinity among the 32: byte 255, all of them read as NaN.
- * D a multiple of 32, the caches' block strides (in elements) too.
+ * D a multiple of 32, the caches' block strides (in elements) too.  No two tokens share a slot.
  */
 int moe_qk_norm_rope_fp4(void *stream, const void *qkv_bf16, int64_t row_stride, int T, int Hq, int Hkv, int D,
                          const int32_t *positions, const float *cos_sin, int P, int R, int interleaved, const void *q_weight,
@@ -512,7 +512,8 @@ int moe_residual_norm(void *stream, const void *x_bf16, int64_t x_stride, int T,
                       int64_t y_stride, void *residual_out, int64_t residual_out_stride);
 
 /*
- * What requests ask of their logits [T, V] (fp32 or bf16, rows row_stride apart), -> out in the same type, which may be logits itself.
+ * What requests ask of their logits [T, V] (fp32 or bf16, rows row_stride apart), -> out in the same type, which may be logits itself and
+ * otherwise lies over nothing that is read (MOE_E_MODE).
  * Request b has rows [cu_tokens[b], cu_tokens[b + 1]) (cu_tokens NULL: row b, B = T) and a history [B, L] int32 (rows history_stride apart) of
  * history_lens[b] tokens (NULL: L), the first prompt_lens[b] of them its prompt (NULL: none).  With tokens [T] int64 a row's history goes on with the
  * tokens of its request that its mask names (masks [T] int64, up to 64 tokens a request; NULL: those up to its own).  Of a

@@ -54,6 +54,9 @@ def test_adjust_logits_refusals(pkg):
     assert call(x=ctypes.c_void_p(0x100001)) == E_ALIGN and call(out=odd, dt=0) == E_ALIGN
     for bad in (dict(out=ctypes.c_void_p(0x100002)), dict(out=ctypes.c_void_p(0x100000 - 7998)), dict(out=at(1), os=1001)):
         assert call(**bad) == E_MODE, bad
+    for name in ("cu", "hist", "lens", "asked", "tok", "masks", "rep", "freq", "pres", "bi", "bv", "al", "rows"):       # out over what is read
+        for there in (0x200000, 0x200000 + 7992, 0x200000 - 4):
+            assert call(**{name: ctypes.c_void_p(there)}) == E_MODE, (name, there)
     assert call(T=0, x=None, out=None) == 0
 
 

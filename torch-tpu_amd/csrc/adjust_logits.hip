@@ -357,6 +357,15 @@ extern "C" int moe_adjust_logits(void *stream, const void *logits, int dtype, in
   const uint8_t *i0 = (const uint8_t *)logits, *o0 = (const uint8_t *)out;
   if (!(i0 == o0 && (row_stride == out_stride || T == 1)) && i0 < o0 + ((T - 1) * out_stride + V) * e && o0 < i0 + ((T - 1) * row_stride + V) * e)
     return MOE_E_MODE;
+  const auto over = [&](const void *p, int64_t rows, int64_t stride, int64_t row, int size) {      // out lies over an input of such rows
+    return p && rows > 0 && row > 0 && (const uint8_t *)p < o0 + ((T - 1) * out_stride + V) * e && o0 < (const uint8_t *)p + ((rows - 1) * stride + row) * size;
+  };
+  if (over(cu_tokens, 1, 0, B + 1ll, 4) || over(history, B, history_stride, L, 4) || over(tokens, 1, 0, T, 8) || over(masks, 1, 0, T, 8) ||
+      over(n_bias ? bias_ids : nullptr, B, bias_ids_stride, n_bias, 4) || over(n_bias ? bias : nullptr, B, bias_stride, n_bias, 4) ||
+      over(allowed, n_allowed, allowed_stride, (V + 31) / 32, 4) || over(allowed ? allowed_rows : nullptr, 1, 0, T, 4))
+    return MOE_E_MODE;
+  for (const void *p : {(const void *)history_lens, (const void *)prompt_lens, (const void *)repetition, (const void *)frequency, (const void *)presence})
+    if (over(p, 1, 0, B, 4)) return MOE_E_MODE;
   const int rows = B > 0 ? (T + B - 1) / B : 1;
   LogitArgs a{logits, out, row_stride, out_stride, T, V, B, L, dtype == MOE_DTYPE_BF16, rows < 4 ? rows : 4, 0, cu_tokens,
               history, history_stride, history_lens, prompt_lens, tokens, masks, repetition, frequency, presence, bias_ids, bias_ids_stride, bias,

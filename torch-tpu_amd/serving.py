@@ -1,9 +1,11 @@
-"""A serving step around the MoE layer: paged cache, attention over it, and what the logits say about given tokens.
+"""A serving step around the MoE layer: paged cache, attention over it, what lies between two blocks, and what is asked of logits and what they say.
 
     plan = cache_plan(block_tables, lens, counts, free_blocks, n_free, page_size, max_tokens, parents)
     q = qk_norm_rope(qkv, plan.positions, cos_sin, heads, kv_heads, q_weight, k_weight,
                      k_cache=k_cache, v_cache=v_cache, slots=plan.slots)                       # each layer
     o = tree_attention(q, k_cache, v_cache, block_tables, plan.kv_lens, plan.cu_tokens, plan.masks)
+    x, residual = residual_norm(projection, residual, weight)
+    logits = adjust_logits(logits, plan.cu_tokens, history, history_lens, prompt_lens, tokens, plan.masks, repetition=repetition)
     said = token_logprobs(logits, tokens, top_k=8)
 
 The functions are thin: the operators of the same names in torch.ops.my_ops check, allocate and launch (csrc/serving_ops.cpp).
@@ -61,7 +63,7 @@ def qk_norm_rope(qkv, positions, cos_sin, n_heads: int, n_kv_heads: int, q_weigh
     and slots [T] int64: stores keys and values, returns q [T, n_heads, D].  Without: returns (q, k).
     Caches in 4 bits are float4_e2m1fn_x2 [blocks, page, n_kv_heads, D / 2] (two elements to a byte, the first in the low bits), their scales
     float8_e8m0fnu [blocks, page, n_kv_heads, D / 32], written beside them: the power of two of 32 neighbouring elements, the least that
-    brings them to 7 or below (the largest code is 6).  D a multiple of 32."""
+    brings them to 7 or below (the largest code is 6).  D a multiple of 32.  Slots inside the cache must differ."""
     q, k = _ops.qk_norm_rope.default(qkv, positions, cos_sin, n_heads, n_kv_heads, q_weight, k_weight, eps, interleaved, k_cache, v_cache,
                                      slots, k_scale, v_scale, out)
     return q if k is None else (q, k)
