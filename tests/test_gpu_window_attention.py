@@ -171,6 +171,40 @@ def test_two_heads_to_a_workgroup(pkg, dev, D, Hq, Hkv, W, sinks):
     assert torch.equal(out, pkg.tree_attention(**s.args(dev)))
 
 
+@pytest.mark.parametrize("cache,D,Hq,Hkv", [("bf16", 128, 8, 4), ("bf16", 64, 12, 6), ("fp8", 128, 4, 4), ("fp8", 64, 16, 8), ("fp4", 128, 6, 2), ("fp4", 64, 8, 4)])
+@pytest.mark.parametrize("W,sinks", [(7000, 300), (7000, 0)])
+def test_two_heads_to_a_workgroup_in_a_wide_window(pkg, dev, cache, D, Hq, Hkv, W, sinks):
+    """The same over every cache, in windows wide enough for it: some texts end inside theirs, some begin before it."""
+    say("tree_attention, two heads", cache, D, Hq, Hkv, W, sinks)
+    g = torch.Generator().manual_seed(D + Hkv)
+    reqs = [(int(n), 1) for n in torch.randint(0, 900, (120 // Hkv,), generator=g)] + [(-1, 1), (0, 0), (7400, 1), (5, 1), (7003, 1), (8191, 1)]
+    s = one_request_in_room(Step(D + W, reqs, Hq, Hkv, D, 64, cache, False, W, sinks, spare_rows=1), 131072)
+    assert len(reqs) * Hkv >= 64 and len(reqs) * Hkv * W >= 3 << 18 and s.rows(pkg) == 16
+    out, lse = pkg.tree_attention(**s.args(dev), return_lse=True)
+    torch.cuda.synchronize()
+    s.check(out, lse)
+    assert torch.equal(out, pkg.tree_attention(**s.args(dev)))
+
+
+@pytest.mark.parametrize("cache", ["bf16", "fp8", "fp4"])
+def test_keys_outside_the_window_are_not_read_into_it(pkg, dev, cache):
+    """Units that hold the ends of first tokens and windows, whose other keys and values are no numbers, for tiles of every size."""
+    for n, Hq, Hkv, as_tree, W, sinks in ((1, 4, 2, False, 200, 5), (1, 4, 2, False, 130, 0), (5, 16, 2, True, 77, 3), (30, 16, 2, True, 100, 1), (300, 8, 2, False, 150, 70)):
+        say("tree_attention, no numbers outside", cache, n, W, sinks)
+        s = one_request_in_room(Step(n + W, [(701, n), (333, n)], Hq, Hkv, 128, 16, cache, as_tree, W, sinks), 131072)
+        for b, (l, new) in enumerate(zip(s.lens, s.counts)):
+            for i in range(sinks, l - new - W):            # cached keys that no row sees
+                where = s.tables[b][i // 16], i % 16
+                if cache == "fp4":
+                    s.ks[where] = s.vs[where] = 255
+                else:
+                    s.k[where] = s.v[where] = torch.tensor(math.nan).to(s.k.dtype)
+        out, lse = pkg.tree_attention(**s.args(dev), return_lse=True)
+        torch.cuda.synchronize()
+        assert bool(out.isfinite().all())
+        s.check(out, lse)
+
+
 @pytest.mark.parametrize("cache,reqs,Hq,Hkv,D,W,sinks", [
     # a tile to each workgroup or several, parts of one, and lengths too different for either
     ("bf16", [(400 + b, 1) for b in range(100)], 8, 4, 64, 200, 4), ("bf16", [(300, 1)] * 260, 4, 2, 128, 100, 0), ("fp8", [(900, 1)] * 3, 4, 2, 64, 500, 1),

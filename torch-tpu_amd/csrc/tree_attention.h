@@ -68,21 +68,24 @@ __device__ __forceinline__ int attn_tile_end(const AttnArgs &a, const AttnReques
   return r.prefix + min(r.n, (min((m + 1) * ROWS, r.n * a.G) - 1) / a.G + 1);
 }
 // The units of keys that tile m goes over: without a window units 0 .. u, with one the first tokens' and then those from the lowest
-// key that one of its rows sees in its window on.
+// key that one of its rows sees in its window on.  Of the units at the two ends only keys that a row may see are read: in place of the others their
+// nearest such neighbour, whose line is on its way anyway.  (64 single tokens in a window of 1024 with 4 first ones, units of 128: 36.6 us, 41.4 with all ten units read whole.)
 struct AttnReach {
   int units, first, skip;              // in all; of the first tokens; left out behind them
   int every;                           // every row of the tile sees keys from here on (up to where the new tokens begin)
+  int high, low;                       // no row sees a key above `high` in the first tokens' units, nor one below `low` in those behind them
   __device__ __forceinline__ int unit(int c) const { return c + (c >= first ? skip : 0); }
+  __device__ __forceinline__ int read(int c, int key) const { return max(min(key, c < first ? high : 0x7fffffff), c < first ? 0 : low); }
 };
 template <int ROWS, int UNIT, bool LOCAL>
 __device__ __forceinline__ AttnReach attn_reach(const AttnArgs &a, const AttnRequest &r, int m) {
   const int end = attn_tile_end<ROWS>(a, r, m), upto = (end + UNIT - 1) / UNIT;
-  if (!LOCAL) return {upto, 0, 0, 0};
+  if (!LOCAL) return {upto, 0, 0, 0, 0, 0};
   // (the window may be 2^31 - 1: each line's first term is a length)
   const int j0 = a.masks ? -1 : m * ROWS / a.G, j1 = a.masks ? r.n - 1 : (min((m + 1) * ROWS, r.n * a.G) - 1) / a.G;
-  const int lowest = max(r.prefix + j0 + 1 - a.window, 0) / UNIT, first = (min(a.sinks, end) + UNIT - 1) / UNIT;
-  const int skip = max(lowest - first, 0);
-  return {upto - skip, first, skip, r.prefix + j1 + 1 - a.window};
+  const int low = max(r.prefix + j0 + 1 - a.window, 0), head = min(a.sinks, end), first = (head + UNIT - 1) / UNIT;
+  const int skip = max(low / UNIT - first, 0);
+  return {upto - skip, first, skip, r.prefix + j1 + 1 - a.window, low >= first * UNIT ? head - 1 : 0x7fffffff, low};
 }
 template <int ROWS, int UNIT>
 __device__ __forceinline__ int attn_head_units(const AttnArgs &a, const AttnRequest &r) {
@@ -179,7 +182,7 @@ __device__ __forceinline__ void attn_walk(const AttnArgs &a, Segment segment) {
 // The same for LOCAL kernels.  With a window most tiles are equally long, and lengths may be alike without one: where all tiles filled up to the longest
 // one's length are not more than an eighth longer, the line has every tile at that length, and stretches are whole tiles or a tile's equal parts, so that
 // none holds the end of one tile and the beginning of the next and, of whole tiles, nothing is left to join (two chunks of 1021 tokens
-// in a window of 1024, 32 query heads: 84 us with stretches across tiles, 59 so; 64 single tokens: 42.6 and 41.4).  A lane adds up
+// in a window of 1024, 32 query heads: 84 us with stretches across tiles, 59 so).  A lane adds up
 // a tile of a causal request, 64 at once.
 template <int ROWS, int UNIT, int HEADS, typename Segment>
 __device__ __forceinline__ void attn_walk_local(const AttnArgs &a, Segment segment) {
@@ -676,8 +679,9 @@ __device__ __forceinline__ void attn_store(const AttnArgs &a, const AttnRequest 
 // barrier, and the next keys and values are asked for before the present ones are worked on.  The wavefronts' results meet in
 // LDS at the end of a tile.
 // In 4 bits a head's key is 64 bytes or 32, half a line of memory or less, so that one head's keys alone come at 2.6 to 2.9 TB/s.  With HEADS = 2 a
-// workgroup reads two neighbouring heads' keys at the same time, a pair of wavefronts (SHARE) to each: 4.0 TB/s (256 requests of up to 8192 keys: 261 us with
-// one head, 174 with two).
+// workgroup reads two neighbouring heads' keys at the same time, a pair of wavefronts (SHARE) to each: 4.0 TB/s (256 requests of up to 8192 keys, 4 heads: 261 us with
+// one head, 174 with two; e4m3 heads of 64: 462 and 269 over 8 heads, 4.9 TB/s).  (Four heads: 246 us where two take 294, 256 requests of 8 heads of
+// 64 in 4 bits; no faster elsewhere, slower where parts have to be joined.)
 template <int D, int C, bool LOCAL, int NQ, int HEADS>
 __global__ __launch_bounds__(256, 2) void attn_keys_kernel(const AttnArgs a) {
   constexpr int ROWS = 16 * NQ, SHARE = 4 / HEADS, UNIT = 32 * SHARE, DT = D / 16, LD = 2 * D + 32;
@@ -705,7 +709,10 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(const AttnArgs a) {
     Piece kr[2][P], vr[2][P];
     uint32_t kp[2], vp[2];                             // their powers of two
     int block[2];
-    const auto key_of = [&](int unit, int kt) { return min(reach.unit(unit) * UNIT + 32 * part_of_unit + 16 * kt + c16, r.kv - 1); };
+    const auto key_of = [&](int unit, int kt) {
+      const int key = reach.unit(unit) * UNIT + 32 * part_of_unit + 16 * kt + c16;
+      return min(LOCAL ? reach.read(unit, key) : key, r.kv - 1);
+    };
     const auto blocks = [&](int unit) {
 #pragma unroll
       for (int kt = 0; kt < 2; kt++) block[kt] = attn_block(a, table, key_of(unit, kt));
@@ -889,7 +896,10 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const AttnArgs a) {
     Piece kr[NU], vr[NU];
     uint32_t kp = 0, vp = 0;                           // their powers of two
     int block;                                         // of the unit that is asked for next
-    const auto key_of = [&](int unit) { return min(reach.unit(min(unit, last)) * UNIT + stage_row, r.kv - 1); };
+    const auto key_of = [&](int unit) {
+      const int c = min(unit, last), key = reach.unit(c) * UNIT + stage_row;
+      return min(LOCAL ? reach.read(c, key) : key, r.kv - 1);
+    };
     const auto is_edge = [&](int unit) { return (reach.unit(unit) + 1) * UNIT > clear || (LOCAL && reach.unit(unit) * UNIT < reach.every); };
     const auto ask = [&](int unit) {
       const int key = key_of(unit);
@@ -1013,7 +1023,10 @@ __global__ __launch_bounds__(512, 2) void attn_pairs_kernel(const AttnArgs a) {
     Piece kr[NU], vr[NU];
     uint32_t kp = 0, vp = 0;                           // their powers of two
     int block, block_v;                                // of the key, of the value that is asked for next
-    const auto key_of = [&](int unit) { return min(reach.unit(min(unit, last)) * UNIT + stage_row, r.kv - 1); };
+    const auto key_of = [&](int unit) {
+      const int c = min(unit, last), key = reach.unit(c) * UNIT + stage_row;
+      return min(LOCAL ? reach.read(c, key) : key, r.kv - 1);
+    };
     const auto is_edge = [&](int unit) { return (reach.unit(unit) + 1) * UNIT > clear || (LOCAL && reach.unit(unit) * UNIT < reach.every); };
     const auto ask = [&](bool values, int blk, int unit, Piece (&to)[NU], uint32_t &power) {
       const int key = key_of(unit);
@@ -1145,20 +1158,37 @@ __global__ __launch_bounds__(512, 2) void attn_pairs_kernel(const AttnArgs a) {
 // tokens from its start takes 1610 us of which 760 are the walk's, and requests without tokens are passed one by one (two single tokens over
 // 2048 keys: 17, with 4000 idle requests between them 54).
 // 4 bits: keys are cheaper to read than to unpack, so that tiles of 128 pay from 33 rows on (32 requests over 8001 keys, 64 and 128 rows a tile: 59 and 59 us
-// at 32 rows, 66 and 64 at 48, 76 and 69 at 64).  Of single tokens two heads to a workgroup where each still finds a tile to itself,
-// from 128 tiles of a head on (64 requests 62 and 56 us with one and two heads, 256 requests 261 and 174; one request of 32767 keys 18.5 and
-// 23), and 512 workgroups (64 requests: 75 us with 256).
-// With a window a tile's keys are at most the window's, which the rule takes for `keys`; the table above holds as it is (16 rows in bf16, 64 requests in
-// a window of 1024: 41.6 us with 256 workgroups, 45.5 with 512; 16 x 64 tokens in one of 1024, 64, 128 and 256 rows: 46, 49 and 52; 32 x 64: 84, 63 and 61).
+// at 32 rows, 66 and 64 at 48, 76 and 69 at 64).
+// LOCAL kernels of more rows go by the same table, with the window's keys where those are fewer (16 x 64 tokens in a window of 1024, 64, 128 and 256
+// rows: 46, 49 and 52 us; 32 x 64: 84, 63 and 61).  Those of 16 rows read two neighbouring heads' keys together, wider pieces of memory with fewer parts to join, where keys
+// are many, and one head's where two would leave workgroups without a tile; and they have 512 workgroups where these find a tile each.  Us, 8
+// cache heads, one and two heads with 256 workgroups, one and two with 512:
+//   B x keys              bf16, 128               e4m3, 128               e4m3, 64                4 bits, 128             4 bits, 64
+//   256 x up to 8192                                                      419  373  462  269                              498  411  462  297
+//   64 x up to 8192       253  242  263  252      168  158  164  144      126  107  114   84      154  137  139  113      119  107  113   77
+//   16 x up to 8192       82   73   84   76       51   48   48   46       32   29   35   27       41   40   40   37       34   32   31   29
+//   128 x up to 1024      96   94   89   90       79   66   61   55       52   42   41   34       70   58   53   48       55   45   42   37
+//   32 x up to 2048       47   45   49   49       34   32   29   30       26   25   23   22       34   32   29   30       27   25   24   24
+//   256 x 1028 (window)                                                   124  104  102  72                               125  105  102  69
+//   128 x 1028            122  114  114  113      89   74   72   69       64   53   55   38       80   71   64   51       66   53   42   37
+//   64 x 1028             74   69   73   76       46   39   40   41       35   27   23   26       42   36   32   35       32   29   25   28
+//   16 x 1028             23   26   28   29       19   21   21   21       15   16   16   17       19   21   21   22       16   16   17   19
+//   1 x 32767, 4 heads    34   37   38   49       20   23   20   23       18   19   18   19       20   24   20   23       18   20   18   20
 struct AttnPlan {
   int rows, groups;                    // rows of a tile; workgroups, a multiple of 8
   float cut;
   int heads;                           // cache heads of a workgroup (of 16 rows)
 };
-inline AttnPlan attn_plan(int T, int Hq, int Hkv, int B, int cache_dtype, bool trees, int64_t keys) {
+inline AttnPlan attn_plan(int T, int Hq, int Hkv, int B, int cache_dtype, bool local, bool trees, int64_t keys) {
   const int64_t rows = B > 0 ? ((int64_t)T * (Hq / Hkv) + B - 1) / B : 1;
-  const int heads = Hkv % 2 == 0 && (int64_t)B * Hkv >= 128 ? 2 : 1;
-  if (rows <= 16) return {16, cache_dtype == MOE_DTYPE_BF16 ? 256 : 512, 0.0625f, cache_dtype == MOE_DTYPE_FP4 ? heads : 1};
+  if (rows <= 16) {
+    const bool bf16 = cache_dtype == MOE_DTYPE_BF16;
+    if (!local) return {16, bf16 ? 256 : 512, 0.0625f, 1};
+    const int64_t tiles = (int64_t)B * Hkv, all = tiles * keys;
+    const int heads = Hkv % 2 == 0 && tiles >= 64 && all >= (bf16 ? 3 << 17 : 3 << 18) ? 2 : 1;
+    const bool more = bf16 ? tiles / heads >= 512 : tiles < 64 || tiles > 128 || all > 1 << 18;
+    return {16, more ? 512 : 256, 0.0625f, heads};
+  }
   if (rows <= (cache_dtype == MOE_DTYPE_FP4 ? 32 : 64) || (int64_t)T * Hq <= (trees ? 20000000 : 8000000) / (keys > 0 ? keys : 1)) return {64, 512, 0.125f, 1};
   if (rows <= 128) return {128, 512, 0.125f, 1};
   return {256, 256, 0.25f, 1};
@@ -1172,12 +1202,12 @@ inline int64_t attn_seen(int64_t room, int window, int sinks) {
 constexpr int attn_cache_bits(int cache_dtype) { return cache_dtype == MOE_DTYPE_BF16 ? 16 : cache_dtype == MOE_DTYPE_FP8 ? 8 : 4; }
 
 // What both entry points check and hand to their kernels.  scales: fp32 of each cache head, or a 4-bit cache's powers of two, whose blocks lie
-// *_scale_stride bytes apart.  window 0: none.  A call with nothing to do: MOE_OK and plan.rows 0.
+// *_scale_stride bytes apart.  window 0: none; local: for the LOCAL kernels.  A call with nothing to do: MOE_OK and plan.rows 0.
 inline int attn_arguments(const void *q_bf16, int64_t q_stride, int T, int Hq, int Hkv, int D, const void *k_cache, const void *v_cache, int cache_dtype,
                           int n_blocks, int64_t k_block_stride, int64_t v_block_stride, int page_size, const int32_t *block_tables,
                           int64_t table_stride, int table_width, const int32_t *kv_lens, const int32_t *cu_tokens, int B, const int64_t *masks,
                           float scale, const void *k_scale, const void *v_scale, int64_t k_scale_stride, int64_t v_scale_stride, int window,
-                          int sinks, void *out_bf16, float *lse, void *workspace, size_t workspace_bytes, AttnPlan &plan, AttnArgs &a) {
+                          int sinks, bool local, void *out_bf16, float *lse, void *workspace, size_t workspace_bytes, AttnPlan &plan, AttnArgs &a) {
   plan.rows = 0;
   const bool four = cache_dtype == MOE_DTYPE_FP4;
   if (T < 0 || B < 0 || B > MOE_MAX_REQUESTS || Hq < 1 || Hkv < 1 || Hq > 4096 || Hq % Hkv || (D != 64 && D != 128) || window < 0 || sinks < 0) return MOE_E_SHAPE;
@@ -1198,7 +1228,7 @@ inline int attn_arguments(const void *q_bf16, int64_t q_stride, int T, int Hq, i
   if ((uintptr_t)workspace % 256) return MOE_E_ALIGN;
   if (workspace_bytes < moe_tree_attention_workspace_bytes(T, Hq, Hkv, D, B, cache_dtype)) return MOE_E_WORKSPACE;
   const int64_t room = (int64_t)table_width * page_size;
-  const AttnPlan p = attn_plan(T, Hq, Hkv, B, cache_dtype, masks != nullptr, attn_seen(room, window, sinks));
+  const AttnPlan p = attn_plan(T, Hq, Hkv, B, cache_dtype, local, masks != nullptr, attn_seen(room, window, sinks));
   const int64_t most_units = ((int64_t)T * (Hq / Hkv) / p.rows + B) * Hkv * ((room + 63) / 64);
   if (most_units >= (1ll << 31)) return MOE_E_SHAPE;
   const size_t parts = 2 * p.groups;
@@ -1220,7 +1250,7 @@ template <int D, int C, bool LOCAL>
 void attn_main(const AttnArgs &a, const AttnPlan &plan, hipStream_t st) {
   if (plan.rows == 16 && plan.heads == 1) attn_keys_kernel<D, C, LOCAL, 1, 1><<<a.groups, 256, 0, st>>>(a);
   else if (plan.rows == 16) {
-    if constexpr (C == MOE_DTYPE_FP4) attn_keys_kernel<D, C, LOCAL, 1, 2><<<a.groups, 256, 0, st>>>(a);
+    if constexpr (LOCAL) attn_keys_kernel<D, C, LOCAL, 1, 2><<<a.groups, 256, 0, st>>>(a);
   }
   else if (plan.rows == 64) attn_rows_kernel<D, C, LOCAL, 1><<<a.groups, 256, 0, st>>>(a);
   else if (plan.rows == 128) attn_rows_kernel<D, C, LOCAL, 2><<<a.groups, 256, 0, st>>>(a);

@@ -1,4 +1,5 @@
 // Attention over the paged cache in bf16 and e4m3, every key seen: the kernels of tree_attention.h, and the join of all of them.
+#include <algorithm>
 #include "tree_attention.h"
 
 namespace moe {
@@ -111,9 +112,14 @@ void attn_join(const AttnArgs &a, const AttnPlan &plan, int D, hipStream_t st) {
 extern "C" size_t moe_tree_attention_workspace_bytes(int T, int Hq, int Hkv, int D, int B, int cache_dtype) {
   using namespace moe;
   if (T < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || D < 1 || B < 0 || cache_dtype < MOE_DTYPE_BF16 || cache_dtype > MOE_DTYPE_FP4) return 0;
-  const AttnPlan plan = attn_plan(T, Hq, Hkv, B, cache_dtype, false, 1ll << 31);      // (shorter caches need no more)
-  const size_t rows = (size_t)plan.rows * plan.heads, parts = 2 * plan.groups;
-  return align_up(parts * rows * D * 4, 256) + align_up(parts * rows * 8, 256) + plan.groups * 32;
+  size_t most = 0;                                     // of calls with a window and without, over the longest cache and the shortest
+  for (const bool local : {false, true})
+    for (const int64_t keys : {(int64_t)1 << 31, (int64_t)1}) {
+      const AttnPlan plan = attn_plan(T, Hq, Hkv, B, cache_dtype, local, false, keys);
+      const size_t rows = (size_t)plan.rows * plan.heads, parts = 2 * plan.groups;
+      most = std::max(most, align_up(parts * rows * D * 4, 256) + align_up(parts * rows * 8, 256) + plan.groups * 32);
+    }
+  return most;
 }
 
 extern "C" int moe_tree_attention_tile_rows(int T, int Hq, int Hkv, int B, int cache_dtype, int trees, int table_width, int page_size) {
@@ -121,7 +127,7 @@ extern "C" int moe_tree_attention_tile_rows(int T, int Hq, int Hkv, int B, int c
   if (T < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || B < 0 || B > MOE_MAX_REQUESTS || (cache_dtype != MOE_DTYPE_BF16 && cache_dtype != MOE_DTYPE_FP8) ||
       table_width < 0 || page_size < 1 || page_size > MOE_MAX_PAGE || (page_size & (page_size - 1)))
     return 0;
-  return attn_plan(T, Hq, Hkv, B, cache_dtype, trees != 0, (int64_t)table_width * page_size).rows;
+  return attn_plan(T, Hq, Hkv, B, cache_dtype, false, trees != 0, (int64_t)table_width * page_size).rows;
 }
 
 extern "C" int moe_tree_attention(void *stream, const void *q_bf16, int64_t q_stride, int T, int Hq, int Hkv, int D,
@@ -135,8 +141,8 @@ extern "C" int moe_tree_attention(void *stream, const void *q_bf16, int64_t q_st
   AttnPlan plan;
   AttnArgs a;
   const int rc = attn_arguments(q_bf16, q_stride, T, Hq, Hkv, D, k_cache, v_cache, cache_dtype, n_blocks, k_block_stride, v_block_stride, page_size,
-                                block_tables, table_stride, table_width, kv_lens, cu_tokens, B, masks, scale, k_scale, v_scale, 0, 0, 0, 0, out_bf16,
-                                lse, workspace, workspace_bytes, plan, a);
+                                block_tables, table_stride, table_width, kv_lens, cu_tokens, B, masks, scale, k_scale, v_scale, 0, 0, 0, 0, false,
+                                out_bf16, lse, workspace, workspace_bytes, plan, a);
   if (rc || !plan.rows) return rc;
   hipStream_t st = (hipStream_t)stream;
   const bool fp8 = cache_dtype == MOE_DTYPE_FP8;
