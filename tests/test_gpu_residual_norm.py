@@ -87,6 +87,24 @@ def test_strided_rows_and_in_place(pkg, dev, H, at):
         assert bool((big[k][:, :at] == -3).all()) and bool((big[k][:, at + H:] == -3).all())
 
 
+@pytest.mark.parametrize("H", [*range(1, 18), *range(505, 522), 1029, 2049, 4103, 8191, 8195, 16386])
+def test_last_pieces(pkg, dev, H):
+    """Rows of every length around a piece's and a wavefront's, in place, in types of their own, beside values that stay."""
+    say("residual_norm, last piece", H)
+    for wide, gate in ((False, "column"), (True, "full")):
+        a = make(5, H, H, wide, gate, gate_f32=wide, weights_f32=not wide)
+        big = {k: torch.full((5, H + 3), -3.0, dtype=a[k].dtype, device=dev) for k in ("x", "residual")}
+        for k, t in big.items():
+            t[:, 1:H + 1] = a[k].to(dev)
+        view = {k: t[:, 1:H + 1] for k, t in big.items()}
+        y, h = pkg.residual_norm(view["x"], view["residual"], a["weight"].to(dev), a["post_weight"].to(dev), a["gate"].to(dev), out=view["x"],
+                                 residual_out=view["residual"])
+        torch.cuda.synchronize()
+        check(a, (y, h), 1.0, 1e-6)
+        for t in big.values():
+            assert bool((t[:, 0] == -3).all()) and bool((t[:, H + 1:] == -3).all())
+
+
 def test_two_halves_of_one_buffer(pkg, dev):
     """Results in the columns beside what is read share no value with it."""
     a = make(6, 256, 5)

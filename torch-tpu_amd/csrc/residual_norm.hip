@@ -8,8 +8,8 @@
 // Bound by bytes: every value is read once and written once, so a row stays in the registers of the wavefronts that share it, sums of
 // squares are added over lanes by data-parallel moves and over wavefronts in LDS, and y is formed from the h in registers, before
 // its rounding.  All of it in fp32 with one rounding to each output.
-// 16384 rows of 7168 bf16 values with both norms and a gate per column: 189 us, 5.0 TB/s, where a large copy reaches 4.85; of 1999 values, whose rows
-// begin anywhere, 3.3 TB/s; one row of 7168: 3.2 us, the chain of row, sum over the wavefronts and store.
+// 16384 rows of 7168 bf16 values with both norms and a gate per column: 189 us, 5.0 TB/s, where a large copy reaches 4.85; 9808 rows of 1999
+// values, which begin anywhere, 40 us, 3.9 TB/s, of 2000 34; one row of 7168: 2.9 us, the chain of row, sum over the wavefronts and store.
 #include <type_traits>
 #include "moe_common.h"
 #include "lanes.h"
@@ -31,50 +31,85 @@ struct NormArgs {
   int T, H, residual_f32, weight_f32, gate_f32;
 };
 
-// Eight neighbouring values, or the `count` that a row's last piece has.  ALIGNED: on 16 bytes; else on their own size, which the memory path
-// takes in one access too.
+// Eight neighbouring values of a row from `place` on.  kWhole: on 16 bytes, kAny: on their own size, which the memory path takes in one
+// access too, kFew: rows of fewer than eight.  Of kAny a row's last piece of fewer values is loaded as the row's last eight, of which the first `back` are another lane's and
+// count as 0 (they may be overwritten already where a row takes its own place), and stored in pieces of 4, 2 and 1.  (9808 rows of 1999 values with one norm: 38 us,
+// 52 with the last piece value by value.)
+constexpr int kFew = 0, kAny = 1, kWhole = 2;
 typedef v4i __attribute__((aligned(2))) v4i_any;
+typedef v2i __attribute__((aligned(2))) v2i_any;
+typedef int __attribute__((aligned(2))) int_any;
 typedef v4f __attribute__((aligned(4))) v4f_any;
-template <bool ALIGNED>
-__device__ __forceinline__ void norm_load(const void *base, int64_t at, int count, bool f32, float (&v)[8]) {
-  if (!ALIGNED && count < 8) {
-    for (int i = 0; i < 8; i++) v[i] = 0.f;
+typedef float v2f_any __attribute__((ext_vector_type(2), aligned(4)));
+template <int HOW>
+__device__ __forceinline__ void norm_load(const void *row, int place, int H, bool f32, float (&v)[8]) {
+  if constexpr (HOW == kFew) {
 #pragma unroll
-    for (int i = 0; i < 7; i++)
-      if (i < count) v[i] = f32 ? ((const float *)base)[at + i] : bf16_to_f32(((const uint16_t *)base)[at + i]);
-  } else if (f32) {
-    const float *p = (const float *)base + at;
-    const v4f a = ALIGNED ? *(const v4f *)p : *(const v4f_any *)p, b = ALIGNED ? *(const v4f *)(p + 4) : *(const v4f_any *)(p + 4);
-#pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
+    for (int i = 0; i < 8; i++) {
+      v[i] = 0.f;
+      if (i < H) v[i] = f32 ? ((const float *)row)[i] : bf16_to_f32(((const uint16_t *)row)[i]);
+    }
   } else {
-    const uint16_t *p = (const uint16_t *)base + at;
-    const v4i w = ALIGNED ? *(const v4i *)p : *(const v4i_any *)p;
+    const int back = HOW == kWhole ? 0 : max(place + 8 - H, 0), at = place - back;
+    if (f32) {
+      const float *p = (const float *)row + at;
+      const v4f a = HOW == kWhole ? *(const v4f *)p : *(const v4f_any *)p, b = HOW == kWhole ? *(const v4f *)(p + 4) : *(const v4f_any *)(p + 4);
 #pragma unroll
-    for (int i = 0; i < 4; i++) v[2 * i] = __uint_as_float((uint32_t)w[i] << 16), v[2 * i + 1] = __uint_as_float((uint32_t)w[i] & 0xffff0000u);
+      for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
+    } else {
+      const uint16_t *p = (const uint16_t *)row + at;
+      const v4i w = HOW == kWhole ? *(const v4i *)p : *(const v4i_any *)p;
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[2 * i] = __uint_as_float((uint32_t)w[i] << 16), v[2 * i + 1] = __uint_as_float((uint32_t)w[i] & 0xffff0000u);
+    }
+    if constexpr (HOW == kAny) {
+#pragma unroll
+      for (int i = 0; i < 7; i++) v[i] = i < back ? 0.f : v[i];
+    }
   }
 }
-template <bool ALIGNED>
-__device__ __forceinline__ void norm_store(void *base, int64_t at, int count, bool f32, const float (&v)[8]) {
-  if (!ALIGNED && count < 8) {
+template <int HOW>
+__device__ __forceinline__ void norm_store(void *row, int place, int H, bool f32, const float (&v)[8]) {
+  const int count = H - place;
+  if constexpr (HOW == kFew) {
 #pragma unroll
     for (int i = 0; i < 7; i++) {
-      if (i >= count) continue;
-      if (f32) ((float *)base)[at + i] = v[i];
-      else ((uint16_t *)base)[at + i] = (uint16_t)pack2_bf16(v[i], 0.f);
+      if (i >= H) continue;
+      if (f32) ((float *)row)[i] = v[i];
+      else ((uint16_t *)row)[i] = (uint16_t)pack2_bf16(v[i], 0.f);
     }
-  } else if (f32) {
-    float *p = (float *)base + at;
-    const v4f a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
-    if (ALIGNED) *(v4f *)p = a, *(v4f *)(p + 4) = b;
-    else *(v4f_any *)p = a, *(v4f_any *)(p + 4) = b;
+  } else if (HOW == kWhole || count >= 8) {
+    if (f32) {
+      float *p = (float *)row + place;
+      const v4f a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
+      if (HOW == kWhole) *(v4f *)p = a, *(v4f *)(p + 4) = b;
+      else *(v4f_any *)p = a, *(v4f_any *)(p + 4) = b;
+    } else {
+      uint16_t *p = (uint16_t *)row + place;
+      const v4i w = {(int)pack2_bf16(v[0], v[1]), (int)pack2_bf16(v[2], v[3]), (int)pack2_bf16(v[4], v[5]), (int)pack2_bf16(v[6], v[7])};
+      if (HOW == kWhole) *(v4i *)p = w;
+      else *(v4i_any *)p = w;
+    }
   } else {
-    uint16_t *p = (uint16_t *)base + at;
-    const v4i w = {(int)pack2_bf16(v[0], v[1]), (int)pack2_bf16(v[2], v[3]), (int)pack2_bf16(v[4], v[5]), (int)pack2_bf16(v[6], v[7])};
-    if (ALIGNED) *(v4i *)p = w;
-    else *(v4i_any *)p = w;
+    const bool four = count & 4, two = count & 2;
+    const float v1 = v[1], v2 = v[2], v3 = v[3], v5 = v[5], v6 = v[6], v7 = v[7];
+    const float a = four ? v2 : v6, b = four ? v3 : v7, one = four ? (two ? v1 : v3) : two ? v5 : v7;
+    if (f32) {
+      float *end = (float *)row + H;
+      if (four) *(v4f_any *)(end - 4) = (v4f){v[4], v5, v6, v7};
+      if (two) *(v2f_any *)(end - (count & 4) - 2) = (v2f_any){a, b};
+      if (count & 1) end[-count] = one;
+    } else {
+      uint16_t *end = (uint16_t *)row + H;
+      if (four) *(v2i_any *)(end - 4) = (v2i){(int)pack2_bf16(v[4], v5), (int)pack2_bf16(v6, v7)};
+      if (two) *(int_any *)(end - (count & 4) - 2) = (int)pack2_bf16(a, b);
+      if (count & 1) end[-count] = (uint16_t)pack2_bf16(one, 0.f);
+    }
   }
 }
+// row t of a tensor of fp32 or bf16
+__device__ __forceinline__ const void *norm_row(const void *base, int64_t at, bool f32) { return (const uint8_t *)base + (at << (f32 ? 2 : 1)); }
+__device__ __forceinline__ void *norm_row(void *base, int64_t at, bool f32) { return (uint8_t *)base + (at << (f32 ? 2 : 1)); }
 
 // The sum over the WAVES wavefronts of a row; `turn` names the sum, so that a second one needs no barrier of its own.
 template <int WAVES>
@@ -92,7 +127,7 @@ __device__ __forceinline__ float row_sum(float v, int turn) {
 }
 
 // A row to WAVES wavefronts, P pieces of 8 values to a lane.  One wavefront a row: four rows to a workgroup.
-template <int WAVES, int P, bool ALIGNED>
+template <int WAVES, int P, int HOW>
 __global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) void residual_norm_kernel(const NormArgs a) {
   constexpr int ROWS = WAVES > 1 ? 1 : 4, LANES = 64 * WAVES;
   const int64_t t = (int64_t)blockIdx.x * ROWS + (WAVES > 1 ? 0 : threadIdx.x >> 6);
@@ -104,26 +139,25 @@ __global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) void residual_norm_ke
   float u[P][8], h[P][8], w[P][8], w2[EARLY ? P : 1][8], g[EARLY ? P : 1][8];
   const auto place = [&](int p) { return (p * LANES + lane) * 8; };
   const auto live = [&](int p) { return place(p) < a.H; };
-  const auto count = [&](int p) { return a.H - place(p); };
   const auto weights = [&](const void *from, int p, float (&to)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; i++) to[i] = 1.f;
-    if (from && live(p)) norm_load<ALIGNED>(from, place(p), count(p), a.weight_f32, to);
+    if (from && live(p)) norm_load<HOW>(from, place(p), a.H, a.weight_f32, to);
   };
   float one = 1.f;                                     // a gate that is the same for the row
   if (a.gate && !a.gate_col) one = a.gate_f32 ? ((const float *)a.gate)[t * a.gate_row] : bf16_to_f32(((const uint16_t *)a.gate)[t * a.gate_row]);
   const auto gates = [&](int p, float (&to)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; i++) to[i] = one;
-    if (a.gate && a.gate_col && live(p)) norm_load<ALIGNED>(a.gate, t * a.gate_row + place(p), count(p), a.gate_f32, to);
+    if (a.gate && a.gate_col && live(p)) norm_load<HOW>(norm_row(a.gate, t * a.gate_row, a.gate_f32), place(p), a.H, a.gate_f32, to);
   };
 #pragma unroll
   for (int p = 0; p < P; p++) {
 #pragma unroll
     for (int i = 0; i < 8; i++) u[p][i] = h[p][i] = 0.f;
     if (!live(p)) continue;
-    norm_load<ALIGNED>(a.x, t * a.x_stride + place(p), count(p), false, u[p]);
-    if (a.residual) norm_load<ALIGNED>(a.residual, t * a.residual_stride + place(p), count(p), a.residual_f32, h[p]);
+    norm_load<HOW>(norm_row(a.x, t * a.x_stride, false), place(p), a.H, false, u[p]);
+    if (a.residual) norm_load<HOW>(norm_row(a.residual, t * a.residual_stride, a.residual_f32), place(p), a.H, a.residual_f32, h[p]);
   }
   if constexpr (EARLY) {
     if (a.post_weight) weights(a.post_weight, 0, w2[0]);
@@ -164,7 +198,7 @@ __global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) void residual_norm_ke
       h[p][i] = fmaf(a.scale, u[p][i], h[p][i]);
       sum = fmaf(h[p][i], h[p][i], sum);
     }
-    if (live(p) && a.h) norm_store<ALIGNED>(a.h, t * a.h_stride + place(p), count(p), a.residual_f32, h[p]);
+    if (live(p) && a.h) norm_store<HOW>(norm_row(a.h, t * a.h_stride, a.residual_f32), place(p), a.H, a.residual_f32, h[p]);
   }
   const float r = 1.0f / sqrtf(row_sum<WAVES>(sum, 1) * a.over_h + a.eps);
 #pragma unroll
@@ -172,7 +206,7 @@ __global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) void residual_norm_ke
     if (!live(p)) continue;
 #pragma unroll
     for (int i = 0; i < 8; i++) h[p][i] *= r * w[p][i];
-    norm_store<ALIGNED>(a.y, t * a.y_stride + place(p), count(p), false, h[p]);
+    norm_store<HOW>(norm_row(a.y, t * a.y_stride, false), place(p), a.H, false, h[p]);
   }
 }
 
@@ -230,8 +264,8 @@ extern "C" int moe_residual_norm(void *stream, const void *x_bf16, int64_t x_str
     whole = whole && (uintptr_t)p % 16 == 0;
   hipStream_t st = (hipStream_t)stream;
   const unsigned grid = (unsigned)T;
-  const auto run = [&](auto aligned) {
-    constexpr bool A = decltype(aligned)::value;
+  const auto run = [&](auto how) {
+    constexpr int A = decltype(how)::value;
     const int pieces = (H + 7) / 8;
     if (pieces <= 64) residual_norm_kernel<1, 1, A><<<(grid + 3) / 4, 256, 0, st>>>(a);
     else if (pieces <= 128) residual_norm_kernel<2, 1, A><<<grid, 128, 0, st>>>(a);
@@ -241,7 +275,8 @@ extern "C" int moe_residual_norm(void *stream, const void *x_bf16, int64_t x_str
     else if (pieces <= 2048) residual_norm_kernel<16, 2, A><<<grid, 1024, 0, st>>>(a);
     else residual_norm_kernel<16, 4, A><<<grid, 1024, 0, st>>>(a);
   };
-  if (whole) run(std::integral_constant<bool, true>());
-  else run(std::integral_constant<bool, false>());
+  if (whole) run(std::integral_constant<int, kWhole>());
+  else if (H >= 8) run(std::integral_constant<int, kAny>());
+  else residual_norm_kernel<1, 1, kFew><<<(grid + 3) / 4, 256, 0, st>>>(a);
   return (int)hipGetLastError();
 }
