@@ -384,7 +384,7 @@ extern "C" int moe_adjust_logits(void *stream, const void *logits, int dtype, in
       if (a.bf16) adjust_logits_kernel<BYTES, TH, true, M><<<n, TH, 0, st>>>(a);
       else adjust_logits_kernel<BYTES, TH, false, M><<<n, TH, 0, st>>>(a);
     };
-    if constexpr (TH <= 512) {
+    if constexpr (BYTES == 8192 || BYTES == 32768) {
       if (a.rows > 1) launch(std::integral_constant<bool, true>());
       else launch(std::integral_constant<bool, false>());
     } else {
@@ -396,9 +396,12 @@ extern "C" int moe_adjust_logits(void *stream, const void *logits, int dtype, in
   const int64_t work = (int64_t)((T + a.rows - 1) / a.rows) * V * e;
   // Few values: segments of 8 KB, so that the whole chip takes part (a row of 131072 bf16 values 7.2 us, 9.7 with 16 KB).  Else of 32 KB: fewer segments read
   // the histories again, more workgroups share the chip (64 rows of 131072 bf16 values with 8192 tokens of history: 16.8 us, 19.5 with 16 KB, 29 with
-  // 8; 64 of 100003 with 2000, half of them masked: 14.6, 15.5, 19.6).  Long histories of single rows are read by even fewer segments of 64 KB (15.0
-  // and 15.6; fp32 23.8, 25.7 with 32 KB, 28 with 16; of several rows, which wait for each other, 210 and 156).
+  // 8; 64 of 100003 with 2000, half of them masked: 14.6, 15.5, 19.6).  Of single rows three workgroups share a compute unit where there is
+  // work for more than one turn (24 KB; 512 of 100003 bf16 values with 4096 tokens: 66 us, 71 with 32 KB, 88 with 64; 256 of 131072 fp32 with 512: 59, 70, 87; but 64 of
+  // 100003 bf16: 12.0 and 11.3 with 32), and where there is about one turn, the fewest segments read long histories (64 KB; 64 of 131072 fp32 with 8192 tokens: 22.4, 24.9 with
+  // 32, 26.3 with 24; with 1024 tokens 21.7, 19.5, 18.8).  Several rows wait for each other (1290 of 100003 bf16: 156 us, 161 with 24 KB, 210 with 64).
   if (work < (2 << 20)) return run(integral_constant<int, 8192>(), integral_constant<int, 512>());
-  if (a.rows == 1 && history && L >= 4096 && work >= (16 << 20)) return run(integral_constant<int, 65536>(), integral_constant<int, 1024>());
+  if (a.rows == 1 && history && L >= 4096 && work >= (16 << 20) && work <= (32 << 20)) return run(integral_constant<int, 65536>(), integral_constant<int, 1024>());
+  if (a.rows == 1 && work >= (32 << 20)) return run(integral_constant<int, 24576>(), integral_constant<int, 512>());
   return run(integral_constant<int, 32768>(), integral_constant<int, 512>());
 }
