@@ -92,7 +92,7 @@ class Cache:
         self.n_free = p.n_free
         return p
 
-    def keep(self, plan, kept, tokens):
+    def keep(self, plan, kept, tokens=None):
         """kept[b]: the rows of the step that stay, in text order.  Their keys and values move up behind the cached text (their angles
         are already those of their depth), and pages that nothing needs any more go back on the stack."""
         rows = [(b, self.lens[b].item() + i, row) for b, some in enumerate(kept) for i, row in enumerate(some)]
@@ -102,7 +102,8 @@ class Cache:
             for cache in [c for pair in self.layers + self.scales for c in pair if c is not None]:
                 flat = cache.view(torch.uint8).flatten(0, 1)
                 flat[to] = flat[plan.slots[row]]
-            self.text[b, place] = tokens[row].int()
+            if tokens is not None:
+                self.text[b, place] = tokens[row].int()
         had = (plan.kv_lens + self.page - 1) // self.page
         self.lens = self.lens + torch.tensor([len(k) for k in kept], dtype=torch.int32, device=self.lens.device)
         column = torch.arange(self.tables.shape[1], device=self.lens.device)

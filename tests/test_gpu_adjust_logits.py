@@ -191,10 +191,10 @@ def test_cu_tokens_out_of_order_end(pkg, dev):
 
 
 @pytest.mark.parametrize("counts,V,L,bf16,tree,how", [
-    # large enough for segments of 32 KB, and of 64 KB where single rows have long histories
+    # large enough for segments of 24 KB, and of 64 KB where rows have long histories
     ([1] * 40, 60001, 700, True, False, dict(masked="rows")), ([1] * 36, 131072, 4200, False, False, dict(biases=3)), ([3, 16, 5, 1], 100003, 500, True, True, dict(masked="own")),
     ([1] * 70, 130001, 4100, True, False, {}), ([7, 1], 262145, 60, False, True, {}),
-    # and of 24 KB where there are more single rows than that
+    # of 24 KB again where there are more rows than that
     ([1] * 70, 131077, 300, False, False, dict(masked="rows", biases=3)), ([1] * 90, 200003, 4200, True, False, dict(masked="own")), ([1] * 72, 131072, 64, False, False, {})])
 def test_large_vocabularies(pkg, dev, counts, V, L, bf16, tree, how):
     say("adjust_logits, large", len(counts), V, L, bf16)

@@ -6,14 +6,15 @@
 //        -> x + bias of the token                          (of a token named twice the last)
 //        -> -inf unless the grammar allows the token
 //
-// fp32, one rounding at the end.  Bound by bytes: logits once in, once out.  A workgroup takes a segment of the vocabulary for some rows.  It
+// fp32, one rounding at the end.  Bound by bytes: logits once in, once out.  A workgroup takes a segment of a row.  It
 // counts the history's tokens that lie in the segment in LDS, so that no counter per vocabulary entry exists in memory, and a bit per token
 // says which were touched.  A row streams through registers, is stored as it is (but for what its grammar forbids) without waiting for the
 // counts, and the threads that stored the few touched values then store those once more.
-// 64 rows of 131072 fp32 values with up to 8192 tokens of history: 24 us, 14 without the histories (2.8 and 4.9 TB/s); 1290 rows of 100003
-// bf16 values, 128 requests' trees, every other row with a grammar: 156 us, 104 with neither (3.3 and 5.0 TB/s).  What histories cost is the
-// comparisons of every token in every segment and the counting, about 25 instructions a token.  (LDS atomics of all lanes instead of a branch: slower; a list of
-// the touched tokens in place of the bits: 30 and 180 us.)
+// 64 rows of 131072 fp32 values with up to 8192 tokens of history: 22 us, 13 without the histories (3.1 and 5.3 TB/s); 1275 rows of 100003
+// bf16 values, 128 requests' trees, every other row with a grammar: 143 us, 94 with neither (3.6 and 5.4 TB/s).  What histories cost is the
+// comparisons of every token in every segment and the counting, about 25 instructions a token.  (LDS atomics of all lanes instead of a branch, and a list of
+// the touched tokens in place of the bits, took 5 to 15 % longer.  Up to four rows of a request to a workgroup, which then counts once for
+// them: 156 us for the 143, and 25 for 10 where there are 155 rows of 32000 values.)
 #include <math.h>
 #include <type_traits>
 #include "moe_common.h"
@@ -25,7 +26,7 @@ struct LogitArgs {
   const void *in;
   void *out;
   int64_t in_stride, out_stride;
-  int T, V, B, L, bf16, rows, segments;        // rows: of a workgroup
+  int T, V, B, L, bf16, segments;
   const int32_t *cu, *history;
   int64_t history_stride;
   const int32_t *history_lens, *prompt_lens;
@@ -60,9 +61,8 @@ struct LogitTable {
 
 typedef uint16_t __attribute__((aligned(1))) any_u16;
 
-// BYTES of a row to a workgroup: BYTES / 16 groups of 16 bytes, P of them to a thread.  MANY: several rows, of which the next one is on its way
-// while one is worked on.
-template <int BYTES, int THREADS, bool BF16, bool MANY>
+// BYTES of a row to a workgroup: BYTES / 16 groups of 16 bytes, P of them to a thread.
+template <int BYTES, int THREADS, bool BF16>
 __global__ __launch_bounds__(THREADS) void adjust_logits_kernel(const LogitArgs a) {
   constexpr int N = BF16 ? 8 : 4, E = BF16 ? 2 : 4, SEG = BYTES / E;             // values of 16 bytes; bytes of one
   constexpr int P = BYTES / (16 * THREADS), ALL = (1 << N) - 1;
@@ -73,42 +73,21 @@ __global__ __launch_bounds__(THREADS) void adjust_logits_kernel(const LogitArgs 
   const int tid = threadIdx.x, lane = tid & 63;
   const int seg = blockIdx.x % a.segments;
   const int first = seg * SEG, from = first - 8;       // the segment's first token, for a row that begins on 16 bytes; the first counter's
-  const int t0 = (int)(blockIdx.x / a.segments) * a.rows, t1 = min(t0 + a.rows, a.T);
+  const int t = (int)(blockIdx.x / a.segments);
 
   // A row's groups begin on 16 bytes of memory: where the row does not, the first one begins `before` values earlier.  Of most segments all
   // groups lie within the row (inside); of the others some have values before or behind it, which are taken value by value.
-  const auto row_in = [&](int t) { return (const uint8_t *)a.in + t * a.in_stride * E; };
-  const auto before_of = [&](int t) { return (int)((uintptr_t)row_in(t) % 16) / E; };
-  const auto inside_of = [&](int before) { return first >= before && first - before + SEG <= a.V; };
-  const auto token_of = [&](int p, int before) { return first + (p * THREADS + tid) * N - before; };
-  const auto grammar_of = [&](int t) { return !a.allowed ? -1 : a.allowed_row ? a.allowed_row[t] : t; };
-  const auto words_of = [&](int grammar) { return grammar >= 0 && grammar < a.allowed_rows ? (const uint32_t *)a.allowed + grammar * a.allowed_stride : nullptr; };
+  const uint8_t *in = (const uint8_t *)a.in + t * a.in_stride * E;
+  uint8_t *out = (uint8_t *)a.out + t * a.out_stride * E;
+  const int before = (int)((uintptr_t)in % 16) / E;
+  const bool inside = first >= before && first - before + SEG <= a.V;
+  const auto token_of = [&](int p) { return first + (p * THREADS + tid) * N - before; };
+  const int grammar = !a.allowed ? -1 : a.allowed_row ? a.allowed_row[t] : t;
+  const uint32_t *words = grammar >= 0 && grammar < a.allowed_rows ? (const uint32_t *)a.allowed + grammar * a.allowed_stride : nullptr;
   const int last_bits = (a.V + 31) / 32 * 4 - 2;       // a row of the grammar's last two bytes
-  const auto bits_at = [&](const uint32_t *words, int v) {
+  const auto bits_at = [&](int v) {
     const int at = min(v >> 3, last_bits);
     return (uint32_t)*(const any_u16 *)((const uint8_t *)words + at) >> (v - 8 * at) & ALL;
-  };
-  const auto load = [&](int t, const uint32_t *words, Group *g) {
-    const uint8_t *in = row_in(t);
-    const int before = before_of(t);
-    const bool inside = inside_of(before);
-#pragma unroll
-    for (int p = 0; p < P; p++) {
-      const int v = token_of(p, before);
-      g[p].let = ALL;
-      if (inside || (v >= 0 && v + N <= a.V)) {
-        const v4i raw = *(const v4i *)(in + (uint32_t)v * (uint32_t)E);
-#pragma unroll
-        for (int i = 0; i < 4; i++) g[p].w[i] = (uint32_t)raw[i];
-      }
-    }
-    if (words) {
-#pragma unroll
-      for (int p = 0; p < P; p++) {
-        const int v = token_of(p, before);
-        if (inside || (v >= 0 && v + N <= a.V)) g[p].let = bits_at(words, v);
-      }
-    }
   };
   const auto store = [&](uint8_t *out, int v, bool same, const uint32_t (&w)[4]) {
     if (same) {
@@ -122,215 +101,185 @@ __global__ __launch_bounds__(THREADS) void adjust_logits_kernel(const LogitArgs 
     }
   };
 
-  int b = -1, begin = 0, end = 0;                      // the request whose history is counted, its rows
-  uint64_t path = 0;                                   // the tokens of the tree that are counted
-  uint32_t drafted = ~0u;                              // lane i: the counter of the request's token i
-  float rep = 1.f, less = 1.f, freq = 0.f, pres = 0.f; // less: 1 / rep
-  bool counts = false;
-  Group now[P], next[MANY ? P : 1];
-  const uint32_t *words = words_of(grammar_of(t0)), *next_words = nullptr;
-  int next_grammar = MANY && t0 + 1 < t1 ? grammar_of(t0 + 1) : -1;
-  uint64_t next_mask = a.masks ? (uint64_t)a.masks[t0] : 0;
-  load(t0, words, now);
-  for (int t = t0; t < t1; t++) {
-    // What the next rows need is asked for here: nothing below waits for a trip to memory that begins with this row, but its request's
-    // history where a new one begins.
-    const uint64_t mask = next_mask;
-    if (MANY && a.masks && t + 1 < t1) next_mask = (uint64_t)a.masks[t + 1];
-    bool fresh = false;
-    if (a.cu) {
-      if (b < 0 || t >= end) {                         // the last request that begins at t or before
-        int lo = 0, hi = a.B;                          // 64 places at a time
-        while (lo < hi) {
-          const int step = (hi - lo + 63) / 64, at = lo + (1 + lane) * step;
-          const int past = __popcll(__ballot(at <= hi && a.cu[min(at, hi)] <= t));
-          hi = min(lo + (past + 1) * step - 1, hi);
-          lo += past * step;
-        }
-        fresh = true;
-        b = lo < a.B && a.cu[lo] <= t ? lo : a.B;
-        begin = b < a.B ? max(a.cu[b], 0) : t;
-        end = b < a.B ? min(a.cu[b + 1], a.T) : lo < a.B ? min(a.cu[lo], a.T) : a.T;
-      }
-    } else {
-      fresh = true;
-      b = t, begin = t, end = t + 1;
-    }
-    const bool none = b >= a.B;                        // a row of no request passes as it is
-    // The history's first tokens are asked for together with its length and the penalties: one trip to memory.
-    const int32_t *ids = a.history + (none ? 0 : b * a.history_stride);
-    const bool heard = fresh && !none && a.history && a.L > 0;
-    // (Four neighbours to a lane: histories are read by every segment, and single values took more loads than the logits.)
-    v4i asked_for = {-1, -1, -1, -1};
-    int len = 0, asked = 0;
-    const bool whole = (uintptr_t)ids % 16 == 0;
-    const auto ask = [&](int i0) {
-      const int i = i0 + 4 * tid;
-      if (whole && i + 4 <= a.L) {
-        asked_for = *(const v4i *)(ids + i);
-      } else {
+  Group now[P];
 #pragma unroll
-        for (int j = 0; j < 4; j++) asked_for[j] = i + j < a.L ? ids[i + j] : -1;
-      }
-    };
-    if (fresh) {
-      if (heard) ask(0);
-      rep = !none && a.repetition ? a.repetition[b] : 1.f;
-      freq = !none && a.frequency ? a.frequency[b] : 0.f;
-      pres = !none && a.presence ? a.presence[b] : 0.f;
-      len = heard && a.history_lens ? min(a.history_lens[b], a.L) : a.L;
-      asked = heard && a.prompt_lens ? min(a.prompt_lens[b], len) : 0;
-      const int64_t draft = !none && a.tokens && a.masks && tid < 64 && begin + tid < end ? a.tokens[begin + tid] - from : -1;
-      drafted = draft >= 0 && draft < SEG + 8 ? (uint32_t)draft : ~0u;
+  for (int p = 0; p < P; p++) {
+    const int v = token_of(p);
+    now[p].let = ALL;
+    if (inside || (v >= 0 && v + N <= a.V)) {
+      const v4i raw = *(const v4i *)(in + (uint32_t)v * (uint32_t)E);
+#pragma unroll
+      for (int i = 0; i < 4; i++) now[p].w[i] = (uint32_t)raw[i];
     }
-    if (MANY && t + 1 < t1) {
-      next_words = words_of(next_grammar);
-      load(t + 1, next_words, next);
-      if (t + 2 < t1) next_grammar = grammar_of(t + 2);
-    }
-
-    // The row as it is, but for what its grammar forbids: this waits for nothing but the row.
-    const uint8_t *in = row_in(t);
-    uint8_t *out = (uint8_t *)a.out + t * a.out_stride * E;
-    const int before = before_of(t);
-    const bool same = (uintptr_t)out % 16 == (uintptr_t)in % 16, moved = a.out != a.in, inside = inside_of(before);
-    if (none) words = nullptr;
+  }
+  if (words) {
 #pragma unroll
     for (int p = 0; p < P; p++) {
-      const int v = token_of(p, before);
-      uint32_t (&w)[4] = now[p].w;
-      if (inside || (v >= 0 && v + N <= a.V)) {
-        if (words) {
-          const uint32_t let = now[p].let;
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            if (BF16) {
-              const uint32_t keep = ((uint32_t)((int)(let << (31 - 2 * i)) >> 31) & 0xffffu) | ((uint32_t)((int)(let << (30 - 2 * i)) >> 31) & 0xffff0000u);
-              w[i] = (w[i] & keep) | (0xff80ff80u & ~keep);
-            } else {
-              w[i] = let >> i & 1 ? w[i] : 0xff800000u;
-            }
-          }
-        } else {
-          now[p].let = ALL;
-        }
-        if (moved || words) store(out, v, same, w);
-      } else {
-        for (int k = max(v, 0); k < min(v + N, a.V); k++) {
-          const bool may = !words || words[k >> 5] >> (k & 31) & 1;
-          if (BF16) ((uint16_t *)out)[k] = may ? ((const uint16_t *)in)[k] : 0xff80;
-          else ((uint32_t *)out)[k] = may ? ((const uint32_t *)in)[k] : 0xff800000u;
-        }
-      }
+      const int v = token_of(p);
+      if (inside || (v >= 0 && v + N <= a.V)) now[p].let = bits_at(v);
     }
+  }
 
-    if (fresh) {
-      less = 1.0f / rep;
-      counts = rep != 1.f || freq != 0.f || pres != 0.f;
-      path = 0;
-      for (int i = tid; i < SEG / 4 + 2; i += THREADS) *(v4i *)&s.count[4 * i] = (v4i){0, 0, 0, 0};
-      for (int i = tid; i < SEG / 32 + 2; i += THREADS) s.touched[i] = 0;
-      __syncthreads();
-      if (!none && a.n_bias) {
-        for (int i = tid; i < a.n_bias; i += THREADS) {
-          const uint32_t place = (uint32_t)(a.bias_ids[b * a.bias_ids_stride + i] - from);
-          if (place >= SEG + 8) continue;
-          atomicMax(&s.count[place], (uint32_t)(i + 1) << kBiasShift);
-          s.touch(place);
-        }
-        __syncthreads();
-      }
-      if (heard && counts) {
-        for (int i = 0; i < len; i += 4 * THREADS) {
-          const v4i id = asked_for;
-          if (i + 4 * THREADS < len) ask(i + 4 * THREADS);           // (on their way while these are counted)
-            const bool said = i >= asked && i + 4 * THREADS <= len, prompt = i + 4 * THREADS <= asked;       // (elsewhere threads differ)
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-              const uint32_t place = (uint32_t)(id[j] - from);
-              if (place >= SEG + 8) continue;
-              const int at = i + 4 * tid + j;
-              const uint64_t here = __ballot(true);
-              if ((said || prompt) && __popcll(here) > 40) {     // a text that repeats itself: so many additions at one address take as many turns
-                const uint64_t like = __ballot(place == (uint32_t)__builtin_amdgcn_readfirstlane(place));
-                if (like >> lane & 1) {
-                  if (lane == __builtin_ctzll(like)) {
-                    if (prompt) atomicOr(&s.count[place], kHeard);
-                    else atomicAdd(&s.count[place], (uint32_t)__popcll(like) * kOnce);
-                    s.touch(place);
-                  }
-                  continue;
-                }
-              }
-              if (said || (at >= asked && at < len)) atomicAdd(&s.count[place], kOnce);
-              else if (at < asked) atomicOr(&s.count[place], kHeard);
-              s.touch(place);
-            }
-        }
-      }
-      if (!none && counts && a.tokens && !a.masks)     // what stands before the row
-        for (int i = begin + tid; i < t; i += THREADS) s.add(a.tokens[i] - from, kOnce);
+  // The row's request: the last one that begins at t or before.
+  int b = t, begin = t, end = t + 1;
+  if (a.cu) {
+    int lo = 0, hi = a.B;                              // 64 places at a time
+    while (lo < hi) {
+      const int step = (hi - lo + 63) / 64, at = lo + (1 + lane) * step;
+      const int past = __popcll(__ballot(at <= hi && a.cu[min(at, hi)] <= t));
+      hi = min(lo + (past + 1) * step - 1, hi);
+      lo += past * step;
     }
-    if (!none && counts && a.tokens) {
-      if (a.masks) {
-        const int was = path >> lane & 1, is = mask >> lane & 1;
-        if (drafted != ~0u && was != is) {
-          atomicAdd(&s.count[drafted], is ? kOnce : 0u - kOnce);
-          s.touch(drafted);
+    b = lo < a.B && a.cu[lo] <= t ? lo : a.B;
+    begin = b < a.B ? max(a.cu[b], 0) : t;
+    end = b < a.B ? min(a.cu[b + 1], a.T) : t;
+  }
+  const bool none = b >= a.B;                          // a row of no request passes as it is
+  // The history's first tokens are asked for together with its length and the penalties: one trip to memory.
+  const int32_t *ids = a.history + (none ? 0 : b * a.history_stride);
+  const bool heard = !none && a.history && a.L > 0;
+  // (Four neighbours to a lane: histories are read by every segment, and single values took more loads than the logits.)
+  v4i asked_for = {-1, -1, -1, -1};
+  const bool whole = (uintptr_t)ids % 16 == 0;
+  const auto ask = [&](int i0) {
+    const int i = i0 + 4 * tid;
+    if (whole && i + 4 <= a.L) {
+      asked_for = *(const v4i *)(ids + i);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; j++) asked_for[j] = i + j < a.L ? ids[i + j] : -1;
+    }
+  };
+  if (heard) ask(0);
+  const float rep = !none && a.repetition ? a.repetition[b] : 1.f, freq = !none && a.frequency ? a.frequency[b] : 0.f,
+              pres = !none && a.presence ? a.presence[b] : 0.f;
+  const int len = heard && a.history_lens ? min(a.history_lens[b], a.L) : a.L, asked = heard && a.prompt_lens ? min(a.prompt_lens[b], len) : 0;
+  // the drafted tokens on the row's path: those that its mask names, 64 at the most, or those up to its own
+  const uint64_t mask = !none && a.masks ? (uint64_t)a.masks[t] : 0;
+  const bool drafted = !none && a.tokens && a.masks && tid < 64 && begin + tid < end && (mask >> tid & 1);
+  const int64_t draft = drafted ? a.tokens[begin + tid] : 0;
+  for (int i = tid; i < SEG / 4 + 2; i += THREADS) *(v4i *)&s.count[4 * i] = (v4i){0, 0, 0, 0};
+  for (int i = tid; i < SEG / 32 + 2; i += THREADS) s.touched[i] = 0;
+
+  // The row as it is, but for what its grammar forbids: this waits for nothing but the row.
+  const bool same = (uintptr_t)out % 16 == (uintptr_t)in % 16, moved = a.out != a.in;
+  if (none) words = nullptr;
+#pragma unroll
+  for (int p = 0; p < P; p++) {
+    const int v = token_of(p);
+    uint32_t (&w)[4] = now[p].w;
+    if (inside || (v >= 0 && v + N <= a.V)) {
+      if (words) {
+        const uint32_t let = now[p].let;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          if (BF16) {
+            const uint32_t keep = ((uint32_t)((int)(let << (31 - 2 * i)) >> 31) & 0xffffu) | ((uint32_t)((int)(let << (30 - 2 * i)) >> 31) & 0xffff0000u);
+            w[i] = (w[i] & keep) | (0xff80ff80u & ~keep);
+          } else {
+            w[i] = let >> i & 1 ? w[i] : 0xff800000u;
+          }
         }
-        path = mask;
-      } else if (tid == 0) {
-        s.add(a.tokens[t] - from, kOnce);
+      } else {
+        now[p].let = ALL;
       }
+      if (moved || words) store(out, v, same, w);
+    } else {
+      for (int k = max(v, 0); k < min(v + N, a.V); k++) {
+        const bool may = !words || words[k >> 5] >> (k & 31) & 1;
+        if (BF16) ((uint16_t *)out)[k] = may ? ((const uint16_t *)in)[k] : 0xff80;
+        else ((uint32_t *)out)[k] = may ? ((const uint32_t *)in)[k] : 0xff800000u;
+      }
+    }
+  }
+
+  const float less = 1.0f / rep;
+  const bool counts = rep != 1.f || freq != 0.f || pres != 0.f;
+  if (none || !(counts || a.n_bias)) return;
+  __syncthreads();
+  if (a.n_bias) {
+    for (int i = tid; i < a.n_bias; i += THREADS) {
+      const uint32_t place = (uint32_t)(a.bias_ids[b * a.bias_ids_stride + i] - from);
+      if (place >= SEG + 8) continue;
+      atomicMax(&s.count[place], (uint32_t)(i + 1) << kBiasShift);
+      s.touch(place);
     }
     __syncthreads();
-
-    // The touched values, each by the thread that has just stored it.
-    const auto adjusted = [&](float x, uint32_t c) {
-      if (c & kCounts) {
-        const float n = (float)((c & kCounts) >> 1);
-        x = x * (x > 0.f ? less : rep) - (n > 0.f ? fmaf(freq, n, pres) : 0.f);
-      }
-      if (c >> kBiasShift) x += a.bias[b * a.bias_stride + (c >> kBiasShift) - 1];
-      return x;
-    };
-    if (!none && (counts || a.n_bias)) {
-      uint32_t hit[P];
+  }
+  if (heard && counts) {
+    for (int i = 0; i < len; i += 4 * THREADS) {
+      const v4i id = asked_for;
+      if (i + 4 * THREADS < len) ask(i + 4 * THREADS);                 // (on their way while these are counted)
+      const bool said = i >= asked && i + 4 * THREADS <= len, prompt = i + 4 * THREADS <= asked;       // (elsewhere threads differ)
 #pragma unroll
-      for (int p = 0; p < P; p++) {
-        const int at = (p * THREADS + tid) * N - before + 8;         // the first one's counter
-        const uint32_t lo = s.touched[at >> 5], hi = s.touched[(at >> 5) + 1];
-        hit[p] = __builtin_amdgcn_alignbit(hi, lo, at & 31) & ALL;
-      }
-#pragma unroll
-      for (int p = 0; p < P; p++) {
-        const int v = token_of(p, before), at = (p * THREADS + tid) * N - before + 8;
-        if (inside || (v >= 0 && v + N <= a.V)) {
-          const v4i w = {(int)now[p].w[0], (int)now[p].w[1], (int)now[p].w[2], (int)now[p].w[3]};
-          uint32_t left = hit[p] & now[p].let;
-          while (left) {                               // (few, if any: a wavefront passes as often as one of its lanes has hits)
-            const int k = __builtin_ctz(left);
-            left &= left - 1;
-            const int word = BF16 ? k >> 1 : k;
-            const uint32_t low = word & 1 ? w[1] : w[0], high = word & 1 ? w[3] : w[2], one = word & 2 ? high : low;
-            const float x = adjusted(BF16 ? __uint_as_float(one >> (16 * (k & 1)) << 16) : __uint_as_float(one), s.count[at + k]);
-            if (BF16) ((uint16_t *)out)[(uint32_t)(v + k)] = (uint16_t)pack2_bf16(x, 0.f);
-            else ((float *)out)[(uint32_t)(v + k)] = x;
-          }
-        } else if (hit[p]) {
-          for (int k = max(-v, 0); k < N && v + k < a.V; k++) {
-            if (!s.count[at + k] || (words && !(words[(v + k) >> 5] >> ((v + k) & 31) & 1))) continue;
-            const float x = adjusted(BF16 ? bf16_to_f32(((const uint16_t *)in)[v + k]) : ((const float *)in)[v + k], s.count[at + k]);
-            if (BF16) ((uint16_t *)out)[v + k] = (uint16_t)pack2_bf16(x, 0.f);
-            else ((float *)out)[v + k] = x;
+      for (int j = 0; j < 4; j++) {
+        const uint32_t place = (uint32_t)(id[j] - from);
+        if (place >= SEG + 8) continue;
+        const int at = i + 4 * tid + j;
+        const uint64_t here = __ballot(true);
+        if ((said || prompt) && __popcll(here) > 40) {     // a text that repeats itself: so many additions at one address take as many turns
+          const uint64_t like = __ballot(place == (uint32_t)__builtin_amdgcn_readfirstlane(place));
+          if (like >> lane & 1) {
+            if (lane == __builtin_ctzll(like)) {
+              if (prompt) atomicOr(&s.count[place], kHeard);
+              else atomicAdd(&s.count[place], (uint32_t)__popcll(like) * kOnce);
+              s.touch(place);
+            }
+            continue;
           }
         }
+        if (said || (at >= asked && at < len)) atomicAdd(&s.count[place], kOnce);
+        else if (at < asked) atomicOr(&s.count[place], kHeard);
+        s.touch(place);
       }
     }
+  }
+  if (counts && a.tokens) {
+    if (drafted) s.add(draft - from, kOnce);
+    if (!a.masks)
+      for (int i = begin + tid; i <= t; i += THREADS) s.add(a.tokens[i] - from, kOnce);
+  }
+  __syncthreads();
+
+  // The touched values, each by the thread that has just stored it.
+  const auto adjusted = [&](float x, uint32_t c) {
+    if (c & kCounts) {
+      const float n = (float)((c & kCounts) >> 1);
+      x = x * (x > 0.f ? less : rep) - (n > 0.f ? fmaf(freq, n, pres) : 0.f);
+    }
+    if (c >> kBiasShift) x += a.bias[b * a.bias_stride + (c >> kBiasShift) - 1];
+    return x;
+  };
+  uint32_t hit[P];
 #pragma unroll
-    for (int p = 0; p < P; p++) now[p] = next[MANY ? p : 0];
-    words = next_words;
-    if (MANY) __syncthreads();
+  for (int p = 0; p < P; p++) {
+    const int at = (p * THREADS + tid) * N - before + 8;             // the first one's counter
+    const uint32_t lo = s.touched[at >> 5], hi = s.touched[(at >> 5) + 1];
+    hit[p] = __builtin_amdgcn_alignbit(hi, lo, at & 31) & ALL;
+  }
+#pragma unroll
+  for (int p = 0; p < P; p++) {
+    const int v = token_of(p), at = (p * THREADS + tid) * N - before + 8;
+    if (inside || (v >= 0 && v + N <= a.V)) {
+      const v4i w = {(int)now[p].w[0], (int)now[p].w[1], (int)now[p].w[2], (int)now[p].w[3]};
+      uint32_t left = hit[p] & now[p].let;
+      while (left) {                                   // (few, if any: a wavefront passes as often as one of its lanes has hits)
+        const int k = __builtin_ctz(left);
+        left &= left - 1;
+        const int word = BF16 ? k >> 1 : k;
+        const uint32_t low = word & 1 ? w[1] : w[0], high = word & 1 ? w[3] : w[2], one = word & 2 ? high : low;
+        const float x = adjusted(BF16 ? __uint_as_float(one >> (16 * (k & 1)) << 16) : __uint_as_float(one), s.count[at + k]);
+        if (BF16) ((uint16_t *)out)[(uint32_t)(v + k)] = (uint16_t)pack2_bf16(x, 0.f);
+        else ((float *)out)[(uint32_t)(v + k)] = x;
+      }
+    } else if (hit[p]) {
+      for (int k = max(-v, 0); k < N && v + k < a.V; k++) {
+        if (!s.count[at + k] || (words && !(words[(v + k) >> 5] >> ((v + k) & 31) & 1))) continue;
+        const float x = adjusted(BF16 ? bf16_to_f32(((const uint16_t *)in)[v + k]) : ((const float *)in)[v + k], s.count[at + k]);
+        if (BF16) ((uint16_t *)out)[v + k] = (uint16_t)pack2_bf16(x, 0.f);
+        else ((float *)out)[v + k] = x;
+      }
+    }
   }
 }
 
@@ -366,8 +315,7 @@ extern "C" int moe_adjust_logits(void *stream, const void *logits, int dtype, in
     return MOE_E_MODE;
   for (const void *p : {(const void *)history_lens, (const void *)prompt_lens, (const void *)repetition, (const void *)frequency, (const void *)presence})
     if (over(p, 1, 0, B, 4)) return MOE_E_MODE;
-  const int rows = B > 0 ? (T + B - 1) / B : 1;
-  LogitArgs a{logits, out, row_stride, out_stride, T, V, B, L, dtype == MOE_DTYPE_BF16, rows < 4 ? rows : 4, 0, cu_tokens,
+  LogitArgs a{logits, out, row_stride, out_stride, T, V, B, L, dtype == MOE_DTYPE_BF16, 0, cu_tokens,
               history, history_stride, history_lens, prompt_lens, tokens, masks, repetition, frequency, presence, bias_ids, bias_ids_stride, bias,
               bias_stride, n_bias, allowed, allowed_stride, n_allowed, allowed_rows};
   hipStream_t st = (hipStream_t)stream;
@@ -376,32 +324,26 @@ extern "C" int moe_adjust_logits(void *stream, const void *logits, int dtype, in
   const auto run = [&](auto bytes, auto threads) {
     constexpr int BYTES = decltype(bytes)::value, TH = decltype(threads)::value;
     a.segments = (int)((wide * e + BYTES - 1) / BYTES);
-    const int64_t blocks = (int64_t)a.segments * ((T + a.rows - 1) / a.rows);
+    const int64_t blocks = (int64_t)a.segments * T;
     if (blocks > 0x7fffffff) return MOE_E_SHAPE;
-    const unsigned n = (unsigned)blocks;
-    const auto launch = [&](auto many) {
-      constexpr bool M = decltype(many)::value;
-      if (a.bf16) adjust_logits_kernel<BYTES, TH, true, M><<<n, TH, 0, st>>>(a);
-      else adjust_logits_kernel<BYTES, TH, false, M><<<n, TH, 0, st>>>(a);
-    };
-    if constexpr (BYTES == 8192 || BYTES == 32768) {
-      if (a.rows > 1) launch(std::integral_constant<bool, true>());
-      else launch(std::integral_constant<bool, false>());
-    } else {
-      launch(std::integral_constant<bool, false>());
-    }
+    if (a.bf16) adjust_logits_kernel<BYTES, TH, true><<<(unsigned)blocks, TH, 0, st>>>(a);
+    else adjust_logits_kernel<BYTES, TH, false><<<(unsigned)blocks, TH, 0, st>>>(a);
     return (int)hipGetLastError();
   };
   using std::integral_constant;
-  const int64_t work = (int64_t)((T + a.rows - 1) / a.rows) * V * e;
-  // Few values: segments of 8 KB, so that the whole chip takes part (a row of 131072 bf16 values 7.2 us, 9.7 with 16 KB).  Else of 32 KB: fewer segments read
-  // the histories again, more workgroups share the chip (64 rows of 131072 bf16 values with 8192 tokens of history: 16.8 us, 19.5 with 16 KB, 29 with
-  // 8; 64 of 100003 with 2000, half of them masked: 14.6, 15.5, 19.6).  Of single rows three workgroups share a compute unit where there is
-  // work for more than one turn (24 KB; 512 of 100003 bf16 values with 4096 tokens: 66 us, 71 with 32 KB, 88 with 64; 256 of 131072 fp32 with 512: 59, 70, 87; but 64 of
-  // 100003 bf16: 12.0 and 11.3 with 32), and where there is about one turn, the fewest segments read long histories (64 KB; 64 of 131072 fp32 with 8192 tokens: 22.4, 24.9 with
-  // 32, 26.3 with 24; with 1024 tokens 21.7, 19.5, 18.8).  Several rows wait for each other (1290 of 100003 bf16: 156 us, 161 with 24 KB, 210 with 64).
-  if (work < (2 << 20)) return run(integral_constant<int, 8192>(), integral_constant<int, 512>());
-  if (a.rows == 1 && history && L >= 4096 && work >= (16 << 20) && work <= (32 << 20)) return run(integral_constant<int, 65536>(), integral_constant<int, 1024>());
-  if (a.rows == 1 && work >= (32 << 20)) return run(integral_constant<int, 24576>(), integral_constant<int, 512>());
-  return run(integral_constant<int, 32768>(), integral_constant<int, 512>());
+  const int64_t work = (int64_t)T * V * e;
+  // Large segments read the histories and zero the counters less often, small ones put more workgroups to work: of 24 KB three share a compute unit.  Us:
+  //                                                        16 KB     24        32        64
+  //   1 row of 131072 bf16, 4096 tokens of history         7.5       7.6       8.0       8.4
+  //   16 of 131072 bf16, 8192                              8.8       9.7       10.2      10.7
+  //   514 of 5493 bf16 (205 trees), 300 biases             14.2      14.9      19.5      32.6
+  //   155 of 32000 bf16 (16 trees), 2000                   10.1      9.6       10.3      11.8
+  //   64 of 131072 bf16, 8192                              19.5      16.4      16.0      14.0
+  //   64 of 131072 fp32, 8192                              27.9      23.8      23.5      23.6
+  //   320 of 131072 fp32 (64 trees), 2000                  99        78        80        113
+  //   512 of 100003 bf16, 4096                             73        64        69        98
+  //   1275 of 100003 bf16 (128 trees), 2048                160       143       159       252
+  if (work < (6 << 20)) return run(integral_constant<int, 16384>(), integral_constant<int, 512>());
+  if (history && L >= 4096 && work >= (16 << 20) && work <= (32 << 20)) return run(integral_constant<int, 65536>(), integral_constant<int, 1024>());      // (about one turn)
+  return run(integral_constant<int, 24576>(), integral_constant<int, 512>());
 }
