@@ -475,8 +475,10 @@ int moe_tree_attention(void *stream, const void *q_bf16, int64_t q_stride, int T
  *                       times 2^(byte - 127) of its 32 neighbours is its value (255: NaN), blocks *_scale_block_stride bytes apart.  The
  *                       caches' block strides count elements, as ever, and divide by 32.
  *   MOE_DTYPE_BF16, _FP8  k_scale / v_scale are fp32 of each head or NULL, their strides unused.
- * Everything else as moe_tree_attention; the workspace is moe_tree_attention_workspace_bytes of the same arguments.
+ * Everything else as moe_tree_attention; workspace: moe_window_attention_workspace_bytes; that of moe_tree_attention_workspace_bytes is enough
+ * too, but over a bf16 or e4m3 cache may leave no room for the faster of two kernels.
  */
+size_t moe_window_attention_workspace_bytes(int T, int Hq, int Hkv, int D, int B, int cache_dtype);
 int moe_window_attention_tile_rows(int T, int Hq, int Hkv, int B, int cache_dtype, int trees, int table_width, int page_size, int window,
                                    int sinks);
 int moe_window_attention(void *stream, const void *q_bf16, int64_t q_stride, int T, int Hq, int Hkv, int D, const void *k_cache,

@@ -174,3 +174,19 @@ def test_plain_window_by_hand():
     # a tree whose second token does not see the first
     out, _, _ = window.attention(q, k, v, [[0, 1]], [6], [0, 2], [0b01, 0b10], 1.0, 2, 0)
     assert torch.allclose(out[:, 0, 0], torch.tensor([(3 + 4) / 2, (3 + 5) / 2]).double())
+
+
+def test_attention_workspaces(pkg):
+    """Calls without a window ask for one head's parts; with one for two heads' where two share a workgroup."""
+    of = lambda groups, heads, D=128: 2 * groups * 16 * heads * (D * 4 + 8) + groups * 32
+    tree, window = lib().moe_tree_attention_workspace_bytes, lib().moe_window_attention_workspace_bytes
+    for B in (64, 256):
+        assert tree(B, 32, 4, 128, B, 1) == of(256, 1) and tree(B, 32, 4, 128, B, 2) == of(512, 1)
+        assert tree(B, 32, 4, 64, B, 1) == of(256, 1, 64)
+        assert window(B, 32, 4, 128, B, 1) == of(256 if B == 64 else 512, 2) and window(B, 32, 4, 128, B, 2) == of(512, 2)
+        assert tree(B, 32, 4, 128, B, 3) == window(B, 32, 4, 128, B, 3) == of(512, 2)
+    for T in (1, 7, 64, 1000, 5000):                       # a window asks for no less, and over a 4-bit cache there is no other call
+        for B in (1, 3, 40):
+            for cache in (1, 2, 3):
+                assert window(T, 8, 2, 128, B, cache) >= tree(T, 8, 2, 128, B, cache) > 0
+    assert window(4, 8, 3, 128, 3, 1) == 0 and window(4, 8, 2, 128, 3, 0) == 0 and window(4, 8, 2, 128, 3, 4) == 0

@@ -502,3 +502,42 @@ def test_into_a_captured_cache(pkg, dev):
     s.tables = tables.tolist()
     s.q = pkg.qk_norm_rope(qkv, pos, cs, Hq, Hkv)[0].cpu()
     s.check(got, None)
+
+
+# ------------------------------------------------------------------------------------------------ workspaces
+def in_c(pkg, s, dev, workspace, given, window=None, sinks=0):
+    """tree_attention of Step s by its C entry, with `given` bytes of `workspace`: the entry with a window where there is one."""
+    a = s.args(dev)
+    q, k, ptr = a["q"].contiguous(), a["k_cache"], lambda t: None if t is None else t.data_ptr()
+    (T, Hq, D), (n_blocks, page, Hkv, _) = q.shape, k.shape
+    out, tables = torch.zeros_like(q), a["block_tables"].contiguous()
+    stream, block = torch.cuda.current_stream().cuda_stream, page * Hkv * D
+    kind = {"bf16": 1, "fp8": 2}[s.cache]
+    head = (stream, ptr(q), Hq * D, T, Hq, Hkv, D, ptr(k), ptr(a["v_cache"]), kind, n_blocks, block, block, page, ptr(tables), tables.shape[1], tables.shape[1],
+            ptr(a["kv_lens"]), ptr(a["cu_tokens"]), len(s.lens), ptr(a.get("masks")), s.scale, ptr(a.get("k_scale")), ptr(a.get("v_scale")))
+    tail = (ptr(out), None, ptr(workspace), given)
+    lib = pkg._lib.lib
+    rc = lib.moe_window_attention(*head, 0, 0, window, sinks, *tail) if window else lib.moe_tree_attention(*head, *tail)
+    torch.cuda.synchronize()
+    return rc, out
+
+
+@pytest.mark.parametrize("cache,B,Hkv", [("bf16", 70, 4), ("bf16", 260, 2), ("fp8", 70, 4)])
+def test_calls_ask_for_what_they_use(pkg, dev, cache, B, Hkv):
+    """Without a window one head's parts are room enough, with one too, and nothing behind the room is touched."""
+    say("workspaces", cache, B, Hkv)
+    D, W = 128, 8000
+    one = 2 * (256 if cache == "bf16" else 512) * 16 * (D * 4 + 8) + (256 if cache == "bf16" else 512) * 32
+    s = one_request_in_room(Step(B, [(17 * b % 900 + (7500 if b == 3 else 0), 1) for b in range(B)], 2 * Hkv, Hkv, D, 64, cache, False), 131072)
+    lib = pkg._lib.lib
+    more = lib.moe_window_attention_workspace_bytes(B, 2 * Hkv, Hkv, D, B, 1 if cache == "bf16" else 2)
+    room = torch.full((more + 65536,), 7, dtype=torch.uint8, device=dev)
+    for given, window in ((one, None), (one, W), (more, W)):
+        s.window = dict(window=window, sinks=4 if window else 0)
+        room.fill_(7)
+        rc, out = in_c(pkg, s, dev, room, given, window, 4)
+        assert rc == 0
+        assert bool((room[given:] == 7).all())
+        s.check(out, None)
+        if given == more or not window:
+            assert torch.equal(out, pkg.tree_attention(**s.args(dev)))

@@ -1193,6 +1193,11 @@ inline AttnPlan attn_plan(int T, int Hq, int Hkv, int B, int cache_dtype, bool l
   if (rows <= 128) return {128, 512, 0.125f, 1};
   return {256, 256, 0.25f, 1};
 }
+// what a plan's launches leave for each other: the stretches' parts, their maxima and sums, the records
+inline size_t attn_workspace(const AttnPlan &p, int D) {
+  const size_t rows = (size_t)p.rows * p.heads, parts = 2 * p.groups;
+  return align_up(parts * rows * D * 4, 256) + align_up(parts * rows * 8, 256) + p.groups * 32;
+}
 // the keys that a row sees at most, where there is room for so many
 inline int64_t attn_seen(int64_t room, int window, int sinks) {
   const int64_t most = window ? (int64_t)window + sinks : room;
@@ -1226,9 +1231,11 @@ inline int attn_arguments(const void *q_bf16, int64_t q_stride, int T, int Hq, i
   for (const void *p : {q_bf16, k_cache, v_cache, (const void *)out_bf16})
     if ((uintptr_t)p % 16) return MOE_E_ALIGN;
   if ((uintptr_t)workspace % 256) return MOE_E_ALIGN;
-  if (workspace_bytes < moe_tree_attention_workspace_bytes(T, Hq, Hkv, D, B, cache_dtype)) return MOE_E_WORKSPACE;
-  const int64_t room = (int64_t)table_width * page_size;
-  const AttnPlan p = attn_plan(T, Hq, Hkv, B, cache_dtype, local, masks != nullptr, attn_seen(room, window, sinks));
+  const int64_t room = (int64_t)table_width * page_size, seen = attn_seen(room, window, sinks);
+  AttnPlan p = attn_plan(T, Hq, Hkv, B, cache_dtype, local, masks != nullptr, seen);
+  // (A workspace that moe_tree_attention would take is enough here too: then one head to a workgroup.)
+  if (workspace_bytes < attn_workspace(p, D)) p = attn_plan(T, Hq, Hkv, B, cache_dtype, false, masks != nullptr, seen);
+  if (workspace_bytes < attn_workspace(p, D)) return MOE_E_WORKSPACE;
   const int64_t most_units = ((int64_t)T * (Hq / Hkv) / p.rows + B) * Hkv * ((room + 63) / 64);
   if (most_units >= (1ll << 31)) return MOE_E_SHAPE;
   const size_t parts = 2 * p.groups;

@@ -1,5 +1,4 @@
 // Attention over the paged cache in bf16 and e4m3, every key seen: the kernels of tree_attention.h, and the join of all of them.
-#include <algorithm>
 #include "tree_attention.h"
 
 namespace moe {
@@ -112,14 +111,8 @@ void attn_join(const AttnArgs &a, const AttnPlan &plan, int D, hipStream_t st) {
 extern "C" size_t moe_tree_attention_workspace_bytes(int T, int Hq, int Hkv, int D, int B, int cache_dtype) {
   using namespace moe;
   if (T < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || D < 1 || B < 0 || cache_dtype < MOE_DTYPE_BF16 || cache_dtype > MOE_DTYPE_FP4) return 0;
-  size_t most = 0;                                     // of calls with a window and without, over the longest cache and the shortest
-  for (const bool local : {false, true})
-    for (const int64_t keys : {(int64_t)1 << 31, (int64_t)1}) {
-      const AttnPlan plan = attn_plan(T, Hq, Hkv, B, cache_dtype, local, false, keys);
-      const size_t rows = (size_t)plan.rows * plan.heads, parts = 2 * plan.groups;
-      most = std::max(most, align_up(parts * rows * D * 4, 256) + align_up(parts * rows * 8, 256) + plan.groups * 32);
-    }
-  return most;
+  if (cache_dtype == MOE_DTYPE_FP4) return moe_window_attention_workspace_bytes(T, Hq, Hkv, D, B, cache_dtype);
+  return attn_workspace(attn_plan(T, Hq, Hkv, B, cache_dtype, false, false, 1ll << 31), D);          // (shorter caches need no more)
 }
 
 extern "C" int moe_tree_attention_tile_rows(int T, int Hq, int Hkv, int B, int cache_dtype, int trees, int table_width, int page_size) {

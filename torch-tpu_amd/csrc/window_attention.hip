@@ -3,7 +3,15 @@
 //   64 single tokens, 16384 keys in a window of 1024, bf16     36.6 us, 3.7 TB/s: a workgroup's tile at once, then launch, lengths and a tile's end
 //   64 single tokens over up to 8192 keys in 4 bits            55.5 us, 3.2 TB/s: half lines of memory, and the conversions
 //   one token over 32767 keys in 4 bits                        18.5 us: a chain of launch, tables, a few units and the join
+#include <algorithm>
 #include "tree_attention.h"
+
+extern "C" size_t moe_window_attention_workspace_bytes(int T, int Hq, int Hkv, int D, int B, int cache_dtype) {
+  using namespace moe;
+  if (T < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || D < 1 || B < 0 || cache_dtype < MOE_DTYPE_BF16 || cache_dtype > MOE_DTYPE_FP4) return 0;
+  const auto of = [&](int64_t keys) { return attn_workspace(attn_plan(T, Hq, Hkv, B, cache_dtype, true, false, keys), D); };
+  return std::max(of(1ll << 31), of(1));               // (two heads to 256 workgroups or one to 512; what lies between needs no more)
+}
 
 extern "C" int moe_window_attention_tile_rows(int T, int Hq, int Hkv, int B, int cache_dtype, int trees, int table_width, int page_size, int window,
                                               int sinks) {
