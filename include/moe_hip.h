@@ -481,6 +481,8 @@ int moe_tree_attention(void *stream, const void *q_bf16, int64_t q_stride, int T
 size_t moe_window_attention_workspace_bytes(int T, int Hq, int Hkv, int D, int B, int cache_dtype);
 int moe_window_attention_tile_rows(int T, int Hq, int Hkv, int B, int cache_dtype, int trees, int table_width, int page_size, int window,
                                    int sinks);
+/* cache heads whose keys a workgroup reads together in such a call, 1 or 2 (0: not a valid call) */
+int moe_window_attention_heads(int T, int Hq, int Hkv, int B, int cache_dtype, int trees, int table_width, int page_size, int window, int sinks);
 int moe_window_attention(void *stream, const void *q_bf16, int64_t q_stride, int T, int Hq, int Hkv, int D, const void *k_cache,
                          const void *v_cache, int cache_dtype, int n_blocks, int64_t k_block_stride, int64_t v_block_stride,
                          int page_size, const int32_t *block_tables, int64_t table_stride, int table_width, const int32_t *kv_lens,

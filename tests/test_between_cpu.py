@@ -190,3 +190,12 @@ def test_attention_workspaces(pkg):
             for cache in (1, 2, 3):
                 assert window(T, 8, 2, 128, B, cache) >= tree(T, 8, 2, 128, B, cache) > 0
     assert window(4, 8, 3, 128, 3, 1) == 0 and window(4, 8, 2, 128, 3, 0) == 0 and window(4, 8, 2, 128, 3, 4) == 0
+
+
+def test_which_calls_take_two_heads_to_a_workgroup(pkg):
+    heads = lambda *a: lib().moe_window_attention_heads(*a)
+    # 64 single tokens over 4 heads: in 4 bits, in a wide window, in a narrow one; one token; an odd number of heads; trees of many rows
+    assert heads(64, 32, 4, 64, 3, 0, 512, 16, 0, 0) == 2 and heads(64, 32, 4, 64, 1, 0, 1024, 16, 8000, 4) == 2 and heads(64, 32, 4, 64, 1, 0, 1024, 16, 500, 4) == 1
+    assert heads(1, 32, 4, 1, 3, 0, 2048, 16, 0, 0) == 1 and heads(64, 24, 3, 64, 3, 0, 512, 16, 0, 0) == 1 and heads(512, 32, 4, 8, 3, 1, 512, 16, 0, 0) == 1
+    for bad in ((-1, 4, 2, 1, 1, 0, 4, 16, 1, 0), (1, 4, 2, 1, 4, 0, 4, 16, 1, 0), (1, 4, 2, 1, 1, 0, 4, 16, -1, 0), (1, 4, 2, 1, 1, 0, 4, 16, 1, -1)):
+        assert heads(*bad) == 0

@@ -541,3 +541,28 @@ def test_calls_ask_for_what_they_use(pkg, dev, cache, B, Hkv):
         s.check(out, None)
         if given == more or not window:
             assert torch.equal(out, pkg.tree_attention(**s.args(dev)))
+
+
+def heads_of(pkg, s):
+    (T, Hq, _), (_, page, Hkv, _) = s.q.shape, s.k.shape
+    return pkg._lib.lib.moe_window_attention_heads(T, Hq, Hkv, len(s.lens), {"bf16": 1, "fp8": 2, "fp4": 3}[s.cache], s.masks is not None, len(s.tables[0]), page,
+                                                   min(s.window["window"] or 0, 2 ** 31 - 1), s.window["sinks"])
+
+
+@pytest.mark.parametrize("cache,D,Hq,Hkv,W,sinks", [
+    ("fp4", 128, 8, 4, None, 0), ("fp4", 64, 6, 2, None, 0), ("fp4", 64, 16, 8, None, 0), ("fp4", 128, 32, 4, 9000, 5), ("fp4", 64, 4, 4, 9000, 0),
+    ("fp8", 128, 8, 2, 9000, 70), ("fp8", 64, 16, 8, 9000, 0), ("bf16", 128, 8, 4, 9000, 1), ("bf16", 64, 6, 6, 9000, 130)])
+@pytest.mark.parametrize("lengths", ["ragged", "alike", "one long"])
+def test_the_kernel_of_two_heads(pkg, dev, cache, D, Hq, Hkv, W, sinks, lengths):
+    """Two heads to a workgroup: tiles cut across workgroups and joined, whole tiles, and one tile over many workgroups."""
+    say("tree_attention, two heads", cache, D, Hq, Hkv, W, sinks, lengths)
+    g = torch.Generator().manual_seed(D + Hkv)
+    some = torch.randint(0, 700, (130 // Hkv + 30,), generator=g).tolist()
+    cached = {"ragged": some, "alike": [410] * len(some), "one long": [3 + n % 40 for n in some]}[lengths]
+    reqs = [(n, 1) for n in cached] + [(-1, 1), (0, 0), (9100 if lengths != "alike" else 411, 1), (5, 1)]
+    s = one_request_in_room(Step(D, reqs, Hq, Hkv, D, 16, cache, False, W, sinks, spare_rows=2), 131072)
+    assert heads_of(pkg, s) == 2 and s.rows(pkg) == 16
+    out, lse = pkg.tree_attention(**s.args(dev), return_lse=True)
+    torch.cuda.synchronize()
+    s.check(out, lse)
+    assert torch.equal(out, pkg.tree_attention(**s.args(dev)))

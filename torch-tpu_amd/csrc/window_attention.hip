@@ -13,13 +13,19 @@ extern "C" size_t moe_window_attention_workspace_bytes(int T, int Hq, int Hkv, i
   return std::max(of(1ll << 31), of(1));               // (two heads to 256 workgroups or one to 512; what lies between needs no more)
 }
 
-extern "C" int moe_window_attention_tile_rows(int T, int Hq, int Hkv, int B, int cache_dtype, int trees, int table_width, int page_size, int window,
-                                              int sinks) {
+static moe::AttnPlan window_plan(int T, int Hq, int Hkv, int B, int cache_dtype, int trees, int table_width, int page_size, int window, int sinks) {
   using namespace moe;
   if (T < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || B < 0 || B > MOE_MAX_REQUESTS || cache_dtype < MOE_DTYPE_BF16 || cache_dtype > MOE_DTYPE_FP4 ||
       table_width < 0 || page_size < 1 || page_size > MOE_MAX_PAGE || (page_size & (page_size - 1)) || window < 0 || sinks < 0)
-    return 0;
-  return attn_plan(T, Hq, Hkv, B, cache_dtype, true, trees != 0, attn_seen((int64_t)table_width * page_size, window, sinks)).rows;
+    return {};
+  return attn_plan(T, Hq, Hkv, B, cache_dtype, true, trees != 0, attn_seen((int64_t)table_width * page_size, window, sinks));
+}
+extern "C" int moe_window_attention_tile_rows(int T, int Hq, int Hkv, int B, int cache_dtype, int trees, int table_width, int page_size, int window,
+                                              int sinks) {
+  return window_plan(T, Hq, Hkv, B, cache_dtype, trees, table_width, page_size, window, sinks).rows;
+}
+extern "C" int moe_window_attention_heads(int T, int Hq, int Hkv, int B, int cache_dtype, int trees, int table_width, int page_size, int window, int sinks) {
+  return window_plan(T, Hq, Hkv, B, cache_dtype, trees, table_width, page_size, window, sinks).heads;
 }
 
 extern "C" int moe_window_attention(void *stream, const void *q_bf16, int64_t q_stride, int T, int Hq, int Hkv, int D, const void *k_cache,
