@@ -199,3 +199,18 @@ def test_which_calls_take_two_heads_to_a_workgroup(pkg):
     assert heads(1, 32, 4, 1, 3, 0, 2048, 16, 0, 0) == 1 and heads(64, 24, 3, 64, 3, 0, 512, 16, 0, 0) == 1 and heads(512, 32, 4, 8, 3, 1, 512, 16, 0, 0) == 1
     for bad in ((-1, 4, 2, 1, 1, 0, 4, 16, 1, 0), (1, 4, 2, 1, 4, 0, 4, 16, 1, 0), (1, 4, 2, 1, 1, 0, 4, 16, -1, 0), (1, 4, 2, 1, 1, 0, 4, 16, 1, -1)):
         assert heads(*bad) == 0
+
+
+def test_four_bits_are_off_by_a_fifth_at_most():
+    """The power leaves the largest of 32 elements above 3.5 and at most 7.  Up to 4 a value is off by 1 / 2 at most, above by 1: a fifth of the
+    largest at most, which the tie at 5 reaches."""
+    import window_plain as window
+    off = lambda x: ((window.decode(*window.encode(x)) - x).abs() / x.abs().amax(-1, keepdim=True)).amax(-1)
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(20000, 32, generator=g).double() * torch.exp2(torch.randint(-30, 30, (20000, 1), generator=g).double())
+    assert off(x).max() <= 0.2 and (off(x) > 1 / 7).double().mean() > 0.2
+    top = torch.linspace(3.5, 7, 7001, dtype=torch.float64)[1:]
+    alone = torch.zeros(len(top), 32, dtype=torch.float64)
+    alone[:, 5] = top
+    assert off(alone).max() == 0.2 and top[off(alone).argmax()] == 5
+    assert off(alone)[top <= 4].max() <= 1 / 7 and off(alone)[top >= 6].max() <= 1 / 7

@@ -6,7 +6,7 @@
 //
 // One rounding at the end: to bf16, to e4m3 after the division by the head's scale, or to 4 bits after the division by a power of two
 // that 32 neighbouring elements share, the least that leaves them at 7 or below: what lies between 6, the largest code, and 7 is then off by no more than the
-// half step of 1 that values above 4 are off by anyway, and a value is never off by more than a seventh of the 32's largest.
+// half step of 1 that values above 4 are off by anyway, and a value is never off by more than a fifth of the 32's largest (5, that goes to 4).
 // It is bound by bytes, so a value is read once and written once.  A lane holds 8 neighbouring elements of a head, D/8 lanes a head
 // (rounded up to a power of two); the sum of squares is taken over those lanes, and the partner of an (i, i + R/2) pair comes
 // from the lane R/16 further as the two bf16 that the register holds.  A lane's angles and weights are the same for every head, so it
