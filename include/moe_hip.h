@@ -469,7 +469,8 @@ int moe_tree_attention(void *stream, const void *q_bf16, int64_t q_stride, int T
  * moe_tree_attention where a token sees a window of the text and its first tokens, and over a cache in 4 bits.
  *
  *   window W, sinks S   the keys that a token may see by moe_tree_attention's rules, numbered from 0 in the cache's order: it sees the last
- *                       W and the first S of them.  W 0: all.  Pages of which no token sees a key are not read.
+ *                       W and the first S of them.  W 0: all.  Pages of which no token sees a key are not read (of a tree: nor one whose mask names
+ *                       no new token would).
  *   MOE_DTYPE_FP4       caches [n_blocks, page_size, Hkv, D / 2] bytes: element 2 i in the low 4 bits of byte i, 2 i + 1 in the high ones; codes 0 to 7 are 0,
  *                       0.5, 1, 1.5, 2, 3, 4, 6, with bit 3 their negatives.  k_scale / v_scale [n_blocks, page_size, Hkv, D / 32] bytes: an element
  *                       times 2^(byte - 127) of its 32 neighbours is its value (255: NaN), blocks *_scale_block_stride bytes apart.  The

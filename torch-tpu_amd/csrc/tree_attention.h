@@ -13,6 +13,7 @@
 #include <type_traits>
 #include "moe_common.h"
 #include "moe_layout.h"
+#include "attn_reach.h"
 #include "lanes.h"
 #include "../../include/moe_hip.h"
 
@@ -61,31 +62,10 @@ __device__ __forceinline__ AttnRequest attn_request(const AttnArgs &a, int b) {
   const int kv = (int)min((int64_t)a.kv_lens[b], (int64_t)a.table_width << a.page_log2);
   return {t0, t1 - t0, kv, kv - (t1 - t0)};
 }
-// rows of tile m see keys below this
-template <int ROWS>
-__device__ __forceinline__ int attn_tile_end(const AttnArgs &a, const AttnRequest &r, int m) {
-  if (a.masks || r.n == 1) return r.kv;
-  return r.prefix + min(r.n, (min((m + 1) * ROWS, r.n * a.G) - 1) / a.G + 1);
-}
-// The units of keys that tile m goes over: without a window units 0 .. u, with one the first tokens' and then those from the lowest
-// key that one of its rows sees in its window on.  Of the units at the two ends only keys that a row may see are read: in place of the others their
-// nearest such neighbour, whose line is on its way anyway.  (64 single tokens in a window of 1024 with 4 first ones, units of 128: 36.6 us, 41.4 with all ten units read whole.)
-struct AttnReach {
-  int units, first, skip;              // in all; of the first tokens; left out behind them
-  int every;                           // every row of the tile sees keys from here on (up to where the new tokens begin)
-  int high, low;                       // no row sees a key above `high` in the first tokens' units, nor one below `low` in those behind them
-  __device__ __forceinline__ int unit(int c) const { return c + (c >= first ? skip : 0); }
-  __device__ __forceinline__ int read(int c, int key) const { return max(min(key, c < first ? high : 0x7fffffff), c < first ? 0 : low); }
-};
 template <int ROWS, int UNIT, bool LOCAL>
 __device__ __forceinline__ AttnReach attn_reach(const AttnArgs &a, const AttnRequest &r, int m) {
-  const int end = attn_tile_end<ROWS>(a, r, m), upto = (end + UNIT - 1) / UNIT;
-  if (!LOCAL) return {upto, 0, 0, 0, 0, 0};
-  // (the window may be 2^31 - 1: each line's first term is a length)
-  const int j0 = a.masks ? -1 : m * ROWS / a.G, j1 = a.masks ? r.n - 1 : (min((m + 1) * ROWS, r.n * a.G) - 1) / a.G;
-  const int low = max(r.prefix + j0 + 1 - a.window, 0), head = min(a.sinks, end), first = (head + UNIT - 1) / UNIT;
-  const int skip = max(low / UNIT - first, 0);
-  return {upto - skip, first, skip, r.prefix + j1 + 1 - a.window, low >= first * UNIT ? head - 1 : 0x7fffffff, low};
+  if (LOCAL) return attn_window_reach(ROWS, UNIT, a.masks, r.n, a.G, r.prefix, a.window, a.sinks, m);
+  return {(attn_tile_end(ROWS, a.masks, r.n, a.G, r.prefix, m) + UNIT - 1) / UNIT, 0, 0, 0, 0, 0};
 }
 template <int ROWS, int UNIT>
 __device__ __forceinline__ int attn_head_units(const AttnArgs &a, const AttnRequest &r) {
@@ -603,11 +583,12 @@ __device__ __forceinline__ void attn_add_no_numbers(const AttnArgs &a, const Att
   const int g4 = 4 * ((threadIdx.x & 63) >> 4);
 #pragma unroll 1
   for (int key = first_key; key < min(first_key + keys, r.kv); key++) {
+    bool sees[NQ], some = false;
+#pragma unroll
+    for (int qc = 0; qc < NQ; qc++) some |= sees[qc] = sight.from(a, r, qc, key) & 1;
+    if (LOCAL && !__any(some)) continue;                // (its page may not be the request's any more)
     const int block = attn_block(a, table, key);
     const uint8_t *row = attn_row<attn_row_bytes(C, 16 * DT)>(a, a.v_cache, a.v_block_bytes, block, kh, key);
-    bool sees[NQ];
-#pragma unroll
-    for (int qc = 0; qc < NQ; qc++) sees[qc] = sight.from(a, r, qc, key) & 1;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
 #pragma unroll
@@ -711,7 +692,7 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(const AttnArgs a) {
     int block[2];
     const auto key_of = [&](int unit, int kt) {
       const int key = reach.unit(unit) * UNIT + 32 * part_of_unit + 16 * kt + c16;
-      return min(LOCAL ? reach.read(unit, key) : key, r.kv - 1);
+      return min(LOCAL ? reach.read(key) : key, r.kv - 1);
     };
     const auto blocks = [&](int unit) {
 #pragma unroll
@@ -898,7 +879,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const AttnArgs a) {
     int block;                                         // of the unit that is asked for next
     const auto key_of = [&](int unit) {
       const int c = min(unit, last), key = reach.unit(c) * UNIT + stage_row;
-      return min(LOCAL ? reach.read(c, key) : key, r.kv - 1);
+      return min(LOCAL ? reach.read(key) : key, r.kv - 1);
     };
     const auto is_edge = [&](int unit) { return (reach.unit(unit) + 1) * UNIT > clear || (LOCAL && reach.unit(unit) * UNIT < reach.every); };
     const auto ask = [&](int unit) {
@@ -1025,7 +1006,7 @@ __global__ __launch_bounds__(512, 2) void attn_pairs_kernel(const AttnArgs a) {
     int block, block_v;                                // of the key, of the value that is asked for next
     const auto key_of = [&](int unit) {
       const int c = min(unit, last), key = reach.unit(c) * UNIT + stage_row;
-      return min(LOCAL ? reach.read(c, key) : key, r.kv - 1);
+      return min(LOCAL ? reach.read(key) : key, r.kv - 1);
     };
     const auto is_edge = [&](int unit) { return (reach.unit(unit) + 1) * UNIT > clear || (LOCAL && reach.unit(unit) * UNIT < reach.every); };
     const auto ask = [&](bool values, int blk, int unit, Piece (&to)[NU], uint32_t &power) {

@@ -1,6 +1,6 @@
 // Attention over the paged cache with a window and first tokens that stay visible, and over a cache in 4 bits: the LOCAL kernels of
 // tree_attention.h.  They are instances of their own, so that calls without a window over bf16 and e4m3 caches keep their registers and times.
-//   64 single tokens, 16384 keys in a window of 1024, bf16     36.6 us, 3.7 TB/s: a workgroup's tile at once, then launch, lengths and a tile's end
+//   64 single tokens, 16384 keys in a window of 1024, bf16     37.2 us, 3.7 TB/s: a workgroup's tile at once, then launch, lengths and a tile's end
 //   64 single tokens over up to 8192 keys in 4 bits            55.5 us, 3.2 TB/s: half lines of memory, and the conversions
 //   one token over 32767 keys in 4 bits                        18.5 us: a chain of launch, tables, a few units and the join
 #include <algorithm>

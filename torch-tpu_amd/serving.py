@@ -77,7 +77,8 @@ def tree_attention(q, k_cache, v_cache, block_tables, kv_lens, cu_tokens, masks=
     q [T, Hq, D] bf16, D 64 or 128, Hq a multiple of the cache's heads; caches [blocks, page, heads, D] bf16 or e4m3 (with the
     scales of qk_norm_rope), or in 4 bits as qk_norm_rope writes them; kv_lens [B] and cu_tokens [B + 1] from the plan; scale, of any sign, defaults to
     D ** -0.5.  window: of the keys that a row may see by these rules, in the cache's order, it sees the last `window` and the first
-    `sinks`; pages that none of a request's rows sees are not read (their table entries may be anything).
+    `sinks`; pages that none of a request's rows sees are not read (their table entries may be anything; of a tree a row that sees no new
+    token counts too).
     Returns out [T, Hq, D] bf16, or (out, lse [T, Hq] float32).  A row that sees no key is 0, its lse -inf."""
     o, lse = _ops.tree_attention.default(q, k_cache, v_cache, block_tables, kv_lens, cu_tokens, masks, scale, k_scale, v_scale, out, return_lse,
                                        window, sinks)
