@@ -216,16 +216,26 @@ def test_four_bits_are_off_by_a_fifth_at_most():
     assert off(alone)[top <= 4].max() <= 1 / 7 and off(alone)[top >= 6].max() <= 1 / 7
 
 
-def test_keys_that_no_row_sees_are_not_read(tmp_path):
-    """The arithmetic of a tile's way over the keys, built with g++ and its sanitizers, against what every row sees (tests/host_reach_check.cpp)."""
+def host_check(tmp_path, name, said):
+    """Builds tests/<name>.cpp with g++ and its sanitizers, and runs it."""
     import os
     import shutil
     import subprocess
     if shutil.which("g++") is None:
         pytest.skip("no g++")
-    exe, src = tmp_path / "host_reach_check", os.path.join(os.path.dirname(os.path.abspath(__file__)), "host_reach_check.cpp")
+    exe, src = tmp_path / name, os.path.join(os.path.dirname(os.path.abspath(__file__)), name + ".cpp")
     r = subprocess.run(["g++", "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", "-fno-sanitize-recover=all", "-static-libasan", src, "-o", str(exe)],
                        stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     assert r.returncode == 0, r.stdout[-3000:]
     r = subprocess.run([str(exe)], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=300)
-    assert r.returncode == 0 and "reach checks passed" in r.stdout, r.stdout[-3000:]
+    assert r.returncode == 0 and said in r.stdout, r.stdout[-3000:]
+
+
+def test_keys_that_no_row_sees_are_not_read(tmp_path):
+    """The arithmetic of a tile's way over the keys against what every row sees."""
+    host_check(tmp_path, "host_reach_check", "reach checks passed")
+
+
+def test_rows_between_rows(tmp_path):
+    """What tells whether results lie over what is read, against a look at every byte."""
+    host_check(tmp_path, "host_rows_check", "row checks passed")

@@ -225,3 +225,21 @@ def test_tokens_beyond_32_bits_are_no_tokens(pkg, dev):
     cu = torch.tensor([0, 2], dtype=torch.int32, device=dev)
     for masks in (None, torch.tensor([1, 3], device=dev)):
         assert not pkg.adjust_logits(x, cu, tokens=tokens, masks=masks, presence=torch.ones(1, device=dev)).any()
+
+
+@pytest.mark.parametrize("bf16,V", [(True, 1003), (False, 4096)])
+def test_results_beside_what_they_come_from(pkg, dev, bf16, V):
+    """Logits and results in the two halves of one buffer, where no row lies over another."""
+    say("adjust_logits, two halves of a buffer", V)
+    c = Case(V + 1, [3, 1, 4], V, 60, bf16, True, biases=3, masked="rows")
+    a = c.args(dev)
+    want = pkg.adjust_logits(**a)
+    both = torch.full((c.T, 2 * V), 5.0, dtype=c.x.dtype, device=dev)
+    for first in (0, V):
+        both[:, first:first + V] = c.x.to(dev)
+        a.update(logits=both[:, first:first + V], out=both[:, V - first:2 * V - first])
+        assert torch.equal(pkg.adjust_logits(**a), want)
+        assert torch.equal(both[:, first:first + V].cpu(), c.x)
+    a.update(logits=both[:, :V], out=both[:, 1:V + 1])
+    with pytest.raises(RuntimeError):
+        pkg.adjust_logits(**a)

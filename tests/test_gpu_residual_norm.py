@@ -162,3 +162,21 @@ def test_offsets_beyond_32_bits(pkg, dev):
     x.copy_(a["x"].to(dev))
     y, h = pkg.residual_norm(x, a["residual"].to(dev), a["weight"].to(dev), a["post_weight"].to(dev))
     check(a, (y, h), 1.0, 1e-6)
+
+
+@pytest.mark.parametrize("gate", ["full", "token"])
+def test_a_gate_beside_what_it_gates(pkg, dev, gate):
+    """A projection's columns hold the block's output and its gate; the results take the output's and the residual's place."""
+    say("residual_norm, gate beside x", gate)
+    H, T = 256, 9
+    a = make(T, H, 11, gate=gate)
+    want = pkg.residual_norm(**{k: v.to(dev) for k, v in a.items()})
+    wide = torch.zeros(T, 2 * H, dtype=torch.bfloat16, device=dev)
+    cols = a["gate"].shape[1]
+    wide[:, :H], wide[:, H:H + cols] = a["x"].to(dev), a["gate"].to(dev)
+    x, g, r = wide[:, :H], wide[:, H:H + cols], a["residual"].to(dev)
+    y, h = pkg.residual_norm(x, r, a["weight"].to(dev), a["post_weight"].to(dev), g, out=x, residual_out=r)
+    assert torch.equal(y, want[0]) and torch.equal(h, want[1]) and torch.equal(g.cpu(), a["gate"])
+    for bad in (wide[:, H:], wide[:, 1:H + 1]):          # over the gate, over part of x
+        with pytest.raises(RuntimeError):
+            pkg.residual_norm(x, r, a["weight"].to(dev), a["post_weight"].to(dev), g, out=bad)

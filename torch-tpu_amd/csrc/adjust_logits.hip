@@ -18,6 +18,7 @@
 #include <math.h>
 #include <type_traits>
 #include "moe_common.h"
+#include "rows_clash.h"
 #include "../../include/moe_hip.h"
 
 namespace moe {
@@ -303,15 +304,13 @@ extern "C" int moe_adjust_logits(void *stream, const void *logits, int dtype, in
   if (!logits || !out || (n_bias && (!bias_ids || !bias)) || (masks && !tokens)) return MOE_E_NULL;
   const int64_t e = dtype == MOE_DTYPE_BF16 ? 2 : 4;
   if ((uintptr_t)logits % e || (uintptr_t)out % e) return MOE_E_ALIGN;
-  const uint8_t *i0 = (const uint8_t *)logits, *o0 = (const uint8_t *)out;
-  if (!(i0 == o0 && (row_stride == out_stride || T == 1)) && i0 < o0 + ((T - 1) * out_stride + V) * e && o0 < i0 + ((T - 1) * row_stride + V) * e)
-    return MOE_E_MODE;
   const auto over = [&](const void *p, int64_t rows, int64_t stride, int64_t row, int size) {      // out lies over an input of such rows
-    return p && rows > 0 && row > 0 && (const uint8_t *)p < o0 + ((T - 1) * out_stride + V) * e && o0 < (const uint8_t *)p + ((rows - 1) * stride + row) * size;
+    return rows_clash(out, out_stride * e, V * e, T, p, stride * size, row * size, rows);
   };
-  if (over(cu_tokens, 1, 0, B + 1ll, 4) || over(history, B, history_stride, L, 4) || over(tokens, 1, 0, T, 8) || over(masks, 1, 0, T, 8) ||
-      over(n_bias ? bias_ids : nullptr, B, bias_ids_stride, n_bias, 4) || over(n_bias ? bias : nullptr, B, bias_stride, n_bias, 4) ||
-      over(allowed, n_allowed, allowed_stride, (V + 31) / 32, 4) || over(allowed ? allowed_rows : nullptr, 1, 0, T, 4))
+  if ((!(logits == out && (row_stride == out_stride || T == 1)) && over(logits, T, row_stride, V, (int)e)) || over(cu_tokens, 1, 0, B + 1ll, 4) ||
+      over(history, B, history_stride, L, 4) || over(tokens, 1, 0, T, 8) || over(masks, 1, 0, T, 8) || over(n_bias ? bias_ids : nullptr, B, bias_ids_stride, n_bias, 4) ||
+      over(n_bias ? bias : nullptr, B, bias_stride, n_bias, 4) || over(allowed, n_allowed, allowed_stride, (V + 31) / 32, 4) ||
+      over(allowed ? allowed_rows : nullptr, 1, 0, T, 4))
     return MOE_E_MODE;
   for (const void *p : {(const void *)history_lens, (const void *)prompt_lens, (const void *)repetition, (const void *)frequency, (const void *)presence})
     if (over(p, 1, 0, B, 4)) return MOE_E_MODE;

@@ -13,6 +13,7 @@
 #include <type_traits>
 #include "moe_common.h"
 #include "lanes.h"
+#include "rows_clash.h"
 #include "../../include/moe_hip.h"
 
 namespace moe {
@@ -210,17 +211,6 @@ __global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) void residual_norm_ke
   }
 }
 
-// Whether rows of `bytes` bytes, T of them `stride` bytes apart, share memory with others; the same rows do not count.
-static bool rows_clash(const void *a, int64_t a_stride, int64_t a_bytes, const void *b, int64_t b_stride, int64_t b_bytes, int64_t T) {
-  if (!a || !b || T == 0) return false;
-  const uint8_t *p = (const uint8_t *)a, *q = (const uint8_t *)b;
-  if (p == q && (T == 1 || a_stride == b_stride) && a_bytes == b_bytes) return false;
-  if (p + (T - 1) * a_stride + a_bytes <= q || q + (T - 1) * b_stride + b_bytes <= p) return false;
-  if (T == 1 || a_stride != b_stride || a_stride <= 0) return true;
-  const int64_t off = ((q - p) % a_stride + a_stride) % a_stride;
-  return off < a_bytes || a_stride - off < b_bytes;
-}
-
 }  // namespace moe
 
 extern "C" int moe_residual_norm(void *stream, const void *x_bf16, int64_t x_stride, int T, int H, const void *residual, int residual_dtype,
@@ -244,15 +234,14 @@ extern "C" int moe_residual_norm(void *stream, const void *x_bf16, int64_t x_str
     return MOE_E_ALIGN;
   // What is written lies over nothing that is read, but a row may take the place of the row that it comes from.
   const int64_t xs = 2 * x_stride, ys = 2 * y_stride, rs = rb * residual_stride, hs = rb * residual_out_stride, row = 2ll * H, wide = rb * H;
-  const int64_t gate_rows = gate_row_stride ? T : 1, gate_row = gb * (gate_col_stride ? H : 1);
+  const int64_t gs = gb * gate_row_stride, gate_rows = gate_row_stride ? T : 1, gate_row = gb * (gate_col_stride ? H : 1);
   const auto over = [&](const void *p, int64_t stride, int64_t bytes) {
-    if (rows_clash(p, stride, bytes, x_bf16, xs, row, T) || rows_clash(p, stride, bytes, residual, rs, wide, T)) return true;
-    for (const void *w : {weight, post_weight})
-      if (w && (const uint8_t *)p < (const uint8_t *)w + wb * H && (const uint8_t *)w < (const uint8_t *)p + (T - 1) * stride + bytes) return true;
-    return gate && (const uint8_t *)p < (const uint8_t *)gate + (gate_rows - 1) * gate_row_stride * gb + gate_row &&
-           (const uint8_t *)gate < (const uint8_t *)p + (T - 1) * stride + bytes;
+    const auto on = [&](const void *q, int64_t q_stride, int64_t q_bytes, int64_t rows) { return rows_clash(p, stride, bytes, T, q, q_stride, q_bytes, rows); };
+    const auto place_of = [&](const void *q, int64_t q_stride, int64_t q_bytes) { return p == q && (T == 1 || stride == q_stride) && bytes == q_bytes; };
+    return (!place_of(x_bf16, xs, row) && on(x_bf16, xs, row, T)) || (!place_of(residual, rs, wide) && on(residual, rs, wide, T)) ||
+           on(weight, 0, wb * H, 1) || on(post_weight, 0, wb * H, 1) || on(gate, gs, gate_row, gate_rows);
   };
-  if (over(y_bf16, ys, row) || (residual_out && (over(residual_out, hs, wide) || residual_out == y_bf16 || rows_clash(residual_out, hs, wide, y_bf16, ys, row, T))))
+  if (over(y_bf16, ys, row) || (residual_out && (over(residual_out, hs, wide) || rows_clash(residual_out, hs, wide, T, y_bf16, ys, row, T))))
     return MOE_E_MODE;
   NormArgs a{(const uint16_t *)x_bf16, x_stride, residual, residual_stride, weight, post_weight, gate, gate_row_stride, gate_col_stride,
              (uint16_t *)y_bf16, residual_out, y_stride, residual_out_stride, scale, eps, 1.0f / (float)H, T, H,
