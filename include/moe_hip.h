@@ -509,7 +509,7 @@ int moe_token_logprobs(void *stream, const void *logits, int logits_dtype, int64
  * weights of 1), gate of gate_dtype or NULL (1), its value of row t and column c at t gate_row_stride + c gate_col_stride, of which either
  * may be 0 and the second at most 1.  y [T, H] bf16 from the h before its rounding; residual_out [T, H] of residual_dtype = h, or NULL.  Rows at any
  * distance.  y and residual_out may each take the place of x or residual, row on row; otherwise nothing written may lie over what is read (MOE_E_MODE).
- * H at most 32768.
+ * H at most 32768, T below 2^32 over a row's lanes, of which there are 64 to 1024, one to 8 values: 2^22 at H 8192.
  */
 int moe_residual_norm(void *stream, const void *x_bf16, int64_t x_stride, int T, int H, const void *residual, int residual_dtype,
                       int64_t residual_stride, const void *weight, const void *post_weight, int weight_dtype, const void *gate,

@@ -216,6 +216,18 @@ def test_four_bits_are_off_by_a_fifth_at_most():
     assert off(alone)[top <= 4].max() <= 1 / 7 and off(alone)[top >= 6].max() <= 1 / 7
 
 
+def test_launches_of_too_many_threads_are_refused(pkg):
+    """Of 2^32 threads and more: by the entry points, not by the launch (nor cut off by it)."""
+    far = lambda n: ctypes.c_void_p(n << 44)
+    norm = lambda T, H: lib().moe_residual_norm(None, far(1), H, T, H, far(2), 1, H, None, None, 1, None, 1, 0, 0, 1.0, 1e-6, far(3), H, far(4), H)
+    for T, H in ((1 << 22, 8192), (1 << 22, 4104), (1 << 26, 512), (1 << 25, 1024), ((1 << 31) - 1, 1), (1 << 22, 32768)):
+        assert norm(T, H) == E_SHAPE, (T, H)
+    assert lib().moe_adjust_logits(None, far(1), 0, 1 << 20, (1 << 20) - 1, 1 << 20, None, (1 << 20) - 1, *[None, 0, 0], *[None] * 7, None, 0, None, 0, 0, None, 0, 0, None,
+                                   far(3), 1 << 20) == E_SHAPE
+    assert lib().moe_qk_norm_rope(None, far(1), 24, 1 << 30, 1, 1, 8, far(2), None, 0, 0, 0, None, None, 1, 1e-6, far(3), None, None, None, 1, 0, 0, 0, 1, None, None,
+                                  None) == E_SHAPE
+
+
 def host_check(tmp_path, name, said):
     """Builds tests/<name>.cpp with g++ and its sanitizers, and runs it."""
     import os

@@ -324,7 +324,7 @@ extern "C" int moe_adjust_logits(void *stream, const void *logits, int dtype, in
     constexpr int BYTES = decltype(bytes)::value, TH = decltype(threads)::value;
     a.segments = (int)((wide * e + BYTES - 1) / BYTES);
     const int64_t blocks = (int64_t)a.segments * T;
-    if (blocks > 0x7fffffff) return MOE_E_SHAPE;
+    if (blocks * TH >> 32) return MOE_E_SHAPE;         // (a launch has fewer than 2^32 threads)
     if (a.bf16) adjust_logits_kernel<BYTES, TH, true><<<(unsigned)blocks, TH, 0, st>>>(a);
     else adjust_logits_kernel<BYTES, TH, false><<<(unsigned)blocks, TH, 0, st>>>(a);
     return (int)hipGetLastError();

@@ -260,7 +260,7 @@ static int norm_rope(void *stream, const void *qkv_bf16, int64_t row_stride, int
   a.groups_per_token = (int)((heads + most - 1) / most);
   const int lph = D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32;
   const int64_t groups = (int64_t)T * a.groups_per_token, blocks = (groups + 256 / lph - 1) / (256 / lph);
-  if (blocks > 0x7fffffff) return MOE_E_SHAPE;
+  if (blocks * 256 >> 32) return MOE_E_SHAPE;          // (a launch has fewer than 2^32 threads)
   hipStream_t st = (hipStream_t)stream;
   const auto run = [&](auto lanes) {
     constexpr int LPH = decltype(lanes)::value;

@@ -223,6 +223,10 @@ extern "C" int moe_residual_norm(void *stream, const void *x_bf16, int64_t x_str
   if (T < 0 || H < 1 || H > 32768 || x_stride < H || y_stride < H || (residual && residual_stride < H) || (residual_out && residual_out_stride < H) ||
       !(eps >= 0.f))
     return MOE_E_SHAPE;
+  const int pieces = (H + 7) / 8;
+  int lanes = 64;                                      // of a row
+  while (lanes < pieces && lanes < 1024) lanes *= 2;
+  if ((T + 3ll) * lanes >> 32) return MOE_E_SHAPE;     // (a launch has fewer than 2^32 threads)
   if (gate && (gate_row_stride < 0 || gate_col_stride < 0 || gate_col_stride > 1 || (gate_row_stride && gate_col_stride && gate_row_stride < H)))
     return MOE_E_SHAPE;
   if (T == 0) return MOE_OK;
@@ -255,7 +259,6 @@ extern "C" int moe_residual_norm(void *stream, const void *x_bf16, int64_t x_str
   const unsigned grid = (unsigned)T;
   const auto run = [&](auto how) {
     constexpr int A = decltype(how)::value;
-    const int pieces = (H + 7) / 8;
     if (pieces <= 64) residual_norm_kernel<1, 1, A><<<(grid + 3) / 4, 256, 0, st>>>(a);
     else if (pieces <= 128) residual_norm_kernel<2, 1, A><<<grid, 128, 0, st>>>(a);
     else if (pieces <= 256) residual_norm_kernel<4, 1, A><<<grid, 256, 0, st>>>(a);
