@@ -529,6 +529,8 @@ int moe_residual_norm(void *stream, const void *x_bf16, int64_t x_stride, int T,
  * outside [0, n_allowed): everything is allowed.  fp32, one rounding.  Ids outside [0, V) are passed over; rows of no request pass
  * as they are.  L + T below 2^20, n_bias at most MOE_MAX_BIASES.
  */
+/* Bytes of a row to a workgroup of such a call, for rows that begin on 16 bytes; L: of the histories, 0 without any.  0: not a valid call. */
+int moe_adjust_logits_segment_bytes(int dtype, int T, int V, int L);
 int moe_adjust_logits(void *stream, const void *logits, int dtype, int64_t row_stride, int T, int V, const int32_t *cu_tokens, int B,
                       const int32_t *history, int64_t history_stride, int L, const int32_t *history_lens, const int32_t *prompt_lens,
                       const int64_t *tokens, const int64_t *masks, const float *repetition, const float *frequency,

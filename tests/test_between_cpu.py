@@ -251,3 +251,15 @@ def test_keys_that_no_row_sees_are_not_read(tmp_path):
 def test_rows_between_rows(tmp_path):
     """What tells whether results lie over what is read, against a look at every byte."""
     host_check(tmp_path, "host_rows_check", "row checks passed")
+
+
+def test_segments_of_logits(pkg):
+    """64 KB to a workgroup where these fill the chip once or twice and histories are long; never for rows that leave them empty."""
+    of = lambda *a: lib().moe_adjust_logits_segment_bytes(*a)
+    for (T, V, L, bf16), kb in {(1, 131072, 4096, 1): 16, (32, 131072, 8192, 1): 24, (20, 131072, 8192, 1): 16, (40, 131072, 8192, 1): 64, (64, 131072, 8192, 1): 64,
+                                (65, 131072, 8192, 1): 24, (80, 131072, 8192, 1): 24, (96, 131072, 8192, 1): 24, (128, 131072, 8192, 1): 64, (128, 131072, 8191, 1): 24,
+                                (129, 131072, 8192, 1): 24, (160, 100003, 4096, 1): 24, (64, 131072, 8192, 0): 64, (64, 131072, 4096, 0): 24, (64, 131072, 4095, 1): 24,
+                                (64, 131072, 0, 1): 24, (256, 1000, 8192, 1): 16, (512, 17000, 8192, 1): 24, (200, 33000, 8192, 1): 24}.items():
+        assert of(bf16, T, V, L) == kb << 10, (T, V, L, bf16)
+    for bad in ((2, 1, 1, 1), (1, 0, 1, 1), (1, 1, 0, 1), (1, 1, 1 << 30, 1), (1, 1, 1, -1)):
+        assert of(*bad) == 0

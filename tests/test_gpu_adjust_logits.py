@@ -243,3 +243,18 @@ def test_results_beside_what_they_come_from(pkg, dev, bf16, V):
     a.update(logits=both[:, :V], out=both[:, 1:V + 1])
     with pytest.raises(RuntimeError):
         pkg.adjust_logits(**a)
+
+
+@pytest.mark.parametrize("counts,V,L,bf16,tree,how,most", [
+    # every size of segment in both types: rows on 16 bytes and beside them, trees, grammars, biases
+    ([1] * 41, 131072, 4200, True, False, dict(masked="rows", biases=3), 64), ([1] * 45, 130001, 4100, True, False, {}, 64), ([1] * 24, 131072, 4096, False, False, dict(masked="own"), 64),
+    ([1] * 22, 130007, 5000, False, False, dict(biases=9), 64), ([16, 3, 22, 4], 131072, 4100, True, True, dict(masked="rows"), 64), ([1] * 128, 32000, 8192, False, False, {}, 64),
+    ([1] * 130, 32000, 8192, False, False, {}, 24), ([1] * 250, 64001, 8192, True, False, {}, 64), ([1] * 66, 131072, 4096, True, False, {}, 24), ([1] * 33, 131072, 4200, False, False, dict(masked="rows"), 24),
+    ([1] * 12, 131072, 8192, False, False, {}, 24), ([1] * 11, 131072, 8192, False, False, {}, 16), ([1] * 20, 131072, 5000, True, False, dict(biases=2), 16)])
+def test_segments_of_every_size(pkg, dev, counts, V, L, bf16, tree, how, most):
+    say("adjust_logits, segments of", most, "KB:", len(counts), V, L, bf16)
+    c = Case(V + L, counts, V, L, bf16, tree, **how)
+    assert pkg._lib.lib.moe_adjust_logits_segment_bytes(1 if bf16 else 0, c.T, V, L) == most << 10
+    got = pkg.adjust_logits(**c.args(dev))
+    torch.cuda.synchronize()
+    c.check(got)

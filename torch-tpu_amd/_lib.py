@@ -90,6 +90,7 @@ SIGNATURES = {
                                      c_void_p, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_size_t]),
     "moe_residual_norm": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int, c_void_p,
                                   c_int, c_int64, c_int64, c_float, c_float, c_void_p, c_int64, c_void_p, c_int64]),
+    "moe_adjust_logits_segment_bytes": (c_int, [c_int, c_int, c_int, c_int]),
     "moe_adjust_logits": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_int, c_void_p, c_int64, c_int, c_void_p,
                                   c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int,
                                   c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64]),

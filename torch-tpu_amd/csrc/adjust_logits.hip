@@ -10,11 +10,14 @@
 // counts the history's tokens that lie in the segment in LDS, so that no counter per vocabulary entry exists in memory, and a bit per token
 // says which were touched.  A row streams through registers, is stored as it is (but for what its grammar forbids) without waiting for the
 // counts, and the threads that stored the few touched values then store those once more.
-// 64 rows of 131072 fp32 values with up to 8192 tokens of history: 22 us, 13 without the histories (3.1 and 5.3 TB/s); 1275 rows of 100003
+// 64 rows of 131072 fp32 values with up to 8192 tokens of history: 22 to 23 us, 13 without the histories (3.0 and 5.3 TB/s); 1275 rows of 100003
 // bf16 values, 128 requests' trees, every other row with a grammar: 143 us, 94 with neither (3.6 and 5.4 TB/s).  What histories cost is the
 // comparisons of every token in every segment and the counting, about 25 instructions a token.  (LDS atomics of all lanes instead of a branch, and a list of
 // the touched tokens in place of the bits, took 5 to 15 % longer.  Up to four rows of a request to a workgroup, which then counts once for
 // them: 156 us for the 143, and 25 for 10 where there are 155 rows of 32000 values.)
+// Histories of one token only, or filled up with -1, cost up to 1.7 times as much in segments of 64 KB, where lanes wait for each other at one counter:
+// equal tokens are added up first only where 4 tokens of every thread, 4096 there, lie behind the prompt as a whole (38 us for the 22; bf16 22 for 13;
+// segments of 24 KB 73 for 83).
 #include <math.h>
 #include <type_traits>
 #include "moe_common.h"
@@ -284,6 +287,43 @@ __global__ __launch_bounds__(THREADS) void adjust_logits_kernel(const LogitArgs 
   }
 }
 
+// Bytes of a row to a workgroup.  Large segments read the histories and zero the counters less often, small ones put more workgroups to work: of 24 KB
+// three share a compute unit.  64 KB pay for long histories where they fill the chip once: a row's segments, times the rows, are workgroups of 1024
+// threads, of which a bf16 one has a compute unit's LDS for itself; a few more than 256 take a second turn.  Two whole turns still pay where
+// histories are longer.  Us, with the workgroups of 64 KB:
+//                                                               16 KB     24        64
+//   1 row of 131072 bf16, 4096 tokens of history      4         6.5       7.1       8.0
+//   32 of 131072 bf16, 8192                           128       11.1      11.4      11.7
+//   36 of 131072 bf16, 8192                           144       13.9      11.7      11.8
+//   40 of 131072 bf16, 8192                           160       13.9      12.1      11.5
+//   64 of 131072 bf16, 8192                           256       18.6      15.8      13.2
+//   256 of 32000 bf16, 8192                           256       21.1      17.6      14.5
+//   32 of 131072 fp32, 8192                           256       16.6      14.5      12.1
+//   64 of 131072 bf16, 2048                           256       12.7      12.0      12.2
+//   66 of 131072 bf16, 4096                           264       16.3      14.3      18.6
+//   72 of 131072 bf16, 8192                           288       20.8      18.6      21.7
+//   96 of 131072 bf16, 8192                           384       24.2      21.3      22.7
+//   160 of 100003 bf16, 4096                          640       25.7      23.9      35.0
+//   56 of 131072 fp32, 8192                           448       24.0      21.1      20.8
+//   500 of 32000 bf16, 8192                           500       33.3      29.4      27.0
+//   64 of 131072 fp32, 8192                           512       26.3      22.8      21.1 to 22.8
+//   64 of 131072 fp32, 4096                           512       21.6      19.5      20.0
+//   128 of 131072 bf16, 8192                          512       29.4      25.6      24.1 to 25.3
+//   128 of 131072 bf16, 4096                          512       25.0      22.1      22.2
+//   66 of 131072 fp32, 8192                           528       27.5      23.7      27.3
+//   514 of 5493 bf16 (205 trees), 300 biases                    14.2      14.9      32.6
+//   155 of 32000 bf16 (16 trees), 2000                155       10.1      9.6       11.8
+//   320 of 131072 fp32 (64 trees), 2000               2560      99        78        113
+//   512 of 100003 bf16, 4096                          2048      73        64        98
+//   1275 of 100003 bf16 (128 trees), 2048             5100      160       143       252
+// wide: a row's values with room for those before its first 16 bytes; L: of the histories, 0 without any.
+static int logit_segment(int64_t wide, int e, int T, int V, int L) {
+  const int64_t work = (int64_t)T * V * e, large = (wide * e + 65535) / 65536 * T;
+  if (L >= 4096 && large >= 160 && large <= 256 && work >= (10 << 20)) return 65536;
+  if (L >= 8192 && large >= 448 && large <= 512 && work >= (27 << 20)) return 65536;
+  return work < (6 << 20) ? 16384 : 24576;
+}
+
 }  // namespace moe
 
 extern "C" int moe_adjust_logits(void *stream, const void *logits, int dtype, int64_t row_stride, int T, int V, const int32_t *cu_tokens, int B,
@@ -330,19 +370,13 @@ extern "C" int moe_adjust_logits(void *stream, const void *logits, int dtype, in
     return (int)hipGetLastError();
   };
   using std::integral_constant;
-  const int64_t work = (int64_t)T * V * e;
-  // Large segments read the histories and zero the counters less often, small ones put more workgroups to work: of 24 KB three share a compute unit.  Us:
-  //                                                        16 KB     24        32        64
-  //   1 row of 131072 bf16, 4096 tokens of history         7.5       7.6       8.0       8.4
-  //   16 of 131072 bf16, 8192                              8.8       9.7       10.2      10.7
-  //   514 of 5493 bf16 (205 trees), 300 biases             14.2      14.9      19.5      32.6
-  //   155 of 32000 bf16 (16 trees), 2000                   10.1      9.6       10.3      11.8
-  //   64 of 131072 bf16, 8192                              19.5      16.4      16.0      14.0
-  //   64 of 131072 fp32, 8192                              27.9      23.8      23.5      23.6
-  //   320 of 131072 fp32 (64 trees), 2000                  99        78        80        113
-  //   512 of 100003 bf16, 4096                             73        64        69        98
-  //   1275 of 100003 bf16 (128 trees), 2048                160       143       159       252
-  if (work < (6 << 20)) return run(integral_constant<int, 16384>(), integral_constant<int, 512>());
-  if (history && L >= 4096 && work >= (16 << 20) && work <= (32 << 20)) return run(integral_constant<int, 65536>(), integral_constant<int, 1024>());      // (about one turn)
+  const int bytes = logit_segment(wide, (int)e, T, V, history ? L : 0);
+  if (bytes == 16384) return run(integral_constant<int, 16384>(), integral_constant<int, 512>());
+  if (bytes == 65536) return run(integral_constant<int, 65536>(), integral_constant<int, 1024>());
   return run(integral_constant<int, 24576>(), integral_constant<int, 512>());
+}
+
+extern "C" int moe_adjust_logits_segment_bytes(int dtype, int T, int V, int L) {
+  if ((dtype != MOE_DTYPE_F32 && dtype != MOE_DTYPE_BF16) || T < 1 || V < 1 || V >= (1 << 30) || L < 0) return 0;
+  return moe::logit_segment(V, dtype == MOE_DTYPE_BF16 ? 2 : 4, T, V, L);
 }
