@@ -283,7 +283,8 @@ def _run_norm(s):
 
 def _run_logits(s):
     return dict(logits=_package().adjust_logits(s["logits"], s["cu"], history=s["history"], history_lens=s["history_lens"],
-                                                prompt_lens=s["prompt_lens"], tokens=s["tokens"], masks=s["masks"],
+                                                prompt_lens=s["prompt_lens"], tokens=s["tokens"],
+                                                masks=s["masks"] if s["tokens"] is not None else None,    # (of no drafted tokens there are none)
                                                 repetition=s["repetition"], frequency=s["frequency"], presence=s["presence"],
                                                 bias_ids=s["bias_ids"], bias=s["bias"], allowed=s["allowed"], allowed_rows=s["allowed_rows"]))
 
