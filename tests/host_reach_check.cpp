@@ -41,7 +41,7 @@ int main() {
       for (int k = 0; k < kv; k++)
         if (k >= (int64_t)prefix - W) seen[k] = 1;
     for (int m = 0; m * rows < n * G; m++) {
-      const moe::AttnReach r = moe::attn_window_reach(rows, unit, masks, n, G, prefix, W, S, m);
+      const moe::AttnReach r = moe::attn_window_reach(rows, unit, masks, n, G, prefix, kv, W, S, m);
       const int clear = masks ? prefix : prefix + m * rows / G + 1;
       std::vector<char> read(kv, 0);
       CHECK(r.units > 0 && r.units <= (kv + unit - 1) / unit, "units %d of %d keys", r.units, kv);

@@ -15,17 +15,17 @@ struct AttnReach {
   constexpr int read(int key) const { return key < head ? key : key > low ? key : low; }
 };
 
-// Rows of tile m, `rows` of them, see keys below this.  A request's n tokens of G rows each stand behind `prefix` cached ones; a token of a tree
-// (masks) may see any new token.
-constexpr int attn_tile_end(int rows, bool masks, int n, int G, int prefix, int m) {
-  if (masks || n == 1) return prefix + n;
+// Rows of tile m, `rows` of them, see keys below this.  A request's n tokens of G rows each stand behind prefix = kv - n cached ones; a token
+// of a tree (masks) may see any new token.
+constexpr int attn_tile_end(int rows, bool masks, int n, int G, int prefix, int kv, int m) {
+  if (masks || n == 1) return kv;
   const int next = (m + 1) * rows < n * G ? (m + 1) * rows : n * G, tokens = (next - 1) / G + 1;
   return prefix + (tokens < n ? tokens : n);
 }
 
 // (The window may be 2^31 - 1: each sum's first term is a length.)  In a tree the lowest key is that of a token that sees no new one.
-constexpr AttnReach attn_window_reach(int rows, int unit, bool masks, int n, int G, int prefix, int window, int sinks, int m) {
-  const int end = attn_tile_end(rows, masks, n, G, prefix, m), upto = (end + unit - 1) / unit;
+constexpr AttnReach attn_window_reach(int rows, int unit, bool masks, int n, int G, int prefix, int kv, int window, int sinks, int m) {
+  const int end = attn_tile_end(rows, masks, n, G, prefix, kv, m), upto = (end + unit - 1) / unit;
   const int next = (m + 1) * rows < n * G ? (m + 1) * rows : n * G;
   const int j0 = masks ? -1 : m * rows / G, j1 = masks ? n - 1 : (next - 1) / G;
   const int below = prefix + j0 + 1 - window, low = below > 0 ? below : 0;

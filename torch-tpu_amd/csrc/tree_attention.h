@@ -64,8 +64,8 @@ __device__ __forceinline__ AttnRequest attn_request(const AttnArgs &a, int b) {
 }
 template <int ROWS, int UNIT, bool LOCAL>
 __device__ __forceinline__ AttnReach attn_reach(const AttnArgs &a, const AttnRequest &r, int m) {
-  if (LOCAL) return attn_window_reach(ROWS, UNIT, a.masks, r.n, a.G, r.prefix, a.window, a.sinks, m);
-  return {(attn_tile_end(ROWS, a.masks, r.n, a.G, r.prefix, m) + UNIT - 1) / UNIT, 0, 0, 0, 0, 0};
+  if (LOCAL) return attn_window_reach(ROWS, UNIT, a.masks, r.n, a.G, r.prefix, r.kv, a.window, a.sinks, m);
+  return {(attn_tile_end(ROWS, a.masks, r.n, a.G, r.prefix, r.kv, m) + UNIT - 1) / UNIT, 0, 0, 0, 0, 0};
 }
 template <int ROWS, int UNIT>
 __device__ __forceinline__ int attn_head_units(const AttnArgs &a, const AttnRequest &r) {
@@ -583,12 +583,17 @@ __device__ __forceinline__ void attn_add_no_numbers(const AttnArgs &a, const Att
   const int g4 = 4 * ((threadIdx.x & 63) >> 4);
 #pragma unroll 1
   for (int key = first_key; key < min(first_key + keys, r.kv); key++) {
-    bool sees[NQ], some = false;
+    if (LOCAL) {                                       // (a page that no row sees may not be the request's any more)
+      bool some = false;
 #pragma unroll
-    for (int qc = 0; qc < NQ; qc++) some |= sees[qc] = sight.from(a, r, qc, key) & 1;
-    if (LOCAL && !__any(some)) continue;                // (its page may not be the request's any more)
+      for (int qc = 0; qc < NQ; qc++) some |= sight.from(a, r, qc, key) & 1;
+      if (!__any(some)) continue;
+    }
     const int block = attn_block(a, table, key);
     const uint8_t *row = attn_row<attn_row_bytes(C, 16 * DT)>(a, a.v_cache, a.v_block_bytes, block, kh, key);
+    bool sees[NQ];
+#pragma unroll
+    for (int qc = 0; qc < NQ; qc++) sees[qc] = sight.from(a, r, qc, key) & 1;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
 #pragma unroll
