@@ -8,8 +8,8 @@
 // Bound by bytes: every value is read once and written once, so a row stays in the registers of the wavefronts that share it, sums of
 // squares are added over lanes by data-parallel moves and over wavefronts in LDS, and y is formed from the h in registers, before
 // its rounding.  All of it in fp32 with one rounding to each output.
-// 16384 rows of 7168 bf16 values with both norms and a gate per column: 189 us, 5.0 TB/s, where a large copy reaches 4.85; 9808 rows of 1999
-// values, which begin anywhere, 40 us, 3.9 TB/s, of 2000 34; one row of 7168: 2.9 us, the chain of row, sum over the wavefronts and store.
+// 16384 rows of 7168 bf16 values with both norms and a gate per column: 185 to 189 us, 5.0 TB/s, where a large copy reaches 4.85; 9808 rows of 1999
+// values, which begin anywhere, with both norms 38 us, 4.1 TB/s, of 2000 32; one row of 7168: 2.9 us, the chain of row, sum over the wavefronts and store.
 #include <type_traits>
 #include "moe_common.h"
 #include "lanes.h"
@@ -34,7 +34,7 @@ struct NormArgs {
 
 // Eight neighbouring values of a row from `place` on.  kWhole: on 16 bytes, kAny: on their own size, which the memory path takes in one
 // access too, kFew: rows of fewer than eight.  Of kAny a row's last piece of fewer values is loaded as the row's last eight, of which the first `back` are another lane's and
-// count as 0 (they may be overwritten already where a row takes its own place), and stored in pieces of 4, 2 and 1.  (9808 rows of 1999 values with one norm: 38 us,
+// count as 0 (they may be overwritten already where a row takes its own place), and stored in pieces of 4, 2 and 1.  (9808 rows of 1999 values with one norm: 34 to 38 us,
 // 52 with the last piece value by value.)
 constexpr int kFew = 0, kAny = 1, kWhole = 2;
 typedef v4i __attribute__((aligned(2))) v4i_any;

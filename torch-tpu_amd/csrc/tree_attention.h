@@ -817,8 +817,10 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(const AttnArgs a) {
 // ---- staging in LDS (the two kernels below) ---------------------------------------------------------------------------
 // Rows of a stage are 32 bytes longer than their values, so that reads of operands spread over the banks.  TPR
 // threads write a row, 16 bytes of it at a time; which row thread group i takes is chosen so that the rows of one write fall into different
-// banks as well: four rows 4 apart, or of bytes widened to 32 apart 0, 1, 8 and 9.  Counted: no conflicts in the kernel of many rows on
-// a bf16 cache; in the one of 128 rows on an e4m3 cache 2.7 of 10.1 million cycles at which LDS is read or written.
+// banks as well: four rows 4 apart, or of bytes widened to 32 apart 0, 1, 8 and 9.  Of 4-bit codes, whose threads write a row's pieces further apart, rows
+// are taken in order: a write's 16-byte pieces fall on every other group of banks, each twice.  Counted: no conflicts in the kernel of many rows on a bf16
+// cache; in the one of 128 rows 2.7 of 10.1 million cycles at which LDS is read or written on an e4m3 cache, 2.7 of 10.0 in 4 bits; in the one of many rows 1.7
+// of 9.7 in 4 bits.
 template <int C, int TPR>
 __device__ __forceinline__ int attn_stage_row(int i) {
   if (C == MOE_DTYPE_FP4) return i;
@@ -987,7 +989,8 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const AttnArgs a) {
 // thousand clocks, the vector unit 220 thousand, of about 460 thousand: the two still add up more than they overlap.
 // 16 trees of up to 64 tokens over up to 12288 keys: 119 to 124 us, 600 to 622 TFLOP/s (tiles that are not full, and a join of 12 us).
 // LOCAL: the chunks in a window of 1024 58 us, 520 TFLOP/s of what the rows see (tiles of 64 tokens over 17 units for 16 units' worth of keys, then
-// the way to the first unit); the trees over a 4-bit cache in a window of 4095 75 us and a join of 10.5.
+// the way to the first unit), 66 over e4m3 and 63 over 4 bits; the trees in a window of 4095 87 to 92 us over each cache, of which 75 and a join of 10.5
+// over 4 bits (97 to 100 us and 700 to 730 TFLOP/s where all texts are equally long).
 template <int D, int C, bool LOCAL, int NQ>
 __global__ __launch_bounds__(512, 2) void attn_pairs_kernel(const AttnArgs a) {
   constexpr int ROWS = 128 * NQ, UNIT = 64, DT = D / 16, X = D / 32, LD = 2 * D + 32, HALF = UNIT * LD;
